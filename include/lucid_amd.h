@@ -52,8 +52,10 @@ extern "C" {
 #define LUCID_PRECISION_FAST 1  /* bf16 products everywhere */
 #define LUCID_PRECISION_EXACT 2 /* hi/lo split products for every head */
 
-/* ABI version of this header (bumped on any signature change or new entry point): 6. */
+/* ABI version of this header (bumped whenever an entry point changes or goes): 6; and the number of
+ * times that entry points have been added to that version: 1 (serving from a paged cache). */
 int lucid_abi_version(void);
+int lucid_abi_minor(void);
 
 /* Text of the last error on the calling thread ("" if none). */
 const char* lucid_last_error(void);
@@ -357,6 +359,75 @@ int lucid_causal_lm_loss_fwd(const void* logits, int64_t row_stride, const int64
                              float* lse, float* loss, float* valid, void* stream);
 int lucid_causal_lm_loss_bwd(const void* logits, int64_t row_stride, const int64_t* labels, int R, int T, int V,
                              const float* lse, const float* valid, const float* scale, void* dlogits, void* stream);
+
+/* ---- Serving from a paged (K, V') cache ----
+ * No counterpart in the reference, whose cache is one buffer per layer with one length for the whole
+ * batch (modeling_lucid.py:475-496).  A layer's two pools hold num_pages pages of page_size rows of
+ * every kv head, bf16 [num_pages, Hkv, page_size, W] at element strides {page, head, row} (multiples of
+ * 8; 16-byte aligned; each pool within 64 GB), W = lucid_page_width(D): the smallest of 64, 80, 96 and
+ * 128 that holds the head dim (0 for D outside [1, 128]).  Columns D .. W-1 are zero (the entry points
+ * write them so).  Row j of sequence b is row j % page_size of page page_table[b * table_stride +
+ * j / page_size]; max_pages ids a sequence.  page_table, cache_lens and new_lens are int32 device memory,
+ * read when the kernels run: a captured call follows what they hold at replay.  Pages may be shared
+ * by sequences as long as nothing is written to them; two sequences of one call must not write to the
+ * same page.  Page ids outside [0, num_pages) are never followed. */
+int lucid_page_width(int D);
+
+/* lucid_decode_tokens against pages: L new tokens of each of B sequences with lengths of their own.
+ * q [B,Hq,L,D], k and v [B,Hkv,L,D] bf16 at strides {batch, head, time} (any; the last axis contiguous
+ * and of exactly D columns), o [B,L,Hq,D] by its strides, vp_new fp32 [B,Hkv,L,D] contiguous.
+ * cache_lens[b] rows of sequence b are cached; its new rows go to rows cache_lens[b] .. + L - 1, whose
+ * pages must be in the table (cache_lens itself is the caller's to advance).  L tokens in one call give
+ * what L calls of one token give: a new token is coupled to, and attends to, the earlier new V' rows as
+ * the cache holds them (bf16).  cache_lens[b] < 0: no sequence, its o and vp_new are zeros.  A sequence
+ * whose table names a page outside the pool among those it needs, or is too short for the new rows,
+ * gets NaN in o and vp_new and nothing is appended to it; the others are not affected.  Cached rows
+ * must be finite (a NaN or an infinity in one gives NaN where it enters).
+ * ws: lucid_decode_paged_workspace_bytes (0 on bad sizes), 256-byte aligned, one per call in flight. */
+size_t lucid_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int L, int page_size, int max_pages, int D);
+int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                       const int64_t* v_strides, void* k_pages, const int64_t* k_page_strides, void* vp_pages,
+                       const int64_t* vp_page_strides, const int32_t* page_table, int64_t table_stride,
+                       const int32_t* cache_lens, void* o, const int64_t* o_strides, float* vp_new, void* ws, int B, int Hq,
+                       int Hkv, int L, int num_pages, int page_size, int max_pages, int D, float scale, float eps,
+                       void* stream);
+
+/* A prefill's rows into the pages: row t < new_lens[b] (all T where new_lens is null) of k (bf16) and
+ * vprime (bf16, or fp32 when vprime_f32 != 0, rounded to bf16), both [B,Hkv,T,D] at strides {batch, head,
+ * time}, goes to row cache_lens[b] + t of sequence b.  Rows of a sequence with a negative length, beyond
+ * its table or of a page id outside the pool are left out. */
+int lucid_write_pages(const void* k, const int64_t* k_strides, const void* vprime, const int64_t* vprime_strides,
+                      int vprime_f32, void* k_pages, const int64_t* k_page_strides, void* vp_pages,
+                      const int64_t* vp_page_strides, const int32_t* page_table, int64_t table_stride,
+                      const int32_t* cache_lens, const int32_t* new_lens, int B, int Hkv, int T, int num_pages,
+                      int page_size, int max_pages, int D, void* stream);
+
+/* Page src[i] copied over page dst[i], i < num_copies, in each of num_pools pools of one layout (pages of
+ * page_bytes contiguous bytes, page_stride_bytes apart).  pools, src and dst are host arrays, read before
+ * the call returns.  A page may be read any number of times, but is written once and not both read and
+ * written.  One launch per 64 pools and 256 pages. */
+int lucid_copy_pages(int num_pools, void* const* pools, int64_t page_stride_bytes, int64_t page_bytes, int num_pages,
+                     int num_copies, const int* src, const int* dst, void* stream);
+
+/* Log probabilities of given tokens under logit rows, with the rows' entropy and `top` most likely
+ * alternatives (0 .. 64; no counterpart in the reference beside the mean loss of
+ * modeling_lucid.py:847-967).  logits (LUCID_DTYPE_BF16 or _F32): R rows of V contiguous values, row r at
+ * (r / T) batch_stride + (r % T) row_stride elements, any alignment of whole elements; x = logits /
+ * temperature.  logprobs[r] = x[tokens[r]] - lse (0 where the token is -100, NaN where it is outside
+ * [0, V)), entropy[r] = lse - sum p x; top_logprobs / top_indices [R][top] by (logit descending, index
+ * ascending).  A logit of -inf has probability 0; a row of -inf alone, or with a NaN or +inf, gives NaN (NaN
+ * logits come first among the alternatives).  stats: 3 floats a row for the backward.  ws: 256-byte
+ * aligned, needed where its size is not 0.
+ * The backward writes dlogits [R][V] (contiguous, the logits' dtype) from any of the three outputs'
+ * gradients (null: none). */
+size_t lucid_token_logprobs_workspace_bytes(int R, int V, int top);
+int lucid_token_logprobs_fwd(const void* logits, int64_t batch_stride, int64_t row_stride, const int64_t* tokens, int R,
+                             int T, int V, int dtype, float temperature, int top, float* logprobs, float* entropy,
+                             float* stats, float* top_logprobs, int64_t* top_indices, void* ws, void* stream);
+int lucid_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t row_stride, const int64_t* tokens, int R,
+                             int T, int V, int dtype, float temperature, int top, const float* stats,
+                             const int64_t* top_indices, const float* dlogprobs, const float* dentropy,
+                             const float* dtop_logprobs, void* dlogits, void* stream);
 
 /* Zero-pad n (1 to 3) tensors [B, H[i], T, d] of one dtype (LUCID_DTYPE_BF16 or
  * LUCID_DTYPE_F32), element strides strides[3 i ..] of their first three axes, unit stride on

@@ -6,6 +6,7 @@ is raised.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -23,10 +24,12 @@ _i64p = ctypes.POINTER(ctypes.c_int64)
 _int = ctypes.c_int
 _flt = ctypes.c_float
 _sz = ctypes.c_size_t
+_i64 = ctypes.c_int64
 
 _SIGS = {
     "liblucid_amd.so": {
         "lucid_abi_version": ([], _int),
+        "lucid_abi_minor": ([], _int),
         "lucid_last_error": ([], ctypes.c_char_p),
         "lucid_fwd_workspace_bytes": ([_int] * 5, _sz),
         "lucid_set_precision": ([_int], _int),
@@ -99,6 +102,19 @@ _SIGS = {
                               _vp], _int),
         "lucid_decode_tokens": ([_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp,
                                  _int, _int, _int, _int, _int, _int, _int, _flt, _flt, _vp], _int),
+        "lucid_page_width": ([_int], _int),
+        "lucid_decode_paged_workspace_bytes": ([_int] * 7, _sz),
+        "lucid_decode_paged": ([_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _i64p,
+                                _vp, _vp, _int, _int, _int, _int, _int, _int, _int, _int, _flt, _flt, _vp], _int),
+        "lucid_write_pages": ([_vp, _i64p, _vp, _i64p, _int, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp,
+                               _int, _int, _int, _int, _int, _int, _int, _vp], _int),
+        "lucid_copy_pages": ([_int, ctypes.POINTER(_vp), _i64, _i64, _int, _int, ctypes.POINTER(_int),
+                              ctypes.POINTER(_int), _vp], _int),
+        "lucid_token_logprobs_workspace_bytes": ([_int] * 3, _sz),
+        "lucid_token_logprobs_fwd": ([_vp, _i64, _i64, _vp, _int, _int, _int, _int, _flt, _int, _vp, _vp, _vp, _vp, _vp,
+                                      _vp, _vp], _int),
+        "lucid_token_logprobs_bwd": ([_vp, _i64, _i64, _vp, _int, _int, _int, _int, _flt, _int, _vp, _vp, _vp, _vp, _vp,
+                                      _vp, _vp], _int),
         "lucid_profile_enable": ([_int], None),
         "lucid_profile_collect": ([], _int),
         "lucid_profile_entry": ([_int, ctypes.c_char_p, _int, ctypes.POINTER(ctypes.c_double),
@@ -216,6 +232,13 @@ def strides3(t: torch.Tensor, dims: tuple[int, int, int]):
 
 def ptr(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.data_ptr())
+
+
+def on(device: torch.device):
+    """A context in which ``device`` is the current one (kernels launch on the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def stream_handle(device: torch.device) -> ctypes.c_void_p:

@@ -1,6 +1,8 @@
 // C ABI of the LUCID attention kernels (declared in include/lucid_amd.h).
 // One translation unit: the kernel files are included so that every template
 // instantiation lives next to its launcher.
+#include <algorithm>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <string>
@@ -10,7 +12,9 @@
 #include "lucid_bwd.hip"
 #include "lucid_decode.hip"
 #include "lucid_fwd.hip"
+#include "lucid_paged.hip"
 #include "model_ops.hip"
+#include "token_logprobs.hip"
 #include "chain_guard.h"
 #include "profiling.h"
 
@@ -1820,3 +1824,5 @@ int lucid_adamw_step(int n, void* const* params, const void* const* grads, void*
 }
 
 }  // extern "C"
+
+#include "serving_capi.hip"

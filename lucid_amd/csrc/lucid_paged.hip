@@ -1,0 +1,672 @@
+// Paged (K, V') caches on CDNA4 (gfx950): decoding against them, writing a prefill's rows into them
+// and copying their pages (modeling_lucid.py:475-496, 576-598 is the cached path of the reference,
+// whose cache is one buffer per layer and one length for the whole batch).
+//
+// Row j of sequence b is row j % page of page table[b][j / page] of a layer's two pools (keys with
+// RoPE applied, V' rows; bf16 [P][Hkv][page][W] by their strides, W = 64, 80, 96 or 128 the smallest
+// that holds the head dim, columns beyond it zero).  Each sequence has its own length lens[b]; a
+// negative one marks a batch slot without a sequence.  For a new token t of a sequence:
+//   P_tj = exp(s r_t r_j (k_t . k_j) - 1/s),  r = 1 / rms(k)  (j < t, cached or new)
+//   v'_t = (v_t - sum_{j<t} P_tj w_j) / P_tt,  P_tt = exp(s dn ms_t / (ms_t + eps) - 1/s)
+//   o_tg = softmax_j(s q_tg . k_j) w_j over j <= t, for the G query heads of the kv head
+// with w_j the V' row as the cache holds it (bf16), new rows too, so that L tokens in one call are L
+// calls of one token.  The products with the cached rows read each of them once (bytes bound it):
+//   lucid_paged_split_kernel    a chunk of a sequence's rows of one kv head: partial sum_j P_tj w_j and
+//                               the online-softmax state of every (token, query head)
+//   lucid_paged_combine_kernel  the chunks merged, the new tokens solved in order, the outputs, and
+//                               (k_t, v'_t) appended to the pages
+#include "lucid_common.h"
+
+namespace lucid {
+
+constexpr float PAGED_NEG = -1e30f;    // finite "minus infinity" for empty softmax states
+constexpr int kPagedChunkRows = 128;   // rows of a chunk: a multiple of this (four waves' tiles)
+constexpr int kPagedMaxTokens = 16;    // new tokens of a pass
+
+struct PagedBatch {
+  const int32_t* table;  // [B][M] page ids, rows tstride apart
+  int64_t tstride;
+  const int32_t* lens;  // [B] rows cached before the call
+  int B, M, P, page;
+  int L;     // new tokens of the call
+  int done;  // of earlier passes
+};
+
+// A pool by its strides in units of 16 bytes (8 elements); the host checks that every row's offset
+// fits 32 bits, a pool of 64 GB.
+struct PagedPool {
+  bf16* base;
+  unsigned page, head, row;
+};
+__device__ __forceinline__ bf16* paged_at(const PagedPool& p, unsigned off) { return p.base + (size_t)off * 8; }
+
+// Rows of sequence b before this pass; -1: no sequence, -2: its new rows do not fit its table
+__device__ __forceinline__ int paged_rows(const PagedBatch& s, int b) {
+  const int n = s.lens[b];
+  if (n < 0) return -1;
+  return (int64_t)n + s.L > (int64_t)s.M * s.page ? -2 : n + s.done;
+}
+
+// The sequences' rows are cut into chunks of one length, so that the work of a workgroup does not
+// depend on how the rows are spread over the sequences: the least multiple of kPagedChunkRows that
+// gives at most target chunks, and one more for the remainder of each sequence.
+__device__ __forceinline__ int paged_chunk(const PagedBatch& s, int target) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;
+  for (int b = lane; b < s.B; b += 64) total += max(paged_rows(s, b), 0);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor((long long)total, o, 64);
+  const int64_t ks = (total + target - 1) / target;
+  return (int)((max(ks, (int64_t)1) + kPagedChunkRows - 1) / kPagedChunkRows) * kPagedChunkRows;
+}
+__device__ __forceinline__ int paged_chunks(const PagedBatch& s, int b, int ks) {
+  return b < s.B ? (max(paged_rows(s, b), 0) + ks - 1) / ks : 0;
+}
+// Chunks of the sequences before b, and of b itself (every lane of the wave)
+__device__ __forceinline__ void paged_span(const PagedBatch& s, int b, int ks, int& base, int& n) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0;
+  for (int i = lane; i < b; i += 64) sum += paged_chunks(s, i, ks);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  base = sum;
+  n = paged_chunks(s, b, ks);
+}
+// The sequence of chunk slot, and which of its chunks that is; false beyond the last
+__device__ __forceinline__ bool paged_find(const PagedBatch& s, int slot, int ks, int& b, int& chunk) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int c0 = 0; c0 < s.B; c0 += 64) {
+    const int own = paged_chunks(s, c0 + lane, ks);
+    int incl = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += x;
+    }
+    const unsigned long long at = __ballot(slot < base + incl);
+    if (at) {
+      const int l = __ffsll(at) - 1;
+      b = c0 + l;
+      chunk = slot - base - __shfl(incl - own, l, 64);
+      return true;
+    }
+    base += __shfl(incl, 63, 64);
+  }
+  return false;
+}
+
+// Four consecutive columns c .. c+3 of a row of d, zeros beyond d; vec: the row starts at an 8-byte
+// boundary
+__device__ __forceinline__ bf16x4 ld4_cols(const bf16* row, int c, int d, bool vec) {
+  if (vec && c + 4 <= d) return *reinterpret_cast<const bf16x4*>(row + c);
+  bf16x4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = c + e < d ? row[c + e] : (bf16)0.f;
+  return x;
+}
+
+// Partials of the chunks, slot-major; tokens of the pass Lp, columns t Gs + g
+struct PagedPartials {
+  float* a;  // [slots][Hkv][Lp][W]      sum_j P_tj w_j
+  float* m;  // [slots][Hkv][Lp*Gs]      running max (log2 domain); NaN: a page id outside the pool
+  float* l;  // [slots][Hkv][Lp*Gs]      running sum
+  float* o;  // [slots][Hkv][Lp*Gs][W]   unnormalised output
+};
+
+// V' tile of 32 rows in LDS as the direct loads write it: W / 8 chunks of 16 bytes a row, chunk c of
+// row r at c ^ (r & 7) for rows of 128 and 256 bytes; rows of 160 and 192 bytes fall on different
+// banks by themselves.
+template <int W>
+struct PagedSmem {
+  static constexpr bool kSwz = W == 64 || W == 128;
+  union {
+    bf16 v[4][2][32 * W + 64];  // per wave, double buffered (the last tile's transposing reads of W = 80 end 32 bytes behind it)
+    struct {
+      float so[4][32][W + 1];
+      float m[4][32], l[4][32];
+    } fin;
+  } u;
+  float nn[4][32];  // per wave: squared norms of the tile's keys
+  int bad[4];
+};
+
+// MFMA A operand of 16 rows from row0 and columns col0 + lane % 32 of a V' tile (lds_tr_a of
+// lucid_common.h for the row widths of a page)
+template <int W>
+__device__ __forceinline__ bf16x8 paged_tr_a(const bf16* tile, int row0, int col0) {
+  typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+  if constexpr (PagedSmem<W>::kSwz) {
+    return lds_tr_a<W / 8>(tile, row0, col0);
+  } else {
+    const int lane = threadIdx.x & 63, s = lane & 15;
+    const int col = col0 + 16 * ((lane >> 4) & 1) + 4 * (s & 3);
+    const int r1 = row0 + 4 * (lane >> 5) + (s >> 2);
+    const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + r1 * W + col));
+    const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + (r1 + 8) * W + col));
+    return bf16x8{v1[0], v1[1], v1[2], v1[3], v2[0], v2[1], v2[2], v2[3]};
+  }
+}
+
+// Grid (slots, Hkv).  As lucid_decode_split_kernel: each wave sweeps its own 32-row tiles of the
+// chunk, one MFMA score tile S^T[j][c] = K_j . X_c of the columns c = t (Gs + 1) + i (query head
+// g0 + i of token t, its key at i = Gs), then O^T[d][c] += w^T[d][j] p^T[j][c].  p enters the second
+// product as a bf16 pair (hi + lo, 2^-17), since V' is returned in fp32 and one bf16 term of P
+// would be seen in it.  Page ids reach registers two tiles ahead, rows one.  Columns of the NCT
+// 32-column tiles: Lp (Gs + 1) <= 32 NCT.
+template <int W, int NCT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NCT > 1 ? (W <= 64 ? 2 : 1) : (W <= 64 ? 3 : 2)))) void
+lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __restrict__ kn, Strides kns, int vec,
+                         PagedPool kp, PagedPool vp, PagedBatch seq, int target, int Hkv, int Lp, float scale, float eps,
+                         int d, PagedPartials part, int Gs, int Gt, int g0) {
+  constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = 32 * CPR / 64;
+  __shared__ __attribute__((aligned(16))) PagedSmem<W> sm;
+  const int h = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
+  const int ks = paged_chunk(seq, target);
+  int b, chunk;
+  if (!paged_find(seq, blockIdx.x, ks, b, chunk)) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  chunk = __builtin_amdgcn_readfirstlane(chunk);
+  const int rows = paged_rows(seq, b);
+  const int j0 = chunk * ks, j1 = min(rows, j0 + ks);
+  const float sl2 = scale * LOG2E_F, c0 = LOG2E_F / scale, dn = (float)d;
+
+  // B operand: column 32 ct + l32 of X^T (k = d), zero for the padding columns
+  bool valid[NCT], isq[NCT];
+  bf16x8 xb[NCT][NKS];
+  float c1[NCT];
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const int col = 32 * ct + l32, tok = col / (Gs + 1), hi = col - tok * (Gs + 1);
+    valid[ct] = tok < Lp;
+    isq[ct] = valid[ct] && hi < Gs;
+    const int64_t t = seq.done + tok;
+    const bf16* x = isq[ct] ? q + b * qs.b + (h * Gt + g0 + hi) * qs.h + t * qs.t : kn + b * kns.b + h * kns.h + t * kns.t;
+    float nt = 0.f;
+#pragma unroll
+    for (int st = 0; st < NKS; ++st) {
+      bf16x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (bf16)0.f;
+      if (valid[ct]) {
+        const bf16x4 a = ld4_cols(x, 16 * st + 8 * g, d, vec), c = ld4_cols(x, 16 * st + 8 * g + 4, d, vec);
+        v = bf16x8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) nt = fmaf((float)v[e], (float)v[e], nt);
+      }
+      xb[ct][st] = v;
+    }
+    nt = wave_sum32(nt);  // squared norm of this column's key (both lane halves)
+    c1[ct] = sl2 * rsqrtf(nt / dn + eps);
+  }
+
+  f32x16 oacc[NCT][NDT];
+  float m[NCT], l[NCT];
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    m[ct] = PAGED_NEG;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t) oacc[ct][t] = zero16();
+  }
+
+  const int32_t* tbl = seq.table + b * seq.tstride;
+  const int ntile = (j1 - j0 + 31) / 32;  // tiles of the chunk; wave w takes w, w + 4, ...
+  bool bad = false;
+  // this lane's row of tile t (rows beyond the chunk: its last row, masked below)
+  auto row_of = [&](int t) { return min(j0 + 32 * t + l32, j1 - 1); };
+  auto page_id = [&](int t) { return tbl[row_of(t) / seq.page]; };
+  unsigned koff, voff;  // of this lane's row
+  auto place = [&](int t, int id) {
+    const int j = row_of(t);
+    if ((unsigned)id >= (unsigned)seq.P) {
+      bad = true;
+      id = 0;
+    }
+    const unsigned in = j % seq.page;
+    koff = id * kp.page + h * kp.head + in * kp.row;
+    voff = id * vp.page + h * vp.head + in * vp.row;
+  };
+  bf16x8 kcur[NKS], knx[NKS];  // this tile's and the next tile's key rows
+  auto kload = [&](bf16x8* dst) {
+    const bf16* r = paged_at(kp, koff);
+#pragma unroll
+    for (int st = 0; st < NKS; ++st) dst[st] = ld8(r + 16 * st + 8 * g);
+  };
+  auto vstage = [&](bf16* dst) {  // 32 V' rows into this wave's buffer
+#pragma unroll
+    for (int i = 0; i < NST; ++i) {
+      const int qq = i * 64 + lane, r = qq / CPR;
+      int c = qq % CPR;
+      if constexpr (PagedSmem<W>::kSwz) c ^= r & 7;
+      const bf16* src = paged_at(vp, __shfl((int)voff, r, 64)) + c * 8;
+      __builtin_amdgcn_global_load_lds(src, dst + i * 512, 16, 0, 0);
+    }
+  };
+  int it = 0, idn = 0;
+  if (w < ntile) {
+    const int id = page_id(w);
+    if (w + 4 < ntile) idn = page_id(w + 4);
+    place(w, id);
+    kload(kcur);
+    vstage(sm.u.v[w][0]);
+  }
+  for (int t = w; t < ntile; t += 4, ++it) {
+    const int cur = it & 1;
+    const bool more = t + 4 < ntile;
+    if (more) {
+      place(t + 4, idn);
+      if (t + 8 < ntile) idn = page_id(t + 8);
+      kload(knx);
+      vstage(sm.u.v[w][cur ^ 1]);
+      asm volatile("" ::: "memory");  // the loads stay before the wait that counts them
+    }
+    const int jb = j0 + 32 * t;
+    f32x16 scs[NCT];
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) scs[ct] = zero16();
+    float nn = 0.f;
+#pragma unroll
+    for (int st = 0; st < NKS; ++st) {
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) scs[ct] = mfma32(kcur[st], xb[ct][st], scs[ct]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) nn = fmaf((float)kcur[st][e], (float)kcur[st][e], nn);
+    }
+    nn = wave_sum32(nn);
+    if (g == 0) sm.nn[w][l32] = rsqrtf(nn / dn + eps);
+    float nr[16];
+    lds_rows16(&sm.nn[w][0], g, nr);
+    bf16x8 ph[NCT][2], pl[NCT][2];
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      f32x16& sc = scs[ct];
+      // online max of the query columns (lazy: rescale only when a row grows by 2^8)
+      float mx = PAGED_NEG;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (jb + drow(e, g) < j1) mx = fmaxf(mx, sc[e] * sl2);
+      mx = isq[ct] ? wave_max32(mx) : PAGED_NEG;
+      if (__builtin_amdgcn_ballot_w64(mx > m[ct] + 8.0f)) {
+        const float mnew = fmaxf(m[ct], mx);
+        const float al = __builtin_amdgcn_exp2f(m[ct] - mnew);
+        m[ct] = mnew;
+        l[ct] *= al;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) oacc[ct][dt][e] *= isq[ct] ? al : 1.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool ok = jb + drow(e, g) < j1 && valid[ct];
+        const float arg = isq[ct] ? fmaf(sc[e], sl2, -m[ct]) : fmaf(c1[ct] * nr[e], sc[e], -c0);
+        const float p = ok ? __builtin_amdgcn_exp2f(arg) : 0.f;
+        if (isq[ct]) l[ct] += p;
+        sc[e] = p;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        ph[ct][k] = pack_b(sc, k);
+        pl[ct][k] = pack_lo(sc, k, ph[ct][k]);
+      }
+    }
+    // this tile's V' rows have landed once at most the next tile's loads are in flight (its page
+    // ids came before them)
+    if (more)
+      dma_wait_but<NKS + NST>();
+    else
+      dma_wait();
+    asm volatile("" ::: "memory");
+    const bf16* vt = sm.u.v[w][cur];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const bf16x8 va = paged_tr_a<W>(vt, 16 * k, dt * 32);
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) {
+          oacc[ct][dt] = mfma32(va, ph[ct][k], oacc[ct][dt]);
+          oacc[ct][dt] = mfma32(va, pl[ct][k], oacc[ct][dt]);
+        }
+      }
+    }
+    if (more) {
+#pragma unroll
+      for (int st = 0; st < NKS; ++st) kcur[st] = knx[st];
+    }
+  }
+  // the four waves' columns merged, one column tile at a time: wave -> every fourth column, lane ->
+  // its elements
+  const unsigned long long anybad = __ballot(bad);
+  if (lane == 0) sm.bad[w] = anybad != 0;
+  const int64_t at = (int64_t)blockIdx.x * Hkv + h;
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const float lw = wave_sum32(l[ct]);
+    __syncthreads();  // every wave is done with the staging buffers (the first tile's columns)
+    if (valid[ct]) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (32 * dt + drow(e, g) < W) sm.u.fin.so[w][l32][32 * dt + drow(e, g)] = oacc[ct][dt][e];
+      if (isq[ct] && g == 0) {
+        sm.u.fin.m[w][l32] = m[ct];
+        sm.u.fin.l[w][l32] = lw;
+      }
+    }
+    __syncthreads();
+    const bool poison = sm.bad[0] | sm.bad[1] | sm.bad[2] | sm.bad[3];
+#pragma unroll 1
+    for (int cl = w; cl < 32; cl += 4) {
+      const int t = (32 * ct + cl) / (Gs + 1), gg = 32 * ct + cl - t * (Gs + 1);
+      if (t >= Lp) break;
+      if (gg == Gs) {
+#pragma unroll
+        for (int c = lane; c < W; c += 64)
+          part.a[(at * Lp + t) * W + c] =
+              (sm.u.fin.so[0][cl][c] + sm.u.fin.so[1][cl][c]) + (sm.u.fin.so[2][cl][c] + sm.u.fin.so[3][cl][c]);
+        continue;
+      }
+      const float mn = fmaxf(fmaxf(sm.u.fin.m[0][cl], sm.u.fin.m[1][cl]), fmaxf(sm.u.fin.m[2][cl], sm.u.fin.m[3][cl]));
+      float al[4], lt = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < 4; ++ww) {
+        al[ww] = __builtin_amdgcn_exp2f(sm.u.fin.m[ww][cl] - mn);
+        lt = fmaf(sm.u.fin.l[ww][cl], al[ww], lt);
+      }
+      const int64_t pi = at * (Lp * Gs) + t * Gs + gg;
+#pragma unroll
+      for (int c = lane; c < W; c += 64) {
+        float ot = 0.f;
+#pragma unroll
+        for (int ww = 0; ww < 4; ++ww) ot = fmaf(sm.u.fin.so[ww][cl][c], al[ww], ot);
+        part.o[pi * W + c] = ot;
+      }
+      if (lane == 0) {
+        part.m[pi] = poison ? __builtin_nanf("") : mn;
+        part.l[pi] = lt;
+      }
+    }
+  }
+}
+
+// Threads of the combine kernel: W / 4 groups of 4 columns, each on NSL lanes that take a chunk in
+// turn
+template <int W>
+constexpr int paged_nsl() {
+  return W == 64 ? 16 : 8;
+}
+
+// Grid (B Hkv, Gs): workgroup (sequence, kv head, query head g0 + g), for the Lp <= LM tokens of the
+// pass.  Merges the chunks of each token, solves the new tokens in order (a column group needs only
+// its own columns), writes the outputs; the g = 0 workgroups of the first group of query heads append
+// (k_t, v'_t).  A slot without a sequence gets zeros; one whose table names a page outside the
+// pool, or that has no room for the new rows, gets NaN, and nothing is appended to it.
+template <int W, int LM>
+__global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_kernel(
+    const bf16* __restrict__ q, Strides qs, const bf16* __restrict__ kn, Strides kns, const bf16* __restrict__ vn,
+    Strides vns, int vec, PagedPool kp, PagedPool vp, PagedBatch seq, int target, bf16* __restrict__ o, Strides os,
+    float* __restrict__ vp_new, int Hkv, int Lp, float scale, float eps, int d, PagedPartials part, int Gs, int Gt,
+    int g0, int append) {
+  constexpr int CG = W / 4, NSL = paged_nsl<W>(), NT = CG * NSL;
+  __shared__ float kk[LM][LM], qk[LM][LM];  // k_t . k_u and q_tg . k_u (u <= t)
+  __shared__ __attribute__((aligned(16))) float ovs[LM][W], avs[LM][W], vps[LM][W];
+  __shared__ float ms_[LM], ls_[LM];
+  __shared__ unsigned krow[LM], vrow[LM];
+  __shared__ int bads;
+  const int bh = blockIdx.x, g = blockIdx.y;
+  const int b = bh / Hkv, h = bh - b * Hkv;
+  const int tid = threadIdx.x, cg = tid / NSL, sl = tid - cg * NSL, d0 = 4 * cg;
+  const int hq = h * Gt + g0 + g;
+  const int rows = paged_rows(seq, b);
+  const bf16* kb = kn + b * kns.b + h * kns.h + (int64_t)seq.done * kns.t;
+  const bf16* vb = vn + b * vns.b + h * vns.h + (int64_t)seq.done * vns.t;
+  const bf16* qb = q + b * qs.b + hq * qs.h + (int64_t)seq.done * qs.t;
+  bf16* ob = o + b * os.b + hq * os.h + (int64_t)seq.done * os.t;
+  float* vo = vp_new + ((int64_t)bh * seq.L + seq.done) * d;
+  const bool write_v = g == 0 && append;
+  if (rows < 0) {  // no sequence (zeros), or no room (NaN)
+    const float x = rows == -1 ? 0.f : __builtin_nanf("");
+    for (int i = tid; i < Lp * d; i += NT) {
+      ob[(i / d) * os.t + i % d] = (bf16)x;
+      if (write_v) vo[i] = x;
+    }
+    return;
+  }
+  const int ks = paged_chunk(seq, target);
+  int base, nchunk;
+  paged_span(seq, b, ks, base, nchunk);
+  if (tid == 0) bads = 0;
+  __syncthreads();
+  // the pages that the call's new rows go to
+  for (int t = tid; t < seq.L; t += NT) {
+    const int j = rows - seq.done + t;
+    const int id = seq.table[b * seq.tstride + j / seq.page];
+    if ((unsigned)id >= (unsigned)seq.P) atomicOr(&bads, 1);
+    const int u = t - seq.done;
+    if (u >= 0 && u < Lp) {
+      const unsigned in = j % seq.page;
+      krow[u] = id * kp.page + h * kp.head + in * kp.row;
+      vrow[u] = id * vp.page + h * vp.head + in * vp.row;
+    }
+  }
+  // dot products among the new tokens, 16 lanes a pair
+  for (int idx = tid / 16; idx < Lp * Lp; idx += NT / 16) {
+    const int t = idx / Lp, u = idx - t * Lp;
+    if (u > t) continue;
+    float dkk = 0.f, dqk = 0.f;
+    for (int c = tid % 16; c < d; c += 16) {
+      const float ku = (float)kb[u * kns.t + c];
+      dkk = fmaf((float)kb[t * kns.t + c], ku, dkk);
+      dqk = fmaf((float)qb[t * qs.t + c], ku, dqk);
+    }
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+      dkk += __shfl_xor(dkk, off, 64);
+      dqk += __shfl_xor(dqk, off, 64);
+    }
+    if (tid % 16 == 0) {
+      kk[t][u] = dkk;
+      qk[t][u] = dqk;
+    }
+  }
+  // the chunks' partials of every token: its key column and its query column
+  float M[LM], lv[LM];
+  f32x4 ov[LM], av[LM];
+  bool bad = false;
+#pragma unroll
+  for (int t = 0; t < LM; ++t) {
+    M[t] = PAGED_NEG;
+    lv[t] = 0.f;
+    ov[t] = av[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int s = sl; s < nchunk; s += NSL) {
+    const int64_t at = (int64_t)(base + s) * Hkv + h;
+#pragma unroll
+    for (int t = 0; t < LM; ++t) {
+      if (t < Lp) {
+        const int64_t i = at * (Lp * Gs) + t * Gs + g;
+        const float mi = part.m[i], li = part.l[i];
+        bad |= mi != mi;
+        const f32x4 oi = *reinterpret_cast<const f32x4*>(part.o + i * W + d0);
+        const f32x4 ai = *reinterpret_cast<const f32x4*>(part.a + (at * Lp + t) * W + d0);
+        const float mn = fmaxf(M[t], mi);
+        const float c = __builtin_amdgcn_exp2f(M[t] - mn), e = __builtin_amdgcn_exp2f(mi - mn);
+        lv[t] = fmaf(lv[t], c, li * e);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          ov[t][x] = fmaf(ov[t][x], c, oi[x] * e);
+          av[t][x] += ai[x];
+        }
+        M[t] = mn;
+      }
+    }
+  }
+  if (bad) atomicOr(&bads, 1);
+#pragma unroll
+  for (int off = 1; off < NSL; off <<= 1) {
+#pragma unroll
+    for (int t = 0; t < LM; ++t) {
+      if (t < Lp) {
+        const float mo = __shfl_xor(M[t], off, 64), lo = __shfl_xor(lv[t], off, 64);
+        const float mn = fmaxf(M[t], mo);
+        const float c = __builtin_amdgcn_exp2f(M[t] - mn), co = __builtin_amdgcn_exp2f(mo - mn);
+        lv[t] = fmaf(lv[t], c, lo * co);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          ov[t][x] = fmaf(ov[t][x], c, __shfl_xor(ov[t][x], off, 64) * co);
+          av[t][x] += __shfl_xor(av[t][x], off, 64);
+        }
+        M[t] = mn;
+      }
+    }
+  }
+  if (sl == 0) {
+#pragma unroll
+    for (int t = 0; t < LM; ++t) {
+      if (t < Lp) {
+        *reinterpret_cast<f32x4*>(&ovs[t][d0]) = ov[t];
+        *reinterpret_cast<f32x4*>(&avs[t][d0]) = av[t];
+        if (cg == 0) {
+          ms_[t] = M[t];
+          ls_[t] = lv[t];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const bool poison = bads != 0;
+  // the new rows in order (columns d0 .. d0+3): v'_t = (v_t - a_t - sum_{u<t} P_tu w_u) / P_tt
+  const float sl2 = scale * LOG2E_F, c0 = LOG2E_F / scale, dn = (float)d;
+  for (int t = 0; sl == 0 && t < Lp; ++t) {
+    const float rt = rsqrtf(kk[t][t] / dn + eps);
+    const bf16x4 v4 = ld4_cols(vb + t * vns.t, d0, d, vec);
+    const f32x4 a4 = *reinterpret_cast<const f32x4*>(&avs[t][d0]);
+    f32x4 x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (float)v4[j] - a4[j];
+    for (int u = 0; u < t; ++u) {
+      const float ru = rsqrtf(kk[u][u] / dn + eps);
+      const float p = __builtin_amdgcn_exp2f(fmaf(sl2 * rt * ru, kk[t][u], -c0));
+      const f32x4 vu = *reinterpret_cast<const f32x4*>(&vps[u][d0]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = fmaf(-p, (float)(bf16)vu[j], x[j]);
+    }
+    // 1 / P_tt; the exponent is the small difference of two terms of size sqrt(d): in fp64
+    const double ms = (double)kk[t][t] / d;
+    const float inv = __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / scale - scale * d * ms / (ms + eps))));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] *= inv;
+    *reinterpret_cast<f32x4*>(&vps[t][d0]) = x;
+  }
+  __syncthreads();
+  // outputs, a token per split lane: the cached part merged with the new keys u <= t
+  for (int t = sl; t < Lp; t += NSL) {
+    float M2 = ms_[t];
+    for (int u = 0; u <= t; ++u) M2 = fmaxf(M2, qk[t][u] * sl2);
+    const float c = __builtin_amdgcn_exp2f(ms_[t] - M2);
+    const f32x4 o4 = *reinterpret_cast<const f32x4*>(&ovs[t][d0]);
+    f32x4 num;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) num[j] = o4[j] * c;
+    float den = ls_[t] * c;
+    for (int u = 0; u <= t; ++u) {
+      const float es = __builtin_amdgcn_exp2f(fmaf(qk[t][u], sl2, -M2));
+      const f32x4 vu = *reinterpret_cast<const f32x4*>(&vps[u][d0]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) num[j] = fmaf(es, (float)(bf16)vu[j], num[j]);
+      den += es;
+    }
+    const float rden = poison ? __builtin_nanf("") : 1.f / den;
+    const f32x4 vt = *reinterpret_cast<const f32x4*>(&vps[t][d0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (d0 + j >= d) break;
+      ob[t * os.t + d0 + j] = (bf16)(num[j] * rden);
+      if (write_v) vo[t * d + d0 + j] = poison ? rden : vt[j];
+    }
+    if (write_v && !poison) {
+      bf16x4 v4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v4[j] = (bf16)(d0 + j < d ? vt[j] : 0.f);
+      *reinterpret_cast<bf16x4*>(paged_at(kp, krow[t]) + d0) = ld4_cols(kb + t * kns.t, d0, d, vec);
+      *reinterpret_cast<bf16x4*>(paged_at(vp, vrow[t]) + d0) = v4;
+    }
+  }
+}
+
+// Rows t < count_b of k and v' [B][Hkv][T][d] into the pages from row lens[b] on, columns d .. W-1 zero;
+// rows whose page id lies outside the pool, or beyond the table, are left out.  A lane per 8 columns of a
+// row of both.  Grid (rows Hkv CPR / 256, B).
+template <int W, typename TV>
+__global__ __launch_bounds__(256) void lucid_write_pages_kernel(const bf16* __restrict__ k, Strides kst, int kvec,
+                                                                const TV* __restrict__ v, Strides vst, int vvec,
+                                                                PagedPool kp, PagedPool vp, PagedBatch seq,
+                                                                const int32_t* __restrict__ counts, int Hkv, int T,
+                                                                int d) {
+  constexpr int CPR = W / 8;
+  const int b = blockIdx.y;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int c = (int)(idx % CPR) * 8;
+  const int64_t th = idx / CPR;
+  const int h = (int)(th % Hkv);
+  const int64_t t = th / Hkv;
+  if (t >= T || (counts && t >= counts[b])) return;
+  const int64_t j = seq.lens[b] + t;
+  if (seq.lens[b] < 0 || j >= (int64_t)seq.M * seq.page) return;
+  const int id = seq.table[b * seq.tstride + j / seq.page];
+  if ((unsigned)id >= (unsigned)seq.P) return;
+  const unsigned in = (unsigned)(j % seq.page);
+  const bf16* kr = k + b * kst.b + h * kst.h + t * kst.t;
+  const TV* vr = v + b * vst.b + h * vst.h + t * vst.t;
+  bf16x8 x, y;
+  const bf16x4 a = ld4_cols(kr, c, d, kvec), e = ld4_cols(kr, c + 4, d, kvec);
+  x = bf16x8{a[0], a[1], a[2], a[3], e[0], e[1], e[2], e[3]};
+  if constexpr (sizeof(TV) == 2) {
+    const bf16x4 f = ld4_cols(vr, c, d, vvec), i = ld4_cols(vr, c + 4, d, vvec);
+    y = bf16x8{f[0], f[1], f[2], f[3], i[0], i[1], i[2], i[3]};
+  } else {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      f32x4 f;
+      if (vvec && c + 4 * q + 4 <= d) {
+        f = *reinterpret_cast<const f32x4*>(vr + c + 4 * q);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = c + 4 * q + i < d ? vr[c + 4 * q + i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[4 * q + i] = (bf16)f[i];
+    }
+  }
+  *reinterpret_cast<bf16x8*>(paged_at(kp, id * kp.page + h * kp.head + in * kp.row) + c) = x;
+  *reinterpret_cast<bf16x8*>(paged_at(vp, id * vp.page + h * vp.head + in * vp.row) + c) = y;
+}
+
+// Pages copied within each of several pools of one layout.  Pool pointers and page pairs travel in the
+// kernel argument: no upload, and a captured launch keeps them.  Grid (pieces, pairs, pools); a
+// workgroup copies one piece of kCopyUnits units U a lane.
+constexpr int kCopyPools = 64, kCopyPairs = 256;
+constexpr int kCopyUnits = 4;
+struct CopyPages {
+  char* pool[kCopyPools];
+  int src[kCopyPairs], dst[kCopyPairs];
+};
+template <typename U>
+__global__ __launch_bounds__(256) void lucid_copy_pages_kernel(const CopyPages a, int64_t stride, int64_t units) {
+  const U* s = reinterpret_cast<const U*>(a.pool[blockIdx.z] + a.src[blockIdx.y] * stride);
+  U* t = reinterpret_cast<U*>(a.pool[blockIdx.z] + a.dst[blockIdx.y] * stride);
+  const int64_t i0 = (int64_t)blockIdx.x * 256 * kCopyUnits + threadIdx.x;
+  U x[kCopyUnits];
+#pragma unroll
+  for (int i = 0; i < kCopyUnits; ++i)
+    if (i0 + 256 * i < units) x[i] = s[i0 + 256 * i];
+#pragma unroll
+  for (int i = 0; i < kCopyUnits; ++i)
+    if (i0 + 256 * i < units) t[i0 + 256 * i] = x[i];
+}
+
+}  // namespace lucid

@@ -1,0 +1,394 @@
+// C ABI of the serving operators (declared in include/lucid_amd.h): paged (K, V') caches and token log
+// probabilities.  Part of lucid_capi.hip's translation unit, whose helpers it uses.
+
+namespace {
+
+// Workgroups of one resident round of the split pass: three to a CU at rows of 64, two above
+int paged_round(int W) { return W == 64 ? 768 : 512; }
+
+// Row width of a page for a head dim (0: unsupported)
+int page_width(int D) { return D < 1 ? 0 : D <= 64 ? 64 : D <= 80 ? 80 : D <= 96 ? 96 : D <= 128 ? 128 : 0; }
+
+// Chunks wanted of each kv head's rows (all sequences together)
+int paged_target(int B, int Hkv, int64_t cap, int W) {
+  const int64_t most = (int64_t)B * ((cap + lucid::kPagedChunkRows - 1) / lucid::kPagedChunkRows);
+  const int64_t want = (paged_round(W) + Hkv - 1) / Hkv;
+  return (int)std::max<int64_t>(1, std::min(most, want));
+}
+
+// Query heads of a chunk of a group (at most 31 and their key fill the columns of a score tile), and new
+// tokens of a pass: one 32-column tile, or two where the tokens do not fit one
+int paged_heads(int G) {
+  const int chunks = (G + 30) / 31;
+  return (G + chunks - 1) / chunks;
+}
+int paged_tiles(int Gs, int L) { return L > std::min(32 / (Gs + 1), lucid::kPagedMaxTokens) ? 2 : 1; }
+int paged_pass(int Gs, int L) {
+  return std::min(L, std::min(32 * paged_tiles(Gs, L) / (Gs + 1), lucid::kPagedMaxTokens));
+}
+
+lucid::PagedPartials carve_paged(void* base, int64_t slots, int Hkv, int Gs, int Lp, int W, size_t* bytes) {
+  const size_t n = (size_t)slots * Hkv * Lp;
+  size_t off = 0;
+  char* p = static_cast<char*>(base);
+  auto take = [&](size_t floats) {
+    float* r = reinterpret_cast<float*>(p ? p + off : nullptr);
+    off += align256(floats * 4);
+    return r;
+  };
+  lucid::PagedPartials part;
+  part.a = take(n * W);
+  part.m = take(n * Gs);
+  part.l = take(n * Gs);
+  part.o = take(n * Gs * W);
+  if (bytes) *bytes = off;
+  return part;
+}
+
+bool paged_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int D) {
+  return B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && L > 0 && page > 0 && max_pages > 0 && page_width(D) &&
+         (int64_t)page * max_pages <= (1 << 30) && (int64_t)B * Hkv <= (1 << 23) && B <= (1 << 20) && Hkv <= 65535;
+}
+
+int check_pool(const char* name, void* p, const int64_t* s, int pages, int Hkv, int page, int W, lucid::PagedPool* out) {
+  if (!p || !s) return fail(std::string(name) + " or its strides are null");
+  if (misaligned16(p)) return fail(std::string(name) + " must be 16-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    if (s[i] < 0 || s[i] % 8) return fail(std::string(name) + " strides must be non-negative multiples of 8 elements");
+  // offsets in units of 16 bytes have to fit 32 bits; each factor first, so that the sum cannot wrap
+  const int64_t most = (int64_t)1 << 32;
+  const int64_t n[3] = {pages, Hkv, page};
+  int64_t end = W / 8;
+  for (int i = 0; i < 3; ++i) {
+    if (s[i] / 8 >= most || (n[i] > 1 && s[i] / 8 > most / (n[i] - 1)))
+      return fail(std::string(name) + " spans more than 64 GB");
+    end += (n[i] - 1) * (s[i] / 8);
+  }
+  if (end > most) return fail(std::string(name) + " spans more than 64 GB");
+  *out = lucid::PagedPool{(bf16*)p, (unsigned)(s[0] / 8), (unsigned)(s[1] / 8), (unsigned)(s[2] / 8)};
+  return LUCID_OK;
+}
+
+// Whether rows of these tensors start at boundaries of 4 elements
+bool rows_of_4(const void* p, const int64_t* s, size_t size) {
+  return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
+}
+
+struct PagedCall {
+  const void *q, *k, *v;
+  const int64_t *qs, *ks, *vs, *os;
+  lucid::PagedPool kp, vp;
+  lucid::PagedBatch seq;
+  void *o, *ws;
+  float* vp_new;
+  int Hq, Hkv, D;
+  float scale, eps;
+  hipStream_t st;
+};
+
+template <int W, int LM>
+int paged_combine(const PagedCall& c, int vec, const lucid::PagedBatch& seq, int target, int Lp,
+                  const lucid::PagedPartials& part, int Gs, int g0, int gc) {
+  LUCID_LAUNCH_B("lucid_paged_combine_kernel", (lucid::lucid_paged_combine_kernel<W, LM>), dim3(seq.B * c.Hkv, gc),
+                 dim3(W / 4 * lucid::paged_nsl<W>()), c.st, (const bf16*)c.q, S(c.qs), (const bf16*)c.k, S(c.ks),
+                 (const bf16*)c.v, S(c.vs), vec, c.kp, c.vp, seq, target, (bf16*)c.o, S(c.os), c.vp_new, c.Hkv, Lp, c.scale,
+                 c.eps, c.D, part, gc, c.Hq / c.Hkv, g0, g0 == 0 ? 1 : 0);
+  return LUCID_OK;
+}
+
+template <int W>
+int paged_decode(const PagedCall& c) {
+  const int G = c.Hq / c.Hkv, Gs = paged_heads(G), L = c.seq.L;
+  const int tiles = paged_tiles(Gs, L), most = paged_pass(Gs, L);
+  const int target = paged_target(c.seq.B, c.Hkv, (int64_t)c.seq.M * c.seq.page, W), slots = target + c.seq.B;
+  const int vec = rows_of_4(c.q, c.qs, 2) && rows_of_4(c.k, c.ks, 2) && rows_of_4(c.v, c.vs, 2);
+  lucid::PagedBatch seq = c.seq;
+  for (int t0 = 0; t0 < L; t0 += most) {
+    const int Lp = std::min(most, L - t0);
+    seq.done = t0;
+    for (int g0 = 0; g0 < G; g0 += Gs) {
+      const int gc = std::min(Gs, G - g0);  // query heads of this chunk
+      const lucid::PagedPartials part = carve_paged(c.ws, slots, c.Hkv, gc, Lp, W, nullptr);
+      const dim3 grid(slots, c.Hkv);
+      if (tiles == 2)
+        LUCID_LAUNCH("lucid_paged_split_kernel", (lucid::lucid_paged_split_kernel<W, 2>), grid, c.st, (const bf16*)c.q,
+                     S(c.qs), (const bf16*)c.k, S(c.ks), vec, c.kp, c.vp, seq, target, c.Hkv, Lp, c.scale, c.eps, c.D, part, gc,
+                     G, g0);
+      else
+        LUCID_LAUNCH("lucid_paged_split_kernel", (lucid::lucid_paged_split_kernel<W, 1>), grid, c.st, (const bf16*)c.q,
+                     S(c.qs), (const bf16*)c.k, S(c.ks), vec, c.kp, c.vp, seq, target, c.Hkv, Lp, c.scale, c.eps, c.D, part, gc,
+                     G, g0);
+      const int rc = Lp == 1   ? paged_combine<W, 1>(c, vec, seq, target, Lp, part, gc, g0, gc)
+                     : Lp <= 4 ? paged_combine<W, 4>(c, vec, seq, target, Lp, part, gc, g0, gc)
+                               : paged_combine<W, lucid::kPagedMaxTokens>(c, vec, seq, target, Lp, part, gc, g0, gc);
+      if (rc) return rc;
+    }
+  }
+  return LUCID_OK;
+}
+
+template <int W>
+int write_pages(const void* k, const int64_t* ks, const void* v, const int64_t* vs, int v_f32, const lucid::PagedPool& kp,
+                const lucid::PagedPool& vp, const lucid::PagedBatch& seq, const int32_t* counts, int Hkv, int T, int D,
+                hipStream_t st) {
+  const int64_t blocks = ((int64_t)T * Hkv * (W / 8) + 255) / 256;
+  if (blocks > (1 << 23)) return fail("lucid_write_pages: too many rows");
+  const dim3 grid((unsigned)blocks, seq.B);
+  const int kvec = rows_of_4(k, ks, 2), vvec = rows_of_4(v, vs, v_f32 ? 4 : 2);
+  if (v_f32)
+    LUCID_LAUNCH("lucid_write_pages_kernel", (lucid::lucid_write_pages_kernel<W, float>), grid, st, (const bf16*)k, S(ks),
+                 kvec, (const float*)v, S(vs), vvec, kp, vp, seq, counts, Hkv, T, D);
+  else
+    LUCID_LAUNCH("lucid_write_pages_kernel", (lucid::lucid_write_pages_kernel<W, bf16>), grid, st, (const bf16*)k, S(ks),
+                 kvec, (const bf16*)v, S(vs), vvec, kp, vp, seq, counts, Hkv, T, D);
+  return LUCID_OK;
+}
+
+// Token log probabilities: workgroups of 256 lanes for rows of up to 8192 values (and what a
+// misaligned row's first chunk leaves out), else of 1024 on segments of 32768
+int lp_threads(int V) { return V + lucid::kLpChunk - 1 <= 256 * lucid::kLpChunks * lucid::kLpChunk ? 256 : 1024; }
+int lp_segs(int V) {
+  const int seg = lp_threads(V) * lucid::kLpChunks * lucid::kLpChunk;
+  return (int)(((int64_t)V + lucid::kLpChunk - 1 + seg - 1) / seg);
+}
+
+lucid::LpOut carve_lp(void* base, int64_t R, int segs, int top, size_t* bytes) {
+  lucid::LpOut o{};
+  size_t off = 0;
+  char* p = static_cast<char*>(base);
+  auto take = [&](size_t n) {
+    char* r = p ? p + off : nullptr;
+    off += align256(n);
+    return r;
+  };
+  if (segs > 1) {
+    o.pm = reinterpret_cast<float*>(take((size_t)R * segs * 4));
+    o.ps = reinterpret_cast<float*>(take((size_t)R * segs * 4));
+    o.pt = reinterpret_cast<float*>(take((size_t)R * segs * 4));
+    o.pkey = reinterpret_cast<unsigned long long*>(take((size_t)R * segs * top * 8));
+  }
+  if (bytes) *bytes = off;
+  return o;
+}
+
+int check_lp(const char* what, const void* logits, int64_t sb, int64_t st, const int64_t* tokens, int R, int Tn, int V,
+             int dtype, float temperature, int top) {
+  const std::string w = what;
+  if (dtype != LUCID_DTYPE_BF16 && dtype != LUCID_DTYPE_F32) return fail(w + ": dtype LUCID_DTYPE_BF16 or LUCID_DTYPE_F32");
+  if (R < 0 || Tn < 1 || R % Tn) return fail(w + ": R a multiple of the rows of a batch, got R=" + std::to_string(R));
+  if (V < 1 || V > 2000000) return fail(w + ": V from 1 to 2000000, got " + std::to_string(V));
+  if (top < 0 || top > lucid::kLpMaxTop || top > V) return fail(w + ": top from 0 to 64 and at most V, got " + std::to_string(top));
+  if (!(temperature > 0.f) || std::isinf(temperature)) return fail(w + ": the temperature must be positive and finite");
+  if (sb < 0 || st < 0) return fail(w + ": negative strides");
+  if (R == 0) return LUCID_OK;
+  if (!logits || !tokens) return fail(w + ": logits or tokens are null");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == LUCID_DTYPE_F32 ? 4 : 2)) return fail(w + ": logits are misaligned");
+  if ((int64_t)R * lp_segs(V) * lp_threads(V) >= ((int64_t)1 << 32)) return fail(w + ": too many rows");
+  return LUCID_OK;
+}
+
+template <typename T>
+int lp_fwd(const void* logits, int64_t sb, int64_t st, const int64_t* tokens, int R, int Tn, int V, float inv_temp, int top,
+           const lucid::LpOut& out, hipStream_t stream) {
+  const int segs = lp_segs(V), nt = lp_threads(V);
+  const dim3 grid((unsigned)R * segs);
+  if (nt == 256)
+    LUCID_LAUNCH("lucid_token_logprobs_kernel", (lucid::lucid_token_logprobs_kernel<T, 256>), grid, stream, (const T*)logits,
+                 sb, st, Tn, tokens, V, inv_temp, top, segs, out);
+  else
+    LUCID_LAUNCH_B("lucid_token_logprobs_kernel", (lucid::lucid_token_logprobs_kernel<T, 1024>), grid, dim3(1024), stream,
+                   (const T*)logits, sb, st, Tn, tokens, V, inv_temp, top, segs, out);
+  if (segs > 1)
+    LUCID_LAUNCH("lucid_token_logprobs_merge_kernel", lucid::lucid_token_logprobs_merge_kernel<T>, dim3(R), stream,
+                 (const T*)logits, sb, st, Tn, tokens, V, inv_temp, top, segs, out);
+  return LUCID_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lucid_page_width(int D) { return page_width(D); }
+
+size_t lucid_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int L, int page_size, int max_pages, int D) {
+  if (!paged_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D)) return 0;
+  const int W = page_width(D), Gs = paged_heads(Hq / Hkv);
+  const int slots = paged_target(B, Hkv, (int64_t)page_size * max_pages, W) + B;
+  size_t bytes = 0;
+  carve_paged(nullptr, slots, Hkv, Gs, paged_pass(Gs, L), W, &bytes);
+  return bytes;
+}
+
+int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                       const int64_t* v_strides, void* k_pages, const int64_t* k_page_strides, void* vp_pages,
+                       const int64_t* vp_page_strides, const int32_t* page_table, int64_t table_stride,
+                       const int32_t* cache_lens, void* o, const int64_t* o_strides, float* vp_new, void* ws, int B, int Hq,
+                       int Hkv, int L, int num_pages, int page_size, int max_pages, int D, float scale, float eps,
+                       void* stream) {
+  g_last_error.clear();
+  if (!page_width(D)) return fail("head_dim must be in [1, 128], got " + std::to_string(D));
+  if (!paged_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D))
+    return fail("lucid_decode_paged: B, Hq, Hkv, L, page_size and max_pages positive, Hq a multiple of Hkv, at most 2^30 "
+                "rows a sequence and 2^23 kv heads in the batch");
+  if (num_pages < 1) return fail("lucid_decode_paged: the pools have no pages");
+  if (!q || !q_strides || !k || !k_strides || !v || !v_strides || !o || !o_strides || !vp_new || !page_table ||
+      !cache_lens || !ws)
+    return fail("lucid_decode_paged: null argument");
+  if (table_stride < 0) return fail("lucid_decode_paged: negative table stride");
+  if (scale == 0.f) return fail("lucid_decode_paged: scale must not be 0");
+  if (int rc = check_ws("ws", ws)) return rc;
+  PagedCall c{q, k, v, q_strides, k_strides, v_strides, o_strides, {}, {}, {}, o, ws, vp_new, Hq, Hkv, D, scale, eps,
+              static_cast<hipStream_t>(stream)};
+  const int W = page_width(D);
+  if (int rc = check_pool("k_pages", k_pages, k_page_strides, num_pages, Hkv, page_size, W, &c.kp)) return rc;
+  if (int rc = check_pool("vp_pages", vp_pages, vp_page_strides, num_pages, Hkv, page_size, W, &c.vp)) return rc;
+  c.seq = lucid::PagedBatch{page_table, table_stride, cache_lens, B, max_pages, num_pages, page_size, L, 0};
+  switch (W) {
+    case 64: return paged_decode<64>(c);
+    case 80: return paged_decode<80>(c);
+    case 96: return paged_decode<96>(c);
+    default: return paged_decode<128>(c);
+  }
+}
+
+int lucid_write_pages(const void* k, const int64_t* k_strides, const void* vprime, const int64_t* vprime_strides,
+                      int vprime_f32, void* k_pages, const int64_t* k_page_strides, void* vp_pages,
+                      const int64_t* vp_page_strides, const int32_t* page_table, int64_t table_stride,
+                      const int32_t* cache_lens, const int32_t* new_lens, int B, int Hkv, int T, int num_pages,
+                      int page_size, int max_pages, int D, void* stream) {
+  g_last_error.clear();
+  if (!page_width(D)) return fail("head_dim must be in [1, 128], got " + std::to_string(D));
+  if (B < 0 || T < 0 || B > 65535 || !paged_sizes_ok(1, Hkv, Hkv, 1, page_size, max_pages, D))
+    return fail("lucid_write_pages: B in [0, 65535], T >= 0, Hkv, page_size and max_pages positive, at most 2^30 rows a "
+                "sequence");
+  if (B == 0 || T == 0) return LUCID_OK;
+  if (num_pages < 1) return fail("lucid_write_pages: the pools have no pages");
+  if (!k || !k_strides || !vprime || !vprime_strides || !page_table || !cache_lens)
+    return fail("lucid_write_pages: null argument");
+  if (table_stride < 0) return fail("lucid_write_pages: negative table stride");
+  const int W = page_width(D);
+  lucid::PagedPool kp, vp;
+  if (int rc = check_pool("k_pages", k_pages, k_page_strides, num_pages, Hkv, page_size, W, &kp)) return rc;
+  if (int rc = check_pool("vp_pages", vp_pages, vp_page_strides, num_pages, Hkv, page_size, W, &vp)) return rc;
+  const lucid::PagedBatch seq{page_table, table_stride, cache_lens, B, max_pages, num_pages, page_size, 0, 0};
+  auto* run = W == 64 ? write_pages<64> : W == 80 ? write_pages<80> : W == 96 ? write_pages<96> : write_pages<128>;
+  return run(k, k_strides, vprime, vprime_strides, vprime_f32 != 0, kp, vp, seq, new_lens, Hkv, T, D,
+             static_cast<hipStream_t>(stream));
+}
+
+int lucid_copy_pages(int num_pools, void* const* pools, int64_t page_stride_bytes, int64_t page_bytes, int num_pages,
+                     int num_copies, const int* src, const int* dst, void* stream) {
+  g_last_error.clear();
+  if (num_pools < 0 || num_copies < 0 || num_pages < 0 || page_bytes < 0 || page_stride_bytes < page_bytes)
+    return fail("lucid_copy_pages: negative size, or pages that overlap");
+  if (num_pools == 0 || num_copies == 0) return LUCID_OK;
+  if (!pools || !src || !dst) return fail("lucid_copy_pages: null argument");
+  try {
+    std::vector<unsigned char> used(num_pages);  // 1: read, 2: written
+    for (int i = 0; i < num_copies; ++i) {
+      if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages)
+        return fail("lucid_copy_pages: page " + std::to_string(src[i]) + " -> " + std::to_string(dst[i]) +
+                    " outside the pool's " + std::to_string(num_pages));
+      if (used[dst[i]] & 2) return fail("lucid_copy_pages: page " + std::to_string(dst[i]) + " is written twice");
+      used[src[i]] |= 1;
+      used[dst[i]] |= 2;
+    }
+    for (int i = 0; i < num_copies; ++i)
+      if (used[dst[i]] & 1) return fail("lucid_copy_pages: page " + std::to_string(dst[i]) + " is both read and written");
+  } catch (const std::exception&) {
+    return fail("lucid_copy_pages: out of host memory");
+  }
+  if (page_bytes == 0) return LUCID_OK;
+  uintptr_t bits = (uintptr_t)page_bytes | (uintptr_t)page_stride_bytes;
+  for (int i = 0; i < num_pools; ++i) {
+    if (!pools[i]) return fail("lucid_copy_pages: pool " + std::to_string(i) + " is null");
+    bits |= reinterpret_cast<uintptr_t>(pools[i]);
+  }
+  const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+  const int64_t units = page_bytes / unit, pieces = (units + 256 * lucid::kCopyUnits - 1) / (256 * lucid::kCopyUnits);
+  if (pieces > (1 << 23)) return fail("lucid_copy_pages: pages of more than 2^33 units");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  for (int p0 = 0; p0 < num_pools; p0 += lucid::kCopyPools)
+    for (int c0 = 0; c0 < num_copies; c0 += lucid::kCopyPairs) {
+      lucid::CopyPages a;
+      const int np = std::min(lucid::kCopyPools, num_pools - p0), nc = std::min(lucid::kCopyPairs, num_copies - c0);
+      std::copy(pools + p0, pools + p0 + np, reinterpret_cast<void**>(a.pool));
+      std::copy(src + c0, src + c0 + nc, a.src);
+      std::copy(dst + c0, dst + c0 + nc, a.dst);
+      const dim3 grid((unsigned)pieces, nc, np);
+      if (unit == 16)
+        LUCID_LAUNCH("lucid_copy_pages_kernel", lucid::lucid_copy_pages_kernel<u32x4>, grid, st, a, page_stride_bytes, units);
+      else if (unit == 4)
+        LUCID_LAUNCH("lucid_copy_pages_kernel", lucid::lucid_copy_pages_kernel<uint32_t>, grid, st, a, page_stride_bytes,
+                     units);
+      else
+        LUCID_LAUNCH("lucid_copy_pages_kernel", lucid::lucid_copy_pages_kernel<uint8_t>, grid, st, a, page_stride_bytes,
+                     units);
+    }
+  return LUCID_OK;
+}
+
+size_t lucid_token_logprobs_workspace_bytes(int R, int V, int top) {
+  if (R < 0 || V < 1 || top < 0) return 0;
+  size_t bytes = 0;
+  carve_lp(nullptr, R, lp_segs(V), top, &bytes);
+  return bytes;
+}
+
+int lucid_token_logprobs_fwd(const void* logits, int64_t batch_stride, int64_t row_stride, const int64_t* tokens, int R,
+                             int T, int V, int dtype, float temperature, int top, float* logprobs, float* entropy,
+                             float* stats, float* top_logprobs, int64_t* top_indices, void* ws, void* stream) {
+  g_last_error.clear();
+  if (int rc = check_lp("lucid_token_logprobs_fwd", logits, batch_stride, row_stride, tokens, R, T, V, dtype, temperature,
+                        top))
+    return rc;
+  if (R == 0) return LUCID_OK;
+  const int segs = lp_segs(V);
+  if (!logprobs || !entropy || !stats || (top && (!top_logprobs || !top_indices)) || (segs > 1 && !ws))
+    return fail("lucid_token_logprobs_fwd: null output or workspace");
+  if (segs > 1)
+    if (int rc = check_ws("ws", ws)) return rc;
+  lucid::LpOut out = carve_lp(ws, R, segs, top, nullptr);
+  out.logprob = logprobs;
+  out.entropy = entropy;
+  out.stats = reinterpret_cast<lucid::LpStats*>(stats);
+  out.top_lp = top_logprobs;
+  out.top_idx = top_indices;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return (dtype == LUCID_DTYPE_F32 ? lp_fwd<float> : lp_fwd<bf16>)(logits, batch_stride, row_stride, tokens, R, T, V,
+                                                                   1.f / temperature, top, out, st);
+}
+
+int lucid_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t row_stride, const int64_t* tokens, int R,
+                             int T, int V, int dtype, float temperature, int top, const float* stats,
+                             const int64_t* top_indices, const float* dlogprobs, const float* dentropy,
+                             const float* dtop_logprobs, void* dlogits, void* stream) {
+  g_last_error.clear();
+  if (int rc = check_lp("lucid_token_logprobs_bwd", logits, batch_stride, row_stride, tokens, R, T, V, dtype, temperature,
+                        top))
+    return rc;
+  if (R == 0) return LUCID_OK;
+  if (!stats || !dlogits || (top && !top_indices)) return fail("lucid_token_logprobs_bwd: null argument");
+  if (reinterpret_cast<uintptr_t>(dlogits) % (dtype == LUCID_DTYPE_F32 ? 4 : 2))
+    return fail("lucid_token_logprobs_bwd: dlogits are misaligned");
+  const int per = 256 * lucid::kLpChunks * lucid::kLpChunk;
+  const int blocks = (int)(((int64_t)V + lucid::kLpChunk - 1 + per - 1) / per);
+  if ((int64_t)R * blocks * 256 >= ((int64_t)1 << 32)) return fail("lucid_token_logprobs_bwd: too many rows");
+  const dim3 grid((unsigned)R * blocks);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const lucid::LpGrads g{dlogprobs, dentropy, dtop_logprobs};
+  const auto* z = reinterpret_cast<const lucid::LpStats*>(stats);
+  if (dtype == LUCID_DTYPE_F32)
+    LUCID_LAUNCH("lucid_token_logprobs_bwd_kernel", lucid::lucid_token_logprobs_bwd_kernel<float>, grid, st,
+                 (const float*)logits, batch_stride, row_stride, T, tokens, V, 1.f / temperature, top, z, top_indices, g,
+                 (float*)dlogits, blocks);
+  else
+    LUCID_LAUNCH("lucid_token_logprobs_bwd_kernel", lucid::lucid_token_logprobs_bwd_kernel<bf16>, grid, st,
+                 (const bf16*)logits, batch_stride, row_stride, T, tokens, V, 1.f / temperature, top, z, top_indices, g,
+                 (bf16*)dlogits, blocks);
+  return LUCID_OK;
+}
+
+int lucid_abi_minor(void) { return 1; }
+
+}  // extern "C"

@@ -1,0 +1,369 @@
+// Log probabilities of given tokens, entropy and the top alternatives of logit rows, and their
+// gradient, on CDNA4 (gfx950); stands beside the causal-LM loss of model_ops.hip
+// (modeling_lucid.py:847-967 has the logits; the reference reads nothing but the mean loss from
+// them).  With x = logits / temperature, a row of V values:
+//   lse = log sum_j exp x_j,  p_j = exp(x_j - lse)
+//   logprob = x_tok - lse,  entropy H = -sum_j p_j log p_j = log s - t / s,
+//     s = sum_j exp(x_j - m), t = sum_j exp(x_j - m) (x_j - m), m = max_j x_j
+//   alternatives: the `top` largest logits, ties by the lowest index, with x_i - lse
+//   dx_j = [j = tok] g_lp + sum_i [j = top_i] g_i - p_j (g_lp + sum_i g_i + g_H (log p_j + H))
+//
+//   lucid_token_logprobs_kernel        a workgroup per row (or per 32768-value segment of it) keeps
+//                                      its values in registers: one read of the logits serves the
+//                                      maximum, the sums and the alternatives
+//   lucid_token_logprobs_merge_kernel  rows of several segments: the segments' sums and sorted
+//                                      alternatives joined
+//   lucid_token_logprobs_bwd_kernel    one read of the logits and one write of their gradient
+#include "lucid_common.h"
+
+namespace lucid {
+
+constexpr int kLpChunk = 8;     // consecutive logits per load of a lane
+constexpr int kLpChunks = 4;    // chunks a lane holds
+constexpr int kLpMaxTop = 64;   // alternatives of a row
+constexpr int kLpMaxSegs = 64;  // segments of a row
+constexpr float kLpNone = -1000.f;  // a log2 probability whose exp2 is 0: stands for every lower one
+
+// What a forward row leaves for the backward: p_j = exp2((logit_j - m) c - l2), c = log2 e / temperature
+struct LpStats {
+  float m, l2, ent;
+};
+
+// A row of logits as aligned chunks: chunk q holds the values 8 q - shift + e, e = 0 .. 7, so that
+// every whole chunk starts at a 16-byte boundary (rows of odd V do not); the first and the last
+// chunk may lie partly outside the row and are read value by value.
+template <typename T>
+struct LpRow {
+  typedef T V8 __attribute__((ext_vector_type(8)));
+  const T* row;
+  int V, shift;
+  __device__ __forceinline__ LpRow(const T* r, int v)
+      : row(r), V(v), shift((int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T))) {}
+  __device__ __forceinline__ int first(int q) const { return q * kLpChunk - shift; }
+  __device__ __forceinline__ bool whole(int q) const { return first(q) >= 0 && first(q) + kLpChunk <= V; }
+  __device__ __forceinline__ V8 load(int q) const {  // outside the row: -inf
+    const int j = first(q);
+    V8 x;
+    if (whole(q)) {
+      if constexpr (sizeof(T) == 2) {
+        x = *reinterpret_cast<const V8*>(row + j);
+      } else {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(row + j), b = *reinterpret_cast<const f32x4*>(row + j + 4);
+        x = V8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kLpChunk; ++e) x[e] = j + e >= 0 && j + e < V ? row[j + e] : (T)(-INFINITY);
+    }
+    return x;
+  }
+};
+
+// Row r of [R / Tn][Tn] rows at element strides sb, st
+template <typename T>
+__device__ __forceinline__ const T* lp_row(const T* logits, int64_t sb, int64_t st, int Tn, int r) {
+  return logits + (int64_t)(r / Tn) * sb + (int64_t)(r % Tn) * st;
+}
+
+// Order of the alternatives as one unsigned number: by value (NaN above everything, as torch sorts;
+// -0 as 0), then the lowest index.  0 is below every value's key.
+__device__ __forceinline__ unsigned long long lp_key(float x, int j) {
+  unsigned u = __builtin_bit_cast(unsigned, x + 0.f);
+  u = (u >> 31) ? ~u : u | 0x80000000u;
+  if (x != x) u = 0xffffffffu;
+  return ((unsigned long long)u << 32) | (0xffffffffu - (unsigned)j);
+}
+__device__ __forceinline__ int lp_index(unsigned long long key) { return (int)(0xffffffffu - (unsigned)key); }
+// the value of a key (any NaN for a NaN's)
+__device__ __forceinline__ float lp_value(unsigned long long key) {
+  const unsigned u = (unsigned)(key >> 32);
+  return __builtin_bit_cast(float, u == 0xffffffffu ? 0x7fc00000u : (u >> 31) ? u & 0x7fffffffu : ~u);
+}
+
+__device__ __forceinline__ float lp_wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ float lp_wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ unsigned long long lp_wave_max(unsigned long long v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const unsigned long long w = __shfl_xor(v, o, 64);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+struct LpOut {
+  float* logprob;    // [R]
+  float* entropy;    // [R]
+  LpStats* stats;    // [R]
+  float* top_lp;     // [R][top]
+  int64_t* top_idx;  // [R][top]
+  // partials of rows of several segments
+  float* pm;                 // [R][segs] maximum
+  float* ps;                 // [R][segs] sum
+  float* pt;                 // [R][segs] entropy sum, log2 units
+  unsigned long long* pkey;  // [R][segs][top], descending
+};
+
+constexpr int64_t kLpIgnore = -100;  // the loss's ignore index
+
+// The row's results from its maximum m (raw logits), s = sum exp2((x - m) c) and
+// t = sum exp2((x - m) c) (x - m) c
+__device__ __forceinline__ float lp_finish(const LpOut& out, int r, float m, float s, float t, float inv_temp,
+                                           const int64_t* tokens, int V, float xtok) {
+  constexpr float kLn2 = 0.69314718055994531f;
+  const float l2 = log2f(s), ent = kLn2 * (l2 - t / s);
+  const int64_t tok = tokens[r];
+  float lp = 0.f;
+  if (tok != kLpIgnore)
+    lp = tok < 0 || tok >= V ? __builtin_nanf("") : (xtok - m) * inv_temp - kLn2 * l2;
+  out.logprob[r] = lp;
+  out.entropy[r] = ent;
+  out.stats[r] = LpStats{m, l2, ent};
+  return l2;
+}
+
+// Grid R x segs; NT threads.  top <= kLpMaxTop.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __restrict__ logits, int64_t sb, int64_t st,
+                                                                  int Tn, const int64_t* __restrict__ tokens, int V,
+                                                                  float inv_temp, int top, int segs, LpOut out) {
+  constexpr int NW = NT / 64;
+  __shared__ float red[3][NW];
+  __shared__ unsigned long long kred[NW], best[kLpMaxTop];
+  const int r = blockIdx.x / segs, seg = blockIdx.x - r * segs;
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const LpRow<T> row(lp_row(logits, sb, st, Tn, r), V);
+  const int q0 = seg * NT * kLpChunks + tid;
+  typename LpRow<T>::V8 x[kLpChunks];
+#pragma unroll
+  for (int c = 0; c < kLpChunks; ++c) x[c] = row.load(q0 + c * NT);
+
+  float m = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < kLpChunks; ++c)
+#pragma unroll
+    for (int e = 0; e < kLpChunk; ++e) m = fmaxf(m, (float)x[c][e]);
+  m = lp_wave_max(m);
+  if (lane == 0) red[0][w] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NW; ++i) m = fmaxf(m, red[0][i]);
+  // a segment of -inf alone adds nothing to the others (its own sums would be NaN)
+  const float mref = segs > 1 && m == -INFINITY ? 0.f : m;
+  const float c2 = LOG2E_F * inv_temp;
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int c = 0; c < kLpChunks; ++c) {
+#pragma unroll
+    for (int e = 0; e < kLpChunk; ++e) {
+      const float a = ((float)x[c][e] - mref) * c2;
+      const float p = __builtin_amdgcn_exp2f(a);
+      s += p;
+      t = fmaf(p, fmaxf(a, kLpNone), t);  // p = 0 where a = -inf
+    }
+  }
+  s = lp_wave_sum(s);
+  t = lp_wave_sum(t);
+  if (lane == 0) {
+    red[1][w] = s;
+    red[2][w] = t;
+  }
+  // the alternatives, one a round: each lane offers its largest key below the last one taken
+  if (top > 0) {
+    unsigned long long mine = 0, bound = ~0ull;
+    bool scan = true;
+#pragma unroll 1
+    for (int k = 0; k < top; ++k) {
+      if (scan) {
+        mine = 0;
+#pragma unroll
+        for (int c = 0; c < kLpChunks; ++c) {
+          const int j = row.first(q0 + c * NT);
+#pragma unroll
+          for (int e = 0; e < kLpChunk; ++e) {
+            const unsigned long long key = lp_key((float)x[c][e], j + e);
+            if (j + e >= 0 && j + e < V && key < bound && key > mine) mine = key;
+          }
+        }
+      }
+      unsigned long long b = lp_wave_max(mine);
+      if (lane == 0) kred[w] = b;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NW; ++i) b = kred[i] > b ? kred[i] : b;
+      if (tid == 0) best[k] = b;
+      scan = mine == b;  // (also where nothing is left: key 0)
+      bound = b;
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  s = t = 0.f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    s += red[1][i];
+    t += red[2][i];
+  }
+  if (segs == 1) {
+    float l2 = log2f(s);
+    if (tid == 0) {
+      const int64_t tok = tokens[r];
+      lp_finish(out, r, m, s, t, inv_temp, tokens, V, tok >= 0 && tok < V ? (float)row.row[tok] : 0.f);
+    }
+    if (tid < top) {
+      out.top_idx[(int64_t)r * top + tid] = lp_index(best[tid]);
+      out.top_lp[(int64_t)r * top + tid] = (lp_value(best[tid]) - m) * inv_temp - 0.69314718055994531f * l2;
+    }
+  } else {
+    const int64_t at = (int64_t)r * segs + seg;
+    if (tid == 0) {
+      out.pm[at] = m;
+      out.ps[at] = s;
+      out.pt[at] = t;
+    }
+    if (tid < top) out.pkey[at * top + tid] = best[tid];
+  }
+}
+
+// Rows of several segments, one workgroup each: with M the largest maximum and f = exp2((m - M) c) of a
+// segment, s = sum s_i f_i and t = sum f_i (t_i + s_i (m_i - M) c).  Each of the segments' keys counts
+// those above it: its place among the row's alternatives.
+template <typename T>
+__global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T* __restrict__ logits, int64_t sb,
+                                                                         int64_t st, int Tn,
+                                                                         const int64_t* __restrict__ tokens, int V,
+                                                                         float inv_temp, int top, int segs, LpOut out) {
+  __shared__ unsigned long long keys[kLpMaxSegs * kLpMaxTop];
+  __shared__ float stat[2];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const float c2 = LOG2E_F * inv_temp;
+  const int64_t at = (int64_t)r * segs;
+  const int n = segs * top;
+  for (int i = tid; i < n; i += 256) keys[i] = out.pkey[at * top + i];
+  if (tid < 64) {
+    const bool on = lane < segs;
+    const float mi = on ? out.pm[at + lane] : -INFINITY;
+    const float m = lp_wave_max(mi);
+    float f = 0.f, d = 0.f;
+    if (on && mi != -INFINITY) {  // (a segment of -inf alone has the sums 0; NaN sums have to go through)
+      d = (mi - m) * c2;
+      f = __builtin_amdgcn_exp2f(d);
+    }
+    const float si = on ? out.ps[at + lane] : 0.f, ti = on ? out.pt[at + lane] : 0.f;
+    const bool gone = !on || (mi == -INFINITY && si == 0.f);
+    const float s = lp_wave_sum(gone ? (m == -INFINITY && lane == 0 ? __builtin_nanf("") : 0.f) : mi == -INFINITY ? si : si * f);
+    const float t = lp_wave_sum(gone ? 0.f : mi == -INFINITY ? ti : f * fmaf(si, fmaxf(d, kLpNone), ti));
+    if (lane == 0) {
+      const int64_t tok = tokens[r];
+      const T* row = lp_row(logits, sb, st, Tn, r);
+      stat[0] = m;
+      stat[1] = lp_finish(out, r, m, s, t, inv_temp, tokens, V, tok >= 0 && tok < V ? (float)row[tok] : 0.f);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += 256) {
+    const unsigned long long key = keys[i];
+    if (!key) continue;
+    int above = 0;
+    for (int k = 0; k < n; ++k) above += keys[k] > key;
+    if (above >= top) continue;
+    out.top_idx[(int64_t)r * top + above] = lp_index(key);
+    out.top_lp[(int64_t)r * top + above] = (lp_value(key) - stat[0]) * inv_temp - 0.69314718055994531f * stat[1];
+  }
+}
+
+struct LpGrads {
+  const float* lp;   // [R] or null: gradients of the log probability,
+  const float* ent;  // [R] or null: of the entropy,
+  const float* top;  // [R][top] or null: of the alternatives' log probabilities
+};
+
+// Grid R x blocks (column blocks of a row).  Every value gets the softmax part; then the values that a token or an
+// alternative names are written once more with their whole gradient (rounded once).
+template <typename T>
+__global__ __launch_bounds__(256) void lucid_token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t sb,
+                                                                       int64_t st, int Tn,
+                                                                       const int64_t* __restrict__ tokens, int V,
+                                                                       float inv_temp, int top,
+                                                                       const LpStats* __restrict__ stats,
+                                                                       const int64_t* __restrict__ top_idx, LpGrads g,
+                                                                       T* __restrict__ dlogits, int blocks) {
+  constexpr int NT = 256;
+  __shared__ int name[kLpMaxTop + 1];
+  __shared__ float gain[kLpMaxTop + 1];
+  const int r = blockIdx.x / blocks, col = blockIdx.x - r * blocks, tid = threadIdx.x;
+  const LpRow<T> row(lp_row(logits, sb, st, Tn, r), V);
+  T* drow = dlogits + (int64_t)r * V;
+  const LpStats z = stats[r];
+  const float c2 = LOG2E_F * inv_temp;
+  const int64_t tok = tokens[r];
+  float glp = g.lp && tok != kLpIgnore ? g.lp[r] : 0.f;
+  if (g.lp && tok != kLpIgnore && (tok < 0 || tok >= V)) glp = __builtin_nanf("");
+  if (tid == 0) {
+    name[0] = tok >= 0 && tok < V ? (int)tok : -1;
+    gain[0] = glp;
+  }
+  if (tid < top) {
+    name[tid + 1] = (int)top_idx[(int64_t)r * top + tid];
+    gain[tid + 1] = g.top ? g.top[(int64_t)r * top + tid] : 0.f;
+  }
+  __syncthreads();
+  float all = glp;
+  for (int k = 1; k <= top; ++k) all += gain[k];
+  const float gh = g.ent ? g.ent[r] : 0.f;
+  // dx of the softmax part: -p (all + gh (ln p + H)), ln p = ln2 a
+  const float ka = all + gh * z.ent, kb = gh * 0.69314718055994531f;
+  auto soft = [&](float x) {
+    const float a = (x - z.m) * c2 - z.l2;
+    const float p = __builtin_amdgcn_exp2f(a);
+    return -p * fmaf(kb, fmaxf(a, kLpNone), ka);
+  };
+  const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) / sizeof(T) == (unsigned)row.shift;
+  const int q0 = col * NT * kLpChunks + tid;
+#pragma unroll
+  for (int c = 0; c < kLpChunks; ++c) {
+    const int q = q0 + c * NT, j = row.first(q);
+    if (j >= V) break;
+    const typename LpRow<T>::V8 x = row.load(q);
+    typename LpRow<T>::V8 o;
+#pragma unroll
+    for (int e = 0; e < kLpChunk; ++e) o[e] = (T)(soft((float)x[e]) * inv_temp);
+    if (same && row.whole(q)) {
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<bf16x8*>(drow + j) = o;
+      } else {
+        *reinterpret_cast<f32x4*>(drow + j) = f32x4{o[0], o[1], o[2], o[3]};
+        *reinterpret_cast<f32x4*>(drow + j + 4) = f32x4{o[4], o[5], o[6], o[7]};
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kLpChunk; ++e)
+        if (j + e >= 0 && j + e < V) drow[j + e] = o[e];
+    }
+  }
+  __syncthreads();
+  if (tid <= top) {
+    const int j = name[tid];
+    const int lo = row.first(col * NT * kLpChunks), hi = lo + NT * kLpChunks * kLpChunk;
+    if (j >= 0 && j >= lo && j < hi) {
+      bool firstly = true;
+      float add = 0.f;
+      for (int k = 0; k <= top; ++k) {
+        if (name[k] != j) continue;
+        if (k < tid) firstly = false;
+        add += gain[k];
+      }
+      if (firstly) drow[j] = (T)((add + soft((float)row.row[j])) * inv_temp);
+    }
+  }
+}
+
+}  // namespace lucid

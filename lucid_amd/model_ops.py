@@ -17,14 +17,19 @@ one kernel pass forward and one backward:
   reference rounds silu(g) to bf16 before the product).
 * :func:`causal_lm_loss` -- the shifted cross entropy on bf16 logits, one read of the logits
   forward (per-row logsumexp) and one read + write backward, instead of fp32 copies of them.
+* :func:`token_logprobs` -- log probabilities of given tokens, entropy and the top alternatives of
+  logit rows (bf16 or fp32, any vocabulary), and the gradient of all three.
 
-All take bf16 GPU tensors only (RMSNorm: hidden sizes 512, 1024, 2048 or 4096; RoPE: head
+The others take bf16 GPU tensors only (RMSNorm: hidden sizes 512, 1024, 2048 or 4096; RoPE: head
 dim 64; the loss: a vocabulary that is a multiple of 8) and raise otherwise; the
 ``*_supported`` predicates tell the model which inputs they cover.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -273,3 +278,101 @@ def causal_lm_loss(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     """Mean cross entropy of logits[:, :-1] against labels[:, 1:] with -100 ignored, computed in
     fp32 (``LlamaForCausalLM.forward``'s loss, modeling_lucid.py:847-967); a float32 scalar."""
     return CausalLMLossFunction.apply(logits, labels)
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` gives for logits ``[..., V]`` (fp32, indices int64)."""
+
+    logprobs: torch.Tensor       # [...] log probability of the given token
+    entropy: torch.Tensor        # [...] of the row's distribution
+    top_logprobs: torch.Tensor   # [..., top] log probabilities of the most likely tokens
+    top_indices: torch.Tensor    # [..., top] those tokens
+
+
+_LP_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+MAX_TOP = 64
+
+
+def _logit_rows(logits: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """``logits`` as the kernels read them, with rows per batch entry and the two strides: [R, V] and
+    [B, T, V] views with contiguous rows are read as they are, anything else as one run of rows."""
+    if logits.stride(-1) == 1 or logits.shape[-1] == 1:
+        if logits.dim() == 1:
+            return logits, 1, 0, 0
+        if logits.dim() == 2:
+            return logits, max(logits.shape[0], 1), 0, logits.stride(0)
+        if logits.dim() == 3:
+            return logits, max(logits.shape[1], 1), logits.stride(0), logits.stride(1)
+    rows = logits.reshape(-1, logits.shape[-1])
+    rows = rows if rows.stride(1) == 1 or rows.shape[1] == 1 else rows.contiguous()
+    return rows, max(rows.shape[0], 1), 0, rows.stride(0)
+
+
+class TokenLogprobsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits: torch.Tensor, tokens: torch.Tensor, top: int, temperature: float):
+        shape, V, dev = tokens.shape, logits.shape[-1], logits.device
+        rows, T, sb, st = _logit_rows(logits)
+        tok = tokens.contiguous()
+        R = tok.numel()
+        lib = _lib.load()
+        logprobs, entropy = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(2))
+        stats = torch.empty(R, 3, dtype=torch.float32, device=dev)
+        top_lp = torch.empty(*shape, top, dtype=torch.float32, device=dev)
+        top_idx = torch.empty(*shape, top, dtype=torch.int64, device=dev)
+        nbytes = lib.lucid_token_logprobs_workspace_bytes(R, V, top)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with _lib.on(dev):
+            rc = lib.lucid_token_logprobs_fwd(
+                rows.data_ptr(), sb, st, tok.data_ptr(), R, T, V, _LP_DTYPES[logits.dtype], temperature, top,
+                logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top_lp.data_ptr(), top_idx.data_ptr(),
+                None if ws is None else ws.data_ptr(), _lib.stream_handle(dev))
+        _lib.check(lib, rc, "lucid_token_logprobs_fwd")
+        ctx.save_for_backward(logits, tok, stats, top_idx)
+        ctx.top, ctx.temperature = top, temperature
+        ctx.mark_non_differentiable(top_idx)
+        ctx.set_materialize_grads(False)
+        return logprobs, entropy, top_lp, top_idx
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlp, dent, dtop, _didx):
+        logits, tok, stats, top_idx = ctx.saved_tensors
+        if dlp is None and dent is None and dtop is None:
+            return None, None, None, None
+        rows, T, sb, st = _logit_rows(logits)
+        dlp, dent, dtop = (None if g is None else g.contiguous() for g in (dlp, dent, dtop))
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        lib = _lib.load()
+        with _lib.on(logits.device):
+            rc = lib.lucid_token_logprobs_bwd(
+                rows.data_ptr(), sb, st, tok.data_ptr(), tok.numel(), T, logits.shape[-1], _LP_DTYPES[logits.dtype],
+                ctx.temperature, ctx.top, stats.data_ptr(), top_idx.data_ptr(),
+                *(None if g is None else g.data_ptr() for g in (dlp, dent, dtop)), dlogits.data_ptr(),
+                _lib.stream_handle(logits.device))
+        _lib.check(lib, rc, "lucid_token_logprobs_bwd")
+        return dlogits, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` under ``softmax(logits / temperature)``, with the rows' entropy and their
+    ``top`` most likely tokens (0 .. 64), from one read of the logits; differentiable w.r.t. ``logits`` through all
+    three (one more read and one write).
+
+    ``logits [..., V]`` bf16 or fp32 on the GPU, ``tokens [...]`` int64; results in fp32.  A token of -100 (the
+    loss's ignore index) has the log probability 0 and no gradient, one outside ``[0, V)`` NaN.  The alternatives are
+    ordered by their logits, equal ones by the lower index.  Logits of -inf have probability 0; a row of -inf
+    alone, or with a NaN or +inf, gives NaN as torch's log_softmax does."""
+    if not logits.is_cuda:
+        raise RuntimeError("lucid_amd: logits must be a GPU tensor (no CPU path)")
+    if logits.dtype not in _LP_DTYPES or tokens.dtype != torch.int64 or tokens.device != logits.device:
+        raise TypeError("lucid_amd.token_logprobs: bf16 or fp32 logits and int64 tokens on one GPU, got "
+                        f"{logits.dtype} / {tokens.dtype} on {tokens.device}")
+    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape or logits.shape[-1] < 1:
+        raise ValueError(f"lucid_amd.token_logprobs: logits [..., V] and tokens [...], got {tuple(logits.shape)} and "
+                         f"{tuple(tokens.shape)}")
+    if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
+        raise ValueError(f"lucid_amd.token_logprobs: top must be in [0, min({MAX_TOP}, V)], got {top}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"lucid_amd.token_logprobs: the temperature must be positive and finite, got {temperature}")
+    return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, int(top), float(temperature)))
