@@ -147,9 +147,14 @@ int write_pages(const void* k, const int64_t* ks, const void* v, const int64_t* 
 // Token log probabilities: workgroups of 256 lanes for rows of up to 8192 values (and what a
 // misaligned row's first chunk leaves out), else of 1024 on segments of 32768
 int lp_threads(int V) { return V + lucid::kLpChunk - 1 <= 256 * lucid::kLpChunks * lucid::kLpChunk ? 256 : 1024; }
-int lp_segs(int V) {
+int lp_segs(int V, bool aligned = false) {
   const int seg = lp_threads(V) * lucid::kLpChunks * lucid::kLpChunk;
-  return (int)(((int64_t)V + lucid::kLpChunk - 1 + seg - 1) / seg);
+  return (int)(((int64_t)V + (aligned ? 0 : lucid::kLpChunk - 1) + seg - 1) / seg);
+}
+// whether every row starts at a 16-byte boundary (its first chunk is whole)
+bool lp_aligned(const void* logits, int64_t sb, int64_t st, int dtype) {
+  const int64_t es = dtype == LUCID_DTYPE_F32 ? 4 : 2;
+  return reinterpret_cast<uintptr_t>(logits) % 16 == 0 && sb * es % 16 == 0 && st * es % 16 == 0;
 }
 
 lucid::LpOut carve_lp(void* base, int64_t R, int segs, int top, size_t* bytes) {
@@ -188,9 +193,9 @@ int check_lp(const char* what, const void* logits, int64_t sb, int64_t st, const
 }
 
 template <typename T>
-int lp_fwd(const void* logits, int64_t sb, int64_t st, const int64_t* tokens, int R, int Tn, int V, float inv_temp, int top,
-           const lucid::LpOut& out, hipStream_t stream) {
-  const int segs = lp_segs(V), nt = lp_threads(V);
+int lp_fwd(const void* logits, int64_t sb, int64_t st, const int64_t* tokens, int R, int Tn, int V, int segs, float inv_temp,
+           int top, const lucid::LpOut& out, hipStream_t stream) {
+  const int nt = lp_threads(V);
   const dim3 grid((unsigned)R * segs);
   if (nt == 256)
     LUCID_LAUNCH("lucid_token_logprobs_kernel", (lucid::lucid_token_logprobs_kernel<T, 256>), grid, stream, (const T*)logits,
@@ -343,7 +348,7 @@ int lucid_token_logprobs_fwd(const void* logits, int64_t batch_stride, int64_t r
                         top))
     return rc;
   if (R == 0) return LUCID_OK;
-  const int segs = lp_segs(V);
+  const int segs = lp_segs(V, lp_aligned(logits, batch_stride, row_stride, dtype));
   if (!logprobs || !entropy || !stats || (top && (!top_logprobs || !top_indices)) || (segs > 1 && !ws))
     return fail("lucid_token_logprobs_fwd: null output or workspace");
   if (segs > 1)
@@ -355,7 +360,7 @@ int lucid_token_logprobs_fwd(const void* logits, int64_t batch_stride, int64_t r
   out.top_lp = top_logprobs;
   out.top_idx = top_indices;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return (dtype == LUCID_DTYPE_F32 ? lp_fwd<float> : lp_fwd<bf16>)(logits, batch_stride, row_stride, tokens, R, T, V,
+  return (dtype == LUCID_DTYPE_F32 ? lp_fwd<float> : lp_fwd<bf16>)(logits, batch_stride, row_stride, tokens, R, T, V, segs,
                                                                    1.f / temperature, top, out, st);
 }
 

@@ -21,6 +21,7 @@ namespace lucid {
 constexpr int kLpChunk = 8;     // consecutive logits per load of a lane
 constexpr int kLpChunks = 4;    // chunks a lane holds
 constexpr int kLpMaxTop = 64;   // alternatives of a row
+constexpr int kLpCand = 1024;   // values considered for the alternatives of a segment
 constexpr int kLpMaxSegs = 64;  // segments of a row
 constexpr float kLpNone = -1000.f;  // a log2 probability whose exp2 is 0: stands for every lower one
 
@@ -131,13 +132,21 @@ __device__ __forceinline__ float lp_finish(const LpOut& out, int r, float m, flo
 }
 
 // Grid R x segs; NT threads.  top <= kLpMaxTop.
+// Alternatives: the lanes form 64 groups, and the top-th largest of the groups' maxima is a bound that
+// at least `top` values reach and, over values in no order, few more than that (20 alternatives: 24).  Those
+// are collected and each counts the ones before it.  Rows with more than kLpCand values at or above the
+// bound (masks of one finite value, few allowed tokens, ordered logits) are tried again with the equal ones
+// limited to low indices, which is enough wherever such values are dense, and else taken one a round.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __restrict__ logits, int64_t sb, int64_t st,
                                                                   int Tn, const int64_t* __restrict__ tokens, int V,
                                                                   float inv_temp, int top, int segs, LpOut out) {
   constexpr int NW = NT / 64;
-  __shared__ float red[3][NW];
-  __shared__ unsigned long long kred[NW], best[kLpMaxTop];
+  constexpr int GL = NT / 64;  // lanes of one of 64 groups
+  __shared__ float red[3][NW], gmax[64];
+  __shared__ unsigned long long kred[NW], best[kLpMaxTop], cand[kLpCand];
+  __shared__ float bound_;
+  __shared__ int found[2];
   const int r = blockIdx.x / segs, seg = blockIdx.x - r * segs;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const LpRow<T> row(lp_row(logits, sb, st, Tn, r), V);
@@ -151,9 +160,24 @@ __global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __res
   for (int c = 0; c < kLpChunks; ++c)
 #pragma unroll
     for (int e = 0; e < kLpChunk; ++e) m = fmaxf(m, (float)x[c][e]);
-  m = lp_wave_max(m);
+#pragma unroll
+  for (int o = 1; o < GL; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if (top > 0 && tid % GL == 0) gmax[tid / GL] = m;
+#pragma unroll
+  for (int o = GL; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   if (lane == 0) red[0][w] = m;
+  if (tid < 2) found[tid] = 0;
   __syncthreads();
+  if (top > 0 && w == 0) {  // the top-th largest group maximum
+    const float mine = gmax[lane];
+    int above = 0;
+#pragma unroll 16
+    for (int i = 0; i < 64; ++i) {
+      const float o = gmax[i];
+      above += o > mine || (o == mine && i < lane);
+    }
+    if (above == top - 1) bound_ = mine;
+  }
 #pragma unroll
   for (int i = 0; i < NW; ++i) m = fmaxf(m, red[0][i]);
   // a segment of -inf alone adds nothing to the others (its own sums would be NaN)
@@ -176,33 +200,75 @@ __global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __res
     red[1][w] = s;
     red[2][w] = t;
   }
-  // the alternatives, one a round: each lane offers its largest key below the last one taken
   if (top > 0) {
-    unsigned long long mine = 0, bound = ~0ull;
-    bool scan = true;
-#pragma unroll 1
-    for (int k = 0; k < top; ++k) {
-      if (scan) {
-        mine = 0;
+    __syncthreads();
+    const float bound = bound_;
+    const int lo = max(row.first(seg * NT * kLpChunks), 0);  // the segment's first index
+    // Offers what passes: everything from the bound up (and NaN), or, the second time, the values above it and
+    // those equal to it among the segment's first kLpCand / 2.
+    auto offer = [&](int pass) {
 #pragma unroll
-        for (int c = 0; c < kLpChunks; ++c) {
-          const int j = row.first(q0 + c * NT);
+      for (int c = 0; c < kLpChunks; ++c) {
+        const int j = row.first(q0 + c * NT);
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < kLpChunk; ++e) any |= !((float)x[c][e] < bound);
+        if (any) {
 #pragma unroll
           for (int e = 0; e < kLpChunk; ++e) {
-            const unsigned long long key = lp_key((float)x[c][e], j + e);
-            if (j + e >= 0 && j + e < V && key < bound && key > mine) mine = key;
+            const float v = (float)x[c][e];
+            if (v < bound || j + e < 0 || j + e >= V) continue;
+            if (pass == 1 && v == bound && j + e - lo >= kLpCand / 2) continue;
+            const int at = atomicAdd(&found[pass], 1);
+            if (at < kLpCand) cand[at] = lp_key(v, j + e);
           }
         }
       }
-      unsigned long long b = lp_wave_max(mine);
-      if (lane == 0) kred[w] = b;
+    };
+    offer(0);
+    __syncthreads();
+    int n = found[0];
+    if (n > kLpCand) {
+      offer(1);
       __syncthreads();
+      n = found[1];
+    }
+    if (n <= kLpCand && (n >= top || found[0] <= kLpCand)) {
+      if (tid < top && tid >= n) best[tid] = 0;  // a short last segment
+      for (int i = tid; i < n; i += NT) {
+        const unsigned long long key = cand[i];
+        int above = 0;
+        for (int k = 0; k < n; ++k) above += cand[k] > key;
+        if (above < top) best[above] = key;
+      }
+    } else {
+      // one a round: each lane offers its largest key below the last one taken
+      unsigned long long mine = 0, last = ~0ull;
+      bool scan = true;
+#pragma unroll 1
+      for (int k = 0; k < top; ++k) {
+        if (scan) {
+          mine = 0;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) b = kred[i] > b ? kred[i] : b;
-      if (tid == 0) best[k] = b;
-      scan = mine == b;  // (also where nothing is left: key 0)
-      bound = b;
-      __syncthreads();
+          for (int c = 0; c < kLpChunks; ++c) {
+            const int j = row.first(q0 + c * NT);
+#pragma unroll
+            for (int e = 0; e < kLpChunk; ++e) {
+              const unsigned long long key = lp_key((float)x[c][e], j + e);
+              if (j + e >= 0 && j + e < V && key < last && key > mine) mine = key;
+            }
+          }
+        }
+        unsigned long long b = lp_wave_max(mine);
+        if (lane == 0) kred[w] = b;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NW; ++i) b = kred[i] > b ? kred[i] : b;
+        if (tid == 0) best[k] = b;
+        scan = mine == b;
+        last = b;
+        __syncthreads();
+      }
     }
   }
   __syncthreads();
