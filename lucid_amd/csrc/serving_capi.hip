@@ -198,11 +198,13 @@ int lp_fwd(const void* logits, int64_t sb, int64_t st, const int64_t* tokens, in
   const int nt = lp_threads(V);
   const dim3 grid((unsigned)R * segs);
   if (nt == 256)
-    LUCID_LAUNCH("lucid_token_logprobs_kernel", (lucid::lucid_token_logprobs_kernel<T, 256>), grid, stream, (const T*)logits,
-                 sb, st, Tn, tokens, V, inv_temp, top, segs, out);
+    LUCID_LAUNCH("lucid_token_logprobs_kernel",
+                 (top ? lucid::lucid_token_logprobs_kernel<T, 256, true> : lucid::lucid_token_logprobs_kernel<T, 256, false>),
+                 grid, stream, (const T*)logits, sb, st, Tn, tokens, V, inv_temp, top, segs, out);
   else
-    LUCID_LAUNCH_B("lucid_token_logprobs_kernel", (lucid::lucid_token_logprobs_kernel<T, 1024>), grid, dim3(1024), stream,
-                   (const T*)logits, sb, st, Tn, tokens, V, inv_temp, top, segs, out);
+    LUCID_LAUNCH_B("lucid_token_logprobs_kernel",
+                   (top ? lucid::lucid_token_logprobs_kernel<T, 1024, true> : lucid::lucid_token_logprobs_kernel<T, 1024, false>),
+                   grid, dim3(1024), stream, (const T*)logits, sb, st, Tn, tokens, V, inv_temp, top, segs, out);
   if (segs > 1)
     LUCID_LAUNCH("lucid_token_logprobs_merge_kernel", lucid::lucid_token_logprobs_merge_kernel<T>, dim3(R), stream,
                  (const T*)logits, sb, st, Tn, tokens, V, inv_temp, top, segs, out);

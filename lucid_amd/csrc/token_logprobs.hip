@@ -25,7 +25,9 @@ constexpr int kLpCand = 1024;   // values considered for the alternatives of a s
 constexpr int kLpMaxSegs = 64;  // segments of a row
 constexpr float kLpNone = -1000.f;  // a log2 probability whose exp2 is 0: stands for every lower one
 
-// What a forward row leaves for the backward: p_j = exp2((logit_j - m) c - l2), c = log2 e / temperature
+// What a forward row leaves for the backward: p_j = exp2(a_j - l2), a_j = (logit_j - m) c with c = log2 e /
+// temperature (the difference first: one of two logits of the type's lowest value is 0, where their products
+// with c overflow)
 struct LpStats {
   float m, l2, ent;
 };
@@ -115,8 +117,7 @@ struct LpOut {
 
 constexpr int64_t kLpIgnore = -100;  // the loss's ignore index
 
-// The row's results from its maximum m (raw logits), s = sum exp2((x - m) c) and
-// t = sum exp2((x - m) c) (x - m) c
+// The row's results from s = sum exp2(a_j) and t = sum exp2(a_j) a_j; returns log2 s
 __device__ __forceinline__ float lp_finish(const LpOut& out, int r, float m, float s, float t, float inv_temp,
                                            const int64_t* tokens, int V, float xtok) {
   constexpr float kLn2 = 0.69314718055994531f;
@@ -137,14 +138,14 @@ __device__ __forceinline__ float lp_finish(const LpOut& out, int r, float m, flo
 // are collected and each counts the ones before it.  Rows with more than kLpCand values at or above the
 // bound (masks of one finite value, few allowed tokens, ordered logits) are tried again with the equal ones
 // limited to low indices, which is enough wherever such values are dense, and else taken one a round.
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __restrict__ logits, int64_t sb, int64_t st,
+template <typename T, int NT, bool TOP>
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8))) void lucid_token_logprobs_kernel(const T* __restrict__ logits, int64_t sb, int64_t st,
                                                                   int Tn, const int64_t* __restrict__ tokens, int V,
                                                                   float inv_temp, int top, int segs, LpOut out) {
   constexpr int NW = NT / 64;
   constexpr int GL = NT / 64;  // lanes of one of 64 groups
-  __shared__ float red[3][NW], gmax[64];
-  __shared__ unsigned long long kred[NW], best[kLpMaxTop], cand[kLpCand];
+  __shared__ float red[3][NW], gmax[TOP ? 64 : 1];
+  __shared__ unsigned long long kred[TOP ? NW : 1], best[TOP ? kLpMaxTop : 1], cand[TOP ? kLpCand : 1];
   __shared__ float bound_;
   __shared__ int found[2];
   const int r = blockIdx.x / segs, seg = blockIdx.x - r * segs;
@@ -162,13 +163,13 @@ __global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __res
     for (int e = 0; e < kLpChunk; ++e) m = fmaxf(m, (float)x[c][e]);
 #pragma unroll
   for (int o = 1; o < GL; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if (top > 0 && tid % GL == 0) gmax[tid / GL] = m;
+  if (TOP && tid % GL == 0) gmax[tid / GL] = m;
 #pragma unroll
   for (int o = GL; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   if (lane == 0) red[0][w] = m;
-  if (tid < 2) found[tid] = 0;
+  if (TOP && tid < 2) found[tid] = 0;
   __syncthreads();
-  if (top > 0 && w == 0) {  // the top-th largest group maximum
+  if (TOP && w == 0) {  // the top-th largest group maximum
     const float mine = gmax[lane];
     int above = 0;
 #pragma unroll 16
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __res
     red[1][w] = s;
     red[2][w] = t;
   }
-  if (top > 0) {
+  if constexpr (TOP) {
     __syncthreads();
     const float bound = bound_;
     const int lo = max(row.first(seg * NT * kLpChunks), 0);  // the segment's first index
@@ -279,12 +280,12 @@ __global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __res
     t += red[2][i];
   }
   if (segs == 1) {
-    float l2 = log2f(s);
+    const float l2 = log2f(s);
     if (tid == 0) {
       const int64_t tok = tokens[r];
       lp_finish(out, r, m, s, t, inv_temp, tokens, V, tok >= 0 && tok < V ? (float)row.row[tok] : 0.f);
     }
-    if (tid < top) {
+    if (TOP && tid < top) {
       out.top_idx[(int64_t)r * top + tid] = lp_index(best[tid]);
       out.top_lp[(int64_t)r * top + tid] = (lp_value(best[tid]) - m) * inv_temp - 0.69314718055994531f * l2;
     }
@@ -295,12 +296,12 @@ __global__ __launch_bounds__(NT) void lucid_token_logprobs_kernel(const T* __res
       out.ps[at] = s;
       out.pt[at] = t;
     }
-    if (tid < top) out.pkey[at * top + tid] = best[tid];
+    if (TOP && tid < top) out.pkey[at * top + tid] = best[tid];
   }
 }
 
-// Rows of several segments, one workgroup each: with M the largest maximum and f = exp2((m - M) c) of a
-// segment, s = sum s_i f_i and t = sum f_i (t_i + s_i (m_i - M) c).  Each of the segments' keys counts
+// Rows of several segments, one workgroup each: with M the largest of the segments' maxima m_i and
+// d_i = (m_i - M) c, s = sum s_i exp2(d_i) and t = sum exp2(d_i) (t_i + s_i d_i).  Each of the segments' keys counts
 // those above it: its place among the row's alternatives.
 template <typename T>
 __global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T* __restrict__ logits, int64_t sb,
@@ -388,7 +389,7 @@ __global__ __launch_bounds__(256) void lucid_token_logprobs_bwd_kernel(const T* 
   // dx of the softmax part: -p (all + gh (ln p + H)), ln p = ln2 a
   const float ka = all + gh * z.ent, kb = gh * 0.69314718055994531f;
   auto soft = [&](float x) {
-    const float a = (x - z.m) * c2 - z.l2;
+    const float a = fmaf(x - z.m, c2, -z.l2);
     const float p = __builtin_amdgcn_exp2f(a);
     return -p * fmaf(kb, fmaxf(a, kLpNone), ka);
   };
