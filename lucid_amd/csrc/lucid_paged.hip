@@ -11,16 +11,18 @@
 //   o_tg = softmax_j(s q_tg . k_j) w_j over j <= t, for the G query heads of the kv head
 // with w_j the V' row as the cache holds it (bf16), new rows too, so that L tokens in one call are L
 // calls of one token.  The products with the cached rows read each of them once (bytes bound it):
-//   lucid_paged_split_kernel    a chunk of a sequence's rows of one kv head: partial sum_j P_tj w_j and
-//                               the online-softmax state of every (token, query head)
-//   lucid_paged_combine_kernel  the chunks merged, the new tokens solved in order, the outputs, and
-//                               (k_t, v'_t) appended to the pages
+//   lucid_paged_split_kernel    a share of the rows of one kv head, all sequences in a line: of each
+//                               sequence that it covers a part of, partial sum_j P_tj w_j and the
+//                               online-softmax state of every (token, query head)
+//   lucid_paged_combine_kernel  a sequence's parts merged, the new tokens solved in order, the outputs,
+//                               and (k_t, v'_t) appended to the pages
 #include "lucid_common.h"
 
 namespace lucid {
 
 constexpr float PAGED_NEG = -1e30f;    // finite "minus infinity" for empty softmax states
-constexpr int kPagedChunkRows = 128;   // rows of a chunk: a multiple of this (four waves' tiles)
+constexpr int kPagedUnit = 128;        // rows that a workgroup takes at a time (four waves' tiles)
+constexpr int kPagedLead = 1;          // places that a sequence takes in the line beside its rows
 constexpr int kPagedMaxTokens = 16;    // new tokens of a pass
 
 struct PagedBatch {
@@ -28,9 +30,11 @@ struct PagedBatch {
   int64_t tstride;
   const int32_t* lens;  // [B] rows cached before the call
   int B, M, P, page;
-  int L;     // new tokens of the call
-  int done;  // of earlier passes
+  int shift;  // log2 of page, -1 where it is no power of two
+  int L;      // new tokens of the call
+  int done;   // of earlier passes
 };
+__device__ __forceinline__ int page_of(const PagedBatch& s, int j) { return s.shift >= 0 ? j >> s.shift : j / s.page; }
 
 // A pool by its strides in units of 16 bytes (8 elements); the host checks that every row's offset
 // fits 32 bits, a pool of 64 GB.
@@ -47,54 +51,76 @@ __device__ __forceinline__ int paged_rows(const PagedBatch& s, int b) {
   return (int64_t)n + s.L > (int64_t)s.M * s.page ? -2 : n + s.done;
 }
 
-// The sequences' rows are cut into chunks of one length, so that the work of a workgroup does not
-// depend on how the rows are spread over the sequences: the least multiple of kPagedChunkRows that
-// gives at most target chunks, and one more for the remainder of each sequence.
-__device__ __forceinline__ int paged_chunk(const PagedBatch& s, int target) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int b = lane; b < s.B; b += 64) total += max(paged_rows(s, b), 0);
+__device__ __forceinline__ int wave_sum_int(int v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor((long long)total, o, 64);
-  const int64_t ks = (total + target - 1) / target;
-  return (int)((max(ks, (int64_t)1) + kPagedChunkRows - 1) / kPagedChunkRows) * kPagedChunkRows;
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
 }
-__device__ __forceinline__ int paged_chunks(const PagedBatch& s, int b, int ks) {
-  return b < s.B ? (max(paged_rows(s, b), 0) + ks - 1) / ks : 0;
-}
-// Chunks of the sequences before b, and of b itself (every lane of the wave)
-__device__ __forceinline__ void paged_span(const PagedBatch& s, int b, int ks, int& base, int& n) {
-  const int lane = threadIdx.x & 63;
-  int sum = 0;
-  for (int i = lane; i < b; i += 64) sum += paged_chunks(s, i, ks);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  base = sum;
-  n = paged_chunks(s, b, ks);
-}
-// The sequence of chunk slot, and which of its chunks that is; false beyond the last
-__device__ __forceinline__ bool paged_find(const PagedBatch& s, int slot, int ks, int& b, int& chunk) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int c0 = 0; c0 < s.B; c0 += 64) {
-    const int own = paged_chunks(s, c0 + lane, ks);
-    int incl = own;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += x;
-    }
-    const unsigned long long at = __ballot(slot < base + incl);
-    if (at) {
-      const int l = __ffsll(at) - 1;
-      b = c0 + l;
-      chunk = slot - base - __shfl(incl - own, l, 64);
-      return true;
-    }
-    base += __shfl(incl, 63, 64);
+
+// The sequences' rows stand in one line, each sequence rounded up to units of kPagedUnit rows and led by
+// kPagedLead units without rows, and workgroup s of a kv head takes the places [s per, (s + 1) per): equal
+// shares whatever the lengths are, with no tail of workgroups that start late (32 sequences of 8192 rows cut
+// into chunks of their own: 580 workgroups for 512 places, 3.6 TB/s against 4.6).  The lead is what another
+// sequence costs a share, whose loads start anew (without it 10 us of 40 at 8 sequences of 200 to 16000
+// rows, five tokens).  The part of sequence b in share s has the slot s + b among the partials: along the line
+// s + b only grows, so the slots are distinct, at most target + B - 1.  Every wave works the line out from the
+// lengths, 64 sequences at a time (the first 64 are read once and stay in registers).
+struct PagedLine {
+  int n0;     // rows of sequence lane (of the first 64; at least 0)
+  int total;  // places (their number fits: the host's check)
+  int per;    // places of a share
+  static __device__ __forceinline__ int places(int rows) {
+    return rows > 0 ? (rows + kPagedUnit - 1) / kPagedUnit + kPagedLead : 0;
   }
-  return false;
-}
+  __device__ __forceinline__ PagedLine(const PagedBatch& s, int target) {
+    const int lane = threadIdx.x & 63;
+    n0 = lane < s.B ? max(paged_rows(s, lane), 0) : 0;
+    int u = places(n0);
+    for (int b = 64 + lane; b < s.B; b += 64) u += places(max(paged_rows(s, b), 0));
+    total = wave_sum_int(u);
+    per = max(1, (total + target - 1) / target);
+  }
+  __device__ __forceinline__ int rows(const PagedBatch& s, int b) const {
+    return b < 64 ? n0 : b < s.B ? max(paged_rows(s, b), 0) : 0;  // b = lane + a multiple of 64
+  }
+  // the shares that hold parts of sequence b: the slot of the first, and how many
+  __device__ __forceinline__ void parts(const PagedBatch& s, int b, int& slot, int& n) const {
+    const int lane = threadIdx.x & 63;
+    int sum = 0, own = 0;
+    for (int i = lane; i <= b; i += 64) {
+      const int u = places(rows(s, i));
+      sum += i < b ? u : 0;
+      own = i == b ? u : own;
+    }
+    const int before = wave_sum_int(sum), u = __shfl(own, b & 63, 64);
+    const int first = (before + kPagedLead) / per;  // the share of its first row
+    slot = first + b;
+    n = u == 0 ? 0 : (before + u - 1) / per - first + 1;
+  }
+  // the sequence at a place: its rows n and the place of its first row
+  __device__ __forceinline__ void find(const PagedBatch& s, int place, int& b, int& n, int& first) const {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int c0 = 0; c0 < s.B; c0 += 64) {
+      const int r = rows(s, c0 + lane), own = places(r);
+      int incl = own;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += x;
+      }
+      const unsigned long long at = __ballot(place < base + incl);
+      if (at) {
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll(at) - 1);
+        b = c0 + l;
+        first = base + __builtin_amdgcn_readlane(incl - own, l) + kPagedLead;
+        n = __builtin_amdgcn_readlane(r, l);
+        return;
+      }
+      base += __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+};
 
 // Four consecutive columns c .. c+3 of a row of d, zeros beyond d; vec: the row starts at an 8-byte
 // boundary
@@ -106,7 +132,7 @@ __device__ __forceinline__ bf16x4 ld4_cols(const bf16* row, int c, int d, bool v
   return x;
 }
 
-// Partials of the chunks, slot-major; tokens of the pass Lp, columns t Gs + g
+// Partials of the sequences' parts, slot-major; tokens of the pass Lp, columns t Gs + g
 struct PagedPartials {
   float* a;  // [slots][Hkv][Lp][W]      sum_j P_tj w_j
   float* m;  // [slots][Hkv][Lp*Gs]      running max (log2 domain); NaN: a page id outside the pool
@@ -148,8 +174,8 @@ __device__ __forceinline__ bf16x8 paged_tr_a(const bf16* tile, int row0, int col
   }
 }
 
-// Grid (slots, Hkv).  As lucid_decode_split_kernel: each wave sweeps its own 32-row tiles of the
-// chunk, one MFMA score tile S^T[j][c] = K_j . X_c of the columns c = t (Gs + 1) + i (query head
+// Grid (target, Hkv).  As lucid_decode_split_kernel: each wave sweeps its own 32-row tiles of a
+// sequence's part of the share, one MFMA score tile S^T[j][c] = K_j . X_c of the columns c = t (Gs + 1) + i (query head
 // g0 + i of token t, its key at i = Gs), then O^T[d][c] += w^T[d][j] p^T[j][c].  p enters the second
 // product as a bf16 pair (hi + lo, 2^-17), since V' is returned in fp32 and one bf16 term of P
 // would be seen in it.  Page ids reach registers two tiles ahead, rows one.  Columns of the NCT
@@ -162,69 +188,34 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
   constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = 32 * CPR / 64;
   __shared__ __attribute__((aligned(16))) PagedSmem<W> sm;
   const int h = blockIdx.y;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
-  const int ks = paged_chunk(seq, target);
-  int b, chunk;
-  if (!paged_find(seq, blockIdx.x, ks, b, chunk)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  chunk = __builtin_amdgcn_readfirstlane(chunk);
-  const int rows = paged_rows(seq, b);
-  const int j0 = chunk * ks, j1 = min(rows, j0 + ks);
+  const PagedLine line(seq, target);
+  const int end = min(line.total, ((int)blockIdx.x + 1) * line.per);
+  int b = 0, next = 0;
+  for (int place = blockIdx.x * line.per; place < end; place = next) {
+  int rows = 0, first = 0;
+  line.find(seq, place, b, rows, first);
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // what follows from it is worked out here, not kept in registers across the sequences
+  const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
+  next = first + (rows + kPagedUnit - 1) / kPagedUnit;
+  const int j0 = max(place - first, 0) * kPagedUnit, j1 = min(rows, (end - first) * kPagedUnit);
+  if (j1 <= j0) break;  // the share ends in the sequence's lead
   const float sl2 = scale * LOG2E_F, c0 = LOG2E_F / scale, dn = (float)d;
 
-  // B operand: column 32 ct + l32 of X^T (k = d), zero for the padding columns
-  bool valid[NCT], isq[NCT];
-  bf16x8 xb[NCT][NKS];
-  float c1[NCT];
-#pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    const int col = 32 * ct + l32, tok = col / (Gs + 1), hi = col - tok * (Gs + 1);
-    valid[ct] = tok < Lp;
-    isq[ct] = valid[ct] && hi < Gs;
-    const int64_t t = seq.done + tok;
-    const bf16* x = isq[ct] ? q + b * qs.b + (h * Gt + g0 + hi) * qs.h + t * qs.t : kn + b * kns.b + h * kns.h + t * kns.t;
-    float nt = 0.f;
-#pragma unroll
-    for (int st = 0; st < NKS; ++st) {
-      bf16x8 v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (bf16)0.f;
-      if (valid[ct]) {
-        const bf16x4 a = ld4_cols(x, 16 * st + 8 * g, d, vec), c = ld4_cols(x, 16 * st + 8 * g + 4, d, vec);
-        v = bf16x8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) nt = fmaf((float)v[e], (float)v[e], nt);
-      }
-      xb[ct][st] = v;
-    }
-    nt = wave_sum32(nt);  // squared norm of this column's key (both lane halves)
-    c1[ct] = sl2 * rsqrtf(nt / dn + eps);
-  }
-
-  f32x16 oacc[NCT][NDT];
-  float m[NCT], l[NCT];
-#pragma unroll
-  for (int ct = 0; ct < NCT; ++ct) {
-    m[ct] = PAGED_NEG;
-    l[ct] = 0.f;
-#pragma unroll
-    for (int t = 0; t < NDT; ++t) oacc[ct][t] = zero16();
-  }
-
   const int32_t* tbl = seq.table + b * seq.tstride;
-  const int ntile = (j1 - j0 + 31) / 32;  // tiles of the chunk; wave w takes w, w + 4, ...
+  const int ntile = (j1 - j0 + 31) / 32;  // tiles of the part; wave w takes w, w + 4, ...
   bool bad = false;
-  // this lane's row of tile t (rows beyond the chunk: its last row, masked below)
+  // this lane's row of tile t (rows beyond the part: its last row, masked below)
   auto row_of = [&](int t) { return min(j0 + 32 * t + l32, j1 - 1); };
-  auto page_id = [&](int t) { return tbl[row_of(t) / seq.page]; };
+  auto page_id = [&](int t) { return tbl[page_of(seq, row_of(t))]; };
   unsigned koff, voff;  // of this lane's row
-  auto place = [&](int t, int id) {
+  auto locate = [&](int t, int id) {
     const int j = row_of(t);
     if ((unsigned)id >= (unsigned)seq.P) {
       bad = true;
       id = 0;
     }
-    const unsigned in = j % seq.page;
+    const unsigned in = j - page_of(seq, j) * seq.page;
     koff = id * kp.page + h * kp.head + in * kp.row;
     voff = id * vp.page + h * vp.head + in * vp.row;
   };
@@ -244,19 +235,63 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
       __builtin_amdgcn_global_load_lds(src, dst + i * 512, 16, 0, 0);
     }
   };
-  int it = 0, idn = 0;
+  // the first pages' ids, then the new tokens' rows, then the first tile: each wait covers the next loads
+  int it = 0, id0 = 0, idn = 0;
+  if (w < ntile) id0 = page_id(w);
+  if (w + 4 < ntile) idn = page_id(w + 4);
+  // B operand: column 32 ct + l32 of X^T (k = d), zero for the padding columns
+  bool valid[NCT], isq[NCT];
+  bf16x8 xb[NCT][NKS];
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const int col = 32 * ct + l32, tok = col / (Gs + 1), hi = col - tok * (Gs + 1);
+    valid[ct] = tok < Lp;
+    isq[ct] = valid[ct] && hi < Gs;
+    const int64_t t = seq.done + tok;
+    const bf16* x = isq[ct] ? q + b * qs.b + (h * Gt + g0 + hi) * qs.h + t * qs.t : kn + b * kns.b + h * kns.h + t * kns.t;
+#pragma unroll
+    for (int st = 0; st < NKS; ++st) {
+      bf16x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (bf16)0.f;
+      if (valid[ct]) {
+        const bf16x4 a = ld4_cols(x, 16 * st + 8 * g, d, vec), c = ld4_cols(x, 16 * st + 8 * g + 4, d, vec);
+        v = bf16x8{a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
+      }
+      xb[ct][st] = v;
+    }
+  }
   if (w < ntile) {
-    const int id = page_id(w);
-    if (w + 4 < ntile) idn = page_id(w + 4);
-    place(w, id);
+    locate(w, id0);
     kload(kcur);
     vstage(sm.u.v[w][0]);
   }
+  float c1[NCT];  // of the key columns: s log2 e / rms
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    float nt = 0.f;
+#pragma unroll
+    for (int st = 0; st < NKS; ++st)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) nt = fmaf((float)xb[ct][st][e], (float)xb[ct][st][e], nt);
+    nt = wave_sum32(nt);  // both lane halves
+    c1[ct] = sl2 * rsqrtf(nt / dn + eps);
+  }
+  f32x16 oacc[NCT][NDT];
+  float m[NCT], l[NCT];
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    m[ct] = PAGED_NEG;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t) oacc[ct][t] = zero16();
+  }
+
   for (int t = w; t < ntile; t += 4, ++it) {
     const int cur = it & 1;
     const bool more = t + 4 < ntile;
     if (more) {
-      place(t + 4, idn);
+      locate(t + 4, idn);
       if (t + 8 < ntile) idn = page_id(t + 8);
       kload(knx);
       vstage(sm.u.v[w][cur ^ 1]);
@@ -341,7 +376,7 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
   // its elements
   const unsigned long long anybad = __ballot(bad);
   if (lane == 0) sm.bad[w] = anybad != 0;
-  const int64_t at = (int64_t)blockIdx.x * Hkv + h;
+  const int64_t at = (int64_t)(blockIdx.x + b) * Hkv + h;
 #pragma unroll
   for (int ct = 0; ct < NCT; ++ct) {
     const float lw = wave_sum32(l[ct]);
@@ -391,6 +426,8 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
       }
     }
   }
+  if (next < end) __syncthreads();  // the columns are read before the next sequence's rows come
+  }
 }
 
 // Threads of the combine kernel: W / 4 groups of 4 columns, each on NSL lanes that take a chunk in
@@ -408,10 +445,11 @@ constexpr int paged_nsl() {
 template <int W, int LM>
 __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_kernel(
     const bf16* __restrict__ q, Strides qs, const bf16* __restrict__ kn, Strides kns, const bf16* __restrict__ vn,
-    Strides vns, int vec, PagedPool kp, PagedPool vp, PagedBatch seq, int target, bf16* __restrict__ o, Strides os,
+    Strides vns, int vec, int ovec, PagedPool kp, PagedPool vp, PagedBatch seq, int target, bf16* __restrict__ o, Strides os,
     float* __restrict__ vp_new, int Hkv, int Lp, float scale, float eps, int d, PagedPartials part, int Gs, int Gt,
     int g0, int append) {
   constexpr int CG = W / 4, NSL = paged_nsl<W>(), NT = CG * NSL;
+  constexpr int UN = LM == 1 ? 4 : LM == 4 ? 2 : 1;  // chunks whose loads a lane has in flight
   __shared__ float kk[LM][LM], qk[LM][LM];  // k_t . k_u and q_tg . k_u (u <= t)
   __shared__ __attribute__((aligned(16))) float ovs[LM][W], avs[LM][W], vps[LM][W];
   __shared__ float ms_[LM], ls_[LM];
@@ -421,6 +459,7 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
   const int b = bh / Hkv, h = bh - b * Hkv;
   const int tid = threadIdx.x, cg = tid / NSL, sl = tid - cg * NSL, d0 = 4 * cg;
   const int hq = h * Gt + g0 + g;
+  const PagedLine line(seq, target);
   const int rows = paged_rows(seq, b);
   const bf16* kb = kn + b * kns.b + h * kns.h + (int64_t)seq.done * kns.t;
   const bf16* vb = vn + b * vns.b + h * vns.h + (int64_t)seq.done * vns.t;
@@ -436,44 +475,65 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
     }
     return;
   }
-  const int ks = paged_chunk(seq, target);
   int base, nchunk;
-  paged_span(seq, b, ks, base, nchunk);
+  line.parts(seq, b, base, nchunk);
   if (tid == 0) bads = 0;
   __syncthreads();
   // the pages that the call's new rows go to
   for (int t = tid; t < seq.L; t += NT) {
-    const int j = rows - seq.done + t;
-    const int id = seq.table[b * seq.tstride + j / seq.page];
+    const int j = rows - seq.done + t, pg = page_of(seq, j);
+    const int id = seq.table[b * seq.tstride + pg];
     if ((unsigned)id >= (unsigned)seq.P) atomicOr(&bads, 1);
     const int u = t - seq.done;
     if (u >= 0 && u < Lp) {
-      const unsigned in = j % seq.page;
+      const unsigned in = j - pg * seq.page;
       krow[u] = id * kp.page + h * kp.head + in * kp.row;
       vrow[u] = id * vp.page + h * vp.head + in * vp.row;
     }
   }
-  // dot products among the new tokens, 16 lanes a pair
-  for (int idx = tid / 16; idx < Lp * Lp; idx += NT / 16) {
-    const int t = idx / Lp, u = idx - t * Lp;
-    if (u > t) continue;
-    float dkk = 0.f, dqk = 0.f;
-    for (int c = tid % 16; c < d; c += 16) {
-      const float ku = (float)kb[u * kns.t + c];
-      dkk = fmaf((float)kb[t * kns.t + c], ku, dkk);
-      dqk = fmaf((float)qb[t * qs.t + c], ku, dqk);
+  // dot products among the new tokens (t, u <= t), 32 lanes a pair, four columns a lane
+  const int npair = Lp * (Lp + 1) / 2;
+  constexpr int PU = LM == 1 ? 1 : LM == 4 ? 2 : 4;
+  for (int i0 = tid / 32; i0 < npair; i0 += PU * (NT / 32)) {
+    float dkk[PU], dqk[PU];
+    int ts[PU], us[PU];
+    bf16x4 kt[PU], ku[PU], qt[PU];
+#pragma unroll
+    for (int p = 0; p < PU; ++p) {
+      const int i = min(i0 + p * (NT / 32), npair - 1);
+      int t = (int)((sqrtf(8.f * i + 1.f) - 1.f) * 0.5f);
+      if ((t + 1) * (t + 2) / 2 <= i) ++t;
+      if (t * (t + 1) / 2 > i) --t;
+      ts[p] = t;
+      us[p] = i - t * (t + 1) / 2;
+      kt[p] = ld4_cols(kb + t * kns.t, 4 * (tid & 31), d, vec);
+      ku[p] = ld4_cols(kb + us[p] * kns.t, 4 * (tid & 31), d, vec);
+      qt[p] = ld4_cols(qb + t * qs.t, 4 * (tid & 31), d, vec);
     }
 #pragma unroll
-    for (int off = 1; off < 16; off <<= 1) {
-      dkk += __shfl_xor(dkk, off, 64);
-      dqk += __shfl_xor(dqk, off, 64);
-    }
-    if (tid % 16 == 0) {
-      kk[t][u] = dkk;
-      qk[t][u] = dqk;
+    for (int p = 0; p < PU; ++p) {
+      dkk[p] = dqk[p] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dkk[p] = fmaf((float)kt[p][e], (float)ku[p][e], dkk[p]);
+        dqk[p] = fmaf((float)qt[p][e], (float)ku[p][e], dqk[p]);
+      }
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        dkk[p] += __shfl_xor(dkk[p], off, 64);
+        dqk[p] += __shfl_xor(dqk[p], off, 64);
+      }
+      if ((tid & 31) == 0) {
+        kk[ts[p]][us[p]] = dkk[p];
+        qk[ts[p]][us[p]] = dqk[p];
+      }
     }
   }
-  // the chunks' partials of every token: its key column and its query column
+  bf16x4 vrows[LM];  // the new tokens' value rows, wanted after the merge
+#pragma unroll
+  for (int t = 0; t < LM; ++t) vrows[t] = ld4_cols(vb + min(t, Lp - 1) * vns.t, d0, d, vec);
+  // the chunks' partials of every token: its key column and its query column (tokens and chunks beyond
+  // the last read the last again, with the weight 0)
   float M[LM], lv[LM];
   f32x4 ov[LM], av[LM];
   bool bad = false;
@@ -483,23 +543,36 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
     lv[t] = 0.f;
     ov[t] = av[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  for (int s = sl; s < nchunk; s += NSL) {
-    const int64_t at = (int64_t)(base + s) * Hkv + h;
+  for (int s0 = sl; s0 < nchunk; s0 += UN * NSL) {
+    float mi[UN][LM], li[UN][LM];
+    f32x4 oi[UN][LM], ai[UN][LM];
 #pragma unroll
-    for (int t = 0; t < LM; ++t) {
-      if (t < Lp) {
-        const int64_t i = at * (Lp * Gs) + t * Gs + g;
-        const float mi = part.m[i], li = part.l[i];
-        bad |= mi != mi;
-        const f32x4 oi = *reinterpret_cast<const f32x4*>(part.o + i * W + d0);
-        const f32x4 ai = *reinterpret_cast<const f32x4*>(part.a + (at * Lp + t) * W + d0);
-        const float mn = fmaxf(M[t], mi);
-        const float c = __builtin_amdgcn_exp2f(M[t] - mn), e = __builtin_amdgcn_exp2f(mi - mn);
-        lv[t] = fmaf(lv[t], c, li * e);
+    for (int k = 0; k < UN; ++k) {
+      const int64_t at = (int64_t)(base + min(s0 + k * NSL, nchunk - 1)) * Hkv + h;
+#pragma unroll
+      for (int t = 0; t < LM; ++t) {
+        const int tt = min(t, Lp - 1);
+        const int64_t i = at * (Lp * Gs) + tt * Gs + g;
+        mi[k][t] = part.m[i];
+        li[k][t] = part.l[i];
+        oi[k][t] = *reinterpret_cast<const f32x4*>(part.o + i * W + d0);
+        ai[k][t] = *reinterpret_cast<const f32x4*>(part.a + (at * Lp + tt) * W + d0);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < UN; ++k) {
+      const bool on = s0 + k * NSL < nchunk;
+#pragma unroll
+      for (int t = 0; t < LM; ++t) {
+        bad |= mi[k][t] != mi[k][t];
+        const float mn = on ? fmaxf(M[t], mi[k][t]) : M[t];
+        const float c = __builtin_amdgcn_exp2f(M[t] - mn), e = on ? __builtin_amdgcn_exp2f(mi[k][t] - mn) : 0.f;
+        const float one = on ? 1.f : 0.f;
+        lv[t] = fmaf(lv[t], c, li[k][t] * e);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          ov[t][x] = fmaf(ov[t][x], c, oi[x] * e);
-          av[t][x] += ai[x];
+          ov[t][x] = fmaf(ov[t][x], c, oi[k][t][x] * e);
+          av[t][x] = fmaf(ai[k][t][x], one, av[t][x]);
         }
         M[t] = mn;
       }
@@ -510,18 +583,16 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
   for (int off = 1; off < NSL; off <<= 1) {
 #pragma unroll
     for (int t = 0; t < LM; ++t) {
-      if (t < Lp) {
-        const float mo = __shfl_xor(M[t], off, 64), lo = __shfl_xor(lv[t], off, 64);
-        const float mn = fmaxf(M[t], mo);
-        const float c = __builtin_amdgcn_exp2f(M[t] - mn), co = __builtin_amdgcn_exp2f(mo - mn);
-        lv[t] = fmaf(lv[t], c, lo * co);
+      const float mo = __shfl_xor(M[t], off, 64), lo = __shfl_xor(lv[t], off, 64);
+      const float mn = fmaxf(M[t], mo);
+      const float c = __builtin_amdgcn_exp2f(M[t] - mn), co = __builtin_amdgcn_exp2f(mo - mn);
+      lv[t] = fmaf(lv[t], c, lo * co);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          ov[t][x] = fmaf(ov[t][x], c, __shfl_xor(ov[t][x], off, 64) * co);
-          av[t][x] += __shfl_xor(av[t][x], off, 64);
-        }
-        M[t] = mn;
+      for (int x = 0; x < 4; ++x) {
+        ov[t][x] = fmaf(ov[t][x], c, __shfl_xor(ov[t][x], off, 64) * co);
+        av[t][x] += __shfl_xor(av[t][x], off, 64);
       }
+      M[t] = mn;
     }
   }
   if (sl == 0) {
@@ -539,54 +610,98 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
   }
   __syncthreads();
   const bool poison = bads != 0;
-  // the new rows in order (columns d0 .. d0+3): v'_t = (v_t - a_t - sum_{u<t} P_tu w_u) / P_tt
+  // the new tokens among themselves, a pair (t, u <= t) a lane: P_tu (1 / P_tt on the diagonal) in place of k_t . k_u,
+  // the softmax weight of u beside token t's cached part in place of q_tg . k_u
   const float sl2 = scale * LOG2E_F, c0 = LOG2E_F / scale, dn = (float)d;
-  for (int t = 0; sl == 0 && t < Lp; ++t) {
-    const float rt = rsqrtf(kk[t][t] / dn + eps);
-    const bf16x4 v4 = ld4_cols(vb + t * vns.t, d0, d, vec);
-    const f32x4 a4 = *reinterpret_cast<const f32x4*>(&avs[t][d0]);
-    f32x4 x;
+  float pk[LM], pq[LM], weight = 0.f, sum = 0.f;
+  const int tt = tid;  // token of this lane
+  if (tt < Lp) {
+    const float rt = rsqrtf(kk[tt][tt] / dn + eps);
+    float M2 = ms_[tt];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (float)v4[j] - a4[j];
-    for (int u = 0; u < t; ++u) {
-      const float ru = rsqrtf(kk[u][u] / dn + eps);
-      const float p = __builtin_amdgcn_exp2f(fmaf(sl2 * rt * ru, kk[t][u], -c0));
-      const f32x4 vu = *reinterpret_cast<const f32x4*>(&vps[u][d0]);
+    for (int u = 0; u < LM; ++u)
+      if (u <= tt) M2 = fmaxf(M2, qk[tt][u] * sl2);
+    weight = __builtin_amdgcn_exp2f(ms_[tt] - M2);
+    sum = ls_[tt] * weight;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = fmaf(-p, (float)(bf16)vu[j], x[j]);
+    for (int u = 0; u < LM; ++u) {
+      if (u <= tt) {
+        pk[u] = __builtin_amdgcn_exp2f(fmaf(sl2 * rt * rsqrtf(kk[u][u] / dn + eps), kk[tt][u], -c0));
+        pq[u] = __builtin_amdgcn_exp2f(fmaf(qk[tt][u], sl2, -M2));
+        sum += pq[u];
+      }
     }
     // 1 / P_tt; the exponent is the small difference of two terms of size sqrt(d): in fp64
-    const double ms = (double)kk[t][t] / d;
+    const double ms = (double)kk[tt][tt] / d;
     const float inv = __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / scale - scale * d * ms / (ms + eps))));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] *= inv;
-    *reinterpret_cast<f32x4*>(&vps[t][d0]) = x;
+    for (int u = 0; u < LM; ++u)
+      if (u == tt) pk[u] = inv;
+  }
+  if constexpr (LM > 1) __syncthreads();  // every lane has read the dot products (one token: its own lane's)
+  if (tt < Lp) {
+#pragma unroll
+    for (int u = 0; u < LM; ++u) {
+      if (u <= tt) {
+        kk[tt][u] = pk[u];
+        qk[tt][u] = pq[u];
+      }
+    }
+    ms_[tt] = weight;
+    ls_[tt] = sum;
+  }
+  __syncthreads();
+  // the new rows in order (columns d0 .. d0+3): v'_t = (v_t - a_t - sum_{u<t} P_tu w_u) / P_tt
+#pragma unroll
+  for (int t = 0; t < LM; ++t) {
+    if (sl == 0 && t < Lp) {
+      const f32x4 a4 = *reinterpret_cast<const f32x4*>(&avs[t][d0]);
+      f32x4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = (float)vrows[t][j] - a4[j];
+      for (int u = 0; u < t; ++u) {
+        const float p = kk[t][u];
+        const f32x4 vu = *reinterpret_cast<const f32x4*>(&vps[u][d0]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fmaf(-p, (float)(bf16)vu[j], x[j]);
+      }
+      const float inv = kk[t][t];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] *= inv;
+      *reinterpret_cast<f32x4*>(&vps[t][d0]) = x;
+    }
   }
   __syncthreads();
   // outputs, a token per split lane: the cached part merged with the new keys u <= t
   for (int t = sl; t < Lp; t += NSL) {
-    float M2 = ms_[t];
-    for (int u = 0; u <= t; ++u) M2 = fmaxf(M2, qk[t][u] * sl2);
-    const float c = __builtin_amdgcn_exp2f(ms_[t] - M2);
+    const float c = ms_[t], den = ls_[t];
     const f32x4 o4 = *reinterpret_cast<const f32x4*>(&ovs[t][d0]);
     f32x4 num;
 #pragma unroll
     for (int j = 0; j < 4; ++j) num[j] = o4[j] * c;
-    float den = ls_[t] * c;
     for (int u = 0; u <= t; ++u) {
-      const float es = __builtin_amdgcn_exp2f(fmaf(qk[t][u], sl2, -M2));
+      const float es = qk[t][u];
       const f32x4 vu = *reinterpret_cast<const f32x4*>(&vps[u][d0]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) num[j] = fmaf(es, (float)(bf16)vu[j], num[j]);
-      den += es;
     }
     const float rden = poison ? __builtin_nanf("") : 1.f / den;
     const f32x4 vt = *reinterpret_cast<const f32x4*>(&vps[t][d0]);
+    if (d0 < d) {
+      if (ovec) {
+        bf16x4 o4b;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (d0 + j >= d) break;
-      ob[t * os.t + d0 + j] = (bf16)(num[j] * rden);
-      if (write_v) vo[t * d + d0 + j] = poison ? rden : vt[j];
+        for (int j = 0; j < 4; ++j) o4b[j] = (bf16)(num[j] * rden);
+        *reinterpret_cast<bf16x4*>(ob + t * os.t + d0) = o4b;
+        if (write_v) *reinterpret_cast<f32x4*>(vo + t * d + d0) = poison ? f32x4{rden, rden, rden, rden} : vt;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (d0 + j >= d) break;
+          ob[t * os.t + d0 + j] = (bf16)(num[j] * rden);
+          if (write_v) vo[t * d + d0 + j] = poison ? rden : vt[j];
+        }
+      }
     }
     if (write_v && !poison) {
       bf16x4 v4;
@@ -617,9 +732,10 @@ __global__ __launch_bounds__(256) void lucid_write_pages_kernel(const bf16* __re
   if (t >= T || (counts && t >= counts[b])) return;
   const int64_t j = seq.lens[b] + t;
   if (seq.lens[b] < 0 || j >= (int64_t)seq.M * seq.page) return;
-  const int id = seq.table[b * seq.tstride + j / seq.page];
+  const int pg = page_of(seq, (int)j);
+  const int id = seq.table[b * seq.tstride + pg];
   if ((unsigned)id >= (unsigned)seq.P) return;
-  const unsigned in = (unsigned)(j % seq.page);
+  const unsigned in = (unsigned)j - pg * seq.page;
   const bf16* kr = k + b * kst.b + h * kst.h + t * kst.t;
   const TV* vr = v + b * vst.b + h * vst.h + t * vst.t;
   bf16x8 x, y;

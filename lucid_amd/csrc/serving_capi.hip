@@ -9,11 +9,12 @@ int paged_round(int W) { return W == 64 ? 768 : 512; }
 // Row width of a page for a head dim (0: unsupported)
 int page_width(int D) { return D < 1 ? 0 : D <= 64 ? 64 : D <= 80 ? 80 : D <= 96 ? 96 : D <= 128 ? 128 : 0; }
 
-// Chunks wanted of each kv head's rows (all sequences together)
+int page_shift(int page) { return page & (page - 1) ? -1 : __builtin_ctz((unsigned)page); }
+
+// Workgroups of each kv head: one resident round, and no more than there can be units of rows
 int paged_target(int B, int Hkv, int64_t cap, int W) {
-  const int64_t most = (int64_t)B * ((cap + lucid::kPagedChunkRows - 1) / lucid::kPagedChunkRows);
-  const int64_t want = (paged_round(W) + Hkv - 1) / Hkv;
-  return (int)std::max<int64_t>(1, std::min(most, want));
+  const int64_t most = (int64_t)B * ((cap + lucid::kPagedUnit - 1) / lucid::kPagedUnit);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, paged_round(W) / Hkv));
 }
 
 // Query heads of a chunk of a group (at most 31 and their key fill the columns of a score tile), and new
@@ -47,7 +48,8 @@ lucid::PagedPartials carve_paged(void* base, int64_t slots, int Hkv, int Gs, int
 
 bool paged_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int D) {
   return B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && L > 0 && page > 0 && max_pages > 0 && page_width(D) &&
-         (int64_t)page * max_pages <= (1 << 30) && (int64_t)B * Hkv <= (1 << 23) && B <= (1 << 20) && Hkv <= 65535;
+         (int64_t)page * max_pages <= (1 << 30) && (int64_t)B * Hkv <= (1 << 23) && B <= (1 << 20) && Hkv <= 65535 &&
+         B * (((int64_t)page * max_pages + lucid::kPagedUnit - 1) / lucid::kPagedUnit + lucid::kPagedLead) < ((int64_t)1 << 31);
 }
 
 int check_pool(const char* name, void* p, const int64_t* s, int pages, int Hkv, int page, int W, lucid::PagedPool* out) {
@@ -89,9 +91,11 @@ struct PagedCall {
 template <int W, int LM>
 int paged_combine(const PagedCall& c, int vec, const lucid::PagedBatch& seq, int target, int Lp,
                   const lucid::PagedPartials& part, int Gs, int g0, int gc) {
+  // whole groups of 4 columns at 8-byte boundaries of o and 16-byte boundaries of vp_new
+  const int ovec = c.D % 4 == 0 && rows_of_4(c.o, c.os, 2) && !misaligned16(c.vp_new);
   LUCID_LAUNCH_B("lucid_paged_combine_kernel", (lucid::lucid_paged_combine_kernel<W, LM>), dim3(seq.B * c.Hkv, gc),
                  dim3(W / 4 * lucid::paged_nsl<W>()), c.st, (const bf16*)c.q, S(c.qs), (const bf16*)c.k, S(c.ks),
-                 (const bf16*)c.v, S(c.vs), vec, c.kp, c.vp, seq, target, (bf16*)c.o, S(c.os), c.vp_new, c.Hkv, Lp, c.scale,
+                 (const bf16*)c.v, S(c.vs), vec, ovec, c.kp, c.vp, seq, target, (bf16*)c.o, S(c.os), c.vp_new, c.Hkv, Lp, c.scale,
                  c.eps, c.D, part, gc, c.Hq / c.Hkv, g0, g0 == 0 ? 1 : 0);
   return LUCID_OK;
 }
@@ -109,7 +113,7 @@ int paged_decode(const PagedCall& c) {
     for (int g0 = 0; g0 < G; g0 += Gs) {
       const int gc = std::min(Gs, G - g0);  // query heads of this chunk
       const lucid::PagedPartials part = carve_paged(c.ws, slots, c.Hkv, gc, Lp, W, nullptr);
-      const dim3 grid(slots, c.Hkv);
+      const dim3 grid(target, c.Hkv);
       if (tiles == 2)
         LUCID_LAUNCH("lucid_paged_split_kernel", (lucid::lucid_paged_split_kernel<W, 2>), grid, c.st, (const bf16*)c.q,
                      S(c.qs), (const bf16*)c.k, S(c.ks), vec, c.kp, c.vp, seq, target, c.Hkv, Lp, c.scale, c.eps, c.D, part, gc,
@@ -120,6 +124,7 @@ int paged_decode(const PagedCall& c) {
                      G, g0);
       const int rc = Lp == 1   ? paged_combine<W, 1>(c, vec, seq, target, Lp, part, gc, g0, gc)
                      : Lp <= 4 ? paged_combine<W, 4>(c, vec, seq, target, Lp, part, gc, g0, gc)
+                     : Lp <= 8 ? paged_combine<W, 8>(c, vec, seq, target, Lp, part, gc, g0, gc)
                                : paged_combine<W, lucid::kPagedMaxTokens>(c, vec, seq, target, Lp, part, gc, g0, gc);
       if (rc) return rc;
     }
@@ -236,7 +241,7 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
   if (!page_width(D)) return fail("head_dim must be in [1, 128], got " + std::to_string(D));
   if (!paged_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D))
     return fail("lucid_decode_paged: B, Hq, Hkv, L, page_size and max_pages positive, Hq a multiple of Hkv, at most 2^30 "
-                "rows a sequence and 2^23 kv heads in the batch");
+                "rows a sequence, 2^38 in the tables together and 2^23 kv heads in the batch");
   if (num_pages < 1) return fail("lucid_decode_paged: the pools have no pages");
   if (!q || !q_strides || !k || !k_strides || !v || !v_strides || !o || !o_strides || !vp_new || !page_table ||
       !cache_lens || !ws)
@@ -249,7 +254,7 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
   const int W = page_width(D);
   if (int rc = check_pool("k_pages", k_pages, k_page_strides, num_pages, Hkv, page_size, W, &c.kp)) return rc;
   if (int rc = check_pool("vp_pages", vp_pages, vp_page_strides, num_pages, Hkv, page_size, W, &c.vp)) return rc;
-  c.seq = lucid::PagedBatch{page_table, table_stride, cache_lens, B, max_pages, num_pages, page_size, L, 0};
+  c.seq = lucid::PagedBatch{page_table, table_stride, cache_lens, B, max_pages, num_pages, page_size, page_shift(page_size), L, 0};
   switch (W) {
     case 64: return paged_decode<64>(c);
     case 80: return paged_decode<80>(c);
@@ -277,7 +282,7 @@ int lucid_write_pages(const void* k, const int64_t* k_strides, const void* vprim
   lucid::PagedPool kp, vp;
   if (int rc = check_pool("k_pages", k_pages, k_page_strides, num_pages, Hkv, page_size, W, &kp)) return rc;
   if (int rc = check_pool("vp_pages", vp_pages, vp_page_strides, num_pages, Hkv, page_size, W, &vp)) return rc;
-  const lucid::PagedBatch seq{page_table, table_stride, cache_lens, B, max_pages, num_pages, page_size, 0, 0};
+  const lucid::PagedBatch seq{page_table, table_stride, cache_lens, B, max_pages, num_pages, page_size, page_shift(page_size), 0, 0};
   auto* run = W == 64 ? write_pages<64> : W == 80 ? write_pages<80> : W == 96 ? write_pages<96> : write_pages<128>;
   return run(k, k_strides, vprime, vprime_strides, vprime_f32 != 0, kp, vp, seq, new_lens, Hkv, T, D,
              static_cast<hipStream_t>(stream));
