@@ -242,4 +242,6 @@ def on(device: torch.device):
 
 
 def stream_handle(device: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    # the raw handle, without a Stream object around it (0.3 of 1.9 us a call)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))

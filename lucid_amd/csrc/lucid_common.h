@@ -10,6 +10,53 @@ struct Strides {
   int64_t b, h, t;
 };
 
+// Reductions over 8, 16, 32 or 64 adjacent lanes and a prefix sum over the wave in the VALU (DPP and row
+// swaps; a ds_bpermute of __shfl_xor costs an LDS round trip a step).  Every lane of a group gets the result;
+// op is commutative, and where it rounds, lanes may differ in the last bit.
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E;           // quad_perm [1,0,3,2] and [2,3,0,1]
+constexpr int kDppMirror8 = 0x141, kDppMirror16 = 0x140;  // the mirrored lane of each 8 and 16
+template <int N, typename OP>
+__device__ __forceinline__ float lanes_reduce(float v, OP op) {
+  static_assert(N == 4 || N == 8 || N == 16 || N == 32 || N == 64, "lanes of a group");
+  v = op(v, dpp_f32<kDppXor1>(v));
+  v = op(v, dpp_f32<kDppXor2>(v));
+  if constexpr (N >= 8) v = op(v, dpp_f32<kDppMirror8>(v));
+  if constexpr (N >= 16) v = op(v, dpp_f32<kDppMirror16>(v));
+  if constexpr (N >= 32) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);  // rows 0,0,2,2 and 1,1,3,3
+    v = op(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+  }
+  if constexpr (N >= 64) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    v = op(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+  }
+  return v;
+}
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return lanes_reduce<N>(v, [](float a, float b) { return a + b; });
+}
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
+  return lanes_reduce<N>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+// v of this lane and of those before it
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the row before's sum to rows 1 and 3,
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the first half's to rows 2 and 3
+  return v;
+}
+
 // Precision of the preconditioner chains, chosen per head.  The off-diagonal products
 // P_ij V'_j (forward), P_ij dV_i (transposed solve) and the M = (dV V'^T) * P sums of the
 // backward accumulate over every earlier (later) key of a row, and with bf16 operands

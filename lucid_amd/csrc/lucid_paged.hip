@@ -51,12 +51,6 @@ __device__ __forceinline__ int paged_rows(const PagedBatch& s, int b) {
   return (int64_t)n + s.L > (int64_t)s.M * s.page ? -2 : n + s.done;
 }
 
-__device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
 // The sequences' rows stand in one line, each sequence rounded up to units of kPagedUnit rows and led by
 // kPagedLead units without rows, and workgroup s of a kv head takes the places [s per, (s + 1) per): equal
 // shares whatever the lengths are, with no tail of workgroups that start late (32 sequences of 8192 rows cut
@@ -66,58 +60,57 @@ __device__ __forceinline__ int wave_sum_int(int v) {
 // s + b only grows, so the slots are distinct, at most target + B - 1.  Every wave works the line out from the
 // lengths, 64 sequences at a time (the first 64 are read once and stay in registers).
 struct PagedLine {
-  int n0;     // rows of sequence lane (of the first 64; at least 0)
-  int total;  // places (their number fits: the host's check)
-  int per;    // places of a share
+  int n0, end0;  // rows of sequence lane (of the first 64; at least 0), and the place behind it
+  int total;     // places (their number fits: the host's check)
+  int per;       // places of a share
   static __device__ __forceinline__ int places(int rows) {
     return rows > 0 ? (rows + kPagedUnit - 1) / kPagedUnit + kPagedLead : 0;
   }
   __device__ __forceinline__ PagedLine(const PagedBatch& s, int target) {
     const int lane = threadIdx.x & 63;
     n0 = lane < s.B ? max(paged_rows(s, lane), 0) : 0;
-    int u = places(n0);
-    for (int b = 64 + lane; b < s.B; b += 64) u += places(max(paged_rows(s, b), 0));
-    total = wave_sum_int(u);
+    end0 = wave_scan(places(n0));
+    total = __builtin_amdgcn_readlane(end0, 63);
+    for (int b0 = 64; b0 < s.B; b0 += 64)
+      total += __builtin_amdgcn_readlane(wave_scan(places(rows(s, b0 + lane))), 63);
     per = max(1, (total + target - 1) / target);
   }
-  __device__ __forceinline__ int rows(const PagedBatch& s, int b) const {
-    return b < 64 ? n0 : b < s.B ? max(paged_rows(s, b), 0) : 0;  // b = lane + a multiple of 64
+  __device__ __forceinline__ int rows(const PagedBatch& s, int b) const {  // b = lane + a multiple of 64
+    return b < 64 ? n0 : b < s.B ? max(paged_rows(s, b), 0) : 0;
+  }
+  // the places behind the sequences of a group of 64 (base: those of the groups before)
+  __device__ __forceinline__ int ends(const PagedBatch& s, int b0, int base, int n) const {
+    return b0 == 0 ? end0 : base + wave_scan(places(n));
   }
   // the shares that hold parts of sequence b: the slot of the first, and how many
   __device__ __forceinline__ void parts(const PagedBatch& s, int b, int& slot, int& n) const {
     const int lane = threadIdx.x & 63;
-    int sum = 0, own = 0;
-    for (int i = lane; i <= b; i += 64) {
-      const int u = places(rows(s, i));
-      sum += i < b ? u : 0;
-      own = i == b ? u : own;
+    int base = 0, end = end0, r = n0;
+    for (int b0 = 0; b0 <= b; b0 += 64) {
+      if (b0) base = __builtin_amdgcn_readlane(end, 63);
+      r = rows(s, b0 + lane);
+      end = ends(s, b0, base, r);
     }
-    const int before = wave_sum_int(sum), u = __shfl(own, b & 63, 64);
-    const int first = (before + kPagedLead) / per;  // the share of its first row
+    const int u = places(__builtin_amdgcn_readlane(r, b & 63)), after = __builtin_amdgcn_readlane(end, b & 63);
+    const int first = (after - u + kPagedLead) / per;  // the share of its first row
     slot = first + b;
-    n = u == 0 ? 0 : (before + u - 1) / per - first + 1;
+    n = u == 0 ? 0 : (after - 1) / per - first + 1;
   }
   // the sequence at a place: its rows n and the place of its first row
   __device__ __forceinline__ void find(const PagedBatch& s, int place, int& b, int& n, int& first) const {
     const int lane = threadIdx.x & 63;
     int base = 0;
-    for (int c0 = 0; c0 < s.B; c0 += 64) {
-      const int r = rows(s, c0 + lane), own = places(r);
-      int incl = own;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += x;
-      }
-      const unsigned long long at = __ballot(place < base + incl);
+    for (int b0 = 0; b0 < s.B; b0 += 64) {
+      const int r = rows(s, b0 + lane), end = ends(s, b0, base, r);
+      const unsigned long long at = __ballot(place < end);
       if (at) {
         const int l = __builtin_amdgcn_readfirstlane(__ffsll(at) - 1);
-        b = c0 + l;
-        first = base + __builtin_amdgcn_readlane(incl - own, l) + kPagedLead;
+        b = b0 + l;
         n = __builtin_amdgcn_readlane(r, l);
+        first = __builtin_amdgcn_readlane(end, l) - places(n) + kPagedLead;
         return;
       }
-      base += __builtin_amdgcn_readlane(incl, 63);
+      base = __builtin_amdgcn_readlane(end, 63);
     }
   }
 };
@@ -430,11 +423,11 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
   }
 }
 
-// Threads of the combine kernel: W / 4 groups of 4 columns, each on NSL lanes that take a chunk in
-// turn
+// Threads of the combine kernel: W / 4 groups of 4 columns, each on NSL lanes that take a part in turn; whole
+// waves (the line of sequences is worked out by all 64 lanes of each)
 template <int W>
 constexpr int paged_nsl() {
-  return W == 64 ? 16 : 8;
+  return W <= 80 ? 16 : 8;
 }
 
 // Grid (B Hkv, Gs): workgroup (sequence, kv head, query head g0 + g), for the Lp <= LM tokens of the
@@ -449,6 +442,7 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
     float* __restrict__ vp_new, int Hkv, int Lp, float scale, float eps, int d, PagedPartials part, int Gs, int Gt,
     int g0, int append) {
   constexpr int CG = W / 4, NSL = paged_nsl<W>(), NT = CG * NSL;
+  static_assert(NT % 64 == 0, "whole waves");
   constexpr int UN = LM == 1 ? 4 : LM == 4 ? 2 : 1;  // chunks whose loads a lane has in flight
   __shared__ float kk[LM][LM], qk[LM][LM];  // k_t . k_u and q_tg . k_u (u <= t)
   __shared__ __attribute__((aligned(16))) float ovs[LM][W], avs[LM][W], vps[LM][W];
@@ -518,11 +512,8 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
         dkk[p] = fmaf((float)kt[p][e], (float)ku[p][e], dkk[p]);
         dqk[p] = fmaf((float)qt[p][e], (float)ku[p][e], dqk[p]);
       }
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        dkk[p] += __shfl_xor(dkk[p], off, 64);
-        dqk[p] += __shfl_xor(dqk[p], off, 64);
-      }
+      dkk[p] = lanes_sum<32>(dkk[p]);
+      dqk[p] = lanes_sum<32>(dqk[p]);
       if ((tid & 31) == 0) {
         kk[ts[p]][us[p]] = dkk[p];
         qk[ts[p]][us[p]] = dqk[p];
@@ -579,20 +570,16 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
     }
   }
   if (bad) atomicOr(&bads, 1);
+  // the NSL lanes of a column group: their common maximum first, then plain sums
 #pragma unroll
-  for (int off = 1; off < NSL; off <<= 1) {
+  for (int t = 0; t < LM; ++t) {
+    const float mn = lanes_max<NSL>(M[t]), c = __builtin_amdgcn_exp2f(M[t] - mn);
+    M[t] = mn;
+    lv[t] = lanes_sum<NSL>(lv[t] * c);
 #pragma unroll
-    for (int t = 0; t < LM; ++t) {
-      const float mo = __shfl_xor(M[t], off, 64), lo = __shfl_xor(lv[t], off, 64);
-      const float mn = fmaxf(M[t], mo);
-      const float c = __builtin_amdgcn_exp2f(M[t] - mn), co = __builtin_amdgcn_exp2f(mo - mn);
-      lv[t] = fmaf(lv[t], c, lo * co);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        ov[t][x] = fmaf(ov[t][x], c, __shfl_xor(ov[t][x], off, 64) * co);
-        av[t][x] += __shfl_xor(av[t][x], off, 64);
-      }
-      M[t] = mn;
+    for (int x = 0; x < 4; ++x) {
+      ov[t][x] = lanes_sum<NSL>(ov[t][x] * c);
+      av[t][x] = lanes_sum<NSL>(av[t][x]);
     }
   }
   if (sl == 0) {

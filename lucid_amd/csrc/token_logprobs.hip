@@ -83,16 +83,6 @@ __device__ __forceinline__ float lp_value(unsigned long long key) {
   return __builtin_bit_cast(float, u == 0xffffffffu ? 0x7fc00000u : (u >> 31) ? u & 0x7fffffffu : ~u);
 }
 
-__device__ __forceinline__ float lp_wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-__device__ __forceinline__ float lp_wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 __device__ __forceinline__ unsigned long long lp_wave_max(unsigned long long v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
@@ -161,11 +151,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
   for (int c = 0; c < kLpChunks; ++c)
 #pragma unroll
     for (int e = 0; e < kLpChunk; ++e) m = fmaxf(m, (float)x[c][e]);
-#pragma unroll
-  for (int o = 1; o < GL; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  m = lanes_max<GL>(m);
   if (TOP && tid % GL == 0) gmax[tid / GL] = m;
-#pragma unroll
-  for (int o = GL; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  m = lanes_max<64>(m);
   if (lane == 0) red[0][w] = m;
   if (TOP && tid < 2) found[tid] = 0;
   __syncthreads();
@@ -195,8 +183,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
       t = fmaf(p, fmaxf(a, kLpNone), t);  // p = 0 where a = -inf
     }
   }
-  s = lp_wave_sum(s);
-  t = lp_wave_sum(t);
+  s = lanes_sum<64>(s);
+  t = lanes_sum<64>(t);
   if (lane == 0) {
     red[1][w] = s;
     red[2][w] = t;
@@ -318,7 +306,7 @@ __global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T
   if (tid < 64) {
     const bool on = lane < segs;
     const float mi = on ? out.pm[at + lane] : -INFINITY;
-    const float m = lp_wave_max(mi);
+    const float m = lanes_max<64>(mi);
     float f = 0.f, d = 0.f;
     if (on && mi != -INFINITY) {  // (a segment of -inf alone has the sums 0; NaN sums have to go through)
       d = (mi - m) * c2;
@@ -326,8 +314,8 @@ __global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T
     }
     const float si = on ? out.ps[at + lane] : 0.f, ti = on ? out.pt[at + lane] : 0.f;
     const bool gone = !on || (mi == -INFINITY && si == 0.f);
-    const float s = lp_wave_sum(gone ? (m == -INFINITY && lane == 0 ? __builtin_nanf("") : 0.f) : mi == -INFINITY ? si : si * f);
-    const float t = lp_wave_sum(gone ? 0.f : mi == -INFINITY ? ti : f * fmaf(si, fmaxf(d, kLpNone), ti));
+    const float s = lanes_sum<64>(gone ? (m == -INFINITY && lane == 0 ? __builtin_nanf("") : 0.f) : mi == -INFINITY ? si : si * f);
+    const float t = lanes_sum<64>(gone ? 0.f : mi == -INFINITY ? ti : f * fmaf(si, fmaxf(d, kLpNone), ti));
     if (lane == 0) {
       const int64_t tok = tokens[r];
       const T* row = lp_row(logits, sb, st, Tn, r);

@@ -15,6 +15,7 @@ columns that holds the head dim, columns from d on zero.  Row j of sequence b is
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 from typing import Sequence
@@ -32,12 +33,26 @@ def page_width(d: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def _i64x3(a: int, b: int, c: int):
-    """Three element strides as the C entry points take them (they only read the array)."""
-    return (ctypes.c_int64 * 3)(a, b, c)
+def _strides(stride: tuple):
+    """The first three of a tensor's strides as the C entry points take them (they only read the array)."""
+    return (ctypes.c_int64 * 3)(*stride[:3])
 
 
-def _check_pools(what, key_pages, vprime_pages, Hkv, d, device):
+def _pools_ok(key_pages, vprime_pages, Hkv, W, device) -> bool:
+    P, H, page, w = key_pages.shape
+    a, b, c, e = s = key_pages.stride()
+    if vprime_pages.stride() != s:
+        x, y, z, f = vprime_pages.stride()
+        a, b, c, e = a | x, b | y, c | z, e if f == 1 else 0
+    return (H == Hkv and w == W and page > 0 and e == 1 and not (a | b | c) & 7
+            and not (key_pages.data_ptr() | vprime_pages.data_ptr()) & 15 and vprime_pages.shape == key_pages.shape
+            and key_pages.dtype is torch.bfloat16 and vprime_pages.dtype is torch.bfloat16
+            and key_pages.device == device and vprime_pages.device == device)
+
+
+def _refuse(what, device, dims, key_pages, vprime_pages, page_table, lens):
+    """Says what is wrong with the pools, the table or the lengths of a call."""
+    B, Hkv, d = dims
     W = page_width(d)
     for name, t in (("key_pages", key_pages), ("vprime_pages", vprime_pages)):
         if t.dtype != torch.bfloat16 or t.dim() != 4 or t.device != device:
@@ -51,15 +66,19 @@ def _check_pools(what, key_pages, vprime_pages, Hkv, d, device):
     if key_pages.shape != vprime_pages.shape:
         raise ValueError(f"lucid_amd.{what}: key_pages {tuple(key_pages.shape)} and vprime_pages "
                          f"{tuple(vprime_pages.shape)} must match")
-
-
-def _check_table(what, page_table, lens, B, device):
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.device != device or \
-            page_table.shape[0] != B or page_table.shape[1] < 1 or page_table.stride(1) != 1:
-        raise ValueError(f"lucid_amd.{what}: page_table must be int32 [{B}, max_pages] on {device}, rows contiguous")
     for name, t in lens:
         if t.dtype != torch.int32 or t.shape != (B,) or t.device != device or not t.is_contiguous():
             raise ValueError(f"lucid_amd.{what}: {name} must be contiguous int32 [{B}] on {device}")
+    raise ValueError(f"lucid_amd.{what}: page_table must be int32 [{B}, max_pages] on {device}, rows contiguous")
+
+
+def _table_ok(page_table, B, device) -> bool:
+    return (page_table.dtype is torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B
+            and page_table.shape[1] > 0 and page_table.stride(1) == 1 and page_table.device == device)
+
+
+def _lens_ok(t, B, device) -> bool:
+    return t.dtype is torch.int32 and t.shape == (B,) and t.is_contiguous() and t.device == device
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -86,17 +105,21 @@ def lucid_decode_paged(query, key, value, key_pages, vprime_pages, page_table, c
     device = query.device
     if not query.is_cuda:
         raise RuntimeError("lucid_amd: query must be a GPU tensor (no CPU path)")
-    for name, t in (("query", query), ("key", key), ("value", value)):
-        if t.dtype != torch.bfloat16 or t.dim() != 4 or t.device != device:
-            raise TypeError(f"lucid_amd.lucid_decode_paged: {name} must be a 4-D bfloat16 tensor on {device}")
+    bf = torch.bfloat16
+    if not (query.dtype is key.dtype is value.dtype is bf and query.dim() == key.dim() == 4 and key.device == device
+            and value.device == device):
+        raise TypeError(f"lucid_amd.lucid_decode_paged: query, key and value must be 4-D bfloat16 tensors on {device}")
     B, Hkv, L, d = key.shape
     Hq = query.shape[1]
     if value.shape != key.shape or query.shape != (B, Hq, L, d) or Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError("lucid_amd.lucid_decode_paged: query [B, Hq, L, d], key and value [B, Hkv, L, d] disagree")
-    _check_pools("lucid_decode_paged", key_pages, vprime_pages, Hkv, d, device)
-    _check_table("lucid_decode_paged", page_table, (("cache_lens", cache_lens),), B, device)
-    o = torch.empty(B, L, Hq, d, dtype=torch.bfloat16, device=device)
-    vp_new = torch.empty(B, Hkv, L, d, dtype=torch.float32, device=device)
+    if not (key_pages.dim() == 4 and vprime_pages.dim() == 4
+            and _pools_ok(key_pages, vprime_pages, Hkv, page_width(d), device)
+            and _table_ok(page_table, B, device) and _lens_ok(cache_lens, B, device)):
+        _refuse("lucid_decode_paged", device, (B, Hkv, d), key_pages, vprime_pages, page_table,
+                (("cache_lens", cache_lens),))
+    o = torch.empty((B, L, Hq, d), dtype=bf, device=device)
+    vp_new = torch.empty((B, Hkv, L, d), dtype=torch.float32, device=device)
     if B == 0 or L == 0:
         return o, vp_new
     lib = _lib.load()
@@ -107,10 +130,10 @@ def lucid_decode_paged(query, key, value, key_pages, vprime_pages, page_table, c
     q, k, v = _rows(query), _rows(key), _rows(value)
     with _lib.on(device):
         rc = lib.lucid_decode_paged(
-            q.data_ptr(), _i64x3(*q.stride()[:3]), k.data_ptr(), _i64x3(*k.stride()[:3]), v.data_ptr(),
-            _i64x3(*v.stride()[:3]), key_pages.data_ptr(), _i64x3(*key_pages.stride()[:3]), vprime_pages.data_ptr(),
-            _i64x3(*vprime_pages.stride()[:3]), page_table.data_ptr(), page_table.stride(0), cache_lens.data_ptr(),
-            o.data_ptr(), _i64x3(L * Hq * d, d, Hq * d), vp_new.data_ptr(), ws.data_ptr(), B, Hq, Hkv, L, P, page, M, d,
+            q.data_ptr(), _strides(q.stride()), k.data_ptr(), _strides(k.stride()), v.data_ptr(), _strides(v.stride()),
+            key_pages.data_ptr(), _strides(key_pages.stride()), vprime_pages.data_ptr(), _strides(vprime_pages.stride()),
+            page_table.data_ptr(), page_table.stride(0), cache_lens.data_ptr(), o.data_ptr(),
+            _strides((L * Hq * d, d, Hq * d)), vp_new.data_ptr(), ws.data_ptr(), B, Hq, Hkv, L, P, page, M, d,
             d ** -0.5 if scaling is None else float(scaling), float(eps), _lib.stream_handle(device))
     _lib.check(lib, rc, "lucid_decode_paged")
     return o, vp_new
@@ -131,17 +154,20 @@ def write_pages(key, v_prime, key_pages, vprime_pages, page_table, cache_lens, n
     if v_prime.dtype not in (torch.bfloat16, torch.float32) or v_prime.shape != key.shape or v_prime.device != device:
         raise ValueError("lucid_amd.write_pages: v_prime must be a bf16 or fp32 tensor shaped like key, on its device")
     B, Hkv, T, d = key.shape
-    _check_pools("write_pages", key_pages, vprime_pages, Hkv, d, device)
-    lens = (("cache_lens", cache_lens),) if new_lens is None else (("cache_lens", cache_lens), ("new_lens", new_lens))
-    _check_table("write_pages", page_table, lens, B, device)
+    if not (key_pages.dim() == 4 and vprime_pages.dim() == 4
+            and _pools_ok(key_pages, vprime_pages, Hkv, page_width(d), device)
+            and _table_ok(page_table, B, device) and _lens_ok(cache_lens, B, device)
+            and (new_lens is None or _lens_ok(new_lens, B, device))):
+        lens = (("cache_lens", cache_lens),) if new_lens is None else (("cache_lens", cache_lens), ("new_lens", new_lens))
+        _refuse("write_pages", device, (B, Hkv, d), key_pages, vprime_pages, page_table, lens)
     lib = _lib.load()
     P, _, page, _ = key_pages.shape
     k, v = _rows(key), _rows(v_prime)
     with _lib.on(device):
         rc = lib.lucid_write_pages(
-            k.data_ptr(), _i64x3(*k.stride()[:3]), v.data_ptr(), _i64x3(*v.stride()[:3]), int(v.dtype == torch.float32),
-            key_pages.data_ptr(), _i64x3(*key_pages.stride()[:3]), vprime_pages.data_ptr(),
-            _i64x3(*vprime_pages.stride()[:3]), page_table.data_ptr(), page_table.stride(0), cache_lens.data_ptr(),
+            k.data_ptr(), _strides(k.stride()), v.data_ptr(), _strides(v.stride()), int(v.dtype == torch.float32),
+            key_pages.data_ptr(), _strides(key_pages.stride()), vprime_pages.data_ptr(),
+            _strides(vprime_pages.stride()), page_table.data_ptr(), page_table.stride(0), cache_lens.data_ptr(),
             None if new_lens is None else new_lens.data_ptr(), B, Hkv, T, P, page, page_table.shape[1], d,
             _lib.stream_handle(device))
     _lib.check(lib, rc, "lucid_write_pages")
@@ -161,18 +187,25 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
     device, shape, stride = first.device, first.shape, first.stride()
     if not first.is_cuda:
         raise RuntimeError("lucid_amd: pools must be GPU tensors (no CPU path)")
-    for t in pools:
-        if t.shape != shape or t.stride() != stride or t.dtype != first.dtype or t.device != device:
-            raise ValueError("lucid_amd.copy_pages: pools must share shape, strides, dtype and device")
+    n, m = len(pools), len(src)
+    tensor = torch.Tensor
+    # (whole lists at a time: this is most of a small call's time)
+    if (n > 1 and (list(map(tensor.size, pools)) != [shape] * n or list(map(tensor.stride, pools)) != [stride] * n
+                   or list(map(tensor.get_device, pools)) != [device.index] * n
+                   or any(t.dtype is not first.dtype for t in pools))):
+        raise ValueError("lucid_amd.copy_pages: pools must share shape, strides, dtype and device")
     if first.dim() < 1 or (shape[0] > 0 and not first[0].is_contiguous()):
         raise ValueError("lucid_amd.copy_pages: a page must be contiguous")
     size = first.element_size()
     page_bytes = size * (first.numel() // shape[0] if shape[0] else 0)
+    try:
+        s, t = array.array("i", src), array.array("i", dst)
+    except OverflowError:
+        raise ValueError("lucid_amd.copy_pages: page outside the pool") from None
     lib = _lib.load()
-    n, m = len(pools), len(src)
     with _lib.on(device):
-        rc = lib.lucid_copy_pages(n, (ctypes.c_void_p * n)(*(t.data_ptr() for t in pools)),
+        rc = lib.lucid_copy_pages(n, (ctypes.c_void_p * n)(*map(tensor.data_ptr, pools)),
                                   max(stride[0] * size, page_bytes) if shape[0] < 2 else stride[0] * size, page_bytes,
-                                  shape[0], m, (ctypes.c_int * m)(*src), (ctypes.c_int * m)(*dst),
+                                  shape[0], m, (ctypes.c_int * m).from_buffer(s), (ctypes.c_int * m).from_buffer(t),
                                   _lib.stream_handle(device))
     _lib.check(lib, rc, "lucid_copy_pages")

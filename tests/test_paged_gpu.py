@@ -189,6 +189,8 @@ def test_many_sequences_of_uneven_lengths():
     lens[149] = 700
     _go(_case(lens, 4, 2, 1, 64, 16, seed=2), 16)
     _go(_case(lens[60:90], 8, 2, 3, 128, 32, seed=3), 32)
+    for d in (68, 96, 128):  # each row width's own number of lanes
+        _go(_case(lens[:100], 2, 1, 2, d, 16, seed=d), 16)
 
 
 def test_sharp_softmax_shared_keys_and_other_scales():
