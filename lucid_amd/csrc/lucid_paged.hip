@@ -423,35 +423,40 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
   }
 }
 
-// Threads of the combine kernel: W / 4 groups of 4 columns, each on NSL lanes that take a part in turn; whole
-// waves (the line of sequences is worked out by all 64 lanes of each)
-template <int W>
-constexpr int paged_nsl() {
-  return W <= 80 ? 16 : 8;
+// The combine kernel's workgroup: CGP lanes (W / 4 of them, 4 columns each) for every token and slice of
+// the parts.
+template <int LM>
+constexpr int paged_threads() {
+  return LM == 1 ? 256 : 512;
 }
 
 // Grid (B Hkv, Gs): workgroup (sequence, kv head, query head g0 + g), for the Lp <= LM tokens of the
-// pass.  Merges the chunks of each token, solves the new tokens in order (a column group needs only
-// its own columns), writes the outputs; the g = 0 workgroups of the first group of query heads append
-// (k_t, v'_t).  A slot without a sequence gets zeros; one whose table names a page outside the
-// pool, or that has no room for the new rows, gets NaN, and nothing is appended to it.
+// pass.  Merges the parts of each token (a slice of them per lane group, the slices through LDS), solves the new
+// tokens in order (a column group needs only its own columns), writes the outputs; the g = 0 workgroups of
+// the first group of query heads append (k_t, v'_t).  A slot without a sequence gets zeros; one whose table
+// names a page outside the pool, or that has no room for the new rows, gets NaN, and nothing is appended to
+// it.  What bounds it is the chain of dependent loads (lengths, partials) and three barriers: 6 us at
+// one token, 9 at five; with every lane holding all tokens of its columns the reductions over lanes
+// alone took 4 of 19.
 template <int W, int LM>
-__global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_kernel(
+__global__ __launch_bounds__(paged_threads<LM>()) void lucid_paged_combine_kernel(
     const bf16* __restrict__ q, Strides qs, const bf16* __restrict__ kn, Strides kns, const bf16* __restrict__ vn,
     Strides vns, int vec, int ovec, PagedPool kp, PagedPool vp, PagedBatch seq, int target, bf16* __restrict__ o, Strides os,
     float* __restrict__ vp_new, int Hkv, int Lp, float scale, float eps, int d, PagedPartials part, int Gs, int Gt,
     int g0, int append) {
-  constexpr int CG = W / 4, NSL = paged_nsl<W>(), NT = CG * NSL;
-  static_assert(NT % 64 == 0, "whole waves");
-  constexpr int UN = LM == 1 ? 4 : LM == 4 ? 2 : 1;  // chunks whose loads a lane has in flight
+  constexpr int CG = W / 4, CGP = W == 64 ? 16 : 32, NT = paged_threads<LM>(), NG = NT / CGP, SL = NG / LM;
+  static_assert(SL >= 1, "a lane group for every token");
+  constexpr int UN = 4;  // parts whose loads a lane has in flight
   __shared__ float kk[LM][LM], qk[LM][LM];  // k_t . k_u and q_tg . k_u (u <= t)
-  __shared__ __attribute__((aligned(16))) float ovs[LM][W], avs[LM][W], vps[LM][W];
-  __shared__ float ms_[LM], ls_[LM];
+  __shared__ float pp[LM][LM], ww[LM][LM];  // P_tu (1 / P_tt), and u's weight in token t's softmax
+  __shared__ f32x4 os_[NG][CGP], as_[NG][CGP], vps[LM][CGP];
+  __shared__ float ms_[NG], ls_[NG], top_[LM];
   __shared__ unsigned krow[LM], vrow[LM];
   __shared__ int bads;
   const int bh = blockIdx.x, g = blockIdx.y;
   const int b = bh / Hkv, h = bh - b * Hkv;
-  const int tid = threadIdx.x, cg = tid / NSL, sl = tid - cg * NSL, d0 = 4 * cg;
+  const int tid = threadIdx.x, grp = tid / CGP, cg = tid % CGP, d0 = 4 * cg;
+  const int t = grp % LM, slice = grp / LM;
   const int hq = h * Gt + g0 + g;
   const PagedLine line(seq, target);
   const int rows = paged_rows(seq, b);
@@ -469,223 +474,202 @@ __global__ __launch_bounds__(W / 4 * paged_nsl<W>()) void lucid_paged_combine_ke
     }
     return;
   }
-  int base, nchunk;
-  line.parts(seq, b, base, nchunk);
+  int base, nparts;
+  line.parts(seq, b, base, nparts);
   if (tid == 0) bads = 0;
   __syncthreads();
   // the pages that the call's new rows go to
-  for (int t = tid; t < seq.L; t += NT) {
-    const int j = rows - seq.done + t, pg = page_of(seq, j);
+  for (int i = tid; i < seq.L; i += NT) {
+    const int j = rows - seq.done + i, pg = page_of(seq, j);
     const int id = seq.table[b * seq.tstride + pg];
     if ((unsigned)id >= (unsigned)seq.P) atomicOr(&bads, 1);
-    const int u = t - seq.done;
+    const int u = i - seq.done;
     if (u >= 0 && u < Lp) {
       const unsigned in = j - pg * seq.page;
       krow[u] = id * kp.page + h * kp.head + in * kp.row;
       vrow[u] = id * vp.page + h * vp.head + in * vp.row;
     }
   }
+  bf16x4 vrows[LM];  // the new tokens' value rows, for the lanes that solve
+  if (grp == 0) {
+#pragma unroll
+    for (int i = 0; i < LM; ++i)
+      if (i < Lp) vrows[i] = ld4_cols(vb + i * vns.t, d0, d, vec);
+  }
   // dot products among the new tokens (t, u <= t), 32 lanes a pair, four columns a lane
   const int npair = Lp * (Lp + 1) / 2;
-  constexpr int PU = LM == 1 ? 1 : LM == 4 ? 2 : 4;
+  auto pair = [&](int i, int& x, int& y) {  // i = x (x + 1) / 2 + y
+    x = (int)((sqrtf(8.f * i + 1.f) - 1.f) * 0.5f);
+    if ((x + 1) * (x + 2) / 2 <= i) ++x;
+    if (x * (x + 1) / 2 > i) --x;
+    y = i - x * (x + 1) / 2;
+  };
+  constexpr int PU = LM <= 4 ? 1 : LM == 8 ? 2 : 4;
   for (int i0 = tid / 32; i0 < npair; i0 += PU * (NT / 32)) {
-    float dkk[PU], dqk[PU];
     int ts[PU], us[PU];
     bf16x4 kt[PU], ku[PU], qt[PU];
 #pragma unroll
     for (int p = 0; p < PU; ++p) {
-      const int i = min(i0 + p * (NT / 32), npair - 1);
-      int t = (int)((sqrtf(8.f * i + 1.f) - 1.f) * 0.5f);
-      if ((t + 1) * (t + 2) / 2 <= i) ++t;
-      if (t * (t + 1) / 2 > i) --t;
-      ts[p] = t;
-      us[p] = i - t * (t + 1) / 2;
-      kt[p] = ld4_cols(kb + t * kns.t, 4 * (tid & 31), d, vec);
+      pair(min(i0 + p * (NT / 32), npair - 1), ts[p], us[p]);
+      kt[p] = ld4_cols(kb + ts[p] * kns.t, 4 * (tid & 31), d, vec);
       ku[p] = ld4_cols(kb + us[p] * kns.t, 4 * (tid & 31), d, vec);
-      qt[p] = ld4_cols(qb + t * qs.t, 4 * (tid & 31), d, vec);
+      qt[p] = ld4_cols(qb + ts[p] * qs.t, 4 * (tid & 31), d, vec);
     }
 #pragma unroll
     for (int p = 0; p < PU; ++p) {
-      dkk[p] = dqk[p] = 0.f;
+      float dkk = 0.f, dqk = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        dkk[p] = fmaf((float)kt[p][e], (float)ku[p][e], dkk[p]);
-        dqk[p] = fmaf((float)qt[p][e], (float)ku[p][e], dqk[p]);
+        dkk = fmaf((float)kt[p][e], (float)ku[p][e], dkk);
+        dqk = fmaf((float)qt[p][e], (float)ku[p][e], dqk);
       }
-      dkk[p] = lanes_sum<32>(dkk[p]);
-      dqk[p] = lanes_sum<32>(dqk[p]);
+      dkk = lanes_sum<32>(dkk);
+      dqk = lanes_sum<32>(dqk);
       if ((tid & 31) == 0) {
-        kk[ts[p]][us[p]] = dkk[p];
-        qk[ts[p]][us[p]] = dqk[p];
+        kk[ts[p]][us[p]] = dkk;
+        qk[ts[p]][us[p]] = dqk;
       }
     }
   }
-  bf16x4 vrows[LM];  // the new tokens' value rows, wanted after the merge
+  // this group's slice of the parts of its token: the key column and the query column (parts beyond the
+  // last: the last again, with the weight 0)
+  float M = PAGED_NEG, lv = 0.f;
+  f32x4 ov = {0.f, 0.f, 0.f, 0.f}, av = {0.f, 0.f, 0.f, 0.f};
+  if (t < Lp) {
+    const int dc = CG == CGP ? d0 : min(d0, W - 4);
+    bool bad = false;
+    for (int p0 = slice; p0 < nparts; p0 += UN * SL) {
+      float mi[UN], li[UN];
+      f32x4 oi[UN], ai[UN];
 #pragma unroll
-  for (int t = 0; t < LM; ++t) vrows[t] = ld4_cols(vb + min(t, Lp - 1) * vns.t, d0, d, vec);
-  // the chunks' partials of every token: its key column and its query column (tokens and chunks beyond
-  // the last read the last again, with the weight 0)
-  float M[LM], lv[LM];
-  f32x4 ov[LM], av[LM];
-  bool bad = false;
-#pragma unroll
-  for (int t = 0; t < LM; ++t) {
-    M[t] = PAGED_NEG;
-    lv[t] = 0.f;
-    ov[t] = av[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  for (int s0 = sl; s0 < nchunk; s0 += UN * NSL) {
-    float mi[UN][LM], li[UN][LM];
-    f32x4 oi[UN][LM], ai[UN][LM];
-#pragma unroll
-    for (int k = 0; k < UN; ++k) {
-      const int64_t at = (int64_t)(base + min(s0 + k * NSL, nchunk - 1)) * Hkv + h;
-#pragma unroll
-      for (int t = 0; t < LM; ++t) {
-        const int tt = min(t, Lp - 1);
-        const int64_t i = at * (Lp * Gs) + tt * Gs + g;
-        mi[k][t] = part.m[i];
-        li[k][t] = part.l[i];
-        oi[k][t] = *reinterpret_cast<const f32x4*>(part.o + i * W + d0);
-        ai[k][t] = *reinterpret_cast<const f32x4*>(part.a + (at * Lp + tt) * W + d0);
+      for (int k = 0; k < UN; ++k) {
+        const int64_t at = (int64_t)(base + min(p0 + k * SL, nparts - 1)) * Hkv + h;
+        const int64_t i = at * (Lp * Gs) + t * Gs + g;
+        mi[k] = part.m[i];
+        li[k] = part.l[i];
+        oi[k] = *reinterpret_cast<const f32x4*>(part.o + i * W + dc);
+        ai[k] = *reinterpret_cast<const f32x4*>(part.a + (at * Lp + t) * W + dc);
       }
-    }
 #pragma unroll
-    for (int k = 0; k < UN; ++k) {
-      const bool on = s0 + k * NSL < nchunk;
-#pragma unroll
-      for (int t = 0; t < LM; ++t) {
-        bad |= mi[k][t] != mi[k][t];
-        const float mn = on ? fmaxf(M[t], mi[k][t]) : M[t];
-        const float c = __builtin_amdgcn_exp2f(M[t] - mn), e = on ? __builtin_amdgcn_exp2f(mi[k][t] - mn) : 0.f;
+      for (int k = 0; k < UN; ++k) {
+        const bool on = p0 + k * SL < nparts;
+        bad |= mi[k] != mi[k];
+        const float mn = on ? fmaxf(M, mi[k]) : M;
+        const float c = __builtin_amdgcn_exp2f(M - mn), e = on ? __builtin_amdgcn_exp2f(mi[k] - mn) : 0.f;
         const float one = on ? 1.f : 0.f;
-        lv[t] = fmaf(lv[t], c, li[k][t] * e);
+        lv = fmaf(lv, c, li[k] * e);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          ov[t][x] = fmaf(ov[t][x], c, oi[k][t][x] * e);
-          av[t][x] = fmaf(ai[k][t][x], one, av[t][x]);
+          ov[x] = fmaf(ov[x], c, oi[k][x] * e);
+          av[x] = fmaf(ai[k][x], one, av[x]);
         }
-        M[t] = mn;
+        M = mn;
       }
     }
+    if (bad) atomicOr(&bads, 1);
   }
-  if (bad) atomicOr(&bads, 1);
-  // the NSL lanes of a column group: their common maximum first, then plain sums
-#pragma unroll
-  for (int t = 0; t < LM; ++t) {
-    const float mn = lanes_max<NSL>(M[t]), c = __builtin_amdgcn_exp2f(M[t] - mn);
-    M[t] = mn;
-    lv[t] = lanes_sum<NSL>(lv[t] * c);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      ov[t][x] = lanes_sum<NSL>(ov[t][x] * c);
-      av[t][x] = lanes_sum<NSL>(av[t][x]);
-    }
-  }
-  if (sl == 0) {
-#pragma unroll
-    for (int t = 0; t < LM; ++t) {
-      if (t < Lp) {
-        *reinterpret_cast<f32x4*>(&ovs[t][d0]) = ov[t];
-        *reinterpret_cast<f32x4*>(&avs[t][d0]) = av[t];
-        if (cg == 0) {
-          ms_[t] = M[t];
-          ls_[t] = lv[t];
-        }
-      }
-    }
+  os_[grp][cg] = ov;
+  as_[grp][cg] = av;
+  if (cg == 0) {
+    ms_[grp] = M;
+    ls_[grp] = lv;
   }
   __syncthreads();
   const bool poison = bads != 0;
-  // the new tokens among themselves, a pair (t, u <= t) a lane: P_tu (1 / P_tt on the diagonal) in place of k_t . k_u,
-  // the softmax weight of u beside token t's cached part in place of q_tg . k_u
   const float sl2 = scale * LOG2E_F, c0 = LOG2E_F / scale, dn = (float)d;
-  float pk[LM], pq[LM], weight = 0.f, sum = 0.f;
-  const int tt = tid;  // token of this lane
-  if (tt < Lp) {
-    const float rt = rsqrtf(kk[tt][tt] / dn + eps);
-    float M2 = ms_[tt];
+  // the largest score of a token: over the slices and the new keys
+  auto top_of = [&](int x) {
+    float m = ms_[x];
 #pragma unroll
-    for (int u = 0; u < LM; ++u)
-      if (u <= tt) M2 = fmaxf(M2, qk[tt][u] * sl2);
-    weight = __builtin_amdgcn_exp2f(ms_[tt] - M2);
-    sum = ls_[tt] * weight;
-#pragma unroll
-    for (int u = 0; u < LM; ++u) {
-      if (u <= tt) {
-        pk[u] = __builtin_amdgcn_exp2f(fmaf(sl2 * rt * rsqrtf(kk[u][u] / dn + eps), kk[tt][u], -c0));
-        pq[u] = __builtin_amdgcn_exp2f(fmaf(qk[tt][u], sl2, -M2));
-        sum += pq[u];
-      }
-    }
-    // 1 / P_tt; the exponent is the small difference of two terms of size sqrt(d): in fp64
-    const double ms = (double)kk[tt][tt] / d;
-    const float inv = __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / scale - scale * d * ms / (ms + eps))));
-#pragma unroll
-    for (int u = 0; u < LM; ++u)
-      if (u == tt) pk[u] = inv;
-  }
-  if constexpr (LM > 1) __syncthreads();  // every lane has read the dot products (one token: its own lane's)
-  if (tt < Lp) {
-#pragma unroll
-    for (int u = 0; u < LM; ++u) {
-      if (u <= tt) {
-        kk[tt][u] = pk[u];
-        qk[tt][u] = pq[u];
-      }
-    }
-    ms_[tt] = weight;
-    ls_[tt] = sum;
-  }
-  __syncthreads();
-  // the new rows in order (columns d0 .. d0+3): v'_t = (v_t - a_t - sum_{u<t} P_tu w_u) / P_tt
-#pragma unroll
-  for (int t = 0; t < LM; ++t) {
-    if (sl == 0 && t < Lp) {
-      const f32x4 a4 = *reinterpret_cast<const f32x4*>(&avs[t][d0]);
-      f32x4 x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = (float)vrows[t][j] - a4[j];
-      for (int u = 0; u < t; ++u) {
-        const float p = kk[t][u];
-        const f32x4 vu = *reinterpret_cast<const f32x4*>(&vps[u][d0]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = fmaf(-p, (float)(bf16)vu[j], x[j]);
-      }
-      const float inv = kk[t][t];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] *= inv;
-      *reinterpret_cast<f32x4*>(&vps[t][d0]) = x;
+    for (int s = 1; s < SL; ++s) m = fmaxf(m, ms_[x + s * LM]);
+    for (int u = 0; u <= x; ++u) m = fmaxf(m, qk[x][u] * sl2);
+    return m;
+  };
+  // the new tokens among themselves, a pair a lane
+  if (tid < npair) {
+    int x, u;
+    pair(tid, x, u);
+    const float m = top_of(x);
+    ww[x][u] = __builtin_amdgcn_exp2f(fmaf(qk[x][u], sl2, -m));
+    if (u < x) {
+      const float rx = rsqrtf(kk[x][x] / dn + eps), ru = rsqrtf(kk[u][u] / dn + eps);
+      pp[x][u] = __builtin_amdgcn_exp2f(fmaf(sl2 * rx * ru, kk[x][u], -c0));
+    } else {
+      // 1 / P_tt; the exponent is the small difference of two terms of size sqrt(d): in fp64
+      const double ms = (double)kk[x][x] / d;
+      pp[x][x] = __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / scale - scale * d * ms / (ms + eps))));
+      top_[x] = m;
     }
   }
   __syncthreads();
-  // outputs, a token per split lane: the cached part merged with the new keys u <= t
-  for (int t = sl; t < Lp; t += NSL) {
-    const float c = ms_[t], den = ls_[t];
-    const f32x4 o4 = *reinterpret_cast<const f32x4*>(&ovs[t][d0]);
-    f32x4 num;
+  // the slices of a token merged at its largest score; the sum with the new keys' weights
+  float den = 1.f;
+  if (slice == 0 && t < Lp) {
+    const float m = top_[t];
+    den = 0.f;
+    ov = av = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) num[j] = o4[j] * c;
+    for (int s = 0; s < SL; ++s) {
+      const float e = __builtin_amdgcn_exp2f(ms_[t + s * LM] - m);
+      den = fmaf(ls_[t + s * LM], e, den);
+      const f32x4 os4 = os_[t + s * LM][cg], as4 = as_[t + s * LM][cg];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        ov[x] = fmaf(os4[x], e, ov[x]);
+        av[x] += as4[x];
+      }
+    }
+    for (int u = 0; u <= t; ++u) den += ww[t][u];
+    as_[t][cg] = av;  // (read by this lane alone so far)
+  }
+  __syncthreads();
+  // the new rows in order (this lane's columns): v'_t = (v_t - a_t - sum_{u<t} P_tu w_u) / P_tt
+  if (grp == 0) {
+    f32x4 held[LM];
+#pragma unroll
+    for (int x = 0; x < LM; ++x) {
+      if (x < Lp) {
+        f32x4 v = as_[x][cg];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (float)vrows[x][j] - v[j];
+#pragma unroll
+        for (int u = 0; u < x; ++u) {
+          const float p = pp[x][u];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = fmaf(-p, held[u][j], v[j]);
+        }
+        const float inv = pp[x][x];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[j] *= inv;
+          held[x][j] = (float)(bf16)v[j];
+        }
+        vps[x][cg] = v;
+      }
+    }
+  }
+  __syncthreads();
+  if (slice == 0 && t < Lp && cg < CG) {
     for (int u = 0; u <= t; ++u) {
-      const float es = qk[t][u];
-      const f32x4 vu = *reinterpret_cast<const f32x4*>(&vps[u][d0]);
+      const float es = ww[t][u];
+      const f32x4 vu = vps[u][cg];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) num[j] = fmaf(es, (float)(bf16)vu[j], num[j]);
+      for (int j = 0; j < 4; ++j) ov[j] = fmaf(es, (float)(bf16)vu[j], ov[j]);
     }
     const float rden = poison ? __builtin_nanf("") : 1.f / den;
-    const f32x4 vt = *reinterpret_cast<const f32x4*>(&vps[t][d0]);
+    const f32x4 vt = vps[t][cg];
     if (d0 < d) {
       if (ovec) {
-        bf16x4 o4b;
+        bf16x4 o4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o4b[j] = (bf16)(num[j] * rden);
-        *reinterpret_cast<bf16x4*>(ob + t * os.t + d0) = o4b;
+        for (int j = 0; j < 4; ++j) o4[j] = (bf16)(ov[j] * rden);
+        *reinterpret_cast<bf16x4*>(ob + t * os.t + d0) = o4;
         if (write_v) *reinterpret_cast<f32x4*>(vo + t * d + d0) = poison ? f32x4{rden, rden, rden, rden} : vt;
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (d0 + j >= d) break;
-          ob[t * os.t + d0 + j] = (bf16)(num[j] * rden);
+          ob[t * os.t + d0 + j] = (bf16)(ov[j] * rden);
           if (write_v) vo[t * d + d0 + j] = poison ? rden : vt[j];
         }
       }

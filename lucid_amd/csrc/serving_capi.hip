@@ -94,7 +94,7 @@ int paged_combine(const PagedCall& c, int vec, const lucid::PagedBatch& seq, int
   // whole groups of 4 columns at 8-byte boundaries of o and 16-byte boundaries of vp_new
   const int ovec = c.D % 4 == 0 && rows_of_4(c.o, c.os, 2) && !misaligned16(c.vp_new);
   LUCID_LAUNCH_B("lucid_paged_combine_kernel", (lucid::lucid_paged_combine_kernel<W, LM>), dim3(seq.B * c.Hkv, gc),
-                 dim3(W / 4 * lucid::paged_nsl<W>()), c.st, (const bf16*)c.q, S(c.qs), (const bf16*)c.k, S(c.ks),
+                 dim3(lucid::paged_threads<LM>()), c.st, (const bf16*)c.q, S(c.qs), (const bf16*)c.k, S(c.ks),
                  (const bf16*)c.v, S(c.vs), vec, ovec, c.kp, c.vp, seq, target, (bf16*)c.o, S(c.os), c.vp_new, c.Hkv, Lp, c.scale,
                  c.eps, c.D, part, gc, c.Hq / c.Hkv, g0, g0 == 0 ? 1 : 0);
   return LUCID_OK;
