@@ -151,10 +151,10 @@ int write_pages(const void* k, const int64_t* ks, const void* v, const int64_t* 
 
 // Token log probabilities: workgroups of 256 lanes for rows of up to 8192 values (and what a
 // misaligned row's first chunk leaves out), else of 1024 on segments of 32768
-int lp_threads(int V) { return V + lucid::kLpChunk - 1 <= 256 * lucid::kLpChunks * lucid::kLpChunk ? 256 : 1024; }
+int lp_threads(int V) { return V + 7 <= 256 * lucid::kLpLane ? 256 : 1024; }
 int lp_segs(int V, bool aligned = false) {
-  const int seg = lp_threads(V) * lucid::kLpChunks * lucid::kLpChunk;
-  return (int)(((int64_t)V + (aligned ? 0 : lucid::kLpChunk - 1) + seg - 1) / seg);
+  const int seg = lp_threads(V) * lucid::kLpLane;
+  return (int)(((int64_t)V + (aligned ? 0 : 7) + seg - 1) / seg);
 }
 // whether every row starts at a 16-byte boundary (its first chunk is whole)
 bool lp_aligned(const void* logits, int64_t sb, int64_t st, int dtype) {
@@ -383,8 +383,8 @@ int lucid_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t r
   if (!stats || !dlogits || (top && !top_indices)) return fail("lucid_token_logprobs_bwd: null argument");
   if (reinterpret_cast<uintptr_t>(dlogits) % (dtype == LUCID_DTYPE_F32 ? 4 : 2))
     return fail("lucid_token_logprobs_bwd: dlogits are misaligned");
-  const int per = 256 * lucid::kLpChunks * lucid::kLpChunk;
-  const int blocks = (int)(((int64_t)V + lucid::kLpChunk - 1 + per - 1) / per);
+  const int per = 256 * lucid::kLpLane;
+  const int blocks = (int)(((int64_t)V + 7 + per - 1) / per);
   if ((int64_t)R * blocks * 256 >= ((int64_t)1 << 32)) return fail("lucid_token_logprobs_bwd: too many rows");
   const dim3 grid((unsigned)R * blocks);
   hipStream_t st = static_cast<hipStream_t>(stream);

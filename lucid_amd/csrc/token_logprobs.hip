@@ -18,8 +18,7 @@
 
 namespace lucid {
 
-constexpr int kLpChunk = 8;     // consecutive logits per load of a lane
-constexpr int kLpChunks = 4;    // chunks a lane holds
+constexpr int kLpLane = 32;     // logits a lane holds, in chunks of 16 bytes
 constexpr int kLpMaxTop = 64;   // alternatives of a row
 constexpr int kLpCand = 1024;   // values considered for the alternatives of a segment
 constexpr int kLpMaxSegs = 64;  // segments of a row
@@ -32,32 +31,25 @@ struct LpStats {
   float m, l2, ent;
 };
 
-// A row of logits as aligned chunks: chunk q holds the values 8 q - shift + e, e = 0 .. 7, so that
-// every whole chunk starts at a 16-byte boundary (rows of odd V do not); the first and the last
-// chunk may lie partly outside the row and are read value by value.
+// A row of logits as aligned chunks of N = 16 bytes: chunk q holds the values N q - shift + e, e < N, so that
+// every whole chunk starts at a 16-byte boundary (rows of odd V do not); the first and the last chunk may lie
+// partly outside the row and are read value by value.
 template <typename T>
 struct LpRow {
-  typedef T V8 __attribute__((ext_vector_type(8)));
+  static constexpr int N = 16 / sizeof(T), C = kLpLane / N;  // values of a chunk, chunks of a lane
+  typedef T V __attribute__((ext_vector_type(N)));
   const T* row;
-  int V, shift;
+  int len, shift;
   __device__ __forceinline__ LpRow(const T* r, int v)
-      : row(r), V(v), shift((int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T))) {}
-  __device__ __forceinline__ int first(int q) const { return q * kLpChunk - shift; }
-  __device__ __forceinline__ bool whole(int q) const { return first(q) >= 0 && first(q) + kLpChunk <= V; }
-  __device__ __forceinline__ V8 load(int q) const {  // outside the row: -inf
+      : row(r), len(v), shift((int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T))) {}
+  __device__ __forceinline__ int first(int q) const { return q * N - shift; }
+  __device__ __forceinline__ bool whole(int q) const { return first(q) >= 0 && first(q) + N <= len; }
+  __device__ __forceinline__ V load(int q) const {  // outside the row: -inf
     const int j = first(q);
-    V8 x;
-    if (whole(q)) {
-      if constexpr (sizeof(T) == 2) {
-        x = *reinterpret_cast<const V8*>(row + j);
-      } else {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(row + j), b = *reinterpret_cast<const f32x4*>(row + j + 4);
-        x = V8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-      }
-    } else {
+    if (whole(q)) return *reinterpret_cast<const V*>(row + j);
+    V x;
 #pragma unroll
-      for (int e = 0; e < kLpChunk; ++e) x[e] = j + e >= 0 && j + e < V ? row[j + e] : (T)(-INFINITY);
-    }
+    for (int e = 0; e < N; ++e) x[e] = j + e >= 0 && j + e < len ? row[j + e] : (T)(-INFINITY);
     return x;
   }
 };
@@ -141,16 +133,17 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
   const int r = blockIdx.x / segs, seg = blockIdx.x - r * segs;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const LpRow<T> row(lp_row(logits, sb, st, Tn, r), V);
-  const int q0 = seg * NT * kLpChunks + tid;
-  typename LpRow<T>::V8 x[kLpChunks];
+  constexpr int N = LpRow<T>::N, C = LpRow<T>::C;
+  const int q0 = seg * NT * C + tid;
+  typename LpRow<T>::V x[C];
 #pragma unroll
-  for (int c = 0; c < kLpChunks; ++c) x[c] = row.load(q0 + c * NT);
+  for (int c = 0; c < C; ++c) x[c] = row.load(q0 + c * NT);
 
   float m = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < kLpChunks; ++c)
+  for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int e = 0; e < kLpChunk; ++e) m = fmaxf(m, (float)x[c][e]);
+    for (int e = 0; e < N; ++e) m = fmaxf(m, (float)x[c][e]);
   m = lanes_max<GL>(m);
   if (TOP && tid % GL == 0) gmax[tid / GL] = m;
   m = lanes_max<64>(m);
@@ -174,9 +167,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
   const float c2 = LOG2E_F * inv_temp;
   float s = 0.f, t = 0.f;
 #pragma unroll
-  for (int c = 0; c < kLpChunks; ++c) {
+  for (int c = 0; c < C; ++c) {
 #pragma unroll
-    for (int e = 0; e < kLpChunk; ++e) {
+    for (int e = 0; e < N; ++e) {
       const float a = ((float)x[c][e] - mref) * c2;
       const float p = __builtin_amdgcn_exp2f(a);
       s += p;
@@ -192,19 +185,19 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
   if constexpr (TOP) {
     __syncthreads();
     const float bound = bound_;
-    const int lo = max(row.first(seg * NT * kLpChunks), 0);  // the segment's first index
+    const int lo = max(row.first(seg * NT * C), 0);  // the segment's first index
     // Offers what passes: everything from the bound up (and NaN), or, the second time, the values above it and
     // those equal to it among the segment's first kLpCand / 2.
     auto offer = [&](int pass) {
 #pragma unroll
-      for (int c = 0; c < kLpChunks; ++c) {
+      for (int c = 0; c < C; ++c) {
         const int j = row.first(q0 + c * NT);
         bool any = false;
 #pragma unroll
-        for (int e = 0; e < kLpChunk; ++e) any |= !((float)x[c][e] < bound);
+        for (int e = 0; e < N; ++e) any |= !((float)x[c][e] < bound);
         if (any) {
 #pragma unroll
-          for (int e = 0; e < kLpChunk; ++e) {
+          for (int e = 0; e < N; ++e) {
             const float v = (float)x[c][e];
             if (v < bound || j + e < 0 || j + e >= V) continue;
             if (pass == 1 && v == bound && j + e - lo >= kLpCand / 2) continue;
@@ -239,10 +232,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
         if (scan) {
           mine = 0;
 #pragma unroll
-          for (int c = 0; c < kLpChunks; ++c) {
+          for (int c = 0; c < C; ++c) {
             const int j = row.first(q0 + c * NT);
 #pragma unroll
-            for (int e = 0; e < kLpChunk; ++e) {
+            for (int e = 0; e < N; ++e) {
               const unsigned long long key = lp_key((float)x[c][e], j + e);
               if (j + e >= 0 && j + e < V && key < last && key > mine) mine = key;
             }
@@ -351,7 +344,7 @@ __global__ __launch_bounds__(256) void lucid_token_logprobs_bwd_kernel(const T* 
                                                                        const LpStats* __restrict__ stats,
                                                                        const int64_t* __restrict__ top_idx, LpGrads g,
                                                                        T* __restrict__ dlogits, int blocks) {
-  constexpr int NT = 256;
+  constexpr int NT = 256, N = LpRow<T>::N, C = LpRow<T>::C;
   __shared__ int name[kLpMaxTop + 1];
   __shared__ float gain[kLpMaxTop + 1];
   const int r = blockIdx.x / blocks, col = blockIdx.x - r * blocks, tid = threadIdx.x;
@@ -382,32 +375,27 @@ __global__ __launch_bounds__(256) void lucid_token_logprobs_bwd_kernel(const T* 
     return -p * fmaf(kb, fmaxf(a, kLpNone), ka);
   };
   const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) / sizeof(T) == (unsigned)row.shift;
-  const int q0 = col * NT * kLpChunks + tid;
+  const int q0 = col * NT * C + tid;
 #pragma unroll
-  for (int c = 0; c < kLpChunks; ++c) {
+  for (int c = 0; c < C; ++c) {
     const int q = q0 + c * NT, j = row.first(q);
     if (j >= V) break;
-    const typename LpRow<T>::V8 x = row.load(q);
-    typename LpRow<T>::V8 o;
+    const typename LpRow<T>::V x = row.load(q);
+    typename LpRow<T>::V o;
 #pragma unroll
-    for (int e = 0; e < kLpChunk; ++e) o[e] = (T)(soft((float)x[e]) * inv_temp);
+    for (int e = 0; e < N; ++e) o[e] = (T)(soft((float)x[e]) * inv_temp);
     if (same && row.whole(q)) {
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<bf16x8*>(drow + j) = o;
-      } else {
-        *reinterpret_cast<f32x4*>(drow + j) = f32x4{o[0], o[1], o[2], o[3]};
-        *reinterpret_cast<f32x4*>(drow + j + 4) = f32x4{o[4], o[5], o[6], o[7]};
-      }
+      *reinterpret_cast<typename LpRow<T>::V*>(drow + j) = o;
     } else {
 #pragma unroll
-      for (int e = 0; e < kLpChunk; ++e)
+      for (int e = 0; e < N; ++e)
         if (j + e >= 0 && j + e < V) drow[j + e] = o[e];
     }
   }
   __syncthreads();
   if (tid <= top) {
     const int j = name[tid];
-    const int lo = row.first(col * NT * kLpChunks), hi = lo + NT * kLpChunks * kLpChunk;
+    const int lo = row.first(col * NT * C), hi = lo + NT * kLpLane;
     if (j >= 0 && j >= lo && j < hi) {
       bool firstly = true;
       float add = 0.f;
