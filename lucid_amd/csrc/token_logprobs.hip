@@ -99,12 +99,11 @@ struct LpOut {
 
 constexpr int64_t kLpIgnore = -100;  // the loss's ignore index
 
-// The row's results from s = sum exp2(a_j) and t = sum exp2(a_j) a_j; returns log2 s
-__device__ __forceinline__ float lp_finish(const LpOut& out, int r, float m, float s, float t, float inv_temp,
-                                           const int64_t* tokens, int V, float xtok) {
+// The row's results from its maximum m, s = sum exp2(a_j) and t = sum exp2(a_j) a_j; returns log2 s
+__device__ __forceinline__ float lp_finish(const LpOut& out, int r, float m, float s, float t, float inv_temp, int64_t tok,
+                                           int V, float xtok) {
   constexpr float kLn2 = 0.69314718055994531f;
   const float l2 = log2f(s), ent = kLn2 * (l2 - t / s);
-  const int64_t tok = tokens[r];
   float lp = 0.f;
   if (tok != kLpIgnore)
     lp = tok < 0 || tok >= V ? __builtin_nanf("") : (xtok - m) * inv_temp - kLn2 * l2;
@@ -114,21 +113,35 @@ __device__ __forceinline__ float lp_finish(const LpOut& out, int r, float m, flo
   return l2;
 }
 
-// Grid R x segs; NT threads.  top <= kLpMaxTop.
+// The parts (m, s, t) of a row that K adjacent lanes hold, joined in each of them: with M the largest m_i and
+// d_i = (m_i - M) c, s = sum s_i exp2(d_i), t = sum exp2(d_i) (t_i + s_i d_i).  A part of -inf alone has
+// m = -inf and adds its sums as they are: 0, or NaN where there was one.
+template <int K>
+__device__ __forceinline__ void lp_join(float& m, float& s, float& t, float c2) {
+  const float M = lanes_max<K>(m);
+  const bool has = m != -INFINITY;
+  const float d = (m - M) * c2, f = __builtin_amdgcn_exp2f(d);
+  t = lanes_sum<K>(has ? f * fmaf(s, fmaxf(d, kLpNone), t) : t);
+  s = lanes_sum<K>(has ? s * f : s);
+  m = M;
+}
+
+// Grid R x segs; NT threads.  top <= kLpMaxTop.  Each wave takes its own maximum for the reference of its
+// sums, so that nothing waits for the row's; one wave joins the waves.
 // Alternatives: the lanes form 64 groups, and the top-th largest of the groups' maxima is a bound that
 // at least `top` values reach and, over values in no order, few more than that (20 alternatives: 24).  Those
 // are collected and each counts the ones before it.  Rows with more than kLpCand values at or above the
 // bound (masks of one finite value, few allowed tokens, ordered logits) are tried again with the equal ones
 // limited to low indices, which is enough wherever such values are dense, and else taken one a round.
 template <typename T, int NT, bool TOP>
-__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8))) void lucid_token_logprobs_kernel(const T* __restrict__ logits, int64_t sb, int64_t st,
-                                                                  int Tn, const int64_t* __restrict__ tokens, int V,
-                                                                  float inv_temp, int top, int segs, LpOut out) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lucid_token_logprobs_kernel(
+    const T* __restrict__ logits, int64_t sb, int64_t st, int Tn, const int64_t* __restrict__ tokens, int V,
+    float inv_temp, int top, int segs, LpOut out) {
   constexpr int NW = NT / 64;
   constexpr int GL = NT / 64;  // lanes of one of 64 groups
   __shared__ float red[3][NW], gmax[TOP ? 64 : 1];
   __shared__ unsigned long long kred[TOP ? NW : 1], best[TOP ? kLpMaxTop : 1], cand[TOP ? kLpCand : 1];
-  __shared__ float bound_;
+  __shared__ float bound_, stat[2];
   __shared__ int found[2];
   const int r = blockIdx.x / segs, seg = blockIdx.x - r * segs;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
@@ -139,6 +152,13 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
 #pragma unroll
   for (int c = 0; c < C; ++c) x[c] = row.load(q0 + c * NT);
 
+  constexpr int JW = TOP ? 1 : 0;  // the joining wave (the first one finds the alternatives' bound)
+  int64_t tok = kLpIgnore;
+  float xtok = 0.f;
+  if (segs == 1 && w == JW) {  // wanted at the end
+    tok = tokens[r];
+    if (tok >= 0 && tok < V) xtok = (float)row.row[tok];
+  }
   float m = -INFINITY;
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -146,41 +166,68 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
     for (int e = 0; e < N; ++e) m = fmaxf(m, (float)x[c][e]);
   m = lanes_max<GL>(m);
   if (TOP && tid % GL == 0) gmax[tid / GL] = m;
-  m = lanes_max<64>(m);
-  if (lane == 0) red[0][w] = m;
+  m = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, lanes_max<64>(m))));
+  const float c2 = LOG2E_F * inv_temp, mref = m == -INFINITY ? 0.f : m, mc = mref * c2;
+  float s = 0.f, t = 0.f;  // p = 0 where a = -inf
+  if (fabsf(mc) < 1e37f) {  // a = x c - m c in one step
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float a = fmaf((float)x[c][e], c2, -mc), p = __builtin_amdgcn_exp2f(a);
+        s += p;
+        t = fmaf(p, fmaxf(a, kLpNone), t);
+      }
+    }
+  } else {  // a maximum near the type's lowest or largest value (or inf), whose product overflows
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float a = ((float)x[c][e] - mref) * c2, p = __builtin_amdgcn_exp2f(a);
+        s += p;
+        t = fmaf(p, fmaxf(a, kLpNone), t);
+      }
+    }
+  }
+  s = lanes_sum<64>(s);
+  t = lanes_sum<64>(t);
+  if (lane == 0) {
+    // m c was rounded: every a is larger by the difference (exact in one fma), which leaves here
+    const float off = fabsf(mc) < 1e37f ? fmaf(mref, c2, -mc) : 0.f, f = __builtin_amdgcn_exp2f(-off);
+    red[0][w] = m;
+    red[1][w] = s * f;
+    red[2][w] = fmaf(-off, s, t) * f;
+  }
   if (TOP && tid < 2) found[tid] = 0;
   __syncthreads();
   if (TOP && w == 0) {  // the top-th largest group maximum
     const float mine = gmax[lane];
     int above = 0;
-#pragma unroll 16
+#pragma unroll 8
     for (int i = 0; i < 64; ++i) {
       const float o = gmax[i];
       above += o > mine || (o == mine && i < lane);
     }
     if (above == top - 1) bound_ = mine;
   }
-#pragma unroll
-  for (int i = 0; i < NW; ++i) m = fmaxf(m, red[0][i]);
-  // a segment of -inf alone adds nothing to the others (its own sums would be NaN)
-  const float mref = segs > 1 && m == -INFINITY ? 0.f : m;
-  const float c2 = LOG2E_F * inv_temp;
-  float s = 0.f, t = 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float a = ((float)x[c][e] - mref) * c2;
-      const float p = __builtin_amdgcn_exp2f(a);
-      s += p;
-      t = fmaf(p, fmaxf(a, kLpNone), t);  // p = 0 where a = -inf
+  if (w == JW) {
+    const bool on = lane < NW;
+    m = on ? red[0][lane % NW] : -INFINITY;
+    s = on ? red[1][lane % NW] : 0.f;
+    t = on ? red[2][lane % NW] : 0.f;
+    lp_join<NW>(m, s, t, c2);
+    if (lane == 0) {
+      if (segs == 1) {
+        stat[0] = m;
+        stat[1] = lp_finish(out, r, m, s, t, inv_temp, tok, V, xtok);
+      } else {
+        const int64_t at = (int64_t)r * segs + seg;
+        out.pm[at] = m;
+        out.ps[at] = s;
+        out.pt[at] = t;
+      }
     }
-  }
-  s = lanes_sum<64>(s);
-  t = lanes_sum<64>(t);
-  if (lane == 0) {
-    red[1][w] = s;
-    red[2][w] = t;
   }
   if constexpr (TOP) {
     __syncthreads();
@@ -188,30 +235,31 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
     const int lo = max(row.first(seg * NT * C), 0);  // the segment's first index
     // Offers what passes: everything from the bound up (and NaN), or, the second time, the values above it and
     // those equal to it among the segment's first kLpCand / 2.
-    auto offer = [&](int pass) {
+    auto offer = [&](int pass, typename LpRow<T>::V xv, int j) {
+      bool any = false;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int j = row.first(q0 + c * NT);
-        bool any = false;
+      for (int e = 0; e < N; ++e) any |= !((float)xv[e] < bound);
+      if (any) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) any |= !((float)x[c][e] < bound);
-        if (any) {
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float v = (float)x[c][e];
-            if (v < bound || j + e < 0 || j + e >= V) continue;
-            if (pass == 1 && v == bound && j + e - lo >= kLpCand / 2) continue;
-            const int at = atomicAdd(&found[pass], 1);
-            if (at < kLpCand) cand[at] = lp_key(v, j + e);
-          }
+        for (int e = 0; e < N; ++e) {
+          const float v = (float)xv[e];
+          if (v < bound || j + e < 0 || j + e >= V) continue;
+          if (pass == 1 && v == bound && j + e - lo >= kLpCand / 2) continue;
+          const int at = atomicAdd(&found[pass], 1);
+          if (at < kLpCand) cand[at] = lp_key(v, j + e);
         }
       }
     };
-    offer(0);
+    int qa = q0;
+    asm volatile("" : "+v"(qa));  // the indices are worked out here, not kept from the loads
+#pragma unroll
+    for (int c = 0; c < C; ++c) offer(0, x[c], row.first(qa + c * NT));
     __syncthreads();
     int n = found[0];
     if (n > kLpCand) {
-      offer(1);
+      // (from here on the row is read again: its registers would cost the rows that never get here)
+#pragma unroll 1
+      for (int c = 0; c < C; ++c) offer(1, row.load(qa + c * NT), row.first(qa + c * NT));
       __syncthreads();
       n = found[1];
     }
@@ -231,12 +279,13 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
       for (int k = 0; k < top; ++k) {
         if (scan) {
           mine = 0;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < C; ++c) {
-            const int j = row.first(q0 + c * NT);
+            const int j = row.first(qa + c * NT);
+            const typename LpRow<T>::V xv = row.load(qa + c * NT);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-              const unsigned long long key = lp_key((float)x[c][e], j + e);
+              const unsigned long long key = lp_key((float)xv[e], j + e);
               if (j + e >= 0 && j + e < V && key < last && key > mine) mine = key;
             }
           }
@@ -253,37 +302,22 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(TOP ? 4 : 8)
       }
     }
   }
-  __syncthreads();
-  s = t = 0.f;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    s += red[1][i];
-    t += red[2][i];
-  }
-  if (segs == 1) {
-    const float l2 = log2f(s);
-    if (tid == 0) {
-      const int64_t tok = tokens[r];
-      lp_finish(out, r, m, s, t, inv_temp, tokens, V, tok >= 0 && tok < V ? (float)row.row[tok] : 0.f);
+  if constexpr (TOP) {
+    __syncthreads();
+    if (tid < top) {
+      const unsigned long long key = best[tid];
+      if (segs == 1) {
+        out.top_idx[(int64_t)r * top + tid] = lp_index(key);
+        out.top_lp[(int64_t)r * top + tid] = (lp_value(key) - stat[0]) * inv_temp - 0.69314718055994531f * stat[1];
+      } else {
+        out.pkey[((int64_t)r * segs + seg) * top + tid] = key;
+      }
     }
-    if (TOP && tid < top) {
-      out.top_idx[(int64_t)r * top + tid] = lp_index(best[tid]);
-      out.top_lp[(int64_t)r * top + tid] = (lp_value(best[tid]) - m) * inv_temp - 0.69314718055994531f * l2;
-    }
-  } else {
-    const int64_t at = (int64_t)r * segs + seg;
-    if (tid == 0) {
-      out.pm[at] = m;
-      out.ps[at] = s;
-      out.pt[at] = t;
-    }
-    if (TOP && tid < top) out.pkey[at * top + tid] = best[tid];
   }
 }
 
-// Rows of several segments, one workgroup each: with M the largest of the segments' maxima m_i and
-// d_i = (m_i - M) c, s = sum s_i exp2(d_i) and t = sum exp2(d_i) (t_i + s_i d_i).  Each of the segments' keys counts
-// those above it: its place among the row's alternatives.
+// Rows of several segments, one workgroup each.  Each of the segments' keys counts those above it: its place among
+// the row's alternatives.
 template <typename T>
 __global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T* __restrict__ logits, int64_t sb,
                                                                          int64_t st, int Tn,
@@ -298,22 +332,13 @@ __global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T
   for (int i = tid; i < n; i += 256) keys[i] = out.pkey[at * top + i];
   if (tid < 64) {
     const bool on = lane < segs;
-    const float mi = on ? out.pm[at + lane] : -INFINITY;
-    const float m = lanes_max<64>(mi);
-    float f = 0.f, d = 0.f;
-    if (on && mi != -INFINITY) {  // (a segment of -inf alone has the sums 0; NaN sums have to go through)
-      d = (mi - m) * c2;
-      f = __builtin_amdgcn_exp2f(d);
-    }
-    const float si = on ? out.ps[at + lane] : 0.f, ti = on ? out.pt[at + lane] : 0.f;
-    const bool gone = !on || (mi == -INFINITY && si == 0.f);
-    const float s = lanes_sum<64>(gone ? (m == -INFINITY && lane == 0 ? __builtin_nanf("") : 0.f) : mi == -INFINITY ? si : si * f);
-    const float t = lanes_sum<64>(gone ? 0.f : mi == -INFINITY ? ti : f * fmaf(si, fmaxf(d, kLpNone), ti));
+    float m = on ? out.pm[at + lane] : -INFINITY, s = on ? out.ps[at + lane] : 0.f, t = on ? out.pt[at + lane] : 0.f;
+    const int64_t tok = tokens[r];
+    const float xtok = tok >= 0 && tok < V ? (float)lp_row(logits, sb, st, Tn, r)[tok] : 0.f;
+    lp_join<64>(m, s, t, c2);
     if (lane == 0) {
-      const int64_t tok = tokens[r];
-      const T* row = lp_row(logits, sb, st, Tn, r);
       stat[0] = m;
-      stat[1] = lp_finish(out, r, m, s, t, inv_temp, tokens, V, tok >= 0 && tok < V ? (float)row[tok] : 0.f);
+      stat[1] = lp_finish(out, r, m, s, t, inv_temp, tok, V, xtok);
     }
   }
   __syncthreads();
