@@ -316,8 +316,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lu
   }
 }
 
-// Rows of several segments, one workgroup each.  Each of the segments' keys counts those above it: its place among
-// the row's alternatives.
+// Rows of several segments, one workgroup each.  A key's place among the row's alternatives is
+// the number above it: its place in its own segment's list and those that it would have in the others'.
 template <typename T>
 __global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T* __restrict__ logits, int64_t sb,
                                                                          int64_t st, int Tn,
@@ -345,8 +345,21 @@ __global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T
   for (int i = tid; i < n; i += 256) {
     const unsigned long long key = keys[i];
     if (!key) continue;
-    int above = 0;
-    for (int k = 0; k < n; ++k) above += keys[k] > key;
+    // every segment's keys are in descending order
+    const int own = i / top;
+    int above = i - own * top;
+    for (int g = 0; g < segs; ++g) {
+      if (g == own) continue;
+      int lo = 0, hi = top;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (keys[g * top + mid] > key)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      above += lo;
+    }
     if (above >= top) continue;
     out.top_idx[(int64_t)r * top + above] = lp_index(key);
     out.top_lp[(int64_t)r * top + above] = (lp_value(key) - stat[0]) * inv_temp - 0.69314718055994531f * stat[1];
