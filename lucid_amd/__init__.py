@@ -8,7 +8,8 @@ Operator entry points (drop-ins for the reference seams):
 * :func:`lucid_amd.lucid.set_precision` (bf16 or hi/lo-split chain products, chosen per head by default)
 * :func:`lucid_amd.lucid.set_fused_forward` (one fused chain + attention kernel, or two kernels)
 * :mod:`lucid_amd.modeling_lucid` (the reference model file's classes on these operators)
-* :mod:`lucid_amd.paged` (decoding against a paged (K, V') cache, writing and copying its pages)
+* :mod:`lucid_amd.paged` (decoding against a paged (K, V') cache, writing, copying, forking and freeing its
+  pages)
 * :mod:`lucid_amd.model_ops` (fused RMSNorm, RoPE, SwiGLU gate and causal-LM loss of the decoder; token
   log probabilities)
 * :mod:`lucid_amd.optim` (AdamW on one HIP pass per step)
@@ -17,10 +18,11 @@ Operator entry points (drop-ins for the reference seams):
 from .lucid import (LucidAttentionFunction, causal_attention, eager_lucid_attention_forward, get_fused_forward,
                     get_precision, get_v_prime, lucid_attention, lucid_decode, set_fused_forward, set_precision)
 from .model_ops import token_logprobs
-from .paged import copy_pages, lucid_decode_paged, write_pages
+from .paged import LucidPagedCache, copy_pages, lucid_decode_paged, write_pages
 
 __all__ = [
     "LucidAttentionFunction",
+    "LucidPagedCache",
     "causal_attention",
     "copy_pages",
     "eager_lucid_attention_forward",

@@ -15,7 +15,8 @@ Decoding with a cache (``get_new_v_prime``, ``modeling_lucid.py:576-598``) keeps
 follow the prefill definition exactly:
 v'_t = (v_t - sum_{j<t} P_tj v'_j) / P_tt with the non-unit diagonal
 P_tt = exp(s |K^_t|^2 - 1/s), so a decoded token gets the same V' row as the same
-token inside a prefill (the reference's decode path drops the division by P_tt).
+token inside a prefill (the reference's decode path drops the division by P_tt).  Sequences of
+different lengths are served from a :class:`lucid_amd.paged.LucidPagedCache` in the same argument.
 """
 from __future__ import annotations
 
@@ -27,8 +28,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .lucid import _padded_dim, lucid_attention, lucid_decode
-from .model_ops import (apply_rope, causal_lm_loss, causal_lm_loss_supported, qkv_rope, rms_norm,
-                        rms_norm_supported, rope_supported, swiglu, swiglu_supported)
+from .model_ops import (TokenLogprobs, apply_rope, causal_lm_loss, causal_lm_loss_supported, qkv_rope, rms_norm,
+                        rms_norm_supported, rope_supported, swiglu, swiglu_supported, token_logprobs)
+from .paged import LucidPagedCache, lucid_decode_paged, write_pages
 
 
 @dataclass
@@ -239,6 +241,9 @@ class LucidAttention(nn.Module):
             cos, sin = position_embeddings
             if self.use_rope:
                 q, k = apply_rotary_pos_emb(q, k, cos, sin)
+        if isinstance(past_key_value, LucidPagedCache):
+            out = self._paged(q, k, v, past_key_value)
+            return self.o_proj(out.reshape(*input_shape, -1)), None
         past = 0 if past_key_value is None else past_key_value.get_seq_length(self.layer_idx)
         if past == 0:
             # training / prefill: the fused HIP op (P never materialised, causal mask implicit)
@@ -284,6 +289,21 @@ class LucidAttention(nn.Module):
         return o
 
 
+    def _paged(self, q, k, v, cache: LucidPagedCache) -> torch.Tensor:
+        """A pass over the sequences that the cache has selected: a prefill of empty ones through the
+        fused op, whose rows are written into their pages, else the new tokens through one paged
+        decoding call (which appends them); returns [B, T, Hq, d]."""
+        step = cache.step
+        pools = cache.pools(self.layer_idx, k.shape[1], self.head_dim)
+        if step.prefill:
+            out, v_prime = lucid_attention(q, k, v, scaling=self.scaling, eps=self.config.rms_norm_eps,
+                                           return_vprime=True)
+            write_pages(k, v_prime, *pools, step.table, step.lens, step.counts)
+            return out
+        return lucid_decode_paged(q, k, v, *pools, step.table, step.lens, scaling=self.scaling,
+                                  eps=self.config.rms_norm_eps)[0]
+
+
 class LlamaDecoderLayer(nn.Module):
     """modeling_lucid.py:621-684 (pre-norm residual blocks)."""
 
@@ -311,13 +331,21 @@ class LlamaModel(nn.Module):
         self.norm = LlamaRMSNorm(config.hidden_size, eps=config.rms_norm_eps)
         self.rotary_emb = LlamaRotaryEmbedding(config)
 
-    def forward(self, input_ids: torch.Tensor, past_key_values: Optional[LucidCache] = None) -> torch.Tensor:
+    def forward(self, input_ids: torch.Tensor,
+                past_key_values: Optional[LucidCache | LucidPagedCache] = None) -> torch.Tensor:
         h = self.embed_tokens(input_ids)
-        past = past_key_values.get_seq_length() if past_key_values is not None else 0
-        pos = torch.arange(past, past + input_ids.shape[1], device=input_ids.device)[None].expand(input_ids.shape[0], -1)
+        paged = isinstance(past_key_values, LucidPagedCache)
+        if paged:
+            pos = past_key_values.begin(*input_ids.shape).positions
+        else:
+            past = past_key_values.get_seq_length() if past_key_values is not None else 0
+            pos = torch.arange(past, past + input_ids.shape[1],
+                               device=input_ids.device)[None].expand(input_ids.shape[0], -1)
         pe = self.rotary_emb(h, pos)
         for layer in self.layers:
             h = layer(h, pe, past_key_value=past_key_values)
+        if paged:
+            past_key_values.commit()
         return self.norm(h)
 
 
@@ -346,7 +374,7 @@ class LlamaForCausalLM(nn.Module):
             module.weight.data.fill_(1.0)
 
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
-                past_key_values: Optional[LucidCache] = None):
+                past_key_values: Optional[LucidCache | LucidPagedCache] = None):
         hidden = self.model(input_ids, past_key_values=past_key_values)
         logits = self.lm_head(hidden)
         loss = None
@@ -355,6 +383,16 @@ class LlamaForCausalLM(nn.Module):
         elif labels is not None:
             loss = F.cross_entropy(logits[:, :-1].float().reshape(-1, logits.shape[-1]), labels[:, 1:].reshape(-1))
         return loss, logits
+
+
+    def token_logprobs(self, input_ids: torch.Tensor, top: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+        """Log probabilities that the model gives each token of ``input_ids [B, T]`` after those before it, with the
+        entropy and the ``top`` most likely tokens at each place (:func:`lucid_amd.model_ops.token_logprobs` on the
+        logits; differentiable).  Position t holds those of token t + 1; the last one, which has no next token, the log
+        probability 0."""
+        logits = self.lm_head(self.model(input_ids))
+        after = F.pad(input_ids[:, 1:], (0, min(1, input_ids.shape[1])), value=-100)
+        return token_logprobs(logits, after, top, temperature)
 
 
 def count_parameters(model: nn.Module) -> int:
@@ -367,6 +405,6 @@ def c3_config() -> LucidConfig:
                        num_attention_heads=32, head_dim=64, rope_theta=10000.0)
 
 
-__all__ = ["LucidConfig", "LucidCache", "LucidAttention", "LlamaDecoderLayer", "LlamaModel", "LlamaForCausalLM",
-           "LlamaRMSNorm", "LlamaMLP", "LlamaRotaryEmbedding", "apply_rotary_pos_emb", "c3_config",
+__all__ = ["LucidConfig", "LucidCache", "LucidPagedCache", "LucidAttention", "LlamaDecoderLayer", "LlamaModel",
+           "LlamaForCausalLM", "LlamaRMSNorm", "LlamaMLP", "LlamaRotaryEmbedding", "apply_rotary_pos_emb", "c3_config",
            "count_parameters"]
