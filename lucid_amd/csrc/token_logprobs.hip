@@ -201,15 +201,14 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lu
   }
   if (TOP && tid < 2) found[tid] = 0;
   __syncthreads();
-  if (TOP && w == 0) {  // the top-th largest group maximum
-    const float mine = gmax[lane];
-    int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < 64; ++i) {
-      const float o = gmax[i];
-      above += o > mine || (o == mine && i < lane);
-    }
-    if (above == top - 1) bound_ = mine;
+  if (TOP && w == 0) {  // the top-th largest group maximum: its order key (lp_key's upper half) bit by bit
+    const unsigned mine = (unsigned)(lp_key(gmax[lane], 0) >> 32);
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 31; i >= (sizeof(T) == 2 ? 16 : 0); --i)
+      bits = __popcll(__ballot(mine >= (bits | 1u << i))) >= top ? bits | 1u << i : bits;
+    if (sizeof(T) == 2 && !(bits >> 31)) bits |= 0xffff;  // (a negative bf16's key ends in ones)
+    if (lane == 0) bound_ = lp_value((unsigned long long)bits << 32);
   }
   if (w == JW) {
     const bool on = lane < NW;
@@ -265,11 +264,14 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lu
     }
     if (n <= kLpCand && (n >= top || found[0] <= kLpCand)) {
       if (tid < top && tid >= n) best[tid] = 0;  // a short last segment
-      for (int i = tid; i < n; i += NT) {
+      // a wave counts what is above a value; the first 128 stay in its registers
+      const unsigned long long c0 = lane < n ? cand[lane] : 0, c1 = lane + 64 < n ? cand[lane + 64] : 0;
+#pragma unroll 4
+      for (int i = w; i < n; i += NW) {
         const unsigned long long key = cand[i];
-        int above = 0;
-        for (int k = 0; k < n; ++k) above += cand[k] > key;
-        if (above < top) best[above] = key;
+        int above = __popcll(__ballot(c0 > key)) + __popcll(__ballot(c1 > key));
+        for (int k = lane + 128; k - lane < n; k += 64) above += __popcll(__ballot(k < n && cand[k] > key));
+        if (lane == 0 && above < top) best[above] = key;
       }
     } else {
       // one a round: each lane offers its largest key below the last one taken
