@@ -142,7 +142,7 @@ struct PagedSmem {
   union {
     bf16 v[4][2][32 * W + 64];  // per wave, double buffered (the last tile's transposing reads of W = 80 end 32 bytes behind it)
     struct {
-      float so[4][32][W + 1];
+      float so[4][32][W + 4];  // per wave: the columns of O^T (of one column tile at a time)
       float m[4][32], l[4][32];
     } fin;
   } u;
@@ -378,8 +378,10 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (32 * dt + drow(e, g) < W) sm.u.fin.so[w][l32][32 * dt + drow(e, g)] = oacc[ct][dt][e];
+        for (int e = 0; e < 16; e += 4)  // four rows of the tile side by side
+          if (32 * dt + drow(e, 0) < W)
+            *reinterpret_cast<f32x4*>(&sm.u.fin.so[w][l32][32 * dt + drow(e, g)]) =
+                f32x4{oacc[ct][dt][e], oacc[ct][dt][e + 1], oacc[ct][dt][e + 2], oacc[ct][dt][e + 3]};
       if (isq[ct] && g == 0) {
         sm.u.fin.m[w][l32] = m[ct];
         sm.u.fin.l[w][l32] = lw;
@@ -387,33 +389,33 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
     }
     __syncthreads();
     const bool poison = sm.bad[0] | sm.bad[1] | sm.bad[2] | sm.bad[3];
+    // W / 4 lanes a column, two or four columns a wave
+    constexpr int CGP = W == 64 ? 16 : 32, CPW = 64 / CGP;
+    const int cg = lane % CGP;
 #pragma unroll 1
-    for (int cl = w; cl < 32; cl += 4) {
+    for (int cl = w * CPW + lane / CGP; cl < 32; cl += 4 * CPW) {
       const int t = (32 * ct + cl) / (Gs + 1), gg = 32 * ct + cl - t * (Gs + 1);
       if (t >= Lp) break;
-      if (gg == Gs) {
-#pragma unroll
-        for (int c = lane; c < W; c += 64)
-          part.a[(at * Lp + t) * W + c] =
-              (sm.u.fin.so[0][cl][c] + sm.u.fin.so[1][cl][c]) + (sm.u.fin.so[2][cl][c] + sm.u.fin.so[3][cl][c]);
-        continue;
-      }
-      const float mn = fmaxf(fmaxf(sm.u.fin.m[0][cl], sm.u.fin.m[1][cl]), fmaxf(sm.u.fin.m[2][cl], sm.u.fin.m[3][cl]));
-      float al[4], lt = 0.f;
+      if (cg >= W / 4) continue;
+      const bool key = gg == Gs;
+      float mw[4], lt = 0.f, mn = PAGED_NEG;
 #pragma unroll
       for (int ww = 0; ww < 4; ++ww) {
-        al[ww] = __builtin_amdgcn_exp2f(sm.u.fin.m[ww][cl] - mn);
-        lt = fmaf(sm.u.fin.l[ww][cl], al[ww], lt);
+        mw[ww] = sm.u.fin.m[ww][cl];
+        mn = fmaxf(mn, mw[ww]);
+      }
+      f32x4 ot = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ww = 0; ww < 4; ++ww) {
+        const float al = key ? 1.f : __builtin_amdgcn_exp2f(mw[ww] - mn);
+        lt = fmaf(sm.u.fin.l[ww][cl], al, lt);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&sm.u.fin.so[ww][cl][4 * cg]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ot[j] = fmaf(x[j], al, ot[j]);
       }
       const int64_t pi = at * (Lp * Gs) + t * Gs + gg;
-#pragma unroll
-      for (int c = lane; c < W; c += 64) {
-        float ot = 0.f;
-#pragma unroll
-        for (int ww = 0; ww < 4; ++ww) ot = fmaf(sm.u.fin.so[ww][cl][c], al[ww], ot);
-        part.o[pi * W + c] = ot;
-      }
-      if (lane == 0) {
+      *reinterpret_cast<f32x4*>((key ? part.a + (at * Lp + t) * W : part.o + pi * W) + 4 * cg) = ot;
+      if (cg == 0 && !key) {
         part.m[pi] = poison ? __builtin_nanf("") : mn;
         part.l[pi] = lt;
       }
