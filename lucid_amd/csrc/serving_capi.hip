@@ -48,7 +48,7 @@ lucid::PagedPartials carve_paged(void* base, int64_t slots, int Hkv, int Gs, int
 
 bool paged_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int D) {
   return B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && L > 0 && page > 0 && max_pages > 0 && page_width(D) &&
-         (int64_t)page * max_pages <= (1 << 30) && (int64_t)B * Hkv <= (1 << 23) && B <= (1 << 20) && Hkv <= 65535 &&
+         (int64_t)page * max_pages <= (1 << 30) && (int64_t)B * Hkv <= (1 << 22) && B <= (1 << 20) && Hkv <= 65535 &&
          B * (((int64_t)page * max_pages + lucid::kPagedUnit - 1) / lucid::kPagedUnit + lucid::kPagedLead) < ((int64_t)1 << 31);
 }
 
@@ -188,7 +188,8 @@ int check_lp(const char* what, const void* logits, int64_t sb, int64_t st, const
   if (R < 0 || Tn < 1 || R % Tn) return fail(w + ": R a multiple of the rows of a batch, got R=" + std::to_string(R));
   if (V < 1 || V > 2000000) return fail(w + ": V from 1 to 2000000, got " + std::to_string(V));
   if (top < 0 || top > lucid::kLpMaxTop || top > V) return fail(w + ": top from 0 to 64 and at most V, got " + std::to_string(top));
-  if (!(temperature > 0.f) || std::isinf(temperature)) return fail(w + ": the temperature must be positive and finite");
+  if (!(temperature > 0.f) || std::isinf(temperature) || std::isinf(1.f / temperature))
+    return fail(w + ": the temperature and its inverse must be positive and finite");
   if (sb < 0 || st < 0) return fail(w + ": negative strides");
   if (R == 0) return LUCID_OK;
   if (!logits || !tokens) return fail(w + ": logits or tokens are null");
@@ -241,7 +242,7 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
   if (!page_width(D)) return fail("head_dim must be in [1, 128], got " + std::to_string(D));
   if (!paged_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D))
     return fail("lucid_decode_paged: B, Hq, Hkv, L, page_size and max_pages positive, Hq a multiple of Hkv, at most 2^30 "
-                "rows a sequence, 2^38 in the tables together and 2^23 kv heads in the batch");
+                "rows a sequence, 2^38 in the tables together and 2^22 kv heads in the batch");
   if (num_pages < 1) return fail("lucid_decode_paged: the pools have no pages");
   if (!q || !q_strides || !k || !k_strides || !v || !v_strides || !o || !o_strides || !vp_new || !page_table ||
       !cache_lens || !ws)

@@ -26,6 +26,7 @@ dim 64; the loss: a vocabulary that is a multiple of 8) and raise otherwise; the
 """
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple
 
 import torch
@@ -378,10 +379,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     if logits.dim() < 1 or logits.shape[:-1] != tokens.shape or logits.shape[-1] < 1:
         raise ValueError(f"lucid_amd.token_logprobs: logits [..., V] and tokens [...], got {tuple(logits.shape)} and "
                          f"{tuple(tokens.shape)}")
+    top = operator.index(top)
     if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError(f"lucid_amd.token_logprobs: top must be in [0, min({MAX_TOP}, V)], got {top}")
     if not 0.0 < temperature < float("inf"):
         raise ValueError(f"lucid_amd.token_logprobs: the temperature must be positive and finite, got {temperature}")
     if logits.requires_grad and torch.is_grad_enabled():
-        return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, int(top), float(temperature)))
-    return TokenLogprobs(*_token_logprobs(logits.detach(), tokens.contiguous(), int(top), float(temperature))[:4])
+        return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, top, float(temperature)))
+    return TokenLogprobs(*_token_logprobs(logits.detach(), tokens.contiguous(), top, float(temperature))[:4])

@@ -492,3 +492,64 @@ def test_copy_pages_of_many_pools_pairs_and_strides():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(base, want)
+
+
+def test_thousands_of_sequences_equal_smaller_batches():
+    """3000 sequences (the line of 47 groups of 64), each shorter than a share's unit: the bits of batches of 60."""
+    g = torch.Generator().manual_seed(8)
+    lens = torch.randint(-1, 100, (3000,), generator=g).tolist()
+    for Hq, Hkv, L, d in ((2, 1, 1, 64), (4, 2, 2, 68)):
+        c = _case(lens, Hq, Hkv, L, d, 16, seed=d)
+        o, vn = lucid_decode_paged(*(c[n] for n in ("q", "k", "v", "kp", "vp", "table", "lens")))
+        for i in range(0, 3000, 60):
+            part = [c[n][i:i + 60] for n in ("q", "k", "v")] + [c["kp"], c["vp"], c["table"][i:i + 60], c["lens"][i:i + 60]]
+            o2, vn2 = lucid_decode_paged(*part)
+            assert torch.equal(o[i:i + 60], o2) and torch.equal(vn[i:i + 60], vn2), i
+
+
+def test_calls_on_two_streams_at_once():
+    """Two calls in flight (workspaces of their own), each writing its own pools, give what they give one by one."""
+    cases = [_case([3000, 500], 8, 2, 2, 128, 16, seed=s) for s in (1, 2)]
+    names = ("q", "k", "v", "kp", "vp", "table", "lens")
+    want = [lucid_decode_paged(*(c[n].clone() for n in names)) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(lucid_decode_paged(*(c[n] for n in names)))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        assert all(torch.equal(a, b) for r in gs for a, b in zip(r, w))
+
+
+def test_captured_writes_and_shared_pages():
+    """A captured prefill write follows new rows and lengths; two sequences that share full pages (a forked prompt) read
+    the same rows and append to pages of their own."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    B, Hkv, T, d, page = 2, 2, 20, 64, 16
+    table, pages = _tables(g, [0, 0], [40, 40], page)
+    kp, vp = (_pool(g, pages, Hkv, page, d) for _ in range(2))
+    k = torch.randn(B, Hkv, T, d, generator=g, device="cuda").to(BF)
+    v = torch.randn(B, Hkv, T, d, generator=g, device="cuda")
+    lens, counts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 3], [20, 7]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        write_pages(k, v, kp, vp, table, lens, counts)
+    for i in range(3):
+        k.normal_(generator=g)
+        v.normal_(generator=g)
+        lens.copy_(torch.tensor([i, 11 - i], dtype=torch.int32))
+        want_k, want_v = kp.clone(), vp.clone()
+        write_pages(k, v, want_k, want_v, table, lens, counts)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(kp, want_k) and torch.equal(vp, want_v), i
+    c = _case([33, 33], 4, 2, 1, d, page, seed=3)
+    c["table"][1, :2] = c["table"][0, :2]  # rows 0 .. 31 shared, row 32 and the new one its own
+    _go(c, page)

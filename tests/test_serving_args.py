@@ -68,7 +68,8 @@ def _decode(lib, **kw):
     (dict(k_pages=None), b"null"), (dict(k_pages=ctypes.c_void_p((1 << 20) + 8)), b"16-byte"),
     (dict(ks=_s(8192, 4096, 60)), b"multiples of 8"), (dict(vs=_s(8192, -4096, 64)), b"non-negative"),
     (dict(P=(1 << 22) + 1), b"64 GB"), (dict(ks=_s(1 << 40, 64, 64)), b"64 GB"), (dict(scale=0.0), b"scale"),
-    (dict(tstride=-1), b"table stride")])
+    (dict(tstride=-1), b"table stride"), (dict(B=1 << 20, Hq=8, Hkv=8, M=1), b"2^22"),
+    (dict(B=1 << 20, Hq=1, Hkv=1, M=1 << 24, page=64), b"2^38")])
 def test_decode_paged_refuses(lib, kw, text):
     _err(lib, _decode(lib, **kw), text)
 
@@ -113,7 +114,7 @@ def test_token_logprobs_refuses(lib):
     assert fwd(R=0) == 0
     for kw, text in ((dict(dtype=2), b"dtype"), (dict(R=5), b"multiple"), (dict(V=0), b"V from 1"), (dict(V=3000000), b"V from 1"),
                      (dict(top=65), b"top"), (dict(top=4, V=3), b"top"), (dict(top=-1), b"top"), (dict(temp=0.0), b"temperature"),
-                     (dict(temp=float("nan")), b"temperature"), (dict(temp=float("inf")), b"temperature"),
+                     (dict(temp=float("nan")), b"temperature"), (dict(temp=1e-39), b"temperature"), (dict(temp=float("inf")), b"temperature"),
                      (dict(logits=None), b"null"), (dict(logits=ctypes.c_void_p((1 << 20) + 1)), b"misaligned"),
                      (dict(out=None), b"null"), (dict(V=131072, ws=None), b"null"), (dict(st=-8), b"negative"),
                      (dict(V=131072, ws=ctypes.c_void_p((1 << 20) + 8)), b"256-byte"), (dict(R=1 << 30, T=1), b"too many")):
