@@ -3,22 +3,33 @@
 
 namespace {
 
-// Workgroups of one resident round of the split pass: three to a CU at rows of 64, two above
-int paged_round(int W) { return W == 64 ? 768 : 512; }
+// Workgroups of one resident round of the split pass: as many as the registers leave place for, one to a CU
+// with two column tiles of more than 64 columns, else two.  Both sides at 32 sequences of 8000 rows of 4 kv
+// heads, the column tiles of one token and of five of 8 query heads:
+//   rows of 128, five tokens: 160 us with 256 workgroups, 177 with 512
+//   rows of 64, five tokens:  100 us with 256, 81 with 512
+//   rows of 128, one token:   100 us with 512, 112 with 768
+// (a third of rows of 64 with one column tile has its place, and takes as long: 51 us with 512 and with 768)
+int paged_round(int W, int tiles) { return W > 64 && tiles == 2 ? 256 : 512; }
 
 // Row width of a page for a head dim (0: unsupported)
 int page_width(int D) { return D < 1 ? 0 : D <= 64 ? 64 : D <= 80 ? 80 : D <= 96 ? 96 : D <= 128 ? 128 : 0; }
 
+// log2 of a page size that is a power of two, whose rows are found by a shift (-1: by a division, 20.7 against
+// 20.2 us at 32 sequences of up to 3500 rows, nothing at one of 131072)
 int page_shift(int page) { return page & (page - 1) ? -1 : __builtin_ctz((unsigned)page); }
 
 // Workgroups of each kv head: one resident round, and no more than there can be units of rows
-int paged_target(int B, int Hkv, int64_t cap, int W) {
+int paged_target(int B, int Hkv, int64_t cap, int round) {
   const int64_t most = (int64_t)B * ((cap + lucid::kPagedUnit - 1) / lucid::kPagedUnit);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(most, paged_round(W) / Hkv));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, round / Hkv));
 }
 
 // Query heads of a chunk of a group (at most 31 and their key fill the columns of a score tile), and new
-// tokens of a pass: one 32-column tile, or two where the tokens do not fit one
+// tokens of a pass: one 32-column tile, or two where the tokens do not fit one.  At 8 query heads and 32
+// sequences of up to 3500 rows of 68 columns five tokens take 44 us in one pass of two tiles and 58 in two of
+// one; one token takes 20 us with one tile and 30 with two.  The last pass takes what its own tokens need
+// (8 tokens as 7 and 1: 75 us, 84 with two tiles for the one).
 int paged_heads(int G) {
   const int chunks = (G + 30) / 31;
   return (G + chunks - 1) / chunks;
@@ -103,16 +114,17 @@ int paged_combine(const PagedCall& c, int vec, const lucid::PagedBatch& seq, int
 template <int W>
 int paged_decode(const PagedCall& c) {
   const int G = c.Hq / c.Hkv, Gs = paged_heads(G), L = c.seq.L;
-  const int tiles = paged_tiles(Gs, L), most = paged_pass(Gs, L);
-  const int target = paged_target(c.seq.B, c.Hkv, (int64_t)c.seq.M * c.seq.page, W), slots = target + c.seq.B;
+  const int most = paged_pass(Gs, L);
+  // (rows at boundaries of 4 elements: 20.5 us where value by value takes 22.4, at five tokens 43 and 61)
   const int vec = rows_of_4(c.q, c.qs, 2) && rows_of_4(c.k, c.ks, 2) && rows_of_4(c.v, c.vs, 2);
   lucid::PagedBatch seq = c.seq;
   for (int t0 = 0; t0 < L; t0 += most) {
-    const int Lp = std::min(most, L - t0);
+    const int Lp = std::min(most, L - t0), tiles = paged_tiles(Gs, Lp);
+    const int target = paged_target(c.seq.B, c.Hkv, (int64_t)c.seq.M * c.seq.page, paged_round(W, tiles));
     seq.done = t0;
     for (int g0 = 0; g0 < G; g0 += Gs) {
       const int gc = std::min(Gs, G - g0);  // query heads of this chunk
-      const lucid::PagedPartials part = carve_paged(c.ws, slots, c.Hkv, gc, Lp, W, nullptr);
+      const lucid::PagedPartials part = carve_paged(c.ws, target + c.seq.B, c.Hkv, gc, Lp, W, nullptr);
       const dim3 grid(target, c.Hkv);
       if (tiles == 2)
         LUCID_LAUNCH("lucid_paged_split_kernel", (lucid::lucid_paged_split_kernel<W, 2>), grid, c.st, (const bf16*)c.q,
@@ -122,6 +134,9 @@ int paged_decode(const PagedCall& c) {
         LUCID_LAUNCH("lucid_paged_split_kernel", (lucid::lucid_paged_split_kernel<W, 1>), grid, c.st, (const bf16*)c.q,
                      S(c.qs), (const bf16*)c.k, S(c.ks), vec, c.kp, c.vp, seq, target, c.Hkv, Lp, c.scale, c.eps, c.D, part, gc,
                      G, g0);
+      // lane groups for the next 1, 4, 8 or 16 tokens: the instance of 4 takes 25 us of a call of one token where
+      // that of 1 takes 20, that of 16 takes 52 where that of 4 takes 45 at four tokens, 46 where that of 8
+      // takes 43 at five
       const int rc = Lp == 1   ? paged_combine<W, 1>(c, vec, seq, target, Lp, part, gc, g0, gc)
                      : Lp <= 4 ? paged_combine<W, 4>(c, vec, seq, target, Lp, part, gc, g0, gc)
                      : Lp <= 8 ? paged_combine<W, 8>(c, vec, seq, target, Lp, part, gc, g0, gc)
@@ -139,6 +154,7 @@ int write_pages(const void* k, const int64_t* ks, const void* v, const int64_t* 
   const int64_t blocks = ((int64_t)T * Hkv * (W / 8) + 255) / 256;
   if (blocks > (1 << 23)) return fail("lucid_write_pages: too many rows");
   const dim3 grid((unsigned)blocks, seq.B);
+  // (rows at boundaries of 4 elements: 51 us for 30011 rows of 8 heads of 128 columns, value by value 90)
   const int kvec = rows_of_4(k, ks, 2), vvec = rows_of_4(v, vs, v_f32 ? 4 : 2);
   if (v_f32)
     LUCID_LAUNCH("lucid_write_pages_kernel", (lucid::lucid_write_pages_kernel<W, float>), grid, st, (const bf16*)k, S(ks),
@@ -150,7 +166,9 @@ int write_pages(const void* k, const int64_t* ks, const void* v, const int64_t* 
 }
 
 // Token log probabilities: workgroups of 256 lanes for rows of up to 8192 values (and what a
-// misaligned row's first chunk leaves out), else of 1024 on segments of 32768
+// misaligned row's first chunk leaves out), else of 1024 on segments of 32768.  8000 rows of 8184 values take
+// 26 us in workgroups of 256 and 86 in those of 1024, 4 rows 3.5 and 5.3; 4000 of 32000 take 49 in those of
+// 1024, with no second launch to join four segments
 int lp_threads(int V) { return V + 7 <= 256 * lucid::kLpLane ? 256 : 1024; }
 int lp_segs(int V, bool aligned = false) {
   const int seg = lp_threads(V) * lucid::kLpLane;
@@ -226,7 +244,7 @@ int lucid_page_width(int D) { return page_width(D); }
 size_t lucid_decode_paged_workspace_bytes(int B, int Hq, int Hkv, int L, int page_size, int max_pages, int D) {
   if (!paged_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D)) return 0;
   const int W = page_width(D), Gs = paged_heads(Hq / Hkv);
-  const int slots = paged_target(B, Hkv, (int64_t)page_size * max_pages, W) + B;
+  const int slots = paged_target(B, Hkv, (int64_t)page_size * max_pages, paged_round(64, 1)) + B;
   size_t bytes = 0;
   carve_paged(nullptr, slots, Hkv, Gs, paged_pass(Gs, L), W, &bytes);
   return bytes;
@@ -317,6 +335,7 @@ int lucid_copy_pages(int num_pools, void* const* pools, int64_t page_stride_byte
     if (!pools[i]) return fail("lucid_copy_pages: pool " + std::to_string(i) + " is null");
     bits |= reinterpret_cast<uintptr_t>(pools[i]);
   }
+  // (in 16 bytes a lane 12.7 us for 30 pages of 16 layers, in 4 bytes 13.8; 400 pages 213 and 211, and 764 in bytes)
   const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
   const int64_t units = page_bytes / unit, pieces = (units + 256 * lucid::kCopyUnits - 1) / (256 * lucid::kCopyUnits);
   if (pieces > (1 << 23)) return fail("lucid_copy_pages: pages of more than 2^33 units");

@@ -133,6 +133,10 @@ __device__ __forceinline__ void lp_join(float& m, float& s, float& t, float c2) 
 // are collected and each counts the ones before it.  Rows with more than kLpCand values at or above the
 // bound (masks of one finite value, few allowed tokens, ordered logits) are tried again with the equal ones
 // limited to low indices, which is enough wherever such values are dense, and else taken one a round.
+// 4000 rows of 32000 bf16 values (256 MB): 49 us without alternatives, 5.2 TB/s; 73 with 8, 91 with 50, where
+// the workgroup's four barriers and the lists in LDS bound it.  8 rows with 20 alternatives: 8.2 us.  TOP = false
+// leaves the lists out (368 -> 317 us forward and backward of 8192 rows, when they still cost the second workgroup
+// on a CU).
 template <typename T, int NT, bool TOP>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lucid_token_logprobs_kernel(
     const T* __restrict__ logits, int64_t sb, int64_t st, int Tn, const int64_t* __restrict__ tokens, int V,
@@ -319,7 +323,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lu
 }
 
 // Rows of several segments, one workgroup each.  A key's place among the row's alternatives is
-// the number above it: its place in its own segment's list and those that it would have in the others'.
+// the number above it: its place in its own segment's list and those that it would have in the others' (by
+// bisection: 4.4 us for 4 rows with 50 alternatives, 5.5 with all keys compared).
 template <typename T>
 __global__ __launch_bounds__(256) void lucid_token_logprobs_merge_kernel(const T* __restrict__ logits, int64_t sb,
                                                                          int64_t st, int Tn,
@@ -375,7 +380,9 @@ struct LpGrads {
 };
 
 // Grid R x blocks (column blocks of a row).  Every value gets the softmax part; then the values that a token or an
-// alternative names are written once more with their whole gradient (rounded once).
+// alternative names are written once more with their whole gradient (rounded once).  Memory bounds it: 8192 rows of
+// 32000 bf16 values in 165 to 180 us (1.05 GB, 5.8 to 6.3 TB/s: part of the rows is still in the cache from the
+// forward), 1021 of 32003 fp32 values in 44.
 template <typename T>
 __global__ __launch_bounds__(256) void lucid_token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t sb,
                                                                        int64_t st, int Tn,

@@ -137,8 +137,8 @@ def lucid_decode_paged(query, key, value, key_pages, vprime_pages, page_table, c
             q.data_ptr(), _strides(q.stride()), k.data_ptr(), _strides(k.stride()), v.data_ptr(), _strides(v.stride()),
             key_pages.data_ptr(), _strides(key_pages.stride()), vprime_pages.data_ptr(),
             _strides(vprime_pages.stride()), page_table.data_ptr(), page_table.stride(0), cache_lens.data_ptr(),
-            o.data_ptr(), _strides((L * Hq * d, d, Hq * d)), vp_new.data_ptr(), ws.data_ptr(), B, Hq, Hkv, L, P, page, M, d,
-            d ** -0.5 if scaling is None else float(scaling), float(eps), _lib.stream_handle(device))
+            o.data_ptr(), _strides((L * Hq * d, d, Hq * d)), vp_new.data_ptr(), ws.data_ptr(), B, Hq, Hkv, L, P, page,
+            M, d, d ** -0.5 if scaling is None else float(scaling), float(eps), _lib.stream_handle(device))
     _lib.check(lib, rc, "lucid_decode_paged")
     return o, vp_new
 

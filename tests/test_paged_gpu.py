@@ -148,6 +148,13 @@ def test_decode_rows(lens, Hq, Hkv, L, d, page):
     _go(_case(lens, Hq, Hkv, L, d, page, seed=sum(lens) + d), page)
 
 
+@pytest.mark.parametrize("d", [64, 68, 128])
+def test_decode_passes_of_unequal_tokens(d):
+    """Eight tokens of eight query heads in a pass of two column tiles and one of one, in shares of their own."""
+    print(f"case paged decode unequal passes d={d}", flush=True)
+    _go(_case([3000, 40, -1, 700], 16, 2, 8, d, 64, seed=d), 64)
+
+
 @pytest.mark.parametrize("layout", ["rows", "pairs"])
 @pytest.mark.parametrize("d", [64, 68, 128])
 def test_decode_other_pool_layouts(layout, d):
