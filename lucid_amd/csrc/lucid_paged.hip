@@ -21,7 +21,10 @@
 namespace lucid {
 
 constexpr float PAGED_NEG = -1e30f;    // finite "minus infinity" for empty softmax states
-constexpr int kPagedUnit = 128;        // rows that a workgroup takes at a time (four waves' tiles)
+// Rows that a workgroup takes at a time, a tile for each of its four waves.  (Finer units balance the shares better and
+// leave waves without a tile: with 32 rows, and lead to match, 21.7 to 23.3 us for 20.2 at 32 sequences of up
+// to 3500 rows, 110 for 104 at one of 131072.)
+constexpr int kPagedUnit = 128;
 constexpr int kPagedLead = 1;          // places that a sequence takes in the line beside its rows
 constexpr int kPagedMaxTokens = 16;    // new tokens of a pass
 
@@ -691,8 +694,8 @@ __global__ __launch_bounds__(paged_threads<LM>()) void lucid_paged_combine_kerne
 // Rows t < count_b of k and v' [B][Hkv][T][d] into the pages from row lens[b] on, columns d .. W-1 zero;
 // rows whose page id lies outside the pool, or beyond the table, are left out.  A lane per 8 columns of a
 // row of both.  Grid (rows Hkv CPR / 256, B).  30011 rows of 8 heads of 128 columns, V' in fp32 (307 MB
-// read and written): 51 us with the inputs in cache from the call before, 59 without, 5.2 TB/s; the launch
-// alone bounds a batch of 4 x 300 (4.7 us).
+// read and written): 51 us with the inputs in cache from the call before, 59 without, 5.2 TB/s; four prompts
+// of 300 to 2048 rows (4 heads of 68) 4.7 us, which is little more than a launch.
 template <int W, typename TV>
 __global__ __launch_bounds__(256) void lucid_write_pages_kernel(const bf16* __restrict__ k, Strides kst, int kvec,
                                                                 const TV* __restrict__ v, Strides vst, int vvec,
