@@ -416,7 +416,7 @@ int lucid_copy_pages(int num_pools, void* const* pools, int64_t page_stride_byte
  * temperature.  logprobs[r] = x[tokens[r]] - lse (0 where the token is -100, NaN where it is outside
  * [0, V)), entropy[r] = lse - sum p x; top_logprobs / top_indices [R][top] by (logit descending, index
  * ascending).  A logit of -inf has probability 0; a row of -inf alone, or with a NaN or +inf, gives NaN (NaN
- * logits come first among the alternatives).  stats: 3 floats a row for the backward.  ws: 256-byte
+ * logits come first among the alternatives).  stats: 3 floats a row for the backward, or null.  ws: 256-byte
  * aligned, needed where its size is not 0.
  * The backward writes dlogits [R][V] (contiguous, the logits' dtype) from any of the three outputs'
  * gradients (null: none). */

@@ -376,7 +376,7 @@ int lucid_token_logprobs_fwd(const void* logits, int64_t batch_stride, int64_t r
     return rc;
   if (R == 0) return LUCID_OK;
   const int segs = lp_segs(V, lp_aligned(logits, batch_stride, row_stride, dtype));
-  if (!logprobs || !entropy || !stats || (top && (!top_logprobs || !top_indices)) || (segs > 1 && !ws))
+  if (!logprobs || !entropy || (top && (!top_logprobs || !top_indices)) || (segs > 1 && !ws))
     return fail("lucid_token_logprobs_fwd: null output or workspace");
   if (segs > 1)
     if (int rc = check_ws("ws", ws)) return rc;

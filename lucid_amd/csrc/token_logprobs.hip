@@ -87,7 +87,7 @@ __device__ __forceinline__ unsigned long long lp_wave_max(unsigned long long v) 
 struct LpOut {
   float* logprob;    // [R]
   float* entropy;    // [R]
-  LpStats* stats;    // [R]
+  LpStats* stats;    // [R] or null
   float* top_lp;     // [R][top]
   int64_t* top_idx;  // [R][top]
   // partials of rows of several segments
@@ -109,7 +109,7 @@ __device__ __forceinline__ float lp_finish(const LpOut& out, int r, float m, flo
     lp = tok < 0 || tok >= V ? __builtin_nanf("") : (xtok - m) * inv_temp - kLn2 * l2;
   out.logprob[r] = lp;
   out.entropy[r] = ent;
-  out.stats[r] = LpStats{m, l2, ent};
+  if (out.stats) out.stats[r] = LpStats{m, l2, ent};
   return l2;
 }
 

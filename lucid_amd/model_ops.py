@@ -309,15 +309,16 @@ def _logit_rows(logits: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     return rows, max(rows.shape[0], 1), 0, rows.stride(0)
 
 
-def _token_logprobs(logits: torch.Tensor, tok: torch.Tensor, top: int, temperature: float):
-    """(logprobs, entropy, top_logprobs, top_indices) and the rows' state for the backward."""
+def _token_logprobs(logits: torch.Tensor, tok: torch.Tensor, top: int, temperature: float, backward: bool):
+    """(logprobs, entropy, top_logprobs, top_indices) and, for a backward, the rows' state."""
     shape, V, dev = tok.shape, logits.shape[-1], logits.device
     rows, T, sb, st = _logit_rows(logits)
     R = tok.numel()
     lib = _lib.load()
     f32 = torch.float32
-    logprobs, entropy = torch.empty(shape, dtype=f32, device=dev), torch.empty(shape, dtype=f32, device=dev)
-    stats = torch.empty((R, 3), dtype=f32, device=dev)
+    logprobs = torch.empty_like(tok, dtype=f32)
+    entropy = torch.empty_like(logprobs)
+    stats = torch.empty((R, 3), dtype=f32, device=dev) if backward else None
     top_lp = torch.empty((*shape, top), dtype=f32, device=dev)
     top_idx = torch.empty((*shape, top), dtype=torch.int64, device=dev)
     nbytes = lib.lucid_token_logprobs_workspace_bytes(R, V, top)
@@ -325,8 +326,8 @@ def _token_logprobs(logits: torch.Tensor, tok: torch.Tensor, top: int, temperatu
     with _lib.on(dev):
         rc = lib.lucid_token_logprobs_fwd(
             rows.data_ptr(), sb, st, tok.data_ptr(), R, T, V, _LP_DTYPES[logits.dtype], temperature, top,
-            logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top_lp.data_ptr(), top_idx.data_ptr(),
-            None if ws is None else ws.data_ptr(), _lib.stream_handle(dev))
+            logprobs.data_ptr(), entropy.data_ptr(), None if stats is None else stats.data_ptr(),
+            top_lp.data_ptr(), top_idx.data_ptr(), None if ws is None else ws.data_ptr(), _lib.stream_handle(dev))
     _lib.check(lib, rc, "lucid_token_logprobs_fwd")
     return logprobs, entropy, top_lp, top_idx, stats
 
@@ -335,7 +336,7 @@ class TokenLogprobsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits: torch.Tensor, tokens: torch.Tensor, top: int, temperature: float):
         tok = tokens.contiguous()
-        logprobs, entropy, top_lp, top_idx, stats = _token_logprobs(logits, tok, top, temperature)
+        logprobs, entropy, top_lp, top_idx, stats = _token_logprobs(logits, tok, top, temperature, True)
         ctx.save_for_backward(logits, tok, stats, top_idx)
         ctx.top, ctx.temperature = top, temperature
         ctx.mark_non_differentiable(top_idx)
@@ -386,4 +387,4 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
         raise ValueError(f"lucid_amd.token_logprobs: the temperature must be positive and finite, got {temperature}")
     if logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, top, float(temperature)))
-    return TokenLogprobs(*_token_logprobs(logits.detach(), tokens.contiguous(), top, float(temperature))[:4])
+    return TokenLogprobs(*_token_logprobs(logits.detach(), tokens.contiguous(), top, float(temperature), False)[:4])
