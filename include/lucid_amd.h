@@ -389,7 +389,7 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
                        const int64_t* v_strides, void* k_pages, const int64_t* k_page_strides, void* vp_pages,
                        const int64_t* vp_page_strides, const int32_t* page_table, int64_t table_stride,
                        const int32_t* cache_lens, void* o, const int64_t* o_strides, float* vp_new, void* ws, int B, int Hq,
-                       int Hkv, int L, int num_pages, int page_size, int max_pages, int D, float scale, float eps,
+                       int Hkv, int L, int num_pages, int page_size, int max_pages, int D, double scale, float eps,
                        void* stream);
 
 /* A prefill's rows into the pages: row t < new_lens[b] (all T where new_lens is null) of k (bf16) and

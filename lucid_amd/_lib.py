@@ -23,6 +23,7 @@ _vp = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _int = ctypes.c_int
 _flt = ctypes.c_float
+_dbl = ctypes.c_double
 _sz = ctypes.c_size_t
 _i64 = ctypes.c_int64
 
@@ -105,7 +106,7 @@ _SIGS = {
         "lucid_page_width": ([_int], _int),
         "lucid_decode_paged_workspace_bytes": ([_int] * 7, _sz),
         "lucid_decode_paged": ([_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _i64p,
-                                _vp, _vp, _int, _int, _int, _int, _int, _int, _int, _int, _flt, _flt, _vp], _int),
+                                _vp, _vp, _int, _int, _int, _int, _int, _int, _int, _int, _dbl, _flt, _vp], _int),
         "lucid_write_pages": ([_vp, _i64p, _vp, _i64p, _int, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp,
                                _int, _int, _int, _int, _int, _int, _int, _vp], _int),
         "lucid_copy_pages": ([_int, ctypes.POINTER(_vp), _i64, _i64, _int, _int, ctypes.POINTER(_int),

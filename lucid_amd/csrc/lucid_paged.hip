@@ -118,6 +118,12 @@ struct PagedLine {
   }
 };
 
+// The scale s, and s log2 e and log2 e / s as the exponents take them
+struct PagedScale {
+  double s;
+  float sl2, c0;
+};
+
 // Four consecutive columns c .. c+3 of a row of d, zeros beyond d; vec: the row starts at an 8-byte
 // boundary
 __device__ __forceinline__ bf16x4 ld4_cols(const bf16* row, int c, int d, bool vec) {
@@ -182,7 +188,7 @@ __device__ __forceinline__ bf16x8 paged_tr_a(const bf16* tile, int row0, int col
 template <int W, int NCT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NCT > 1 ? (W <= 64 ? 2 : 1) : (W <= 64 ? 3 : 2)))) void
 lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __restrict__ kn, Strides kns, int vec,
-                         PagedPool kp, PagedPool vp, PagedBatch seq, int target, int Hkv, int Lp, float scale, float eps,
+                         PagedPool kp, PagedPool vp, PagedBatch seq, int target, int Hkv, int Lp, PagedScale factor, float eps,
                          int d, PagedPartials part, int Gs, int Gt, int g0) {
   constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = 32 * CPR / 64;
   __shared__ __attribute__((aligned(16))) PagedSmem<W> sm;
@@ -199,7 +205,7 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
   next = first + (rows + kPagedUnit - 1) / kPagedUnit;
   const int j0 = max(place - first, 0) * kPagedUnit, j1 = min(rows, (end - first) * kPagedUnit);
   if (j1 <= j0) break;  // the share ends in the sequence's lead
-  const float sl2 = scale * LOG2E_F, c0 = LOG2E_F / scale, dn = (float)d;
+  const float sl2 = factor.sl2, c0 = factor.c0, dn = (float)d;
 
   const int32_t* tbl = seq.table + b * seq.tstride;
   const int ntile = (j1 - j0 + 31) / 32;  // tiles of the part; wave w takes w, w + 4, ...
@@ -449,7 +455,7 @@ template <int W, int LM>
 __global__ __launch_bounds__(paged_threads<LM>()) void lucid_paged_combine_kernel(
     const bf16* __restrict__ q, Strides qs, const bf16* __restrict__ kn, Strides kns, const bf16* __restrict__ vn,
     Strides vns, int vec, int ovec, PagedPool kp, PagedPool vp, PagedBatch seq, int target, bf16* __restrict__ o, Strides os,
-    float* __restrict__ vp_new, int Hkv, int Lp, float scale, float eps, int d, PagedPartials part, int Gs, int Gt,
+    float* __restrict__ vp_new, int Hkv, int Lp, PagedScale factor, float eps, int d, PagedPartials part, int Gs, int Gt,
     int g0, int append) {
   constexpr int CG = W / 4, CGP = W == 64 ? 16 : 32, NT = paged_threads<LM>(), NG = NT / CGP, SL = NG / LM;
   static_assert(SL >= 1, "a lane group for every token");
@@ -583,7 +589,7 @@ __global__ __launch_bounds__(paged_threads<LM>()) void lucid_paged_combine_kerne
   }
   __syncthreads();
   const bool poison = bads != 0;
-  const float sl2 = scale * LOG2E_F, c0 = LOG2E_F / scale, dn = (float)d;
+  const float sl2 = factor.sl2, c0 = factor.c0, dn = (float)d;
   // the largest score of a token: over the slices and the new keys
   auto top_of = [&](int x) {
     float m = ms_[x];
@@ -602,9 +608,10 @@ __global__ __launch_bounds__(paged_threads<LM>()) void lucid_paged_combine_kerne
       const float rx = rsqrtf(kk[x][x] / dn + eps), ru = rsqrtf(kk[u][u] / dn + eps);
       pp[x][u] = __builtin_amdgcn_exp2f(fmaf(sl2 * rx * ru, kk[x][u], -c0));
     } else {
-      // 1 / P_tt; the exponent is the small difference of two terms of size sqrt(d): in fp64
+      // 1 / P_tt; the exponent is the small difference of two terms of size sqrt(d): in fp64, and from the scale in
+      // fp64 (from its fp32 value every V' was off by up to 2 sqrt(d) 2^-24: 3.4e-7 at d = 68, now 6e-8)
       const double ms = (double)kk[x][x] / d;
-      pp[x][x] = __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / scale - scale * d * ms / (ms + eps))));
+      pp[x][x] = __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / factor.s - factor.s * d * ms / (ms + eps))));
       top_[x] = m;
     }
   }

@@ -95,7 +95,8 @@ struct PagedCall {
   void *o, *ws;
   float* vp_new;
   int Hq, Hkv, D;
-  float scale, eps;
+  lucid::PagedScale scale;
+  float eps;
   hipStream_t st;
 };
 
@@ -254,7 +255,7 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
                        const int64_t* v_strides, void* k_pages, const int64_t* k_page_strides, void* vp_pages,
                        const int64_t* vp_page_strides, const int32_t* page_table, int64_t table_stride,
                        const int32_t* cache_lens, void* o, const int64_t* o_strides, float* vp_new, void* ws, int B, int Hq,
-                       int Hkv, int L, int num_pages, int page_size, int max_pages, int D, float scale, float eps,
+                       int Hkv, int L, int num_pages, int page_size, int max_pages, int D, double scale, float eps,
                        void* stream) {
   g_last_error.clear();
   if (!page_width(D)) return fail("head_dim must be in [1, 128], got " + std::to_string(D));
@@ -266,9 +267,11 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
       !cache_lens || !ws)
     return fail("lucid_decode_paged: null argument");
   if (table_stride < 0) return fail("lucid_decode_paged: negative table stride");
-  if (scale == 0.f) return fail("lucid_decode_paged: scale must not be 0");
+  if (scale == 0.) return fail("lucid_decode_paged: scale must not be 0");
   if (int rc = check_ws("ws", ws)) return rc;
-  PagedCall c{q, k, v, q_strides, k_strides, v_strides, o_strides, {}, {}, {}, o, ws, vp_new, Hq, Hkv, D, scale, eps,
+  constexpr double kLog2e = 1.4426950408889634;
+  PagedCall c{q, k, v, q_strides, k_strides, v_strides, o_strides, {}, {}, {}, o, ws, vp_new, Hq, Hkv, D,
+              {scale, (float)(scale * kLog2e), (float)(kLog2e / scale)}, eps,
               static_cast<hipStream_t>(stream)};
   const int W = page_width(D);
   if (int rc = check_pool("k_pages", k_pages, k_page_strides, num_pages, Hkv, page_size, W, &c.kp)) return rc;

@@ -155,6 +155,18 @@ def test_decode_passes_of_unequal_tokens(d):
     _go(_case([3000, 40, -1, 700], 16, 2, 8, d, 64, seed=d), 64)
 
 
+@pytest.mark.parametrize("d", [58, 68, 125, 127])
+def test_first_token_divides_by_the_exact_diagonal(d):
+    """V' of a sequence's first token is v / P_tt: an exponential (2^-23) and a product (2^-24), with no error from a scale
+    d^-1/2 that fp32 does not hold (which alone makes 15 2^-24 at d = 127)."""
+    print(f"case paged first token d={d}", flush=True)
+    c = _case([0, 0, 0], 2, 2, 1, d, 16, seed=d)
+    _, vnew = _go(c, 16)
+    ms, s = c["k"].double().square().mean(-1, keepdim=True), d ** -0.5
+    want = c["v"].double() / (s * d * ms / (ms + 1e-5) - 1 / s).exp()
+    assert bool(((vnew.double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all())
+
+
 @pytest.mark.parametrize("layout", ["rows", "pairs"])
 @pytest.mark.parametrize("d", [64, 68, 128])
 def test_decode_other_pool_layouts(layout, d):
