@@ -27,6 +27,11 @@ constexpr float PAGED_NEG = -1e30f;    // finite "minus infinity" for empty soft
 constexpr int kPagedUnit = 128;
 constexpr int kPagedLead = 1;          // places that a sequence takes in the line beside its rows
 constexpr int kPagedMaxTokens = 16;    // new tokens of a pass
+// Cache policy of the direct loads of V' (the instruction's nt bit): each line is read once, by one
+// instruction, and need not push others out.  131072 rows of 8 kv heads 106 -> 96 us, 32 sequences of 8192 rows
+// of 4 102 -> 93 at 128 columns and 61 -> 57 at 64, caches changing from call to call.  The keys keep the usual
+// policy: a line of theirs is read by several instructions of a wave (with the bit 125 us).
+constexpr int kPagedOnce = 2;
 
 struct PagedBatch {
   const int32_t* table;  // [B][M] page ids, rows tstride apart
@@ -182,7 +187,7 @@ __device__ __forceinline__ bf16x8 paged_tr_a(const bf16* tile, int row0, int col
 // product as a bf16 pair (hi + lo, 2^-17), since V' is returned in fp32 and one bf16 term of P
 // would be seen in it.  Page ids reach registers two tiles ahead, rows one.  Columns of the NCT
 // 32-column tiles: Lp (Gs + 1) <= 32 NCT.
-// Memory bounds it: 131072 rows of 8 kv heads of 128 columns (537 MB) in 99 us, 5.4 TB/s with nothing read
+// Memory bounds it: 131072 rows of 8 kv heads of 128 columns (537 MB) in 90 us, 6.0 TB/s with nothing read
 // twice by the counters.  At 32 sequences of up to 3500 rows it takes 14 us for 27 MB: the lengths, a page
 // id, a row, each waiting for the one before, take 7 of them.
 template <int W, int NCT>
@@ -237,7 +242,7 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
       int c = qq % CPR;
       if constexpr (PagedSmem<W>::kSwz) c ^= r & 7;
       const bf16* src = paged_at(vp, __shfl((int)voff, r, 64)) + c * 8;
-      __builtin_amdgcn_global_load_lds(src, dst + i * 512, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(src, dst + i * 512, 16, 0, kPagedOnce);
     }
   };
   // the first pages' ids, then the new tokens' rows, then the first tile: each wait covers the next loads
@@ -437,7 +442,8 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
 }
 
 // The combine kernel's workgroup: CGP lanes (W / 4 of them, 4 columns each) for every token and slice of
-// the parts.
+// the parts.  One token of 32 sequences takes 20 us in workgroups of 256 and 25 in those of 512 (five tokens 44 in
+// 512, 57 in 1024): more slices wait for one another.
 template <int LM>
 constexpr int paged_threads() {
   return LM == 1 ? 256 : 512;
@@ -459,7 +465,7 @@ __global__ __launch_bounds__(paged_threads<LM>()) void lucid_paged_combine_kerne
     int g0, int append) {
   constexpr int CG = W / 4, CGP = W == 64 ? 16 : 32, NT = paged_threads<LM>(), NG = NT / CGP, SL = NG / LM;
   static_assert(SL >= 1, "a lane group for every token");
-  constexpr int UN = 4;  // parts whose loads a lane has in flight
+  constexpr int UN = 4;  // parts whose loads a lane has in flight (8: 57 us for 44 at five tokens of 32 sequences)
   __shared__ float kk[LM][LM], qk[LM][LM];  // k_t . k_u and q_tg . k_u (u <= t)
   __shared__ float pp[LM][LM], ww[LM][LM];  // P_tu (1 / P_tt), and u's weight in token t's softmax
   __shared__ f32x4 os_[NG][CGP], as_[NG][CGP], vps[LM][CGP];
@@ -701,8 +707,9 @@ __global__ __launch_bounds__(paged_threads<LM>()) void lucid_paged_combine_kerne
 // Rows t < count_b of k and v' [B][Hkv][T][d] into the pages from row lens[b] on, columns d .. W-1 zero;
 // rows whose page id lies outside the pool, or beyond the table, are left out.  A lane per 8 columns of a
 // row of both.  Grid (rows Hkv CPR / 256, B).  30011 rows of 8 heads of 128 columns, V' in fp32 (307 MB
-// read and written): 51 us with the inputs in cache from the call before, 59 without, 5.2 TB/s; four prompts
-// of 300 to 2048 rows (4 heads of 68) 4.7 us, which is little more than a launch.
+// read and written): 58 us, 5.3 TB/s, with stores that pass the caches by (61 without: a long prompt's pages do
+// not stay there until they are read); four prompts of 300 to 2048 rows (4 heads of 68) 5.7 us both ways, which is
+// little more than a launch.
 template <int W, typename TV>
 __global__ __launch_bounds__(256) void lucid_write_pages_kernel(const bf16* __restrict__ k, Strides kst, int kvec,
                                                                 const TV* __restrict__ v, Strides vst, int vvec,
@@ -745,14 +752,17 @@ __global__ __launch_bounds__(256) void lucid_write_pages_kernel(const bf16* __re
       for (int i = 0; i < 4; ++i) y[4 * q + i] = (bf16)f[i];
     }
   }
-  *reinterpret_cast<bf16x8*>(paged_at(kp, id * kp.page + h * kp.head + in * kp.row) + c) = x;
-  *reinterpret_cast<bf16x8*>(paged_at(vp, id * vp.page + h * vp.head + in * vp.row) + c) = y;
+  bf16* kd = paged_at(kp, id * kp.page + h * kp.head + in * kp.row) + c;
+  bf16* vd = paged_at(vp, id * vp.page + h * vp.head + in * vp.row) + c;
+  __builtin_nontemporal_store(x, reinterpret_cast<bf16x8*>(kd));
+  __builtin_nontemporal_store(y, reinterpret_cast<bf16x8*>(vd));
 }
 
 // Pages copied within each of several pools of one layout.  Pool pointers and page pairs travel in the
 // kernel argument: no upload, and a captured launch keeps them.  Grid (pieces, pairs, pools); a
 // workgroup copies one piece of kCopyUnits units U a lane (8 units: 216 us where 4 take 211).  400 pages of 16
-// layers' pools (524 MB read, 524 written) take 211 us, 5.0 TB/s; 8 pages 3.2 us, a launch.
+// layers' pools (524 MB read, 524 written) take 203 us, 5.2 TB/s, past the caches (through them 214; 100 pages
+// 53 and 56; 30 pages 17 both ways, and 15.5 where 12.7 if they are in the cache); 8 pages 3 us, a launch.
 constexpr int kCopyPools = 64, kCopyPairs = 256;
 constexpr int kCopyUnits = 4;
 struct CopyPages {
@@ -767,10 +777,10 @@ __global__ __launch_bounds__(256) void lucid_copy_pages_kernel(const CopyPages a
   U x[kCopyUnits];
 #pragma unroll
   for (int i = 0; i < kCopyUnits; ++i)
-    if (i0 + 256 * i < units) x[i] = s[i0 + 256 * i];
+    if (i0 + 256 * i < units) x[i] = __builtin_nontemporal_load(s + i0 + 256 * i);
 #pragma unroll
   for (int i = 0; i < kCopyUnits; ++i)
-    if (i0 + 256 * i < units) t[i0 + 256 * i] = x[i];
+    if (i0 + 256 * i < units) __builtin_nontemporal_store(x[i], t + i0 + 256 * i);
 }
 
 }  // namespace lucid

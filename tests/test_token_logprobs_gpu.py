@@ -105,6 +105,15 @@ def test_forward_and_gradient(V, R, top, temperature, dtype):
     _run(logits, tokens, top, temperature)
 
 
+@pytest.mark.parametrize("dtype,R", [(torch.bfloat16, 1600), (torch.float32, 801)])
+def test_gradients_of_100_megabytes(dtype, R):
+    """Gradients from the size on that passes the caches by, the named values among them (written a second time)."""
+    print(f"case large gradient R={R} {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(R)
+    logits = (2.5 * torch.randn(R, 32003, generator=g, device="cuda")).to(dtype)
+    _run(logits, torch.randint(0, 32003, (R,), generator=g, device="cuda"), 8, 1.0)
+
+
 @pytest.mark.parametrize("V", [40, 9000, 32003, 40000])
 @pytest.mark.parametrize("kind", ["inf", "lowest", "few", "const", "steps", "ramp", "fall", "zeros"])
 def test_masked_tied_and_ordered_rows(kind, V):
