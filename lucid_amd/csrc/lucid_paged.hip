@@ -707,7 +707,7 @@ __global__ __launch_bounds__(paged_threads<LM>()) void lucid_paged_combine_kerne
 // Rows t < count_b of k and v' [B][Hkv][T][d] into the pages from row lens[b] on, columns d .. W-1 zero;
 // rows whose page id lies outside the pool, or beyond the table, are left out.  A lane per 8 columns of a
 // row of both.  Grid (rows Hkv CPR / 256, B).  30011 rows of 8 heads of 128 columns, V' in fp32 (307 MB
-// read and written): 58 us, 5.3 TB/s, with stores that pass the caches by (61 without: a long prompt's pages do
+// read and written): 55.5 us, 5.5 TB/s, with stores that pass the caches by (58.5 without: a long prompt's pages do
 // not stay there until they are read); four prompts of 300 to 2048 rows (4 heads of 68) 5.7 us both ways, which is
 // little more than a launch.
 template <int W, typename TV>

@@ -381,8 +381,7 @@ struct LpGrads {
 
 // Grid R x blocks (column blocks of a row).  Every value gets the softmax part; then the values that a token or an
 // alternative names are written once more with their whole gradient (rounded once).  Memory bounds it: 8192 rows of
-// 32000 bf16 values in 165 to 180 us (1.05 GB, 5.8 to 6.3 TB/s: part of the rows is still in the cache from the
-// forward), 1021 of 32003 fp32 values in 44.  PAST: the gradient passes the caches by (the launcher's rule).
+// 32000 bf16 values in 165 to 180 us (1.05 GB, 5.8 to 6.3 TB/s), 1021 of 32003 fp32 values in 44.  PAST: the gradient passes the caches by (the launcher's rule).
 template <typename T, bool PAST>
 __global__ __launch_bounds__(256) void lucid_token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t sb,
                                                                        int64_t st, int Tn,
