@@ -23,6 +23,10 @@ constexpr int kLpMaxTop = 64;   // alternatives of a row
 constexpr int kLpCand = 1024;   // values considered for the alternatives of a segment
 constexpr int kLpMaxSegs = 64;  // segments of a row
 constexpr float kLpNone = -1000.f;  // a log2 probability whose exp2 is 0: stands for every lower one
+// Largest |m c| whose wave takes a = x c - m c in one fma: the product's rounding, by which every a is then off, is
+// at most 2^-5 below it and leaves exactly.  Beyond it (a wave of values all masked with -1e9, say) the rounding grows
+// to whole powers of two, from 2^31 on past exp2's range.
+constexpr float kLpOneStep = 1048576.f;
 
 // What a forward row leaves for the backward: p_j = exp2(a_j - l2), a_j = (logit_j - m) c with c = log2 e /
 // temperature (the difference first: one of two logits of the type's lowest value is 0, where their products
@@ -173,7 +177,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lu
   m = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, lanes_max<64>(m))));
   const float c2 = LOG2E_F * inv_temp, mref = m == -INFINITY ? 0.f : m, mc = mref * c2;
   float s = 0.f, t = 0.f;  // p = 0 where a = -inf
-  if (fabsf(mc) < 1e37f) {  // a = x c - m c in one step
+  const bool one_step = fabsf(mc) < kLpOneStep;
+  if (one_step) {  // a = x c - m c
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -183,7 +188,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lu
         t = fmaf(p, fmaxf(a, kLpNone), t);
       }
     }
-  } else {  // a maximum near the type's lowest or largest value (or inf), whose product overflows
+  } else {  // the difference first: a finite mask's value, or inf
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -198,7 +203,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lu
   t = lanes_sum<64>(t);
   if (lane == 0) {
     // m c was rounded: every a is larger by the difference (exact in one fma), which leaves here
-    const float off = fabsf(mc) < 1e37f ? fmaf(mref, c2, -mc) : 0.f, f = __builtin_amdgcn_exp2f(-off);
+    const float off = one_step ? fmaf(mref, c2, -mc) : 0.f, f = __builtin_amdgcn_exp2f(-off);
     red[0][w] = m;
     red[1][w] = s * f;
     red[2][w] = fmaf(-off, s, t) * f;
