@@ -419,7 +419,8 @@ int lucid_copy_pages(int num_pools, void* const* pools, int64_t page_stride_byte
  * logits come first among the alternatives).  stats: 3 floats a row for the backward, or null.  ws: 256-byte
  * aligned, needed where its size is not 0.
  * The backward writes dlogits [R][V] (contiguous, the logits' dtype) from any of the three outputs'
- * gradients (null: none). */
+ * gradients (null: none); a row whose incoming gradients are all 0, an ignored one, say, gets zeros whatever its
+ * logits are. */
 size_t lucid_token_logprobs_workspace_bytes(int R, int V, int top);
 int lucid_token_logprobs_fwd(const void* logits, int64_t batch_stride, int64_t row_stride, const int64_t* tokens, int R,
                              int T, int V, int dtype, float temperature, int top, float* logprobs, float* entropy,

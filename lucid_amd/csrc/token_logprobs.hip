@@ -416,14 +416,18 @@ __global__ __launch_bounds__(256) void lucid_token_logprobs_bwd_kernel(const T* 
   }
   __syncthreads();
   float all = glp;
-  for (int k = 1; k <= top; ++k) all += gain[k];
   const float gh = g.ent ? g.ent[r] : 0.f;
+  bool wanted = glp != 0.f || gh != 0.f;  // no gradient comes in: none goes out, whatever the row holds
+  for (int k = 1; k <= top; ++k) {
+    all += gain[k];
+    wanted |= gain[k] != 0.f;
+  }
   // dx of the softmax part: -p (all + gh (ln p + H)), ln p = ln2 a
   const float ka = all + gh * z.ent, kb = gh * 0.69314718055994531f;
   auto soft = [&](float x) {
     const float a = fmaf(x - z.m, c2, -z.l2);
     const float p = __builtin_amdgcn_exp2f(a);
-    return -p * fmaf(kb, fmaxf(a, kLpNone), ka);
+    return wanted ? -p * fmaf(kb, fmaxf(a, kLpNone), ka) : 0.f;
   };
   const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) / sizeof(T) == (unsigned)row.shift;
   const int q0 = col * NT * C + tid;

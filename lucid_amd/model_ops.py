@@ -371,7 +371,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     ``logits [..., V]`` bf16 or fp32 on the GPU, ``tokens [...]`` int64; results in fp32.  A token of -100 (the
     loss's ignore index) has the log probability 0 and no gradient, one outside ``[0, V)`` NaN.  The alternatives are
     ordered by their logits, equal ones by the lower index.  Logits of -inf have probability 0; a row of -inf
-    alone, or with a NaN or +inf, gives NaN as torch's log_softmax does."""
+    alone, or with a NaN or +inf, gives NaN as torch's log_softmax does; in the gradient too, unless nothing comes
+    in for it (an ignored row of a padded batch, say): zeros then."""
     if not logits.is_cuda:
         raise RuntimeError("lucid_amd: logits must be a GPU tensor (no CPU path)")
     if logits.dtype not in _LP_DTYPES or tokens.dtype != torch.int64 or tokens.device != logits.device:

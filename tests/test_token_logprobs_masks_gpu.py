@@ -8,6 +8,7 @@ difference and the product, 2^-24 each) as every other one.
 import pytest
 import torch
 
+from lucid_amd.model_ops import token_logprobs
 from test_token_logprobs_gpu import _run
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +57,29 @@ def test_small_temperatures():
     x[1] -= 200.0
     for temperature in (1e-4, 1e-6, 1e-12):
         _run(x, x.argmax(-1), 3, temperature)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,top", [(50, 0), (9001, 4), (40000, 4)])
+def test_ignored_rows_without_a_distribution_have_no_gradient(V, top, dtype):
+    """A token of -100 has no gradient, whatever its row holds: nothing allowed, a NaN, an infinity.  With a gradient of
+    the entropy or of an alternative such a row gives NaN, as ever, and the rows beside it are not affected."""
+    print(f"case ignored rows V={V} top={top} {dtype}", flush=True)
+    x0 = torch.randn(4, V, device="cuda").to(dtype)
+    x0[0] = float("-inf")
+    x0[1, V // 2] = float("nan")
+    x0[2, V - 1] = float("inf")
+    tokens = torch.tensor([-100, -100, -100, 3], device="cuda")
+    x = x0.clone().requires_grad_()
+    r = token_logprobs(x, tokens, top=top)
+    assert r.logprobs[:3].tolist() == [0.0, 0.0, 0.0]
+    dx, = torch.autograd.grad(r.logprobs.sum(), x, retain_graph=True)
+    assert bool((dx[:3] == 0).all()) and bool((dx[3] != 0).any()) and bool(torch.isfinite(dx[3]).all())
+    one = torch.tensor([1.0, 0.0, 0.0, 0.0], device="cuda")
+    dx, = torch.autograd.grad(r.entropy, x, one, retain_graph=True)
+    assert bool(torch.isnan(dx[0]).any()) and bool((dx[1:] == 0).all())
+    if top:
+        g = torch.zeros(4, top, device="cuda")
+        g[1, 1], g[1, 2] = 1.0, -1.0
+        dx, = torch.autograd.grad(r.top_logprobs, x, g)
+        assert bool(torch.isnan(dx[1]).any()) and bool((dx[0] == 0).all()) and bool((dx[2:] == 0).all())
