@@ -30,6 +30,7 @@ import operator
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -372,7 +373,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     loss's ignore index) has the log probability 0 and no gradient, one outside ``[0, V)`` NaN.  The alternatives are
     ordered by their logits, equal ones by the lower index.  Logits of -inf have probability 0; a row of -inf
     alone, or with a NaN or +inf, gives NaN as torch's log_softmax does; in the gradient too, unless nothing comes
-    in for it (an ignored row of a padded batch, say): zeros then."""
+    in for it (an ignored row of a padded batch, say): zeros then.  Forward-mode differentiation is refused
+    (NotImplementedError)."""
     if not logits.is_cuda:
         raise RuntimeError("lucid_amd: logits must be a GPU tensor (no CPU path)")
     if logits.dtype not in _LP_DTYPES or tokens.dtype != torch.int64 or tokens.device != logits.device:
@@ -386,6 +388,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
         raise ValueError(f"lucid_amd.token_logprobs: top must be in [0, min({MAX_TOP}, V)], got {top}")
     if not 0.0 < temperature < float("inf"):
         raise ValueError(f"lucid_amd.token_logprobs: the temperature must be positive and finite, got {temperature}")
-    if logits.requires_grad and torch.is_grad_enabled():
+    # (a tangent of forward-mode differentiation takes the autograd function too, which refuses it)
+    if logits.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(logits).tangent is not None:
         return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, top, float(temperature)))
     return TokenLogprobs(*_token_logprobs(logits.detach(), tokens.contiguous(), top, float(temperature), False)[:4])
