@@ -207,7 +207,8 @@ int check_lp(const char* what, const void* logits, int64_t sb, int64_t st, const
   if (R < 0 || Tn < 1 || R % Tn) return fail(w + ": R a multiple of the rows of a batch, got R=" + std::to_string(R));
   if (V < 1 || V > 2000000) return fail(w + ": V from 1 to 2000000, got " + std::to_string(V));
   if (top < 0 || top > lucid::kLpMaxTop || top > V) return fail(w + ": top from 0 to 64 and at most V, got " + std::to_string(top));
-  if (!(temperature > 0.f) || std::isinf(temperature) || std::isinf(1.f / temperature))
+  // (log2 e / temperature too, the factor of the exponents: from 4.24e-39 down it is infinite)
+  if (!(temperature > 0.f) || std::isinf(temperature) || std::isinf(LOG2E_F * (1.f / temperature)))
     return fail(w + ": the temperature and its inverse must be positive and finite");
   if (sb < 0 || st < 0) return fail(w + ": negative strides");
   if (R == 0) return LUCID_OK;
