@@ -208,7 +208,8 @@ lucid_paged_split_kernel(const bf16* __restrict__ q, Strides qs, const bf16* __r
   asm volatile("" : "+v"(tid));  // what follows from it is worked out here, not kept in registers across the sequences
   const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
   next = first + (rows + kPagedUnit - 1) / kPagedUnit;
-  const int j0 = max(place - first, 0) * kPagedUnit, j1 = min(rows, (end - first) * kPagedUnit);
+  // (a share can hold more rows than 32 bits count, a sequence cannot)
+  const int j0 = max(place - first, 0) * kPagedUnit, j1 = end >= next ? rows : (end - first) * kPagedUnit;
   if (j1 <= j0) break;  // the share ends in the sequence's lead
   const float sl2 = factor.sl2, c0 = factor.c0, dn = (float)d;
 

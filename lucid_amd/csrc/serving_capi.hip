@@ -3,6 +3,9 @@
 
 namespace {
 
+// Most workgroups of one resident round of the split pass for a kv head
+constexpr int kPagedRound = 512;
+
 // Workgroups of one resident round of the split pass: as many as the registers leave place for, one to a CU
 // with two column tiles of more than 64 columns, else two.  Both sides at 32 sequences of 8000 rows of 4 kv
 // heads, the column tiles of one token and of five of 8 query heads:
@@ -10,7 +13,7 @@ namespace {
 //   rows of 64, five tokens:  100 us with 256, 81 with 512
 //   rows of 128, one token:   100 us with 512, 112 with 768
 // (a third of rows of 64 with one column tile has its place, and takes as long: 51 us with 512 and with 768)
-int paged_round(int W, int tiles) { return W > 64 && tiles == 2 ? 256 : 512; }
+int paged_round(int W, int tiles) { return W > 64 && tiles == 2 ? 256 : kPagedRound; }
 
 // Row width of a page for a head dim (0: unsupported)
 int page_width(int D) { return D < 1 ? 0 : D <= 64 ? 64 : D <= 80 ? 80 : D <= 96 ? 96 : D <= 128 ? 128 : 0; }
@@ -57,10 +60,13 @@ lucid::PagedPartials carve_paged(void* base, int64_t slots, int Hkv, int Gs, int
   return part;
 }
 
+// The places of the line of sequences, and those of a share behind its end for every workgroup (the shares are rounded
+// up, and a share's end is worked out before it is cut to the line's), are counted in 32 bits.
 bool paged_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int D) {
   return B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && L > 0 && page > 0 && max_pages > 0 && page_width(D) &&
          (int64_t)page * max_pages <= (1 << 30) && (int64_t)B * Hkv <= (1 << 22) && B <= (1 << 20) && Hkv <= 65535 &&
-         B * (((int64_t)page * max_pages + lucid::kPagedUnit - 1) / lucid::kPagedUnit + lucid::kPagedLead) < ((int64_t)1 << 31);
+         B * (((int64_t)page * max_pages + lucid::kPagedUnit - 1) / lucid::kPagedUnit + lucid::kPagedLead) <
+             ((int64_t)1 << 31) - 2 * kPagedRound;
 }
 
 int check_pool(const char* name, void* p, const int64_t* s, int pages, int Hkv, int page, int W, lucid::PagedPool* out) {
