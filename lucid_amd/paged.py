@@ -240,7 +240,9 @@ class LucidPagedCache:
     shares the full pages of another and has its own copy of the partial last one; :meth:`free` returns pages that no
     sequence uses any more, the lowest free id being given out first; :meth:`compact` moves the pages in use to the
     front of the pools.  The bookkeeping is host work on page ids; only rows and copied pages touch the GPU, on the
-    current stream.  bf16, one device, not thread safe."""
+    current stream.  A graph would not replay the host's part, so passes, forks and compactions are refused while the
+    current stream is being captured (the operators of this module, on tables and lengths of the caller's, are not).
+    bf16, one device, not thread safe."""
 
     def __init__(self, num_pages: int, page_size: int = 64, device="cuda"):
         if num_pages < 1 or page_size < 1:
@@ -257,6 +259,11 @@ class LucidPagedCache:
         self._lengths: Optional[list[int]] = None
         self._dev: Optional[tuple] = None  # (table, lens, 1 in the live rows) of the selection, on the device
         self._step: Optional[PagedStep] = None
+
+    def _not_captured(self, what: str) -> None:
+        if self.device.type == "cuda" and torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"lucid_amd: a LucidPagedCache's {what} cannot be captured into a graph: a replay would "
+                               "not repeat its bookkeeping")
 
     # -- sequences -----------------------------------------------------------------------------
 
@@ -292,6 +299,7 @@ class LucidPagedCache:
     def fork(self, seq: int) -> int:
         """A sequence with the rows of ``seq``: its full pages shared, its partial last page copied (all layers in one
         launch).  Raises :class:`OutOfPages` where there is no page for the copy."""
+        self._not_captured("fork")
         full, part = divmod(self._lens[seq], self.page_size)
         pages = self._pages[seq]
         if part and not self._free:
@@ -323,6 +331,7 @@ class LucidPagedCache:
     def compact(self) -> int:
         """Moves the pages in use to the ids 0 .. n - 1 (all layers in one launch); the number of pages moved.  Those
         beyond n go to the free ids below n, in order."""
+        self._not_captured("compaction")
         n = self.num_pages - len(self._free)
         src = [p for p in range(n, self.num_pages) if self._refs[p]]
         dst = sorted(p for p in self._free if p < n)
@@ -358,6 +367,7 @@ class LucidPagedCache:
     def begin(self, B: int, T: int) -> PagedStep:
         """Makes room for a pass of T tokens a row and describes it to the layers (the model calls this).  Raises
         :class:`OutOfPages` before anything is changed."""
+        self._not_captured("pass")
         if len(self._batch) != B:
             raise ValueError(f"lucid_amd: {B} rows, but {len(self._batch)} selected sequences (LucidPagedCache.select)")
         counts = self._lengths
