@@ -323,7 +323,7 @@ class LucidPagedCache:
             self._lens[seq]  # (KeyError before anything is changed)
         for seq in seqs:
             if seq in self._batch:
-                self._batch, self._dev = (), None
+                self._batch, self._dev, self._step = (), None, None
             del self._lens[seq]
             for page in self._pages.pop(seq):
                 self._drop(page)
@@ -342,7 +342,7 @@ class LucidPagedCache:
         for a, b in to.items():
             self._refs[b], self._refs[a] = self._refs[a], 0
         self._free = list(range(n, self.num_pages))
-        self._dev = None
+        self._dev = self._step = None
         return len(src)
 
     # -- forward passes ------------------------------------------------------------------------
@@ -363,11 +363,13 @@ class LucidPagedCache:
         if seqs != self._batch:
             self._batch, self._dev = seqs, None
         self._lengths = None if lengths is None else [int(n) for n in lengths]
+        self._step = None
 
     def begin(self, B: int, T: int) -> PagedStep:
         """Makes room for a pass of T tokens a row and describes it to the layers (the model calls this).  Raises
         :class:`OutOfPages` before anything is changed."""
         self._not_captured("pass")
+        self._step = None
         if len(self._batch) != B:
             raise ValueError(f"lucid_amd: {B} rows, but {len(self._batch)} selected sequences (LucidPagedCache.select)")
         counts = self._lengths
@@ -400,9 +402,11 @@ class LucidPagedCache:
 
     @property
     def step(self) -> PagedStep:
-        """The pass that :meth:`begin` described."""
+        """The pass that :meth:`begin` described, until it is committed; a selection, a compaction or the end of one of
+        its sequences ends it too, with nothing counted."""
         if self._step is None:
-            raise RuntimeError("lucid_amd: no forward pass has begun (LucidPagedCache.begin)")
+            raise RuntimeError("lucid_amd: no forward pass has begun (LucidPagedCache.begin), or its sequences or pages have "
+                               "changed since")
         return self._step
 
     def commit(self) -> None:
