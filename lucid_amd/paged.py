@@ -78,7 +78,8 @@ def _refuse(what, device, dims, key_pages, vprime_pages, page_table, lens):
 
 def _table_ok(page_table, B, device) -> bool:
     return (page_table.dtype is torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B
-            and page_table.shape[1] > 0 and page_table.stride(1) == 1 and page_table.device == device)
+            and page_table.shape[1] > 0 and (page_table.stride(1) == 1 or page_table.shape[1] == 1)
+            and page_table.device == device)
 
 
 def _lens_ok(t, B, device) -> bool:

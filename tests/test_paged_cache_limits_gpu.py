@@ -42,3 +42,26 @@ def test_a_captured_pass_is_refused_and_the_next_one_runs():
         outs.append(out)
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(*outs))
+
+
+def test_tables_of_one_page():
+    """A table of one column is contiguous whatever its strides say, and its rows may be any distance apart."""
+    from lucid_amd.paged import lucid_decode_paged, write_pages
+    g = torch.Generator(device="cuda").manual_seed(2)
+    kp, vp = (torch.randn(6, 2, 16, 64, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    q, k, v = (torch.randn(3, h, 1, 64, generator=g, device="cuda").to(torch.bfloat16) for h in (4, 2, 2))
+    lens = torch.tensor([3, 0, 15], dtype=torch.int32, device="cuda")
+    ids = torch.tensor([[4, 0, 2]], dtype=torch.int32, device="cuda")
+    wide = torch.full((3, 7), 5, dtype=torch.int32, device="cuda")
+    wide[:, 3] = ids[0]
+    outs = []
+    for table in (ids[0][:, None].clone(), ids.t(), wide[:, 3:4], torch.as_strided(ids, (3, 1), (1, 3))):
+        assert table.shape == (3, 1)
+        a, b = kp.clone(), vp.clone()
+        outs.append([*lucid_decode_paged(q, k, v, a, b, table, lens), a, b])
+        a, b = kp.clone(), vp.clone()
+        write_pages(k, v, a, b, table, lens)
+        outs[-1] += [a, b]
+    assert ids.t().stride() == (1, 3)
+    for other in outs[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(outs[0], other))
