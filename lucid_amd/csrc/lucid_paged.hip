@@ -27,10 +27,15 @@ constexpr float PAGED_NEG = -1e30f;    // finite "minus infinity" for empty soft
 constexpr int kPagedUnit = 128;
 constexpr int kPagedLead = 1;          // places that a sequence takes in the line beside its rows
 constexpr int kPagedMaxTokens = 16;    // new tokens of a pass
-// Cache policy of the direct loads of V' (the instruction's nt bit): each line is read once, by one
-// instruction, and need not push others out.  131072 rows of 8 kv heads 106 -> 96 us, 32 sequences of 8192 rows
-// of 4 102 -> 93 at 128 columns and 61 -> 57 at 64, caches changing from call to call.  The keys keep the usual
-// policy: a line of theirs is read by several instructions of a wave (with the bit 125 us).
+// Cache policy of the direct loads of V' (the instruction's nt bit): where no page is shared, a pass reads each line
+// once, by one instruction, and need not push others out.  131072 rows of 8 kv heads 106 -> 96 us, 32 sequences of
+// 8192 rows of 4 102 -> 93 at 128 columns and 61 -> 57 at 64, caches changing from call to call.  The keys keep the
+// usual policy: a line of theirs is read by several instructions of a wave (with the bit 125 us).
+// Lines that are read again, with the bit and without it: in pages that sequences share it costs up to 5 % (32
+// samples of a prompt of 8192 rows 83 and 79 us, 64 of 1024 37.9 and 36.3, 8 of 8192 36.8 and 36.2, 8 of 32768 the
+// same); by the second chunk of 32 query heads a kv head it still gains (131072 rows 80.5 and 85.7, 16 sequences of
+// 4096 56.6 and 57.8), and by the second pass of eight tokens (94 and 97 at 128 columns, 110 and 111 at 68), while
+// 64 tokens in ten passes lose (342 and 337).
 constexpr int kPagedOnce = 2;
 
 struct PagedBatch {
@@ -185,7 +190,9 @@ __device__ __forceinline__ bf16x8 paged_tr_a(const bf16* tile, int row0, int col
 // sequence's part of the share, one MFMA score tile S^T[j][c] = K_j . X_c of the columns c = t (Gs + 1) + i (query head
 // g0 + i of token t, its key at i = Gs), then O^T[d][c] += w^T[d][j] p^T[j][c].  p enters the second
 // product as a bf16 pair (hi + lo, 2^-17), since V' is returned in fp32 and one bf16 term of P
-// would be seen in it.  Page ids reach registers two tiles ahead, rows one.  Columns of the NCT
+// would be seen in it.  So would that pair's rounding where the coupling is as large as V' itself: with keys so alike
+// that V' is 17 to 33 times V, V' is off by 1.8e-6 to 2.7e-6 of its norm (fp32 throughout: 0.7e-6 to 1.2e-6), with
+// independent keys by 6e-8.  A third term would take half as many products again.  Page ids reach registers two tiles ahead, rows one.  Columns of the NCT
 // 32-column tiles: Lp (Gs + 1) <= 32 NCT.
 // Memory bounds it: 131072 rows of 8 kv heads of 128 columns (537 MB) in 90 us, 6.0 TB/s with nothing read
 // twice by the counters.  At 32 sequences of up to 3500 rows it takes 14 us for 27 MB: the lengths, a page

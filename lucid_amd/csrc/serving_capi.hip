@@ -175,7 +175,9 @@ int write_pages(const void* k, const int64_t* ks, const void* v, const int64_t* 
 // Token log probabilities: workgroups of 256 lanes for rows of up to 8192 values (and what a
 // misaligned row's first chunk leaves out), else of 1024 on segments of 32768.  8000 rows of 8184 values take
 // 26 us in workgroups of 256 and 86 in those of 1024, 4 rows 3.5 and 5.3; 4000 of 32000 take 49 in those of
-// 1024, with no second launch to join four segments
+// 1024, with no second launch to join four segments.  A workgroup costs nearly the same however few of its lanes hold
+// values: 8000 bf16 rows of 2000 take 26 us (7 at the rate of a copy), of 8192 (which an aligned row would fit
+// into 256 lanes) 92 (27), of 16000 86 (53), of 32000 97, of 33000 in two segments 182 (109)
 int lp_threads(int V) { return V + 7 <= 256 * lucid::kLpLane ? 256 : 1024; }
 int lp_segs(int V, bool aligned = false) {
   const int seg = lp_threads(V) * lucid::kLpLane;
@@ -421,8 +423,10 @@ int lucid_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t r
   const lucid::LpGrads g{dlogprobs, dentropy, dtop_logprobs};
   const auto* z = reinterpret_cast<const lucid::LpStats*>(stats);
   // A gradient of 100 MB or more is not kept in the 256 MB cache for what reads it next.  Forward and backward of 8192
-  // rows of 32000 bf16 values 290 -> 274 us, of 4000 147 -> 123, of 1021 of 32003 fp32 ones 84 -> 72; with the
-  // product that reads the gradient 1063 -> 1069, 567 -> 562, of 2000 rows 458 -> 457, but of 1000 322 -> 325.
+  // rows of 32000 bf16 values 290 -> 274 us, of 4000 147 -> 123, of 1021 of 32003 fp32 ones 84 -> 72.  That is the
+  // pair by itself.  With the product that reads the gradient (2048 columns) a step gains nothing: 8192 rows 1042 -> 1047,
+  // 4000 557 -> 555, 3000 441 -> 439, 2000 461 -> 461, 1600 (102 MB) 366 -> 367, 1500 350 -> 350; below the rule it would
+  // lose 1 %: 1250 332 -> 336, 1000 321 -> 324, 500 200 -> 204.
   const bool past = (int64_t)R * V * (dtype == LUCID_DTYPE_F32 ? 4 : 2) >= 100000000;
   auto go = [&](auto zero, auto kernel) -> int {
     using E = decltype(zero);

@@ -138,7 +138,8 @@ __device__ __forceinline__ void lp_join(float& m, float& s, float& t, float c2) 
 // bound (masks of one finite value, few allowed tokens, ordered logits) are tried again with the equal ones
 // limited to low indices, which is enough wherever such values are dense, and else taken one a round.
 // 4000 rows of 32000 bf16 values (256 MB): 49 us without alternatives, 5.2 TB/s; 73 with 8, 91 with 50, where
-// the workgroup's four barriers and the lists in LDS bound it.  8 rows with 20 alternatives: 8.2 us.  TOP = false
+// the workgroup's four barriers and the lists in LDS bound it (the bf16 instances also spill 16 registers, 36 bytes a
+// lane, under the cap of 64 that two workgroups of 1024 on a CU set).  8 rows with 20 alternatives: 8.2 us.  TOP = false
 // leaves the lists out (368 -> 317 us forward and backward of 8192 rows, when they still cost the second workgroup
 // on a CU).
 template <typename T, int NT, bool TOP>
