@@ -392,6 +392,23 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
                        int Hkv, int L, int num_pages, int page_size, int max_pages, int D, double scale, float eps,
                        void* stream);
 
+/* A chunk of new tokens of every sequence behind its cached rows: what lucid_decode_paged gives for
+ * new_lens[b] tokens of sequence b (clamped to 0 .. L; null: L tokens each), for any number of them and at the rate of
+ * a prefill.  The rows of q, k and v behind a sequence's tokens are padding and are not used; o is zero there
+ * and in slots without a sequence.  The new rows' V' go to the pages only (bf16).  Any cutting of a prompt into
+ * calls of this and of lucid_decode_paged gives the same rows up to rounding.  A sequence whose table names a page
+ * outside the pool among those it needs, or is too short for the new rows, gets NaN in o and nothing is
+ * written for it.  Cached rows and the tokens' rows must be finite, scale positive.  At most 65535 sequences and kv heads, 2^24 rows of
+ * query heads (L Hq / Hkv) to a kv head.
+ * ws: lucid_prefill_paged_workspace_bytes (0 on bad sizes), 256-byte aligned, one per call in flight. */
+size_t lucid_prefill_paged_workspace_bytes(int B, int Hq, int Hkv, int L, int page_size, int max_pages, int D);
+int lucid_prefill_paged(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, void* k_pages, const int64_t* k_page_strides, void* vp_pages,
+                        const int64_t* vp_page_strides, const int32_t* page_table, int64_t table_stride,
+                        const int32_t* cache_lens, const int32_t* new_lens, void* o, const int64_t* o_strides, void* ws, int B,
+                        int Hq, int Hkv, int L, int num_pages, int page_size, int max_pages, int D, double scale, float eps,
+                        void* stream);
+
 /* A prefill's rows into the pages: row t < new_lens[b] (all T where new_lens is null) of k (bf16) and
  * vprime (bf16, or fp32 when vprime_f32 != 0, rounded to bf16), both [B,Hkv,T,D] at strides {batch, head,
  * time}, goes to row cache_lens[b] + t of sequence b.  Rows of a sequence with a negative length, beyond

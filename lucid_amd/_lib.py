@@ -107,6 +107,9 @@ _SIGS = {
         "lucid_decode_paged_workspace_bytes": ([_int] * 7, _sz),
         "lucid_decode_paged": ([_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _i64p,
                                 _vp, _vp, _int, _int, _int, _int, _int, _int, _int, _int, _dbl, _flt, _vp], _int),
+        "lucid_prefill_paged_workspace_bytes": ([_int] * 7, _sz),
+        "lucid_prefill_paged": ([_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _vp, _i64p,
+                                 _vp, _int, _int, _int, _int, _int, _int, _int, _int, _dbl, _flt, _vp], _int),
         "lucid_write_pages": ([_vp, _i64p, _vp, _i64p, _int, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp,
                                _int, _int, _int, _int, _int, _int, _int, _vp], _int),
         "lucid_copy_pages": ([_int, ctypes.POINTER(_vp), _i64, _i64, _int, _int, ctypes.POINTER(_int),

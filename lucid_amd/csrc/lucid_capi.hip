@@ -1,6 +1,6 @@
 // C ABI of the LUCID attention kernels (declared in include/lucid_amd.h).
-// One translation unit: the kernel files are included so that every template
-// instantiation lives next to its launcher.
+// The kernel files are included so that every template instantiation lives next to its launcher; those of
+// prompt_capi.hip are the library's other translation unit.
 #include <algorithm>
 #include <cmath>
 #include <map>
@@ -15,12 +15,13 @@
 #include "lucid_paged.hip"
 #include "model_ops.hip"
 #include "token_logprobs.hip"
+#include "capi_common.h"
 #include "chain_guard.h"
-#include "profiling.h"
-
-namespace {
+#include "paged_capi.h"
 
 thread_local std::string g_last_error;
+
+namespace {
 
 // Precision of the preconditioner chains (lucid_set_precision): LUCID_PRECISION_AUTO picks
 // per head from its row mass (lucid_mass_kernel, kExactMass); the others force one kind.
@@ -31,22 +32,6 @@ thread_local int g_precision = LUCID_PRECISION_AUTO;
 // dim 64 with one query head per kv head where it is the faster one (linked_fwd64); off, always
 // the two-kernel sequence.  Per calling thread.
 thread_local bool g_fused_fwd = true;
-
-int fail(const std::string& msg) {
-  g_last_error = msg;
-  return LUCID_EINVAL;
-}
-
-int hip_status(const char* where) {
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) {
-    g_last_error = std::string(where) + ": " + hipGetErrorString(e);
-    return LUCID_EHIP + (int)e;
-  }
-  return LUCID_OK;
-}
-
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // First step of every entry point that launches a chain kernel: set up the bounded waits on
 // this device and report a wait that gave up in an earlier launch.
@@ -238,11 +223,6 @@ int check_dims(int B, int Hq, int Hkv, int T, int D) {
 }
 
 // Workspaces hold the chain operands; their 64-row blocks must fill whole cache lines.
-int check_ws(const char* name, const void* p) {
-  if (reinterpret_cast<uintptr_t>(p) % 256) return fail(std::string(name) + " must be 256-byte aligned");
-  return LUCID_OK;
-}
-
 int check_tensor(const char* name, const void* p, const int64_t* s, int mult = 8) {
   if (!p) return fail(std::string(name) + " is null");
   if (!s) return fail(std::string(name) + " strides are null");
@@ -252,12 +232,6 @@ int check_tensor(const char* name, const void* p, const int64_t* s, int mult = 8
       return fail(std::string(name) + " strides must be multiples of " + std::to_string(mult) + " elements");
   return LUCID_OK;
 }
-
-lucid::Strides S(const int64_t* s) { return lucid::Strides{s[0], s[1], s[2]}; }
-
-#define LUCID_LAUNCH(NAME, KERNEL, GRID, ST, ...) LUCID_TIMED_LAUNCH(hip_status, NAME, KERNEL, GRID, ST, __VA_ARGS__)
-#define LUCID_LAUNCH_B(NAME, KERNEL, GRID, BLOCK, ST, ...) \
-  LUCID_TIMED_LAUNCH_B(hip_status, NAME, KERNEL, GRID, BLOCK, ST, __VA_ARGS__)
 
 // Which chain kernels run the bf16 chains of BH heads.  The 128-row linked chains take about
 // 4.2 us a hand-off (fp32 / exact 5.5) and stage a key tile per 128 rows; the fused forward
@@ -1679,8 +1653,6 @@ int lucid_rope(const void* x, const int64_t x_strides[3], int B, int Hn, int T, 
                  out_strides[0], out_strides[1], out_strides[2]);
   return LUCID_OK;
 }
-
-static bool misaligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 
 int lucid_swiglu_fwd(const void* g, const void* u, void* h, int64_t n, void* stream) {
   g_last_error.clear();

@@ -16,7 +16,7 @@
 //                               online-softmax state of every (token, query head)
 //   lucid_paged_combine_kernel  a sequence's parts merged, the new tokens solved in order, the outputs,
 //                               and (k_t, v'_t) appended to the pages
-#include "lucid_common.h"
+#include "paged_common.h"
 
 namespace lucid {
 
@@ -37,25 +37,6 @@ constexpr int kPagedMaxTokens = 16;    // new tokens of a pass
 // 4096 56.6 and 57.8), and by the second pass of eight tokens (94 and 97 at 128 columns, 110 and 111 at 68), while
 // 64 tokens in ten passes lose (342 and 337).
 constexpr int kPagedOnce = 2;
-
-struct PagedBatch {
-  const int32_t* table;  // [B][M] page ids, rows tstride apart
-  int64_t tstride;
-  const int32_t* lens;  // [B] rows cached before the call
-  int B, M, P, page;
-  int shift;  // log2 of page, -1 where it is no power of two
-  int L;      // new tokens of the call
-  int done;   // of earlier passes
-};
-__device__ __forceinline__ int page_of(const PagedBatch& s, int j) { return s.shift >= 0 ? j >> s.shift : j / s.page; }
-
-// A pool by its strides in units of 16 bytes (8 elements); the host checks that every row's offset
-// fits 32 bits, a pool of 64 GB.
-struct PagedPool {
-  bf16* base;
-  unsigned page, head, row;
-};
-__device__ __forceinline__ bf16* paged_at(const PagedPool& p, unsigned off) { return p.base + (size_t)off * 8; }
 
 // Rows of sequence b before this pass; -1: no sequence, -2: its new rows do not fit its table
 __device__ __forceinline__ int paged_rows(const PagedBatch& s, int b) {
@@ -128,22 +109,6 @@ struct PagedLine {
   }
 };
 
-// The scale s, and s log2 e and log2 e / s as the exponents take them
-struct PagedScale {
-  double s;
-  float sl2, c0;
-};
-
-// Four consecutive columns c .. c+3 of a row of d, zeros beyond d; vec: the row starts at an 8-byte
-// boundary
-__device__ __forceinline__ bf16x4 ld4_cols(const bf16* row, int c, int d, bool vec) {
-  if (vec && c + 4 <= d) return *reinterpret_cast<const bf16x4*>(row + c);
-  bf16x4 x;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = c + e < d ? row[c + e] : (bf16)0.f;
-  return x;
-}
-
 // Partials of the sequences' parts, slot-major; tokens of the pass Lp, columns t Gs + g
 struct PagedPartials {
   float* a;  // [slots][Hkv][Lp][W]      sum_j P_tj w_j
@@ -152,12 +117,9 @@ struct PagedPartials {
   float* o;  // [slots][Hkv][Lp*Gs][W]   unnormalised output
 };
 
-// V' tile of 32 rows in LDS as the direct loads write it: W / 8 chunks of 16 bytes a row, chunk c of
-// row r at c ^ (r & 7) for rows of 128 and 256 bytes; rows of 160 and 192 bytes fall on different
-// banks by themselves.
 template <int W>
 struct PagedSmem {
-  static constexpr bool kSwz = W == 64 || W == 128;
+  static constexpr bool kSwz = paged_swizzled(W);
   union {
     bf16 v[4][2][32 * W + 64];  // per wave, double buffered (the last tile's transposing reads of W = 80 end 32 bytes behind it)
     struct {
@@ -168,23 +130,6 @@ struct PagedSmem {
   float nn[4][32];  // per wave: squared norms of the tile's keys
   int bad[4];
 };
-
-// MFMA A operand of 16 rows from row0 and columns col0 + lane % 32 of a V' tile (lds_tr_a of
-// lucid_common.h for the row widths of a page)
-template <int W>
-__device__ __forceinline__ bf16x8 paged_tr_a(const bf16* tile, int row0, int col0) {
-  typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
-  if constexpr (PagedSmem<W>::kSwz) {
-    return lds_tr_a<W / 8>(tile, row0, col0);
-  } else {
-    const int lane = threadIdx.x & 63, s = lane & 15;
-    const int col = col0 + 16 * ((lane >> 4) & 1) + 4 * (s & 3);
-    const int r1 = row0 + 4 * (lane >> 5) + (s >> 2);
-    const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + r1 * W + col));
-    const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + (r1 + 8) * W + col));
-    return bf16x8{v1[0], v1[1], v1[2], v1[3], v2[0], v2[1], v2[2], v2[3]};
-  }
-}
 
 // Grid (target, Hkv).  As lucid_decode_split_kernel: each wave sweeps its own 32-row tiles of a
 // sequence's part of the share, one MFMA score tile S^T[j][c] = K_j . X_c of the columns c = t (Gs + 1) + i (query head

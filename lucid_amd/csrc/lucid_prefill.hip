@@ -1,0 +1,737 @@
+// A chunk of new tokens of every sequence of a batch against its pages on CDNA4 (gfx950): what lucid_paged.hip does
+// for a few tokens, for as many as a prompt has (modeling_lucid.py:475-496, 576-598 is the cached path of the
+// reference; pages, tables and lengths as in lucid_paged.hip).  Sequence b has n rows cached and brings c
+// tokens of the batch's L (right-padded).  For its tokens t = n .. n + c - 1:
+//   P_tj = exp(s r_t r_j (k_t . k_j) - 1/s),  r = 1 / rms(k)  (j < t, cached or new)
+//   v'_t = (v_t - sum_{j<t} P_tj w_j) / P_tt,  P_tt = exp(s d ms_t / (ms_t + eps) - 1/s)
+//   o_tg = softmax_j(s q_tg . k_j) w_j over j <= t
+// with w_j the V' row as the cache holds it (bf16), new rows too: any cutting of a prompt into chunks, down to
+// single tokens, gives the same rows.  The steps, each a launch:
+//   lucid_prefill_prep_kernel   the batch read and checked; new keys into their pages; for each panel of 256 new
+//                               rows the panel's own P in the form that the solve reads
+//   lucid_prefill_sweep_kernel  (couple) y_t = v_t - sum over the cached rows of P_tj w_j
+//   lucid_prefill_solve_kernel  one panel's rows solved in order and written into their pages; between two panels
+//                               the sweep takes the solved one out of the later rows' y
+//   lucid_prefill_sweep_kernel  (attend) the softmax over all rows, cached and new
+//   lucid_prefill_join_kernel   parts of a sweep that was cut along the keys
+// The sweeps are the work: 4 (Hq + Hkv) d flops for each pair of a token and a row.
+#include "paged_common.h"
+
+namespace lucid {
+
+constexpr int kPanel = 256;      // new rows that one solve takes
+constexpr int kPanelBlocks = 8;  // of 32 rows
+constexpr int kSweepKeys = 128;  // keys of a staged tile
+// A panel's own P: 28 tiles below the diagonal blocks as operands (hi and lo bf16, negated), 8 diagonal blocks
+// transposed in fp32, and 1 / P_tt of its rows
+constexpr int kPanelTile = 4 * 512;                                          // bf16 of an operand tile
+constexpr size_t kPanelDiag = (size_t)28 * kPanelTile * 2;                   // byte offset of the diagonal blocks
+constexpr size_t kPanelInv = kPanelDiag + (size_t)kPanelBlocks * 1024 * 4;   // of the inverses
+constexpr size_t kPanelBytes = kPanelInv + kPanel * 4;
+constexpr float PREFILL_NEG = -1e30f;  // finite "minus infinity" for empty softmax states
+
+struct PrefillBatch {
+  const int32_t* table;  // [B][M] page ids, rows tstride apart
+  int64_t tstride;
+  const int32_t* lens;    // [B] rows cached
+  const int32_t* counts;  // [B] tokens of each sequence, null: L
+  int B, M, P, page;
+  int shift;  // log2 of page, -1 where it is no power of two
+  int L, Hkv;
+  int2* info;  // [B] rows cached and tokens (0: nothing to do), left by the prep kernel
+};
+__device__ __forceinline__ int prefill_page(const PrefillBatch& s, int j) { return s.shift >= 0 ? j >> s.shift : j / s.page; }
+// Offset of row j of a sequence with the page ids tbl in a pool, its head's rows
+__device__ __forceinline__ unsigned prefill_row(const PrefillBatch& s, const PagedPool& p, int id, int j, int h) {
+  return id * p.page + h * p.head + (unsigned)(j - prefill_page(s, j) * s.page) * p.row;
+}
+
+// Eight columns c .. c+7 of a row of d, zeros beyond d
+__device__ __forceinline__ bf16x8 ld8_cols(const bf16* row, int c, int d, bool vec) {
+  const bf16x4 a = ld4_cols(row, c, d, vec), b = ld4_cols(row, c + 4, d, vec);
+  return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// Chunk c (8 columns) of row r of a tile of rows in LDS
+template <int W, typename T>
+__device__ __forceinline__ T* tile_at(T* tile, int r, int c) {
+  if constexpr (paged_swizzled(W)) return tile + r * W + ((c ^ (r & 7)) << 3);
+  return tile + r * W + c * 8;
+}
+
+// --------------------------------------------------------------------------------------------
+// Grid (panels of L, Hkv, B), 512 threads.  Every workgroup of a sequence looks its page ids over itself.
+// --------------------------------------------------------------------------------------------
+template <int W>
+__global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __restrict__ k, Strides ks, int vec,
+                                                                 PagedPool kp, PrefillBatch seq, PagedScale f, float eps, int d,
+                                                                 char* __restrict__ pmat, bf16* __restrict__ o, Strides os,
+                                                                 int G) {
+  constexpr int CPR = W / 8, NKS = W / 16;
+  __shared__ __attribute__((aligned(16))) bf16 rows[kPanel * W];
+  __shared__ float norm[kPanel];
+  __shared__ int bad_;
+  const int panel = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
+  const int32_t* tbl = seq.table + b * seq.tstride;
+  const int n = seq.lens[b];
+  int c = seq.counts ? min(max(seq.counts[b], 0), seq.L) : seq.L;
+  if (n < 0) c = 0;
+  // a page id outside the pool among those that the sequence needs, or a table too short for it
+  bool bad = c > 0 && (int64_t)n + c > (int64_t)seq.M * seq.page;
+  if (tid == 0) bad_ = 0;
+  __syncthreads();
+  if (c > 0 && !bad) {
+    const int ids = prefill_page(seq, n + c - 1) + 1;
+    bool any = false;
+    for (int i = tid; i < ids; i += 512) any |= (unsigned)tbl[i] >= (unsigned)seq.P;
+    if (any) bad_ = 1;
+  }
+  __syncthreads();
+  bad |= bad_ != 0;
+  const int t0 = panel * kPanel;
+  // the outputs of padding (zeros) and of a sequence that is left out (NaN)
+  const int from = bad ? 0 : c;
+  for (int t = max(t0, from); t < min(t0 + kPanel, seq.L); ++t) {
+    const float x = t < c ? __builtin_nanf("") : 0.f;
+    for (int i = tid; i < G * d; i += 512) o[b * os.b + (h * G + i / d) * os.h + t * os.t + i % d] = (bf16)x;
+  }
+  if (bad) c = 0;
+  if (panel == 0 && h == 0 && tid == 0) seq.info[b] = make_int2(max(n, 0), c);
+  if (t0 >= c) return;
+  const int R = min(c - t0, kPanel);
+  const bf16* kb = k + b * ks.b + h * ks.h + (int64_t)t0 * ks.t;
+  for (int i = tid; i < kPanel * CPR; i += 512) {
+    const int r = i / CPR, cc = i % CPR;
+    bf16x8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (bf16)0.f;
+    if (r < R) {
+      x = ld8_cols(kb + r * ks.t, cc * 8, d, vec);
+      const int j = n + t0 + r;
+      *reinterpret_cast<bf16x8*>(paged_at(kp, prefill_row(seq, kp, tbl[prefill_page(seq, j)], j, h)) + cc * 8) = x;
+    }
+    *reinterpret_cast<bf16x8*>(tile_at<W>(rows, r, cc)) = x;
+  }
+  __syncthreads();
+  char* pm = pmat + (((int64_t)b * seq.Hkv + h) * gridDim.x + panel) * kPanelBytes;
+  {
+    const int r = tid >> 1, half = tid & 1;
+    float nn = 0.f;
+    for (int cc = half; cc < CPR; cc += 2) {
+      const bf16x8 x = ld8(tile_at<W>(rows, r, cc));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) nn = fmaf((float)x[e], (float)x[e], nn);
+    }
+    nn += dpp_f32<kDppXor1>(nn);
+    if (half == 0) {
+      norm[r] = rsqrtf(nn / (float)d + eps);
+      // 1 / P_tt; the exponent is the small difference of two terms of size sqrt(d): in fp64
+      const double ms = (double)nn / d;
+      reinterpret_cast<float*>(pm + kPanelInv)[r] =
+          __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / f.s - f.s * d * ms / (ms + eps))));
+    }
+  }
+  __syncthreads();
+  // tiles (i, j), j <= i, of 32 x 32: S^T = K_j . K_i, lane <-> row of i, element <-> row of j
+  for (int idx = w; idx < 36; idx += 8) {
+    int i = (int)((sqrtf(8.f * idx + 1.f) - 1.f) * 0.5f);
+    if ((i + 1) * (i + 2) / 2 <= idx) ++i;
+    if (i * (i + 1) / 2 > idx) --i;
+    const int j = idx - i * (i + 1) / 2;
+    if (32 * i >= R) break;
+    f32x16 sc = zero16();
+#pragma unroll
+    for (int st = 0; st < NKS; ++st)
+      sc = mfma32(ld8(tile_at<W>(rows, 32 * j + l32, 2 * st + g)), ld8(tile_at<W>(rows, 32 * i + l32, 2 * st + g)), sc);
+    float nr[16];
+    lds_rows16(&norm[32 * j], g, nr);
+    const float c1 = f.sl2 * norm[32 * i + l32];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(c1 * nr[e], sc[e], -f.c0));
+    if (i == j) {
+      float* dg = reinterpret_cast<float*>(pm + kPanelDiag) + i * 1024;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dg[drow(e, g) * 32 + l32] = l32 > drow(e, g) ? sc[e] : 0.f;
+    } else {
+      bf16* op = reinterpret_cast<bf16*>(pm) + (i * (i - 1) / 2 + j) * kPanelTile;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = -sc[e];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const bf16x8 hi = pack_b(sc, q), lo = pack_lo(sc, q, hi);
+        *reinterpret_cast<bf16x8*>(op + (2 * q) * 512 + lane * 8) = hi;
+        *reinterpret_cast<bf16x8*>(op + (2 * q + 1) * 512 + lane * 8) = lo;
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------------
+// How a sweep is cut into workgroups, worked out by every wave from the sequences' lengths: tiles of RT of a
+// sequence's rows (GX for each token), for each kv head; and, where there are fewer than `target` of
+// them, cuts along the keys in proportion to their number, so that all items together are at most target + the
+// uncut ones.  A cut item leaves its part in a slot.
+// --------------------------------------------------------------------------------------------
+struct SweepGrid {
+  int GX, RT, attend, target;
+};
+struct SweepItem {
+  int b, h, n, c, tile, j0, j1;
+  int slot, splits, tiles;  // slot -1: not cut
+};
+constexpr int kSweepLeast = 4;  // staged tiles of an item that is cut off
+
+struct SweepPlan {
+  const PrefillBatch& s;
+  const SweepGrid& a;
+  int64_t total;  // staged tiles of all row tiles
+  __device__ __forceinline__ int tiles(const int2& x) const { return (x.y * a.GX + a.RT - 1) / a.RT; }
+  __device__ __forceinline__ int keys(const int2& x) const { return x.x + (a.attend ? x.y : 0); }
+  __device__ __forceinline__ int2 at(int b) const { return b < s.B ? s.info[b] : make_int2(0, 0); }
+  __device__ __forceinline__ int splits(const int2& x) const {
+    const int len = (keys(x) + kSweepKeys - 1) / kSweepKeys;
+    return max(1, min(len / kSweepLeast, (int)((int64_t)len * a.target / max(total, (int64_t)1))));
+  }
+  __device__ __forceinline__ SweepPlan(const PrefillBatch& seq, const SweepGrid& grid) : s(seq), a(grid), total(0) {
+    for (int b0 = 0; b0 < s.B; b0 += 64) {
+      const int2 x = at(b0 + (threadIdx.x & 63));
+      total += (int64_t)s.Hkv * tiles(x) * ((keys(x) + kSweepKeys - 1) / kSweepKeys);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
+  }
+  // Item number `id`; cut: among the row tiles of the sequences that are cut, of which j0 and j1 say nothing
+  __device__ __forceinline__ bool find(int id, bool cut, SweepItem& it) const {
+    const int lane = threadIdx.x & 63;
+    int base = 0, slots = 0;
+    for (int b0 = 0; b0 < s.B; b0 += 64) {
+      const int2 x = at(b0 + lane);
+      const int tl = tiles(x), sp = splits(x);
+      const int own = sp > 1 ? s.Hkv * tl * sp : 0;  // slots
+      const int num = cut ? (sp > 1 ? s.Hkv * tl : 0) : s.Hkv * tl * sp;
+      const int end = base + wave_scan(num), send = slots + wave_scan(own);
+      const unsigned long long hit = __ballot(id < end);
+      if (hit) {
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll(hit) - 1);
+        it.b = b0 + l;
+        it.n = __builtin_amdgcn_readlane(x.x, l);
+        it.c = __builtin_amdgcn_readlane(x.y, l);
+        it.tiles = __builtin_amdgcn_readlane(tl, l);
+        it.splits = __builtin_amdgcn_readlane(sp, l);
+        int k = id - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(num, l));
+        const int first = __builtin_amdgcn_readlane(send, l) - __builtin_amdgcn_readlane(own, l);
+        if (cut) {
+          it.tile = k % it.tiles;
+          it.h = k / it.tiles;
+          it.slot = first + it.h * it.splits * it.tiles + it.tile;
+          return true;
+        }
+        it.slot = it.splits > 1 ? first + k : -1;
+        it.tile = k % it.tiles;
+        k /= it.tiles;
+        const int part = k % it.splits;
+        it.h = k / it.splits;
+        const int len = keys(make_int2(it.n, it.c)), all = (len + kSweepKeys - 1) / kSweepKeys;
+        it.j0 = (int)((int64_t)all * part / it.splits) * kSweepKeys;
+        it.j1 = min(len, (int)((int64_t)all * (part + 1) / it.splits) * kSweepKeys);
+        return true;
+      }
+      base = __builtin_amdgcn_readlane(end, 63);
+      slots = __builtin_amdgcn_readlane(send, 63);
+    }
+    it.tile = base;  // the number of items
+    return false;
+  }
+};
+
+struct SweepParts {
+  float* o;  // [slots][RT][W]
+  float* m;  // [slots][RT]  running max (log2 domain), attend
+  float* l;  // [slots][RT]  running sum, attend
+};
+
+template <int W>
+struct SweepSmem {
+  union {
+    // staged tiles, filled by direct global -> LDS loads (the transposing reads of W = 80 end 32 bytes behind a tile)
+    struct {
+      bf16 k[2][kSweepKeys * W], v[2][kSweepKeys * W + 64];
+    } st;
+    struct {
+      float o[2][64][W + 4], m[4][64], l[4][64];
+    } fin;
+  } u;
+  float nn[8][32];  // per wave: 1 / rms of a sub-tile's keys
+};
+
+// Lane part of the offset of paged_tr_a's first read at row0 = 0 of a tile; the second read is 8 rows on
+template <int W>
+__device__ __forceinline__ int tile_tr_off(int col0) {
+  const int lane = threadIdx.x & 63, s = lane & 15;
+  const int col = col0 + 16 * ((lane >> 4) & 1) + 4 * (s & 3), r1 = 4 * (lane >> 5) + (s >> 2);
+  if constexpr (paged_swizzled(W)) return r1 * W + ((((col >> 3) ^ (r1 & 7)) << 3) | (col & 7));
+  return r1 * W + col;
+}
+template <int W>
+__device__ __forceinline__ bf16x8 tile_tr(const bf16* tile, int off, int row0) {
+  typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+  const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + off + row0 * W));
+  const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + off + (row0 + 8) * W));
+  return bf16x8{v1[0], v1[1], v1[2], v1[3], v2[0], v2[1], v2[2], v2[3]};
+}
+
+// Eight waves over tiles of 128 keys, staged once for all of them; KSP waves share 32 rows and take every KSP-th
+// 32 keys (RT = 256 / KSP rows).  Lane <-> row: S^T[j][i] = K_j . x_i, then acc^T[col][i] += w^T[col][j] p^T[j][i].
+//   attend: x = q, rows (token, query head of the group) token by token, online softmax
+//   couple: x = the new keys, p = P as a bf16 pair; y = v - acc.  panel >= 0: not the cached keys but those of that
+//           panel of new rows, out of the y of the rows behind it.  Grid (row tiles, Hkv, B) then, else by SweepPlan.
+template <int W, bool ATTEND, int KSP>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void lucid_prefill_sweep_kernel(
+    const bf16* __restrict__ x, Strides xs, int vec, const bf16* __restrict__ v, Strides vs, PagedPool kp, PagedPool vp,
+    PrefillBatch seq, SweepGrid grid, int panel, PagedScale f, float eps, int d, float* __restrict__ y, int64_t yrows,
+    bf16* __restrict__ o, Strides os, int ovec, SweepParts part) {
+  constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = CPR / 2, NMT = 4 / KSP, RT = 256 / KSP;
+  __shared__ __attribute__((aligned(16))) SweepSmem<W> sm;
+  SweepItem it;
+  int row_base = 0;
+  if (!ATTEND && panel >= 0) {
+    it.b = blockIdx.z;
+    it.h = blockIdx.y;
+    it.tile = blockIdx.x;
+    const int2 i = seq.info[it.b];
+    it.n = __builtin_amdgcn_readfirstlane(i.x);
+    it.c = __builtin_amdgcn_readfirstlane(i.y);
+    row_base = kPanel * (panel + 1);
+    it.j0 = it.n + kPanel * panel;
+    it.j1 = it.j0 + kPanel;
+    it.slot = -1;
+    if (row_base + it.tile * RT >= it.c) return;
+  } else {
+    const SweepPlan plan(seq, grid);
+    // ids go round robin over the 8 XCDs: each takes a run of items, the row tiles of one part next to each other
+    SweepItem none;
+    plan.find(0x7fffffff, false, none);
+    const int per = (none.tile + 7) >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || !plan.find(id, false, it)) return;
+  }
+  const int b = it.b, h = it.h, n = it.n, GX = grid.GX;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
+  const int rw = w / KSP, kg = w % KSP;
+  const int rows = it.c * GX, row0 = row_base + it.tile * RT + 32 * rw;  // of this wave
+  const bool active = row0 < rows;
+  const int row = row0 + l32, rr = min(row, rows - 1), t = rr / GX, hq = h * GX + (rr - t * GX);
+  // attend: no row of this workgroup sees a key beyond its last token's
+  const int last = min(row_base + (it.tile + 1) * RT, rows) - 1;
+  const int j0 = it.j0, j1 = ATTEND ? min(it.j1, n + last / GX + 1) : it.j1;
+  const int lim = ATTEND ? min(j1 - 1, n + t) : j1 - 1;                         // the lane's last key,
+  const int free = ATTEND ? min(j1 - 1, n + min(row0, rows - 1) / GX) : j1 - 1;  // and one that all lanes of the wave see
+  const int most = ATTEND ? n + min(row0 + 31, rows - 1) / GX : j1 - 1;          // and beyond it none does
+  const int ntile = (j1 - j0 + kSweepKeys - 1) / kSweepKeys;
+
+  // staging: waves 0-3 the keys, 4-7 V', 32 rows each
+  const int32_t* tbl = seq.table + b * seq.tstride;
+  const int quarter = w & 3;
+  const bool isv = w >= 4;
+  const PagedPool pool = isv ? vp : kp;
+  auto key_of = [&](int tile) { return min(j0 + kSweepKeys * tile + 32 * quarter + l32, j1 - 1); };
+  auto page_id = [&](int tile) { return tbl[prefill_page(seq, key_of(tile))]; };
+  auto stage = [&](int tile, int id, int buf) {
+    const unsigned off = prefill_row(seq, pool, id, key_of(tile), h);
+    bf16* dst = (isv ? sm.u.st.v[buf] : sm.u.st.k[buf]) + 32 * quarter * W;
+#pragma unroll
+    for (int i = 0; i < NST; ++i) {
+      const int q = i * 64 + lane, r = q / CPR;
+      int c = q % CPR;
+      if constexpr (paged_swizzled(W)) c ^= r & 7;
+      __builtin_amdgcn_global_load_lds(paged_at(pool, __shfl((int)off, r, 64)) + c * 8, dst + i * 512, 16, 0, 0);
+    }
+  };
+  int idn = 0;
+  if (ntile > 0) {
+    const int id0 = page_id(0);
+    if (ntile > 1) idn = page_id(1);
+    stage(0, id0, 0);
+  }
+  const float c = f.sl2;
+  bf16x8 xb[NKS];
+  {
+    const bf16* xr = x + b * xs.b + (ATTEND ? hq : h) * xs.h + t * xs.t;
+#pragma unroll
+    for (int st = 0; st < NKS; ++st) xb[st] = ld8_cols(xr, 16 * st + 8 * g, d, vec);
+  }
+  float c1 = 0.f;
+  if constexpr (!ATTEND) {
+    float nt = 0.f;
+#pragma unroll
+    for (int st = 0; st < NKS; ++st)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) nt = fmaf((float)xb[st][e], (float)xb[st][e], nt);
+    c1 = c * rsqrtf(wave_sum32(nt) / (float)d + eps);
+  }
+  f32x16 acc[NDT];
+#pragma unroll
+  for (int q = 0; q < NDT; ++q) acc[q] = zero16();
+  float m = PREFILL_NEG, lsum = 0.f;
+  int tr[NDT];
+#pragma unroll
+  for (int q = 0; q < NDT; ++q) tr[q] = tile_tr_off<W>(32 * q);
+  // the rows have landed before the loop (else every tile's first product waits for the next tile's loads)
+#pragma unroll
+  for (int st = 0; st < NKS; ++st) asm volatile("" ::"v"(xb[st]));
+  dma_wait();
+  __syncthreads();
+  for (int jt = 0; jt < ntile; ++jt) {
+    const int buf = jt & 1, jb = j0 + kSweepKeys * jt;
+    if (jt + 1 < ntile) {
+      stage(jt + 1, idn, buf ^ 1);
+      if (jt + 2 < ntile) idn = page_id(jt + 2);
+    }
+    if (active && jb <= most) {
+      const bf16* tk = sm.u.st.k[buf];
+      const bf16* tv = sm.u.st.v[buf];
+      const bool mask = jb + kSweepKeys - 1 > free;
+      if constexpr (ATTEND) {
+        f32x16 s[NMT];
+#pragma unroll
+        for (int i = 0; i < NMT; ++i) {
+          const int mt = kg + KSP * i;
+          s[i] = zero16();
+#pragma unroll
+          for (int st = 0; st < NKS; ++st) s[i] = mfma32(ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g)), xb[st], s[i]);
+        }
+        if (mask) {
+#pragma unroll
+          for (int i = 0; i < NMT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (jb + (kg + KSP * i) * 32 + drow(e, g) > lim) s[i][e] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NMT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[i][e]);
+        mx = wave_max32(mx) * c;
+        if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {  // rescale only where a row grows by 2^8
+          const float mnew = fmaxf(m, mx);
+          const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+          m = mnew;
+          lsum *= alpha;
+#pragma unroll
+          for (int q = 0; q < NDT; ++q)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[q][e] *= alpha;
+        }
+#pragma unroll
+        for (int i = 0; i < NMT; ++i) {
+          const int mt = kg + KSP * i;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], c, -m));
+          const bf16x8 p0 = pack_b(s[i], 0), p1 = pack_b(s[i], 1);
+          lsum = add_sum8(p1, add_sum8(p0, lsum));  // sum of the bf16 P of the product
+#pragma unroll
+          for (int q = 0; q < NDT; ++q) {
+            acc[q] = mfma32(tile_tr<W>(tv, tr[q], mt * 32), p0, acc[q]);
+            acc[q] = mfma32(tile_tr<W>(tv, tr[q], mt * 32 + 16), p1, acc[q]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NMT; ++i) {
+          const int mt = kg + KSP * i;
+          f32x16 s = zero16();
+          float nn = 0.f;
+#pragma unroll
+          for (int st = 0; st < NKS; ++st) {
+            const bf16x8 kf = ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g));
+            s = mfma32(kf, xb[st], s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) nn = fmaf((float)kf[e], (float)kf[e], nn);
+          }
+          nn = wave_sum32(nn);
+          if (g == 0) sm.nn[w][l32] = rsqrtf(nn / (float)d + eps);
+          float nr[16];
+          lds_rows16(&sm.nn[w][0], g, nr);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(c1 * nr[e], s[e], -f.c0));
+            s[e] = mask && jb + mt * 32 + drow(e, g) > lim ? 0.f : p;
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const bf16x8 hi = pack_b(s, k), lo = pack_lo(s, k, hi);
+#pragma unroll
+            for (int q = 0; q < NDT; ++q) {
+              const bf16x8 a = tile_tr<W>(tv, tr[q], mt * 32 + 16 * k);
+              acc[q] = mfma32(a, hi, acc[q]);
+              acc[q] = mfma32(a, lo, acc[q]);
+            }
+          }
+        }
+      }
+    }
+    dma_wait();
+    __syncthreads();
+  }
+  float l = ATTEND ? wave_sum32(lsum) : 0.f;
+  if constexpr (KSP > 1) {  // the key groups' sums joined in the waves of group 0
+    const int r = 32 * rw + l32;
+    if constexpr (ATTEND) {
+      if (g == 0) {
+        sm.u.fin.m[kg][r] = m;
+        sm.u.fin.l[kg][r] = l;
+      }
+      __syncthreads();
+      float M = sm.u.fin.m[0][r];
+#pragma unroll
+      for (int k = 1; k < KSP; ++k) M = fmaxf(M, sm.u.fin.m[k][r]);
+      l = 0.f;
+#pragma unroll
+      for (int k = 0; k < KSP; ++k) l = fmaf(sm.u.fin.l[k][r], __builtin_amdgcn_exp2f(sm.u.fin.m[k][r] - M), l);
+      const float a = __builtin_amdgcn_exp2f(m - M);
+      m = M;
+#pragma unroll
+      for (int q = 0; q < NDT; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[q][e] *= a;
+    }
+#pragma unroll
+    for (int half = KSP / 2; half >= 1; half /= 2) {
+      __syncthreads();
+      if (kg >= half && kg < 2 * half) {
+#pragma unroll
+        for (int q = 0; q < NDT; ++q)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            if (32 * q + drow(e, 0) < W)
+              *reinterpret_cast<f32x4*>(&sm.u.fin.o[kg - half][r][32 * q + drow(e, g)]) =
+                  f32x4{acc[q][e], acc[q][e + 1], acc[q][e + 2], acc[q][e + 3]};
+      }
+      __syncthreads();
+      if (kg < half) {
+#pragma unroll
+        for (int q = 0; q < NDT; ++q)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            if (32 * q + drow(e, 0) < W) {
+              const f32x4 z = *reinterpret_cast<const f32x4*>(&sm.u.fin.o[kg][r][32 * q + drow(e, g)]);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) acc[q][e + u] += z[u];
+            }
+      }
+    }
+    if (kg != 0) return;
+  }
+  if (row >= rows) return;
+  if (it.slot >= 0) {
+    const int64_t at = (int64_t)it.slot * RT + 32 * rw + l32;
+#pragma unroll
+    for (int q = 0; q < NDT; ++q)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        if (32 * q + drow(e, 0) < W)
+          *reinterpret_cast<f32x4*>(part.o + at * W + 32 * q + drow(e, g)) =
+              f32x4{acc[q][e], acc[q][e + 1], acc[q][e + 2], acc[q][e + 3]};
+    if (ATTEND && g == 0) {
+      part.m[at] = m;
+      part.l[at] = l;
+    }
+    return;
+  }
+  if constexpr (ATTEND) {
+    const float inv = 1.f / l;
+    bf16* op = o + b * os.b + hq * os.h + t * os.t;
+#pragma unroll
+    for (int q = 0; q < NDT; ++q)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int col = 32 * q + drow(e, g);
+        bf16x4 z;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) z[u] = (bf16)(acc[q][e + u] * inv);
+        if (ovec && col + 4 <= d) {
+          *reinterpret_cast<bf16x4*>(op + col) = z;
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (col + u < d) op[col + u] = z[u];
+        }
+      }
+  } else {
+    float* yp = y + (((int64_t)b * seq.Hkv + h) * yrows + t) * W;
+    const bf16* vr = v + b * vs.b + h * vs.h + t * vs.t;
+#pragma unroll
+    for (int q = 0; q < NDT; ++q)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int col = 32 * q + drow(e, g);
+        if (32 * q + drow(e, 0) >= W) continue;
+        f32x4 z;
+        if (panel >= 0) {
+          z = *reinterpret_cast<const f32x4*>(yp + col);
+        } else {
+          const bf16x4 r = ld4_cols(vr, col, d, false);
+          z = f32x4{(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) z[u] -= acc[q][e + u];
+        *reinterpret_cast<f32x4*>(yp + col) = z;
+      }
+  }
+}
+
+// --------------------------------------------------------------------------------------------
+// The parts of the row tiles that were cut along the keys, joined.  Grid (target / 2, RT / 16), 256 threads: 16 rows
+// of a row tile, W / 4 lanes a row.
+// --------------------------------------------------------------------------------------------
+template <int W, bool ATTEND>
+__global__ __launch_bounds__(256) void lucid_prefill_join_kernel(const bf16* __restrict__ v, Strides vs, int vec,
+                                                                 PrefillBatch seq, SweepGrid grid, int d, float* __restrict__ y,
+                                                                 int64_t yrows, bf16* __restrict__ o, Strides os, int ovec,
+                                                                 SweepParts part) {
+  constexpr int CG = W / 4;
+  const SweepPlan plan(seq, grid);
+  SweepItem it;
+  if (!plan.find(blockIdx.x, true, it)) return;
+  const int GX = grid.GX, rows = it.c * GX;
+  for (int i = threadIdx.x; i < 16 * CG; i += 256) {
+    const int r = 16 * blockIdx.y + i / CG, col = 4 * (i % CG), row = it.tile * grid.RT + r;
+    if (row >= rows) return;
+    const int t = row / GX, hq = it.h * GX + (row - t * GX);
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    float M = PREFILL_NEG, l = 0.f;
+    for (int p = 0; p < it.splits; ++p) {
+      const int64_t at = ((int64_t)it.slot + (int64_t)p * it.tiles) * grid.RT + r;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(part.o + at * W + col);
+      if constexpr (ATTEND) {
+        const float m = part.m[at], mn = fmaxf(M, m);
+        const float a = __builtin_amdgcn_exp2f(M - mn), e = __builtin_amdgcn_exp2f(m - mn);
+        l = fmaf(l, a, part.l[at] * e);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) z[u] = fmaf(z[u], a, x[u] * e);
+        M = mn;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) z[u] += x[u];
+      }
+    }
+    if constexpr (ATTEND) {
+      const float inv = 1.f / l;
+      bf16* op = o + it.b * os.b + hq * os.h + t * os.t;
+      bf16x4 r4;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) r4[u] = (bf16)(z[u] * inv);
+      if (ovec && col + 4 <= d) {
+        *reinterpret_cast<bf16x4*>(op + col) = r4;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (col + u < d) op[col + u] = r4[u];
+      }
+    } else {
+      const bf16x4 r4 = ld4_cols(v + it.b * vs.b + it.h * vs.h + t * vs.t, col, d, vec);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) z[u] = (float)r4[u] - z[u];
+      *reinterpret_cast<f32x4*>(y + (((int64_t)it.b * seq.Hkv + it.h) * yrows + t) * W + col) = z;
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------------
+// One panel's rows in order: x_t = y_t / P_tt, w_t = bf16(x_t), y_u -= P_ut w_t for u > t.  Grid (Hkv, B), a wave for
+// each 32 columns, which are independent: it holds all rows of the panel (lane <-> column, elements <-> rows), goes
+// through a block of 32 rows by itself, and takes it out of the blocks behind it with MFMAs, the block's rows as
+// they are in its registers as the second operand.
+// --------------------------------------------------------------------------------------------
+template <int W>
+__global__ __launch_bounds__(64 * ((W + 31) / 32)) __attribute__((amdgpu_waves_per_eu(1))) void lucid_prefill_solve_kernel(
+    const char* __restrict__ pmat, int panels, int panel, const float* __restrict__ y, int64_t yrows, PagedPool vp,
+    PrefillBatch seq, int d) {
+  constexpr int NW = (W + 31) / 32;
+  __shared__ __attribute__((aligned(16))) struct {
+    char p[kPanelBytes];
+    unsigned off[kPanel];
+  } sm;
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int2 info = seq.info[b];
+  const int R = min(info.y - panel * kPanel, kPanel);
+  if (R <= 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
+  const int nb = (R + 31) / 32;  // blocks with rows
+  const int64_t bh = (int64_t)b * seq.Hkv + h;
+  const char* pm = pmat + (bh * panels + panel) * kPanelBytes;
+  auto fetch = [&](size_t first, int pieces) {  // 1 KB each
+    for (int i = w; i < pieces; i += NW)
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const bf16*>(pm + first) + i * 512 + lane * 8,
+                                       reinterpret_cast<bf16*>(sm.p + first) + i * 512, 16, 0, 0);
+  };
+  fetch(kPanelInv, 1);
+  fetch(kPanelDiag, 4 * nb);
+  fetch(0, 4 * (nb * (nb - 1) / 2));
+  const int n = info.x + panel * kPanel;
+  for (int r = tid; r < R; r += 64 * NW) {
+    const int j = n + r;
+    sm.off[r] = prefill_row(seq, vp, seq.table[b * seq.tstride + prefill_page(seq, j)], j, h);
+  }
+  const int col = 32 * w + l32;
+  const bool on = col < d;
+  f32x16 acc[kPanelBlocks];
+  const float* yb = y + (bh * yrows + panel * kPanel) * W + col;
+#pragma unroll
+  for (int i = 0; i < kPanelBlocks; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int r = 32 * i + drow(e, g);
+      acc[i][e] = on && r < R ? yb[(int64_t)r * W] : 0.f;
+    }
+  dma_wait();
+  __syncthreads();
+  const bf16* off = reinterpret_cast<const bf16*>(sm.p);
+  const float* inv = reinterpret_cast<const float*>(sm.p + kPanelInv);
+#pragma unroll
+  for (int i = 0; i < kPanelBlocks; ++i) {
+    if (i < nb) {
+      const float* dg = reinterpret_cast<const float*>(sm.p + kPanelDiag) + i * 1024;
+      f32x16 fin;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) fin[e] = 0.f;
+#pragma unroll
+      for (int t = 0; t < 32; ++t) {
+        const int e_t = 4 * (t >> 3) + (t & 3), g_t = (t >> 2) & 1;
+        const float x = acc[i][e_t] * inv[32 * i + t];
+        const unsigned u = __builtin_bit_cast(unsigned, (float)(bf16)x);
+        const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // the first half's, the second's
+        const float wt = __builtin_bit_cast(float, g_t ? (unsigned)both[1] : (unsigned)both[0]);
+        fin[e_t] = g == g_t ? wt : fin[e_t];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (8 * q + 7 <= t) continue;  // no row of these is behind t
+          const f32x4 p = *reinterpret_cast<const f32x4*>(dg + 32 * t + 8 * q + 4 * g);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (8 * q + 4 + k > t) acc[i][4 * q + k] = fmaf(-p[k], wt, acc[i][4 * q + k]);
+        }
+      }
+      const bf16x8 w0 = pack_b(fin, 0), w1 = pack_b(fin, 1);
+#pragma unroll
+      for (int k = i + 1; k < kPanelBlocks; ++k)
+        if (k < nb) {
+          const bf16* tile = off + (k * (k - 1) / 2 + i) * kPanelTile + lane * 8;
+          acc[k] = mfma32(ld8(tile), w0, acc[k]);
+          acc[k] = mfma32(ld8(tile + 512), w0, acc[k]);
+          acc[k] = mfma32(ld8(tile + 1024), w1, acc[k]);
+          acc[k] = mfma32(ld8(tile + 1536), w1, acc[k]);
+        }
+      if (col < W) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int r = 32 * i + drow(e, g);
+          if (r < R) paged_at(vp, sm.off[r])[col] = (bf16)(on ? fin[e] : 0.f);
+        }
+      }
+    }
+  }
+}
+
+}  // namespace lucid

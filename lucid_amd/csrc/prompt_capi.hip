@@ -1,0 +1,160 @@
+// C ABI (declared in include/lucid_amd.h) of the operators around prompts: chunks of new tokens against a paged cache,
+// rotary positions and constraints on logits.  The library's second translation unit.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "lucid_prefill.hip"
+#include "paged_capi.h"
+
+namespace {
+
+// Items that a sweep aims at: one or two rounds of the chip
+constexpr int kPrefillTarget = 512;
+
+struct PrefillWs {
+  int2* info;       // [B]
+  char* pmat;       // [B][Hkv][panels][kPanelBytes]
+  float* y;         // [B][Hkv][256 panels][W]
+  lucid::SweepParts part;  // slots of either sweep
+  size_t bytes;
+};
+
+// Rows of a workgroup of a sweep: 64 with four waves to 32 rows where there are few
+int sweep_rows(int64_t rows) { return rows <= 128 ? 64 : 256; }
+
+PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
+  const size_t panels = ((size_t)L + lucid::kPanel - 1) / lucid::kPanel;
+  size_t off = 0;
+  char* p = static_cast<char*>(base);
+  auto take = [&](size_t n) {
+    char* r = p ? p + off : nullptr;
+    off += align256(n);
+    return r;
+  };
+  PrefillWs w{};
+  w.info = reinterpret_cast<int2*>(take((size_t)B * 8));
+  w.pmat = take((size_t)B * Hkv * panels * lucid::kPanelBytes);
+  w.y = reinterpret_cast<float*>(take((size_t)B * Hkv * panels * lucid::kPanel * W * 4));
+  const size_t rows = (size_t)kPrefillTarget * 256;
+  w.part.o = reinterpret_cast<float*>(take(rows * W * 4));
+  w.part.m = reinterpret_cast<float*>(take(rows * 4));
+  w.part.l = reinterpret_cast<float*>(take(rows * 4));
+  w.bytes = off;
+  return w;
+}
+
+bool prefill_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int D) {
+  return B > 0 && B <= 65535 && Hkv > 0 && Hkv <= 65535 && Hq > 0 && Hq % Hkv == 0 && L > 0 && page > 0 && max_pages > 0 &&
+         page_width(D) && (int64_t)page * max_pages <= (1 << 30) && (int64_t)L * (Hq / Hkv) <= (1 << 24) &&
+         (int64_t)B * Hkv * (((int64_t)L * (Hq / Hkv) + 63) / 64) <= (1 << 24);
+}
+
+struct PrefillCall {
+  const bf16 *q, *k, *v;
+  const int64_t *qs, *ks, *vs, *os;
+  lucid::PagedPool kp, vp;
+  lucid::PrefillBatch seq;
+  bf16* o;
+  PrefillWs ws;
+  int Hq, D;
+  lucid::PagedScale scale;
+  float eps;
+  hipStream_t st;
+};
+
+template <int W, bool ATTEND>
+int prefill_sweep(const PrefillCall& c, int panel) {
+  const int G = c.Hq / c.seq.Hkv, GX = ATTEND ? G : 1;
+  const int panels = (c.seq.L + lucid::kPanel - 1) / lucid::kPanel;
+  const int64_t rows = (int64_t)c.seq.L * GX, yrows = (int64_t)panels * lucid::kPanel;
+  const int RT = panel >= 0 ? 64 : sweep_rows(rows);
+  const lucid::SweepGrid grid{GX, RT, ATTEND, kPrefillTarget};
+  const bf16* x = ATTEND ? c.q : c.k;
+  const int64_t* xs = ATTEND ? c.qs : c.ks;
+  const int vec = rows_of_4(x, xs, 2), vvec = rows_of_4(c.v, c.vs, 2);
+  const int ovec = ATTEND ? c.D % 4 == 0 && rows_of_4(c.o, c.os, 2) : vvec;
+  dim3 blocks;
+  if (panel >= 0) {
+    blocks = dim3((unsigned)((c.seq.L - lucid::kPanel * (panel + 1) + RT - 1) / RT), c.seq.Hkv, c.seq.B);
+  } else {
+    const int64_t most = (int64_t)c.seq.B * c.seq.Hkv * ((rows + RT - 1) / RT) + kPrefillTarget;
+    blocks = dim3((unsigned)((most + 7) / 8 * 8));
+  }
+  auto go = [&](auto kernel) -> int {
+    LUCID_LAUNCH_B(ATTEND ? "lucid_prefill_attend_kernel" : "lucid_prefill_couple_kernel", kernel, blocks, dim3(512), c.st, x,
+                   S(xs), vec, c.v, S(c.vs), c.kp, c.vp, c.seq, grid, panel, c.scale, c.eps, c.D, c.ws.y, yrows, c.o, S(c.os),
+                   ovec, c.ws.part);
+    return LUCID_OK;
+  };
+  const int rc = RT == 64 ? go(lucid::lucid_prefill_sweep_kernel<W, ATTEND, 4>) : go(lucid::lucid_prefill_sweep_kernel<W, ATTEND, 1>);
+  if (rc || panel >= 0) return rc;
+  // (rows of fewer tiles than two least parts are never cut)
+  if ((int64_t)c.seq.M * c.seq.page <= (2 * lucid::kSweepLeast - 1) * lucid::kSweepKeys) return LUCID_OK;
+  LUCID_LAUNCH("lucid_prefill_join_kernel", (lucid::lucid_prefill_join_kernel<W, ATTEND>), dim3(kPrefillTarget / 2, RT / 16), c.st,
+               c.v, S(c.vs), vvec, c.seq, grid, c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
+  return LUCID_OK;
+}
+
+template <int W>
+int prefill(const PrefillCall& c) {
+  const int panels = (c.seq.L + lucid::kPanel - 1) / lucid::kPanel;
+  const int64_t yrows = (int64_t)panels * lucid::kPanel;
+  LUCID_LAUNCH_B("lucid_prefill_prep_kernel", lucid::lucid_prefill_prep_kernel<W>, dim3(panels, c.seq.Hkv, c.seq.B), dim3(512),
+                 c.st, c.k, S(c.ks), (int)rows_of_4(c.k, c.ks, 2), c.kp, c.seq, c.scale, c.eps, c.D, c.ws.pmat, c.o, S(c.os),
+                 c.Hq / c.seq.Hkv);
+  if (int rc = prefill_sweep<W, false>(c, -1)) return rc;
+  for (int p = 0; p < panels; ++p) {
+    LUCID_LAUNCH_B("lucid_prefill_solve_kernel", lucid::lucid_prefill_solve_kernel<W>, dim3(c.seq.Hkv, c.seq.B),
+                   dim3(64 * ((W + 31) / 32)), c.st, c.ws.pmat, panels, p, c.ws.y, yrows, c.vp, c.seq, c.D);
+    if (p + 1 < panels)
+      if (int rc = prefill_sweep<W, false>(c, p)) return rc;
+  }
+  return prefill_sweep<W, true>(c, -1);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t lucid_prefill_paged_workspace_bytes(int B, int Hq, int Hkv, int L, int page_size, int max_pages, int D) {
+  if (!prefill_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D)) return 0;
+  return carve_prefill(nullptr, B, Hkv, L, page_width(D)).bytes;
+}
+
+int lucid_prefill_paged(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, void* k_pages, const int64_t* k_page_strides, void* vp_pages,
+                        const int64_t* vp_page_strides, const int32_t* page_table, int64_t table_stride,
+                        const int32_t* cache_lens, const int32_t* new_lens, void* o, const int64_t* o_strides, void* ws, int B,
+                        int Hq, int Hkv, int L, int num_pages, int page_size, int max_pages, int D, double scale, float eps,
+                        void* stream) {
+  g_last_error.clear();
+  if (!page_width(D)) return fail("head_dim must be in [1, 128], got " + std::to_string(D));
+  if (!prefill_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D))
+    return fail("lucid_prefill_paged: B, Hq, Hkv, L, page_size and max_pages positive, Hq a multiple of Hkv, B and Hkv at most "
+                "65535, at most 2^30 rows a sequence, 2^24 rows of query heads to a kv head and 2^24 tiles of 64 of them in all");
+  if (num_pages < 1) return fail("lucid_prefill_paged: the pools have no pages");
+  if (!q || !q_strides || !k || !k_strides || !v || !v_strides || !o || !o_strides || !page_table || !cache_lens || !ws)
+    return fail("lucid_prefill_paged: null argument");
+  if (table_stride < 0) return fail("lucid_prefill_paged: negative table stride");
+  // (a negative one makes the coupling of unlike keys exp(2/|s|) of a key's own: the solve overflows within a few rows)
+  if (!(scale > 0.) || !std::isfinite(scale)) return fail("lucid_prefill_paged: scale must be positive and finite");
+  if (int rc = check_ws("ws", ws)) return rc;
+  constexpr double kLog2e = 1.4426950408889634;
+  const int W = page_width(D);
+  PrefillCall c{(const bf16*)q, (const bf16*)k, (const bf16*)v, q_strides, k_strides, v_strides, o_strides, {}, {}, {},
+                (bf16*)o, carve_prefill(ws, B, Hkv, L, W), Hq, D,
+                {scale, (float)(scale * kLog2e), (float)(kLog2e / scale)}, eps, static_cast<hipStream_t>(stream)};
+  if (int rc = check_pool("k_pages", k_pages, k_page_strides, num_pages, Hkv, page_size, W, &c.kp)) return rc;
+  if (int rc = check_pool("vp_pages", vp_pages, vp_page_strides, num_pages, Hkv, page_size, W, &c.vp)) return rc;
+  c.seq = lucid::PrefillBatch{page_table, table_stride, cache_lens, new_lens, B, max_pages, num_pages, page_size,
+                              page_shift(page_size), L, Hkv, c.ws.info};
+  switch (W) {
+    case 64: return prefill<64>(c);
+    case 80: return prefill<80>(c);
+    case 96: return prefill<96>(c);
+    default: return prefill<128>(c);
+  }
+}
+
+}  // extern "C"

@@ -15,13 +15,6 @@ constexpr int kPagedRound = 512;
 // (a third of rows of 64 with one column tile has its place, and takes as long: 51 us with 512 and with 768)
 int paged_round(int W, int tiles) { return W > 64 && tiles == 2 ? 256 : kPagedRound; }
 
-// Row width of a page for a head dim (0: unsupported)
-int page_width(int D) { return D < 1 ? 0 : D <= 64 ? 64 : D <= 80 ? 80 : D <= 96 ? 96 : D <= 128 ? 128 : 0; }
-
-// log2 of a page size that is a power of two, whose rows are found by a shift (-1: by a division, 20.7 against
-// 20.2 us at 32 sequences of up to 3500 rows, nothing at one of 131072)
-int page_shift(int page) { return page & (page - 1) ? -1 : __builtin_ctz((unsigned)page); }
-
 // Workgroups of each kv head: one resident round, and no more than there can be units of rows
 int paged_target(int B, int Hkv, int64_t cap, int round) {
   const int64_t most = (int64_t)B * ((cap + lucid::kPagedUnit - 1) / lucid::kPagedUnit);
@@ -67,30 +60,6 @@ bool paged_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int 
          (int64_t)page * max_pages <= (1 << 30) && (int64_t)B * Hkv <= (1 << 22) && B <= (1 << 20) && Hkv <= 65535 &&
          B * (((int64_t)page * max_pages + lucid::kPagedUnit - 1) / lucid::kPagedUnit + lucid::kPagedLead) <
              ((int64_t)1 << 31) - 2 * kPagedRound;
-}
-
-int check_pool(const char* name, void* p, const int64_t* s, int pages, int Hkv, int page, int W, lucid::PagedPool* out) {
-  if (!p || !s) return fail(std::string(name) + " or its strides are null");
-  if (misaligned16(p)) return fail(std::string(name) + " must be 16-byte aligned");
-  for (int i = 0; i < 3; ++i)
-    if (s[i] < 0 || s[i] % 8) return fail(std::string(name) + " strides must be non-negative multiples of 8 elements");
-  // offsets in units of 16 bytes have to fit 32 bits; each factor first, so that the sum cannot wrap
-  const int64_t most = (int64_t)1 << 32;
-  const int64_t n[3] = {pages, Hkv, page};
-  int64_t end = W / 8;
-  for (int i = 0; i < 3; ++i) {
-    if (s[i] / 8 >= most || (n[i] > 1 && s[i] / 8 > most / (n[i] - 1)))
-      return fail(std::string(name) + " spans more than 64 GB");
-    end += (n[i] - 1) * (s[i] / 8);
-  }
-  if (end > most) return fail(std::string(name) + " spans more than 64 GB");
-  *out = lucid::PagedPool{(bf16*)p, (unsigned)(s[0] / 8), (unsigned)(s[1] / 8), (unsigned)(s[2] / 8)};
-  return LUCID_OK;
-}
-
-// Whether rows of these tensors start at boundaries of 4 elements
-bool rows_of_4(const void* p, const int64_t* s, size_t size) {
-  return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
 }
 
 struct PagedCall {

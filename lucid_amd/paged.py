@@ -144,6 +144,61 @@ def lucid_decode_paged(query, key, value, key_pages, vprime_pages, page_table, c
     return o, vp_new
 
 
+def lucid_prefill_paged(query, key, value, key_pages, vprime_pages, page_table, cache_lens, new_lens=None, scaling=None,
+                        eps=1e-5):
+    """A chunk of new tokens of every sequence of a batch behind its cached rows: a prompt that is read in parts, or that
+    follows a cached prefix.
+
+    ``query [B, Hq, L, d]``, ``key/value [B, Hkv, L, d]`` (bf16, any strides with a contiguous last axis; keys with RoPE
+    applied), pages, table and lengths as for :func:`lucid_decode_paged`; ``new_lens`` int32 ``[B]``: the tokens that each
+    sequence brings (rows behind them are padding and not used; a number beyond L counts as L, a negative one as 0;
+    None: L each).  The chunk's K and V' rows are written at rows ``cache_lens[b] ..``, whose pages have to be in the table
+    and belong to that sequence alone; ``cache_lens`` is not advanced.  Any cutting of a prompt into calls of this and of
+    :func:`lucid_decode_paged` gives the same rows up to rounding: a token is coupled to, and attends to, the V' rows
+    before it as the cache holds them.
+
+    Returns O ``[B, L, Hq, d]``, zeros in padding and in slots with a negative length.  A sequence that needs a page id
+    outside the pool, or more rows than its table has, gets NaN results and nothing is written for it.  Cached rows and the
+    tokens' own have to be finite, ``scaling`` positive.  Not differentiable."""
+    device = query.device
+    if not query.is_cuda:
+        raise RuntimeError("lucid_amd: query must be a GPU tensor (no CPU path)")
+    bf = torch.bfloat16
+    if not (query.dtype is key.dtype is value.dtype is bf and query.dim() == key.dim() == 4 and key.device == device
+            and value.device == device):
+        raise TypeError(f"lucid_amd.lucid_prefill_paged: query, key and value must be 4-D bfloat16 tensors on {device}")
+    B, Hkv, L, d = key.shape
+    Hq = query.shape[1]
+    if value.shape != key.shape or query.shape != (B, Hq, L, d) or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError("lucid_amd.lucid_prefill_paged: query [B, Hq, L, d], key and value [B, Hkv, L, d] disagree")
+    if not (key_pages.dim() == 4 and vprime_pages.dim() == 4
+            and _pools_ok(key_pages, vprime_pages, Hkv, page_width(d), device)
+            and _table_ok(page_table, B, device) and _lens_ok(cache_lens, B, device)
+            and (new_lens is None or _lens_ok(new_lens, B, device))):
+        lens = (("cache_lens", cache_lens), ("new_lens", new_lens))
+        _refuse("lucid_prefill_paged", device, (B, Hkv, d), key_pages, vprime_pages, page_table,
+                lens[:1] if new_lens is None else lens)
+    o = torch.empty((B, L, Hq, d), dtype=bf, device=device)
+    if B == 0 or L == 0:
+        return o
+    lib = _lib.load()
+    P, _, page, _ = key_pages.shape
+    M = page_table.shape[1]
+    nbytes = lib.lucid_prefill_paged_workspace_bytes(B, Hq, Hkv, L, page, M, d)
+    ws = cache_lens.new_empty(max(nbytes, 256) // 4)
+    q, k, v = _rows(query), _rows(key), _rows(value)
+    with _lib.on(device):
+        rc = lib.lucid_prefill_paged(
+            q.data_ptr(), _strides(q.stride()), k.data_ptr(), _strides(k.stride()), v.data_ptr(), _strides(v.stride()),
+            key_pages.data_ptr(), _strides(key_pages.stride()), vprime_pages.data_ptr(),
+            _strides(vprime_pages.stride()), page_table.data_ptr(), page_table.stride(0), cache_lens.data_ptr(),
+            None if new_lens is None else new_lens.data_ptr(), o.data_ptr(), _strides((L * Hq * d, d, Hq * d)),
+            ws.data_ptr(), B, Hq, Hkv, L, P, page, M, d, d ** -0.5 if scaling is None else float(scaling), float(eps),
+            _lib.stream_handle(device))
+    _lib.check(lib, rc, "lucid_prefill_paged")
+    return o
+
+
 def write_pages(key, v_prime, key_pages, vprime_pages, page_table, cache_lens, new_lens=None) -> None:
     """The rows of a prefill into their pages: row t of ``key`` (bf16) and ``v_prime`` (bf16, or fp32 as the
     prefill returns it, rounded to bf16), both ``[B, Hkv, T, d]``, goes to row ``cache_lens[b] + t`` of sequence b,
