@@ -447,6 +447,36 @@ int lucid_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t r
                              const int64_t* top_indices, const float* dlogprobs, const float* dentropy,
                              const float* dtop_logprobs, void* dlogits, void* stream);
 
+/* Rotary positions: queries and keys [B,H,T,D] (LUCID_DTYPE_BF16 or _F32 at element strides {batch, head, time}, unit stride on
+ * the last axis) turned by their tokens' positions into q_out and k_out (strides likewise; Hq or Hkv 0: none of that).
+ * The pair (a, b) number i of part / 2 becomes scale (a cos x - b sin x, b cos x + a sin x), x = position inv_freq[i]: columns
+ * i and i + part / 2, or 2 i and 2 i + 1 where interleaved; columns part .. D-1 are copied.  inverse: by -x, which is the
+ * gradient.  positions int32 or int64 (positions_64) at element strides; inv_freq fp32 or fp64 (inv_freq_64) [part / 2]. The
+ * angles are worked out in fp64 (modeling_lucid.py:78-145 has tables in the activations' dtype).  D up to 256, part even,
+ * at most 2048 heads.  Inputs and outputs must not overlap. */
+int lucid_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int Hq, const void* k,
+                 const int64_t* k_strides, void* k_out, const int64_t* k_out_strides, int Hkv, const void* positions,
+                 int positions_64, int64_t position_batch_stride, int64_t position_stride, const void* inv_freq,
+                 int inv_freq_64, int B, int T, int D, int part, double scale, int interleaved, int inverse, int dtype,
+                 void* stream);
+
+/* Logit rows (as for lucid_token_logprobs_fwd) under constraints (no counterpart in the reference), written to out [R][V]
+ * in their dtype.  A token that occurs in the row's history (int64 [R][N], rows history_stride apart, values outside [0, V)
+ * ignored) has its logit x divided by the repetition penalty where x > 0 and multiplied where not; one that occurs n times
+ * from place prompt_lens[r] on (null: from 0) has presence + n frequency taken off.  The three are numbers, or fp32
+ * arrays [R] that replace them.  Then bias (fp32 [R][V], rows bias_stride apart; 0: one row for all) is added, and what the
+ * mask allowed (bit v % 32 of word v / 32, rows allowed_stride words apart) has no bit for becomes -inf, whatever it
+ * was.  The backward gives dlogits [R][V] from dout [R][V], both contiguous in the logits' dtype. */
+int lucid_constrain_logits(const void* logits, int64_t batch_stride, int64_t row_stride, int R, int T, int V, int dtype,
+                           const int64_t* history, int64_t history_stride, int N, const int32_t* prompt_lens,
+                           const float* repetitions, float repetition, const float* presences, float presence,
+                           const float* frequencies, float frequency, const float* bias, int64_t bias_stride,
+                           const uint32_t* allowed, int64_t allowed_stride, void* out, void* stream);
+int lucid_constrain_logits_bwd(const void* logits, int64_t batch_stride, int64_t row_stride, int R, int T, int V, int dtype,
+                               const int64_t* history, int64_t history_stride, int N, const float* repetitions,
+                               float repetition, const uint32_t* allowed, int64_t allowed_stride, const void* dout,
+                               void* dlogits, void* stream);
+
 /* Zero-pad n (1 to 3) tensors [B, H[i], T, d] of one dtype (LUCID_DTYPE_BF16 or
  * LUCID_DTYPE_F32), element strides strides[3 i ..] of their first three axes, unit stride on
  * the last, into contiguous [B, H[i], Tp, dp] tensors (dst 16-byte aligned, dp a multiple of 8):

@@ -119,6 +119,12 @@ _SIGS = {
                                       _vp, _vp], _int),
         "lucid_token_logprobs_bwd": ([_vp, _i64, _i64, _vp, _int, _int, _int, _int, _flt, _int, _vp, _vp, _vp, _vp, _vp,
                                       _vp, _vp], _int),
+        "lucid_rotary": ([_vp, _i64p, _vp, _i64p, _int, _vp, _i64p, _vp, _i64p, _int, _vp, _int, _i64, _i64, _vp, _int,
+                          _int, _int, _int, _int, _dbl, _int, _int, _int, _vp], _int),
+        "lucid_constrain_logits": ([_vp, _i64, _i64, _int, _int, _int, _int, _vp, _i64, _int, _vp, _vp, _flt, _vp, _flt, _vp, _flt,
+                                    _vp, _i64, _vp, _i64, _vp, _vp], _int),
+        "lucid_constrain_logits_bwd": ([_vp, _i64, _i64, _int, _int, _int, _int, _vp, _i64, _int, _vp, _flt, _vp, _i64, _vp, _vp,
+                                        _vp], _int),
         "lucid_profile_enable": ([_int], None),
         "lucid_profile_collect": ([], _int),
         "lucid_profile_entry": ([_int, ctypes.c_char_p, _int, ctypes.POINTER(ctypes.c_double),

@@ -4,8 +4,10 @@
 #include <cmath>
 #include <string>
 
+#include "constrain.hip"
 #include "lucid_prefill.hip"
 #include "paged_capi.h"
+#include "rotary.hip"
 
 namespace {
 
@@ -113,6 +115,56 @@ int prefill(const PrefillCall& c) {
   return prefill_sweep<W, true>(c, -1);
 }
 
+// Pairs of a unit of the rotary kernel: as many as 16 bytes hold (of either half, or of adjacent columns) where
+// rows, halves and head dim are whole numbers of them
+template <typename T, bool INTER>
+int rotary_launch(lucid::RotaryCall c, int V, unsigned blocks, hipStream_t st) {
+  constexpr int most = 16 / (int)sizeof(T) / (INTER ? 2 : 1);
+  c.units = c.part / 2 / V + (c.d - c.part) / V;
+  c.per_unit = 1.f / c.units;
+  c.per_head = 1.f / (c.units * (c.q.heads + c.k.heads));
+  auto go = [&](auto kernel) -> int {
+    LUCID_LAUNCH("lucid_rotary_kernel", kernel, dim3(blocks), st, c);
+    return LUCID_OK;
+  };
+  if constexpr (most >= 8)
+    if (V == 8) return go(lucid::lucid_rotary_kernel<T, 8, INTER>);
+  if constexpr (most >= 4)
+    if (V == 4) return go(lucid::lucid_rotary_kernel<T, 4, INTER>);
+  if (V == 2) return go(lucid::lucid_rotary_kernel<T, 2, INTER>);
+  return go(lucid::lucid_rotary_kernel<T, 1, INTER>);
+}
+
+// Workgroups of a row (a misaligned one's first chunk is not whole)
+int constrain_segs(int V) { return (V + 7 + lucid::kConstrainSeg - 1) / lucid::kConstrainSeg; }
+
+int check_constrain(const std::string& w, const void* logits, int64_t sb, int64_t st, int R, int Tn, int V, int dtype,
+                    const lucid::ConstrainRows& a) {
+  if (dtype != LUCID_DTYPE_BF16 && dtype != LUCID_DTYPE_F32) return fail(w + ": dtype LUCID_DTYPE_BF16 or LUCID_DTYPE_F32");
+  if (R < 0 || Tn < 1 || R % Tn) return fail(w + ": R a multiple of the rows of a batch, got R=" + std::to_string(R));
+  if (V < 1 || V > 2000000) return fail(w + ": V from 1 to 2000000, got " + std::to_string(V));
+  if (sb < 0 || st < 0 || a.hstride < 0 || a.bstride < 0 || a.astride < 0) return fail(w + ": negative strides");
+  if (a.N < 0 || (a.N > 0 && R > 0 && !a.history)) return fail(w + ": a history of N tokens a row, N >= 0");
+  if (!a.rep && !(a.rep0 > 0.f && std::isfinite(a.rep0))) return fail(w + ": the repetition penalty must be positive and finite");
+  if ((!a.pres && !std::isfinite(a.pres0)) || (!a.freq && !std::isfinite(a.freq0))) return fail(w + ": penalties must be finite");
+  if (R > 0 && !logits) return fail(w + ": logits are null");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == LUCID_DTYPE_F32 ? 4 : 2)) return fail(w + ": logits are misaligned");
+  if ((int64_t)R * constrain_segs(V) * 512 >= ((int64_t)1 << 32)) return fail(w + ": too many rows");
+  return LUCID_OK;
+}
+
+template <typename T, bool BWD>
+int constrain_launch(const T* x, int64_t sb, int64_t st, const T* raw, int64_t rb, int64_t rt, int R, int Tn, int V,
+                     lucid::ConstrainRows a, T* out, hipStream_t stream) {
+  const int segs = constrain_segs(V);
+  const dim3 grid((unsigned)R * segs);
+  auto go = [&](auto kernel) -> int {
+    LUCID_LAUNCH_B("lucid_constrain_kernel", kernel, grid, dim3(512), stream, x, sb, st, raw, rb, rt, Tn, V, segs, a, out);
+    return LUCID_OK;
+  };
+  return a.N ? go(lucid::lucid_constrain_kernel<T, true, BWD>) : go(lucid::lucid_constrain_kernel<T, false, BWD>);
+}
+
 }  // namespace
 
 extern "C" {
@@ -155,6 +207,96 @@ int lucid_prefill_paged(const void* q, const int64_t* q_strides, const void* k, 
     case 96: return prefill<96>(c);
     default: return prefill<128>(c);
   }
+}
+
+int lucid_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int Hq, const void* k,
+                 const int64_t* k_strides, void* k_out, const int64_t* k_out_strides, int Hkv, const void* positions,
+                 int positions_64, int64_t position_batch_stride, int64_t position_stride, const void* inv_freq,
+                 int inv_freq_64, int B, int T, int D, int part, double scale, int interleaved, int inverse, int dtype,
+                 void* stream) {
+  g_last_error.clear();
+  if (dtype != LUCID_DTYPE_BF16 && dtype != LUCID_DTYPE_F32) return fail("lucid_rotary: dtype LUCID_DTYPE_BF16 or LUCID_DTYPE_F32");
+  if (B < 0 || T < 0 || Hq < 0 || Hkv < 0) return fail("lucid_rotary: negative size");
+  if (D < 1 || D > 2 * lucid::kRotaryPairs || part < 0 || part > D || part % 2)
+    return fail("lucid_rotary: head_dim from 1 to 256 and an even part of it, got " + std::to_string(D) + " and " + std::to_string(part));
+  if (Hq + (int64_t)Hkv > 2048) return fail("lucid_rotary: at most 2048 heads");
+  if (!std::isfinite(scale)) return fail("lucid_rotary: the scale must be finite");
+  if (B == 0 || T == 0 || Hq + Hkv == 0) return LUCID_OK;
+  if ((Hq && (!q || !q_strides || !q_out || !q_out_strides)) || (Hkv && (!k || !k_strides || !k_out || !k_out_strides)) ||
+      !positions || (part && !inv_freq))
+    return fail("lucid_rotary: null argument");
+  const int64_t size = dtype == LUCID_DTYPE_F32 ? 4 : 2;
+  lucid::RotaryCall c{};
+  // the widest unit that everything is a whole number of
+  int V = (int)(16 / size) / (interleaved ? 2 : 1);
+  auto fits = [&](const void* p, const int64_t* s) {
+    const int64_t n = interleaved ? 2 * V : V;
+    return reinterpret_cast<uintptr_t>(p) % (n * size) == 0 && s[0] % n == 0 && s[1] % n == 0 && s[2] % n == 0;
+  };
+  auto all = [&] {
+    return (part / 2) % V == 0 && (D - part) % V == 0 && (!Hq || (fits(q, q_strides) && fits(q_out, q_out_strides))) &&
+           (!Hkv || (fits(k, k_strides) && fits(k_out, k_out_strides)));
+  };
+  while (V > 1 && !all()) V /= 2;
+  if (reinterpret_cast<uintptr_t>(q) % size || reinterpret_cast<uintptr_t>(k) % size) return fail("lucid_rotary: misaligned operands");
+  if (Hq) c.q = {q, S(q_strides), q_out, S(q_out_strides), Hq};
+  if (Hkv) c.k = {k, S(k_strides), k_out, S(k_out_strides), Hkv};
+  c.pos = positions;
+  c.pos64 = positions_64;
+  c.pb = position_batch_stride;
+  c.pt = position_stride;
+  c.freq = inv_freq;
+  c.freq64 = inv_freq_64;
+  c.B = B;
+  c.T = T;
+  c.d = D;
+  c.part = part;
+  c.scale = (float)scale;
+  c.dir = inverse ? -1.f : 1.f;
+  const int64_t tokens = (int64_t)B * T;
+  c.tokens = tokens >= 4096 ? lucid::kRotaryTokens : 1;
+  const int64_t blocks = (tokens + c.tokens - 1) / c.tokens;
+  if (blocks > 0x7fffffff / 256) return fail("lucid_rotary: too many tokens");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == LUCID_DTYPE_F32)
+    return interleaved ? rotary_launch<float, true>(c, V, (unsigned)blocks, st) : rotary_launch<float, false>(c, V, (unsigned)blocks, st);
+  return interleaved ? rotary_launch<bf16, true>(c, V, (unsigned)blocks, st) : rotary_launch<bf16, false>(c, V, (unsigned)blocks, st);
+}
+
+int lucid_constrain_logits(const void* logits, int64_t batch_stride, int64_t row_stride, int R, int T, int V, int dtype,
+                           const int64_t* history, int64_t history_stride, int N, const int32_t* prompt_lens,
+                           const float* repetitions, float repetition, const float* presences, float presence,
+                           const float* frequencies, float frequency, const float* bias, int64_t bias_stride,
+                           const uint32_t* allowed, int64_t allowed_stride, void* out, void* stream) {
+  g_last_error.clear();
+  const lucid::ConstrainRows a{history, history_stride, N, prompt_lens, repetitions, presences, frequencies, repetition, presence,
+                               frequency, bias, bias_stride, allowed, allowed_stride};
+  if (int rc = check_constrain("lucid_constrain_logits", logits, batch_stride, row_stride, R, T, V, dtype, a)) return rc;
+  if (R == 0) return LUCID_OK;
+  if (!out) return fail("lucid_constrain_logits: null output");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == LUCID_DTYPE_F32)
+    return constrain_launch<float, false>((const float*)logits, batch_stride, row_stride, nullptr, 0, 0, R, T, V, a, (float*)out, st);
+  return constrain_launch<bf16, false>((const bf16*)logits, batch_stride, row_stride, nullptr, 0, 0, R, T, V, a, (bf16*)out, st);
+}
+
+int lucid_constrain_logits_bwd(const void* logits, int64_t batch_stride, int64_t row_stride, int R, int T, int V, int dtype,
+                               const int64_t* history, int64_t history_stride, int N, const float* repetitions,
+                               float repetition, const uint32_t* allowed, int64_t allowed_stride, const void* dout,
+                               void* dlogits, void* stream) {
+  g_last_error.clear();
+  const lucid::ConstrainRows a{history, history_stride, N, nullptr, repetitions, nullptr, nullptr, repetition, 0.f, 0.f, nullptr,
+                               0, allowed, allowed_stride};
+  if (int rc = check_constrain("lucid_constrain_logits_bwd", logits, batch_stride, row_stride, R, T, V, dtype, a)) return rc;
+  if (R == 0) return LUCID_OK;
+  if (!dout || !dlogits) return fail("lucid_constrain_logits_bwd: null argument");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t sb = (int64_t)T * V;
+  if (dtype == LUCID_DTYPE_F32)
+    return constrain_launch<float, true>((const float*)dout, sb, V, (const float*)logits, batch_stride, row_stride, R, T, V, a,
+                                         (float*)dlogits, st);
+  return constrain_launch<bf16, true>((const bf16*)dout, sb, V, (const bf16*)logits, batch_stride, row_stride, R, T, V, a,
+                                      (bf16*)dlogits, st);
 }
 
 }  // extern "C"

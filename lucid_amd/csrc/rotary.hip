@@ -1,0 +1,112 @@
+// Rotary positions on CDNA4 (gfx950): queries and keys turned by their positions (modeling_lucid.py:78-145 is the
+// reference's: tables of cos and sin in the activations' type, the whole head in halves).  With f_i the i-th frequency and p a
+// token's position, the pair (a_i, b_i) of every head becomes
+//   (a_i cos(p f_i) - b_i sin(p f_i), b_i cos(p f_i) + a_i sin(p f_i)) scale,  i < part / 2
+// pairs (i, i + part / 2) in the half layout, (2 i, 2 i + 1) in the interleaved one; columns from part on stay as they
+// are.  The gradient is the turn by -p f_i.  One pass over q and k: a workgroup works the angles of its tokens out
+// once, for all heads, in 64 bits: at position 131072 a product in 32 bits is off by up to 2^-8 of a radian.
+#include "lucid_common.h"
+
+namespace lucid {
+
+constexpr int kRotaryPairs = 128;  // of a head, at most
+constexpr int kRotaryTokens = 4;   // of a workgroup, at most
+
+struct RotaryTensor {
+  const void* x;
+  Strides xs;
+  void* y;
+  Strides ys;
+  int heads;
+};
+struct RotaryCall {
+  RotaryTensor q, k;
+  const void* pos;  // int32 or int64 at element strides pb, pt
+  int64_t pb, pt;
+  int pos64;
+  const void* freq;  // fp64 or fp32 [part / 2]
+  int freq64;
+  int B, T, d, part;
+  int tokens;      // of a workgroup
+  float scale, dir;  // dir -1: the gradient
+  int units;       // of a head: part / 2 / V of pairs, then (d - part) / V of columns that stay
+  float per_unit, per_head;  // 1 / units, 1 / (units (Hq + Hkv))
+};
+
+// i / n by the reciprocal r of n: exact for i < 2^22
+__device__ __forceinline__ int div_by(int i, float r) { return (int)(((float)i + 0.5f) * r); }
+
+// V pairs a unit: V columns of either half, or 2 V adjacent ones.  256 threads.
+template <typename T, int V, bool INTER>
+__global__ __launch_bounds__(256) void lucid_rotary_kernel(const RotaryCall c) {
+  typedef T TV __attribute__((ext_vector_type(V)));
+  typedef T T2 __attribute__((ext_vector_type(2 * V)));
+  __shared__ __attribute__((aligned(16))) float2 turn[kRotaryTokens][kRotaryPairs];
+  const int half = c.part / 2;
+  const int64_t all = (int64_t)c.B * c.T, t0 = (int64_t)blockIdx.x * c.tokens;
+  const int n = (int)min((int64_t)c.tokens, all - t0);
+  for (int i = threadIdx.x; i < n * half; i += 256) {
+    const int tk = i / half, p = i - tk * half;
+    const int64_t tok = t0 + tk, b = tok / c.T, at = b * c.pb + (tok - b * c.T) * c.pt;
+    const double pos = c.pos64 ? (double)static_cast<const int64_t*>(c.pos)[at] : (double)static_cast<const int32_t*>(c.pos)[at];
+    const double f = c.freq64 ? static_cast<const double*>(c.freq)[p] : (double)static_cast<const float*>(c.freq)[p];
+    // in half turns, less whole turns; a quarter of a turn at most is left to 32 bits
+    const double u = pos * f * 0.31830988618379067154, whole = 2.0 * rint(0.5 * u);
+    double r = u - whole;  // -1 .. 1
+    const double q = rint(2.0 * r);
+    const float x = (float)(r - 0.5 * q);  // -1/4 .. 1/4
+    float s, co;
+    sincospif(x, &s, &co);
+    const int quad = (int)q & 3;
+    const float sn = quad == 0 ? s : quad == 1 ? co : quad == 2 ? -s : -co;
+    const float cs = quad == 0 ? co : quad == 1 ? -s : quad == 2 ? -co : s;
+    turn[tk][p] = make_float2(cs * c.scale, sn * c.scale * c.dir);
+  }
+  __syncthreads();
+  const int heads = c.q.heads + c.k.heads, work = n * heads * c.units, turning = half / V;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < work; i += 256) {
+    const int tk = div_by(i, c.per_head), rest = i - tk * heads * c.units;
+    int h = div_by(rest, c.per_unit);
+    const int u = rest - h * c.units;
+    const bool isk = h >= c.q.heads;
+    if (isk) h -= c.q.heads;
+    const int64_t tok = t0 + tk, b = tok / c.T, t = tok - b * c.T;
+    const Strides xs = isk ? c.k.xs : c.q.xs, ys = isk ? c.k.ys : c.q.ys;
+    const T* x = static_cast<const T*>(isk ? c.k.x : c.q.x) + b * xs.b + h * xs.h + t * xs.t;
+    T* y = static_cast<T*>(isk ? c.k.y : c.q.y) + b * ys.b + h * ys.h + t * ys.t;
+    if (u >= turning) {
+      const int col = c.part + (u - turning) * V;
+      *reinterpret_cast<TV*>(y + col) = *reinterpret_cast<const TV*>(x + col);
+      continue;
+    }
+    const float2* tn = &turn[tk][u * V];
+    if constexpr (INTER && V == 1) {  // pairs at any address
+      const float a = (float)x[2 * u], bb = (float)x[2 * u + 1];
+      y[2 * u] = (T)fmaf(a, tn->x, -(bb * tn->y));
+      y[2 * u + 1] = (T)fmaf(bb, tn->x, a * tn->y);
+    } else if constexpr (INTER) {
+      const T2 z = *reinterpret_cast<const T2*>(x + 2 * u * V);
+      T2 o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float a = (float)z[2 * e], bb = (float)z[2 * e + 1];
+        o[2 * e] = (T)fmaf(a, tn[e].x, -(bb * tn[e].y));
+        o[2 * e + 1] = (T)fmaf(bb, tn[e].x, a * tn[e].y);
+      }
+      *reinterpret_cast<T2*>(y + 2 * u * V) = o;
+    } else {
+      const TV a = *reinterpret_cast<const TV*>(x + u * V), bb = *reinterpret_cast<const TV*>(x + half + u * V);
+      TV o, p;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        o[e] = (T)fmaf((float)a[e], tn[e].x, -((float)bb[e] * tn[e].y));
+        p[e] = (T)fmaf((float)bb[e], tn[e].x, (float)a[e] * tn[e].y);
+      }
+      *reinterpret_cast<TV*>(y + u * V) = o;
+      *reinterpret_cast<TV*>(y + half + u * V) = p;
+    }
+  }
+}
+
+}  // namespace lucid

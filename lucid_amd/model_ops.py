@@ -17,6 +17,11 @@ one kernel pass forward and one backward:
   reference rounds silu(g) to bf16 before the product).
 * :func:`causal_lm_loss` -- the shifted cross entropy on bf16 logits, one read of the logits
   forward (per-row logsumexp) and one read + write backward, instead of fp32 copies of them.
+* :func:`rotary` -- queries and keys turned by their positions in one pass: any head dim up to 256, the whole head or a
+  part, in halves or interleaved, frequencies of :func:`rope_frequencies` (scaled for long contexts) or any others,
+  angles in 64 bits (bf16 or fp32).
+* :func:`constrain_logits` -- penalties of tokens that have occurred, biases and bit masks of allowed tokens on logit
+  rows (bf16 or fp32, any vocabulary).
 * :func:`token_logprobs` -- log probabilities of given tokens, entropy and the top alternatives of
   logit rows (bf16 or fp32, any vocabulary), and the gradient of all three.
 
@@ -26,6 +31,8 @@ dim 64; the loss: a vocabulary that is a multiple of 8) and raise otherwise; the
 """
 from __future__ import annotations
 
+import ctypes
+import math
 import operator
 from typing import NamedTuple
 
@@ -198,6 +205,153 @@ def qkv_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, nq: int, n
     """(q, k, v) [B, H, T, 64] from the stacked projection output, q and k rotated
     (apply_rotary_pos_emb, modeling_lucid.py:118-145)."""
     return QKVRopeFunction.apply(qkv, cos, sin, nq, nk)
+
+
+def rope_frequencies(dim: int, theta: float = 10000.0, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
+    """Inverse frequencies (float64 ``[dim / 2]``, on the CPU) of ``dim`` turning columns, and the factor of the turned
+    values: ``theta^(-2 i / dim)`` and 1, or scaled for contexts longer than the model was trained on.
+
+    ``scaling["rope_type"]``: ``"default"``; ``"linear"`` (positions divided by ``factor``); ``"ntk"`` (the base grows to
+    theta factor^(dim / (dim - 2)): the slowest frequency is divided by ``factor``, the fastest stays); ``"llama3"``
+    (wavelengths below ``original_max_position_embeddings / high_freq_factor`` stay, those above ``... / low_freq_factor`` are
+    divided by ``factor``, those between are interpolated over the inverse wavelength); ``"yarn"`` (pairs that turn ``beta_fast`` (32) times
+    or more in ``original_max_position_embeddings`` positions stay, those that turn ``beta_slow`` (1) times or less
+    are divided by ``factor``, with a ramp over the pair's number between, and values are multiplied by ``attention_factor``,
+    0.1 ln(factor) + 1 if it is not given)."""
+    if dim < 0 or dim % 2:
+        raise ValueError(f"lucid_amd.rope_frequencies: an even number of columns, got {dim}")
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    freq = theta ** (-i / max(dim, 1))
+    scaling = {} if scaling is None else dict(scaling)
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "default" or dim == 0:
+        return freq, 1.0
+    known = ("linear", "ntk", "llama3", "yarn")
+    if kind not in known:
+        raise ValueError(f"lucid_amd.rope_frequencies: rope_type one of {('default',) + known}, got {kind!r}")
+    try:
+        factor = float(scaling["factor"])
+        length = float(scaling["original_max_position_embeddings"]) if kind in ("llama3", "yarn") else 0.0
+    except KeyError as e:
+        raise ValueError(f"lucid_amd.rope_frequencies: {kind} needs {e.args[0]!r}") from None
+    if not factor > 0.0 or length < 0.0:
+        raise ValueError(f"lucid_amd.rope_frequencies: the factor must be positive, got {factor}")
+    if kind == "linear":
+        return freq / factor, 1.0
+    if kind == "ntk":
+        return (theta * factor ** (dim / max(dim - 2, 1))) ** (-i / dim), 1.0
+    if kind == "llama3":
+        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        turns = length * freq / (2 * math.pi)
+        keep = ((turns - low) / max(high - low, 1e-9)).clamp(0.0, 1.0)
+        return freq * keep + freq / factor * (1 - keep), 1.0
+
+    def pair(turns):  # the (fractional) number of the pair that turns so often
+        return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+    first = max(math.floor(pair(float(scaling.get("beta_fast", 32.0)))), 0)
+    last = min(math.ceil(pair(float(scaling.get("beta_slow", 1.0)))), dim - 1)
+    keep = 1 - ((torch.arange(dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
+    scale = scaling.get("attention_factor")
+    scale = (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0) if scale is None else float(scale)
+    return freq * keep + freq / factor * (1 - keep), scale
+
+
+class RotaryPositions(NamedTuple):
+    """What :func:`rotary` takes beside queries and keys (a decoder's layers share one)."""
+
+    positions: torch.Tensor     # int32 or int64 [T], [1, T] or [B, T]
+    inv_freq: torch.Tensor      # fp32 or fp64 [part / 2]
+    interleaved: bool = False
+    scale: float = 1.0
+
+
+_ROTARY_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+
+
+def _rotary(q, k, positions, inv_freq, interleaved, scale, inverse):
+    """q and k (either may be None) turned, into new [B, T, H, d] buffers seen as [B, H, T, d]."""
+    some = q if q is not None else k
+    B, _, T, d = some.shape
+    args, outs = [], []
+    for x in (q, k):
+        if x is None:
+            args += [None, None, None, None, 0]
+            outs.append(None)
+            continue
+        x = x if x.stride(3) == 1 or d == 1 else x.contiguous()
+        H = x.shape[1]
+        y = torch.empty((B, T, H, d), dtype=x.dtype, device=x.device)
+        args += [x, (ctypes.c_int64 * 3)(*x.stride()[:3]), y.data_ptr(), (ctypes.c_int64 * 3)(T * H * d, d, H * d), H]
+        outs.append(y.transpose(1, 2))
+    lib = _lib.load()
+    pb, pt = (0, positions.stride(0)) if positions.dim() == 1 else (0 if positions.shape[0] == 1 else positions.stride(0),
+                                                                      positions.stride(1))
+    with _lib.on(some.device):
+        rc = lib.lucid_rotary(*(a.data_ptr() if torch.is_tensor(a) else a for a in args), positions.data_ptr(),
+                              int(positions.dtype == torch.int64), pb, pt, inv_freq.data_ptr(),
+                              int(inv_freq.dtype == torch.float64), B, T, d, 2 * inv_freq.numel(), scale, int(interleaved),
+                              int(inverse), _ROTARY_DTYPES[some.dtype], _lib.stream_handle(some.device))
+    _lib.check(lib, rc, "lucid_rotary")
+    return tuple(outs)
+
+
+class RotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved: bool, scale: float):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = interleaved, scale
+        ctx.set_materialize_grads(False)
+        return _rotary(q, k, positions, inv_freq, interleaved, scale, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        if not ctx.needs_input_grad[0]:
+            dq = None
+        if not ctx.needs_input_grad[1]:
+            dk = None
+        if dq is not None or dk is not None:
+            dq, dk = _rotary(dq, dk, *ctx.saved_tensors, *ctx.how, True)
+        return dq, dk, None, None, None, None
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+           interleaved: bool = False, scale: float = 1.0):
+    """``(q, k)`` turned by their positions, in one pass; differentiable.
+
+    ``q [B, Hq, T, d]`` and ``k [B, Hkv, T, d]`` (or None) bf16 or fp32 on the GPU, any strides; ``positions`` int32 or int64 ``[T]``,
+    ``[1, T]`` or ``[B, T]``; ``inv_freq`` fp32 or fp64 ``[part / 2]`` (:func:`rope_frequencies`), part at most d.  With x =
+    position inv_freq[i], the pair (a, b) number i of a row becomes scale (a cos x - b sin x, b cos x + a sin x): columns i and
+    i + part / 2, or 2 i and 2 i + 1 where ``interleaved``; columns from part on stay as they are.  Angles are worked out in
+    64 bits (good for positions up to 2^31 and beyond), values in 32, rounded once.  Results are ``[B, H, T, d]`` views of
+    ``[B, T, H, d]`` buffers, as the projections leave them."""
+    what = "lucid_amd.rotary"
+    if not q.is_cuda:
+        raise RuntimeError("lucid_amd: query must be a GPU tensor (no CPU path)")
+    dev = q.device
+    if q.dtype not in _ROTARY_DTYPES or (k is not None and (k.dtype != q.dtype or k.device != dev)):
+        raise TypeError(f"{what}: bf16 or fp32 queries and keys of one dtype on one GPU, got {q.dtype}"
+                        + (f" / {k.dtype} on {k.device}" if k is not None else ""))
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or (k.shape[0], *k.shape[2:]) != (q.shape[0], *q.shape[2:]))):
+        raise ValueError(f"{what}: q [B, Hq, T, d] and k [B, Hkv, T, d], got {tuple(q.shape)}"
+                         + (f" and {tuple(k.shape)}" if k is not None else ""))
+    B, _, T, d = q.shape
+    if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev \
+            or tuple(positions.shape) not in ((T,), (1, T), (B, T)):
+        raise ValueError(f"{what}: positions int32 or int64 [{T}] or [{B}, {T}] on {dev}, got {positions.dtype} "
+                         f"{tuple(positions.shape)} on {positions.device}")
+    if inv_freq.dtype not in (torch.float32, torch.float64) or inv_freq.dim() != 1 or inv_freq.device != dev \
+            or 2 * inv_freq.numel() > d or not inv_freq.is_contiguous():
+        raise ValueError(f"{what}: inv_freq contiguous fp32 or fp64 of at most {d // 2} on {dev}, got {inv_freq.dtype} "
+                         f"{tuple(inv_freq.shape)} on {inv_freq.device}")
+    if inv_freq.requires_grad:
+        raise NotImplementedError(f"{what}: no gradient of the frequencies")
+    tracked = [x for x in (q, k) if x is not None]
+    if torch.is_grad_enabled() and any(x.requires_grad for x in tracked) \
+            or any(forward_ad.unpack_dual(x).tangent is not None for x in tracked):
+        return RotaryFunction.apply(q, k, positions, inv_freq, bool(interleaved), float(scale))
+    return _rotary(q, k, positions, inv_freq, bool(interleaved), float(scale), False)
 
 
 def swiglu_supported(g: torch.Tensor, u: torch.Tensor) -> bool:
@@ -392,3 +546,135 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     if logits.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(logits).tangent is not None:
         return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, top, float(temperature)))
     return TokenLogprobs(*_token_logprobs(logits.detach(), tokens.contiguous(), top, float(temperature), False)[:4])
+
+
+class _Constraints(NamedTuple):
+    """Checked arguments of :func:`constrain_logits`: tensors by rows of the logits, or None."""
+
+    history: torch.Tensor | None
+    prompt_lens: torch.Tensor | None
+    repetition: torch.Tensor | float
+    presence: torch.Tensor | float
+    frequency: torch.Tensor | float
+    bias: torch.Tensor | None
+    allowed: torch.Tensor | None
+
+
+def _row_stride(t: torch.Tensor | None) -> int:
+    return 0 if t is None or t.shape[0] == 1 else t.stride(0)
+
+
+def _number(x) -> tuple:
+    return (x.data_ptr(), 0.0) if torch.is_tensor(x) else (None, x)
+
+
+def _at(t: torch.Tensor | None):
+    return None if t is None or t.numel() == 0 else t.data_ptr()
+
+
+def _constrain(logits: torch.Tensor, c: _Constraints) -> torch.Tensor:
+    rows, T, sb, st = _logit_rows(logits)
+    V, dev = logits.shape[-1], logits.device
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    rep, one = _number(c.repetition), 1.0
+    lib = _lib.load()
+    with _lib.on(dev):
+        rc = lib.lucid_constrain_logits(
+            rows.data_ptr(), sb, st, out.numel() // V, T, V, _LP_DTYPES[logits.dtype], _at(c.history), _row_stride(c.history),
+            0 if c.history is None else c.history.shape[1], _at(c.prompt_lens), rep[0], rep[1] if rep[0] is None else one,
+            *_number(c.presence), *_number(c.frequency), _at(c.bias), _row_stride(c.bias), _at(c.allowed),
+            _row_stride(c.allowed), out.data_ptr(), _lib.stream_handle(dev))
+    _lib.check(lib, rc, "lucid_constrain_logits")
+    return out
+
+
+class ConstrainLogitsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits: torch.Tensor, *constraints):
+        c = _Constraints(*constraints)
+        number = not torch.is_tensor(c.repetition)
+        ctx.repetition = c.repetition if number else None
+        ctx.save_for_backward(logits, c.history, None if number else c.repetition, c.allowed)
+        return _constrain(logits, c)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout: torch.Tensor):
+        logits, history, repetition, allowed = ctx.saved_tensors
+        rows, T, sb, st = _logit_rows(logits)
+        V, dev = logits.shape[-1], logits.device
+        g = dout.contiguous()
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        lib = _lib.load()
+        with _lib.on(dev):
+            rc = lib.lucid_constrain_logits_bwd(
+                rows.data_ptr(), sb, st, dlogits.numel() // V, T, V, _LP_DTYPES[logits.dtype], _at(history),
+                _row_stride(history), 0 if history is None else history.shape[1], _at(repetition),
+                1.0 if ctx.repetition is None else ctx.repetition, _at(allowed), _row_stride(allowed), g.data_ptr(),
+                dlogits.data_ptr(), _lib.stream_handle(dev))
+        _lib.check(lib, rc, "lucid_constrain_logits_bwd")
+        return (dlogits,) + (None,) * len(_Constraints._fields)
+
+
+def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                     repetition: torch.Tensor | float = 1.0, presence: torch.Tensor | float = 0.0,
+                     frequency: torch.Tensor | float = 0.0, bias: torch.Tensor | None = None,
+                     allowed: torch.Tensor | None = None) -> torch.Tensor:
+    """Logits under the constraints of a sampling step, in their own shape and dtype, in one pass; differentiable w.r.t.
+    ``logits`` (what :func:`token_logprobs` makes of them included).
+
+    ``logits [..., V]`` bf16 or fp32 on the GPU.  ``history [..., N]`` int64: the tokens so far of each row, values outside
+    ``[0, V)`` (padding) ignored; its first ``prompt_lens [...]`` (int32) are the prompt.  In this order, in 32 bits, rounded
+    once:
+
+    * a token that occurs in the history: x / repetition where x > 0, x repetition where not;
+    * one that occurs n > 0 times behind the prompt: x - presence - n frequency;
+    * ``bias`` (fp32 ``[V]`` or ``[..., V]``) is added;
+    * what ``allowed`` (int32 ``[words]`` or ``[..., words]``, words = ceil(V / 32): bit v % 32 of word v // 32) has no bit for
+      becomes -inf, whatever it was (NaN too); its gradient is 0.
+
+    The three penalties are numbers or fp32 tensors ``[...]`` (positive repetition)."""
+    what = "lucid_amd.constrain_logits"
+    if not logits.is_cuda:
+        raise RuntimeError("lucid_amd: logits must be a GPU tensor (no CPU path)")
+    if logits.dtype not in _LP_DTYPES:
+        raise TypeError(f"{what}: bf16 or fp32 logits, got {logits.dtype}")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits [..., V], got {tuple(logits.shape)}")
+    lead, V, dev = logits.shape[:-1], logits.shape[-1], logits.device
+
+    def rows(name, t, dtype, last, shared):
+        """t [..., last] as [R, last] with contiguous rows ([1, last] for one row that all share)."""
+        if t is None:
+            return None
+        if not torch.is_tensor(t) or t.dtype != dtype or t.device != dev:
+            raise TypeError(f"{what}: {name} must be a {dtype} tensor on {dev}")
+        if t.requires_grad:
+            raise NotImplementedError(f"{what}: no gradient of {name}")
+        if t.dim() < 1 or (last is not None and t.shape[-1] != last) or not (t.shape[:-1] == lead or (shared and t.dim() == 1)):
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} does not fit logits {tuple(logits.shape)}")
+        t = t.reshape(1 if t.shape[:-1] != lead else lead.numel(), t.shape[-1])
+        return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+    def number(name, x):
+        if not torch.is_tensor(x):
+            return float(x)
+        if x.dtype != torch.float32 or x.device != dev or x.shape != lead:
+            raise ValueError(f"{what}: {name} must be a number or fp32 {tuple(lead)} on {dev}")
+        if x.requires_grad:
+            raise NotImplementedError(f"{what}: no gradient of {name}")
+        return x.contiguous()
+
+    if prompt_lens is not None:
+        if history is None:
+            raise ValueError(f"{what}: prompt_lens without a history")
+        if not torch.is_tensor(prompt_lens) or prompt_lens.dtype != torch.int32 or prompt_lens.shape != lead \
+                or prompt_lens.device != dev:
+            raise ValueError(f"{what}: prompt_lens must be int32 {tuple(lead)} on {dev}")
+        prompt_lens = prompt_lens.contiguous()
+    c = _Constraints(rows("history", history, torch.int64, None, False), prompt_lens, number("repetition", repetition),
+                     number("presence", presence), number("frequency", frequency), rows("bias", bias, torch.float32, V, True),
+                     rows("allowed", allowed, torch.int32, -(-V // 32), True))
+    if logits.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(logits).tangent is not None:
+        return ConstrainLogitsFunction.apply(logits, *c)
+    return _constrain(logits.detach(), c)

@@ -28,9 +28,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .lucid import _padded_dim, lucid_attention, lucid_decode
-from .model_ops import (TokenLogprobs, apply_rope, causal_lm_loss, causal_lm_loss_supported, qkv_rope, rms_norm,
-                        rms_norm_supported, rope_supported, swiglu, swiglu_supported, token_logprobs)
-from .paged import LucidPagedCache, lucid_decode_paged, write_pages
+from .model_ops import (RotaryPositions, TokenLogprobs, apply_rope, causal_lm_loss, causal_lm_loss_supported, qkv_rope, rms_norm,
+                        rms_norm_supported, rope_frequencies, rope_supported, rotary, swiglu, swiglu_supported,
+                        token_logprobs)
+from .paged import LucidPagedCache, lucid_decode_paged, lucid_prefill_paged, write_pages
 
 
 @dataclass
@@ -50,6 +51,10 @@ class LucidConfig:
     use_rope: bool = True
     tie_word_embeddings: bool = False
     initializer_range: float = 0.02
+    # beyond the reference's rotary embedding (any of them other than the default: model_ops.rotary)
+    rope_scaling: Optional[dict] = None       # model_ops.rope_frequencies
+    partial_rotary_factor: float = 1.0        # of the head's columns, the first
+    rope_interleaved: bool = False            # pairs of adjacent columns
 
     def __post_init__(self):
         if self.num_key_value_heads is None:
@@ -76,16 +81,27 @@ class LlamaRMSNorm(nn.Module):
 
 
 class LlamaRotaryEmbedding(nn.Module):
-    """Default RoPE (modeling_lucid.py:78-110): cos/sin of position * theta^(-2i/d)."""
+    """Default RoPE (modeling_lucid.py:78-110): cos/sin of position * theta^(-2i/d).  With scaled frequencies, a part of the
+    head or interleaved pairs (the configuration's) it gives what :func:`lucid_amd.model_ops.rotary` takes instead."""
 
     def __init__(self, config: LucidConfig, device=None):
         super().__init__()
         d = config.head_dim
         inv_freq = 1.0 / (config.rope_theta ** (torch.arange(0, d, 2, dtype=torch.int64, device=device).float() / d))
         self.register_buffer("inv_freq", inv_freq, persistent=False)
+        self.plain = config.rope_scaling is None and config.partial_rotary_factor == 1.0 and not config.rope_interleaved
+        if not self.plain:
+            part = int(d * config.partial_rotary_factor)
+            # (float64, so not a buffer: those follow the module's dtype)
+            self._freq, self.scale = rope_frequencies(part, config.rope_theta, config.rope_scaling)
+            self.interleaved = config.rope_interleaved
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, position_ids: torch.Tensor):
+        if not self.plain:
+            if self._freq.device != x.device:
+                self._freq = self._freq.to(x.device)
+            return RotaryPositions(position_ids, self._freq, self.interleaved, self.scale)
         freqs = position_ids[:, :, None].float() * self.inv_freq[None, None, :].to(x.device)
         emb = torch.cat((freqs, freqs), dim=-1)
         return emb.cos().to(x.dtype), emb.sin().to(x.dtype)
@@ -102,6 +118,14 @@ def apply_rotary_pos_emb(q, k, cos, sin, unsqueeze_dim: int = 1):
         return apply_rope(q, cos, sin), apply_rope(k, cos, sin)  # one HIP pass each way
     cos, sin = cos.unsqueeze(unsqueeze_dim), sin.unsqueeze(unsqueeze_dim)
     return (q * cos) + (rotate_half(q) * sin), (k * cos) + (rotate_half(k) * sin)
+
+
+def _turn(q, k, position_embeddings):
+    """q and k [B, H, T, d] turned by what LlamaRotaryEmbedding gives."""
+    if isinstance(position_embeddings, RotaryPositions):
+        p = position_embeddings
+        return rotary(q, k, p.positions, p.inv_freq, p.interleaved, p.scale)
+    return apply_rotary_pos_emb(q, k, *position_embeddings)
 
 
 class LlamaMLP(nn.Module):
@@ -225,22 +249,21 @@ class LucidAttention(nn.Module):
                            None if self.q_proj.bias is None else
                            torch.cat((self.q_proj.bias, self.k_proj.bias, self.v_proj.bias)))
             nq, nk = self.q_proj.out_features, self.k_proj.out_features
-            cos, sin = position_embeddings
-            if self.use_rope and self.head_dim == 64 and rope_supported(qkv.view(*hidden_shape).transpose(1, 2), cos):
+            if self.use_rope and self.head_dim == 64 and not isinstance(position_embeddings, RotaryPositions) \
+                    and rope_supported(qkv.view(*hidden_shape).transpose(1, 2), position_embeddings[0]):
                 # split + rotary embedding in one autograd step: the backward writes dq, dk and
                 # dv into one gradient of qkv instead of concatenating them
-                q, k, v = qkv_rope(qkv, cos, sin, nq, nk)
+                q, k, v = qkv_rope(qkv, *position_embeddings, nq, nk)
             else:
                 q, k, v = (t.view(hidden_shape).transpose(1, 2) for t in qkv.split((nq, nk, nk), dim=-1))
                 if self.use_rope:
-                    q, k = apply_rotary_pos_emb(q, k, cos, sin)
+                    q, k = _turn(q, k, position_embeddings)
         else:
             q = self.q_proj(hidden_states).view(hidden_shape).transpose(1, 2)
             k = self.k_proj(hidden_states).view(hidden_shape).transpose(1, 2)
             v = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
-            cos, sin = position_embeddings
             if self.use_rope:
-                q, k = apply_rotary_pos_emb(q, k, cos, sin)
+                q, k = _turn(q, k, position_embeddings)
         if isinstance(past_key_value, LucidPagedCache):
             out = self._paged(q, k, v, past_key_value)
             return self.o_proj(out.reshape(*input_shape, -1)), None
@@ -291,8 +314,8 @@ class LucidAttention(nn.Module):
 
     def _paged(self, q, k, v, cache: LucidPagedCache) -> torch.Tensor:
         """A pass over the sequences that the cache has selected: a prefill of empty ones through the
-        fused op, whose rows are written into their pages, else the new tokens through one paged
-        decoding call (which appends them); returns [B, T, Hq, d]."""
+        fused op, whose rows are written into their pages, chunks of prompts through one call of the paged prefill,
+        else the new tokens through one paged decoding call (both append them); returns [B, T, Hq, d]."""
         step = cache.step
         pools = cache.pools(self.layer_idx, k.shape[1], self.head_dim)
         if step.prefill:
@@ -300,6 +323,9 @@ class LucidAttention(nn.Module):
                                            return_vprime=True)
             write_pages(k, v_prime, *pools, step.table, step.lens, step.counts)
             return out
+        if step.chunk:
+            return lucid_prefill_paged(q, k, v, *pools, step.table, step.lens, step.counts, scaling=self.scaling,
+                                       eps=self.config.rms_norm_eps)
         return lucid_decode_paged(q, k, v, *pools, step.table, step.lens, scaling=self.scaling,
                                   eps=self.config.rms_norm_eps)[0]
 

@@ -6,6 +6,8 @@ layer's cache is two pools of pages that any number of sequences share out among
 
 * :func:`lucid_decode_paged` -- new tokens of every sequence of a batch against its pages, each sequence at
   its own length (C ``lucid_decode_paged``);
+* :func:`lucid_prefill_paged` -- chunks of prompts behind what is cached, each sequence with its own number of tokens (C
+  ``lucid_prefill_paged``);
 * :func:`write_pages` -- the K and V' rows of a (right-padded) prefill into their pages;
 * :func:`copy_pages` -- pages copied in every layer's pools at once;
 * :class:`LucidPagedCache` -- the pools, page tables and free pages of a model's sequences: forking (full
@@ -284,6 +286,7 @@ class PagedStep(NamedTuple):
     counts: Optional[torch.Tensor]  # int32 [B] real tokens of each right-padded row (None: all)
     positions: torch.Tensor         # int64 [B, T] of the tokens
     prefill: bool                   # every sequence is empty: the pass is a prefill
+    chunk: bool = False             # the rows are chunks of prompts behind what is cached
 
 
 class LucidPagedCache:
@@ -313,6 +316,7 @@ class LucidPagedCache:
         self._next = 0
         self._batch: tuple = ()
         self._lengths: Optional[list[int]] = None
+        self._chunk = False
         self._dev: Optional[tuple] = None  # (table, lens, 1 in the live rows) of the selection, on the device
         self._step: Optional[PagedStep] = None
 
@@ -403,10 +407,12 @@ class LucidPagedCache:
 
     # -- forward passes ------------------------------------------------------------------------
 
-    def select(self, seqs: Sequence[Optional[int]], lengths: Optional[Sequence[int]] = None) -> None:
+    def select(self, seqs: Sequence[Optional[int]], lengths: Optional[Sequence[int]] = None, chunk: bool = False) -> None:
         """The sequence of each row of the passes that follow, each at most once (None: an idle slot, whose row of the
         batch is ignored).  ``lengths``: the real tokens of each row of the next pass, a prefill that is padded on
-        the right."""
+        the right.  ``chunk``: the next pass brings chunks of prompts, behind what the sequences have cached or as their first
+        tokens, padded on the right where ``lengths`` are given (:func:`lucid_prefill_paged`: any number of tokens at the
+        rate of a prefill; one token beside them is a chunk too)."""
         seqs = tuple(seqs)
         live = [s for s in seqs if s is not None]
         if len(set(live)) != len(live):
@@ -419,6 +425,7 @@ class LucidPagedCache:
         if seqs != self._batch:
             self._batch, self._dev = seqs, None
         self._lengths = None if lengths is None else [int(n) for n in lengths]
+        self._chunk = bool(chunk)
         self._step = None
 
     def begin(self, B: int, T: int) -> PagedStep:
@@ -432,8 +439,8 @@ class LucidPagedCache:
         live = [(i, s) for i, s in enumerate(self._batch) if s is not None]
         past = [self._lens[s] for _, s in live]
         prefill = not any(past)
-        if counts is not None and (not prefill or max(counts, default=0) > T):
-            raise ValueError("lucid_amd: lengths are for a prefill of empty sequences, and at most its tokens")
+        if counts is not None and (not (prefill or self._chunk) or max(counts, default=0) > T):
+            raise ValueError("lucid_amd: lengths are for a prefill of empty sequences or for chunks, and at most its tokens")
         more = {s: -(-(n + (T if counts is None else counts[i])) // self.page_size) - len(self._pages[s])
                 for (i, s), n in zip(live, past)}
         need = sum(m for m in more.values() if m > 0)
@@ -453,7 +460,7 @@ class LucidPagedCache:
         table, lens, ones = self._dev
         positions = lens.clamp(min=0).long()[:, None] + torch.arange(T, device=self.device)
         self._step = PagedStep(table, lens, None if counts is None else
-                               torch.tensor(counts, dtype=torch.int32).to(self.device), positions, prefill)
+                               torch.tensor(counts, dtype=torch.int32).to(self.device), positions, prefill, self._chunk)
         return self._step
 
     @property
@@ -476,6 +483,7 @@ class LucidPagedCache:
         table, lens, ones = self._dev
         self._dev = table, lens + (ones * T if step.counts is None else step.counts * ones), ones
         self._lengths = self._step = None
+        self._chunk = False
 
     def pools(self, layer_idx: int, Hkv: int, d: int) -> tuple[torch.Tensor, torch.Tensor]:
         """(key_pages, vprime_pages) of a layer."""
