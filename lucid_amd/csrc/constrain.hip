@@ -8,6 +8,8 @@
 
 namespace lucid {
 
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // four values at any address
+
 constexpr int kConstrainSeg = 8192;  // values of a workgroup, a counter in LDS for each
 constexpr unsigned kConstrainSeen = 0x80000000u;  // of a counter: the token occurs in the prompt
 
@@ -31,74 +33,183 @@ __device__ __forceinline__ unsigned allowed_bits(const uint32_t* m, int j, int V
   return (unsigned)((((uint64_t)hi << 32) | lo) >> (j & 31));
 }
 
-// Grid R x segments, 512 threads.  BWD: x is the incoming gradient and raw the logits' row, whose sign is asked for where a
+// Whether a history's token names a value of the segment from lo on, and which
+__device__ __forceinline__ bool constrain_names(int64_t v, int lo, int V, unsigned& at) {
+  at = (unsigned)((int)v - lo);
+  return (uint64_t)v < (unsigned)V && at < (unsigned)kConstrainSeg;
+}
+
+constexpr int kConstrainThreads = 512;
+constexpr int kConstrainHeld = 8;  // tokens of a history that a lane holds
+
+// How a workgroup finds the tokens of its segment that have occurred
+enum class History {
+  None,
+  Held,  // up to 512 kConstrainHeld tokens: in registers, so that only their own counters are cleared, and a bit each
+         // tells which eight values have none
+  Long,  // any number: all counters cleared, one pass
+};
+
+// Grid R x segments.  BWD: x is the incoming gradient and raw the logits' row, whose sign is asked for where a
 // token has occurred.
-template <typename T, bool HIST, bool BWD>
-__global__ __launch_bounds__(512) void lucid_constrain_kernel(const T* __restrict__ x, int64_t sb, int64_t st,
-                                                              const T* __restrict__ raw, int64_t rb, int64_t rt, int Tn, int V,
-                                                              int segs, ConstrainRows a, T* __restrict__ out) {
-  constexpr int NT = 512, N = LpRow<T>::N, C = kConstrainSeg / NT / N;
-  __shared__ unsigned count[HIST ? kConstrainSeg : 1];
+// PAST: the results pass the caches by (the launcher's rule).
+template <typename T, History H, bool BWD, bool PAST>
+__global__ __launch_bounds__(kConstrainThreads) void lucid_constrain_kernel(const T* __restrict__ x, int64_t sb, int64_t st,
+                                                                            const T* __restrict__ raw, int64_t rb, int64_t rt,
+                                                                            int Tn, int V, int segs, ConstrainRows a,
+                                                                            T* __restrict__ out) {
+  constexpr int NT = kConstrainThreads, N = LpRow<T>::N, C = kConstrainSeg / NT / N;
+  constexpr bool COUNT = H == History::Long || (H == History::Held && !BWD);
+  __shared__ __attribute__((aligned(16))) unsigned count[COUNT ? kConstrainSeg : 4];
+  __shared__ unsigned bits[H == History::Held ? kConstrainSeg / 32 : 1];
+  __shared__ unsigned plus[H == History::Held && BWD ? kConstrainSeg / 32 : 1];  // of tokens whose logit is positive
   const int r = blockIdx.x / segs, seg = blockIdx.x - r * segs, tid = threadIdx.x;
   const LpRow<T> row(lp_row(x, sb, st, Tn, r), V);
-  const int q0 = seg * NT * C + tid, lo = row.first(seg * NT * C);  // (may be negative: the first chunk)
+  const int q0 = seg * NT * C + tid, lo = row.first(seg * NT * C);  // (lo may be negative: the first chunk)
+  const int64_t* h = H == History::None ? nullptr : a.history + r * a.hstride;
+  const int from = H == History::None || BWD || !a.prompt ? 0 : a.prompt[r];
+  const T* rr = BWD ? lp_row(raw, rb, rt, Tn, r) : nullptr;
+  int64_t held[H == History::Held ? kConstrainHeld : 1];
+  if constexpr (H == History::Held) {
+#pragma unroll
+    for (int k = 0; k < kConstrainHeld; ++k)
+      if (k * NT < a.N) held[k] = k * NT + tid < a.N ? h[k * NT + tid] : -1;
+  }
   typename LpRow<T>::V xv[C];
 #pragma unroll
   for (int c = 0; c < C; ++c)
     if (row.first(q0 + c * NT) < V) xv[c] = row.load(q0 + c * NT);
-  if constexpr (HIST) {
+  // what else a value takes is asked for here too, before anything waits
+  const float rho = a.rep ? a.rep[r] : a.rep0, pi = a.pres ? a.pres[r] : a.pres0, phi = a.freq ? a.freq[r] : a.freq0;
+  const uint32_t* mask = a.allowed ? a.allowed + r * a.astride : nullptr;
+  const float* bias = a.bias ? a.bias + r * a.bstride : nullptr;
+  unsigned ok[C];
+  float bv[BWD ? 1 : C][N];
 #pragma unroll
-    for (int i = tid; i < kConstrainSeg; i += NT) count[i] = 0;
+  for (int c = 0; c < C; ++c) {
+    const int q = q0 + c * NT, j = row.first(q);
+    ok[c] = mask && j < V ? allowed_bits(mask, j, V) : ~0u;
+    if constexpr (!BWD) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) bv[c][e] = 0.f;
+      if (bias && row.whole(q)) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const f32x4_any z = *reinterpret_cast<const f32x4_any*>(bias + j + e);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) bv[c][e + k] = z[k];
+        }
+      } else if (bias) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (j + e >= 0 && j + e < V) bv[c][e] = bias[j + e];
+      }
+    }
+  }
+  if constexpr (H == History::Held) {
+    unsigned at;
+    if (tid < kConstrainSeg / 32) {
+      bits[tid] = 0;
+      if (BWD) plus[tid] = 0;
+    }
+    bool up[kConstrainHeld];
+    if constexpr (BWD) {
+#pragma unroll
+      for (int k = 0; k < kConstrainHeld; ++k)
+        up[k] = k * NT < a.N && constrain_names(held[k], lo, V, at) && (float)rr[held[k]] > 0.f;
+    }
+    if constexpr (COUNT) {
+#pragma unroll
+      for (int k = 0; k < kConstrainHeld; ++k)
+        if (k * NT < a.N && constrain_names(held[k], lo, V, at)) count[at] = 0;
+    }
     __syncthreads();
-    const int64_t* h = a.history + r * a.hstride;
-    const int from = a.prompt ? a.prompt[r] : 0;
-#pragma unroll 8
-    for (int i = tid; i < a.N; i += NT) {
-      const int64_t v = h[i];
-      const int64_t at = v - lo;
-      if (v >= 0 && v < V && at >= 0 && at < kConstrainSeg) {
-        if (i >= from)
-          atomicAdd(&count[at], 1u);
-        else
-          atomicOr(&count[at], kConstrainSeen);
+#pragma unroll
+    for (int k = 0; k < kConstrainHeld; ++k)
+      if (k * NT < a.N && constrain_names(held[k], lo, V, at)) {
+        atomicOr(&bits[at >> 5], 1u << (at & 31));
+        if (BWD && up[k]) atomicOr(&plus[at >> 5], 1u << (at & 31));
+        if (COUNT && k * NT + tid >= from) atomicAdd(&count[at], 1u);
+      }
+    __syncthreads();
+  } else if constexpr (H == History::Long) {
+    for (int i = tid; i < kConstrainSeg / 4; i += NT) *reinterpret_cast<u32x4*>(&count[4 * i]) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    for (int i0 = tid; i0 < a.N; i0 += kConstrainHeld * NT) {
+      int64_t v[kConstrainHeld];
+#pragma unroll
+      for (int k = 0; k < kConstrainHeld; ++k) v[k] = i0 + k * NT < a.N ? h[i0 + k * NT] : -1;
+#pragma unroll
+      for (int k = 0; k < kConstrainHeld; ++k) {
+        unsigned at;
+        if (constrain_names(v[k], lo, V, at)) {
+          if (i0 + k * NT >= from)
+            atomicAdd(&count[at], 1u);
+          else
+            atomicOr(&count[at], kConstrainSeen);
+        }
       }
     }
     __syncthreads();
   }
-  const float rho = a.rep ? a.rep[r] : a.rep0, pi = a.pres ? a.pres[r] : a.pres0, phi = a.freq ? a.freq[r] : a.freq0;
-  const uint32_t* mask = a.allowed ? a.allowed + r * a.astride : nullptr;
-  const float* bias = a.bias ? a.bias + r * a.bstride : nullptr;
-  const T* rr = BWD ? lp_row(raw, rb, rt, Tn, r) : nullptr;
   T* orow = out + (int64_t)r * V;
   const bool same = (reinterpret_cast<uintptr_t>(orow) & 15) / sizeof(T) == (unsigned)row.shift;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int q = q0 + c * NT, j = row.first(q);
     if (j >= V) break;
-    const unsigned ok = mask ? allowed_bits(mask, j, V) : ~0u;
-    typename LpRow<T>::V o;
+    float y[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      float y = (float)xv[c][e];
-      if constexpr (HIST) {
-        const unsigned n = count[j + e - lo];
-        if (n) {
-          if constexpr (BWD) {
-            const float z = j + e >= 0 && j + e < V ? (float)rr[j + e] : 0.f;
-            y = z > 0.f ? y / rho : y * rho;
-          } else {
-            y = y > 0.f ? y / rho : y * rho;
-            const unsigned k = n & ~kConstrainSeen;
-            if (k) y = (y - pi) - phi * (float)k;
+    for (int e = 0; e < N; ++e) y[e] = (float)xv[c][e];
+    if constexpr (H != History::None) {
+      const int at = (q - seg * NT * C) * N;  // j - lo
+      unsigned n[N], positive = 0;
+      bool any = false;
+      if constexpr (H == History::Held) {
+        const unsigned b = bits[at >> 5] >> (at & 31);
+        any = (b & ((1u << N) - 1)) != 0;
+        if (BWD) positive = plus[at >> 5] >> (at & 31);
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) n[e] = b >> e & 1 ? kConstrainSeen | (COUNT ? count[at + e] : 0u) : 0u;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const u32x4 z = *reinterpret_cast<const u32x4*>(&count[at + e]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            n[e + k] = z[k];
+            any |= z[k] != 0;
           }
         }
       }
-      if (!BWD && bias && j + e >= 0 && j + e < V) y += bias[j + e];
-      if (!(ok >> e & 1)) y = BWD ? 0.f : -INFINITY;
-      o[e] = (T)y;
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (n[e]) {
+            const bool up = !BWD                      ? y[e] > 0.f
+                            : H == History::Held ? (positive >> e & 1)
+                                                 : j + e >= 0 && j + e < V && (float)rr[j + e] > 0.f;
+            y[e] = up ? y[e] / rho : y[e] * rho;
+            const unsigned k = n[e] & ~kConstrainSeen;
+            if (!BWD && k) y[e] = (y[e] - pi) - phi * (float)k;
+          }
+      }
+    }
+    typename LpRow<T>::V o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (!BWD) y[e] += bv[BWD ? 0 : c][e];
+      if (!(ok[c] >> e & 1)) y[e] = BWD ? 0.f : -INFINITY;
+      o[e] = (T)y[e];
     }
     if (same && row.whole(q)) {
-      *reinterpret_cast<typename LpRow<T>::V*>(orow + j) = o;
+      auto* to = reinterpret_cast<typename LpRow<T>::V*>(orow + j);
+      if constexpr (PAST)
+        __builtin_nontemporal_store(o, to);
+      else
+        *to = o;
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e)

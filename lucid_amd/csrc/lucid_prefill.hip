@@ -15,6 +15,8 @@
 //   lucid_prefill_sweep_kernel  (attend) the softmax over all rows, cached and new
 //   lucid_prefill_join_kernel   parts of a sweep that was cut along the keys
 // The sweeps are the work: 4 (Hq + Hkv) d flops for each pair of a token and a row.
+#include <type_traits>
+
 #include "paged_common.h"
 
 namespace lucid {
@@ -22,7 +24,7 @@ namespace lucid {
 constexpr int kPanel = 256;      // new rows that one solve takes
 constexpr int kPanelBlocks = 8;  // of 32 rows
 constexpr int kSweepKeys = 128;  // keys of a staged tile
-// A panel's own P: 28 tiles below the diagonal blocks as operands (hi and lo bf16, negated), 8 diagonal blocks
+// A panel's own -P_tj / P_tt: 28 tiles below the diagonal blocks as operands (hi and lo bf16), 8 diagonal blocks
 // transposed in fp32, and 1 / P_tt of its rows
 constexpr int kPanelTile = 4 * 512;                                          // bf16 of an operand tile
 constexpr size_t kPanelDiag = (size_t)28 * kPanelTile * 2;                   // byte offset of the diagonal blocks
@@ -46,6 +48,17 @@ __device__ __forceinline__ unsigned prefill_row(const PrefillBatch& s, const Pag
   return id * p.page + h * p.head + (unsigned)(j - prefill_page(s, j) * s.page) * p.row;
 }
 
+// acc + the squares of eight bf16 values
+__device__ __forceinline__ float dot8(const bf16x8& x, float acc) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const bf16x2 y = {x[2 * k], x[2 * k + 1]};
+    acc = __builtin_amdgcn_fdot2_f32_bf16(y, y, acc, false);
+  }
+  return acc;
+}
+
 // Eight columns c .. c+7 of a row of d, zeros beyond d
 __device__ __forceinline__ bf16x8 ld8_cols(const bf16* row, int c, int d, bool vec) {
   const bf16x4 a = ld4_cols(row, c, d, vec), b = ld4_cols(row, c + 4, d, vec);
@@ -60,18 +73,19 @@ __device__ __forceinline__ T* tile_at(T* tile, int r, int c) {
 }
 
 // --------------------------------------------------------------------------------------------
-// Grid (panels of L, Hkv, B), 512 threads.  Every workgroup of a sequence looks its page ids over itself.
+// Grid (4 panels of L, Hkv, B), 512 threads: four workgroups share a panel's rows to write and its tiles.  Every workgroup of
+// a sequence looks its page ids over itself.
 // --------------------------------------------------------------------------------------------
 template <int W>
 __global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __restrict__ k, Strides ks, int vec,
                                                                  PagedPool kp, PrefillBatch seq, PagedScale f, float eps, int d,
                                                                  char* __restrict__ pmat, bf16* __restrict__ o, Strides os,
-                                                                 int G) {
+                                                                 int ovec, int G) {
   constexpr int CPR = W / 8, NKS = W / 16;
   __shared__ __attribute__((aligned(16))) bf16 rows[kPanel * W];
-  __shared__ float norm[kPanel];
+  __shared__ float norm[kPanel], inv[kPanel];
   __shared__ int bad_;
-  const int panel = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int panel = blockIdx.x >> 2, share = blockIdx.x & 3, h = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
   const int32_t* tbl = seq.table + b * seq.tstride;
   const int n = seq.lens[b];
@@ -92,12 +106,20 @@ __global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __r
   const int t0 = panel * kPanel;
   // the outputs of padding (zeros) and of a sequence that is left out (NaN)
   const int from = bad ? 0 : c;
-  for (int t = max(t0, from); t < min(t0 + kPanel, seq.L); ++t) {
-    const float x = t < c ? __builtin_nanf("") : 0.f;
-    for (int i = tid; i < G * d; i += 512) o[b * os.b + (h * G + i / d) * os.h + t * os.t + i % d] = (bf16)x;
+  const int each = kPanel / 4, t1 = min(t0 + each * (share + 1), seq.L);
+  const bool packed = ovec && os.h == d;  // a row of a group's heads is one run
+  for (int t = max(t0 + each * share, from) + w; t < t1; t += 8) {
+    const bf16 x = (bf16)(t < c ? __builtin_nanf("") : 0.f);
+    bf16* op = o + b * os.b + (int64_t)h * G * os.h + t * os.t;
+    if (packed) {
+      for (int i = 4 * lane; i < G * d; i += 256) *reinterpret_cast<bf16x4*>(op + i) = bf16x4{x, x, x, x};
+    } else {
+      for (int q = 0; q < G; ++q)
+        for (int i = lane; i < d; i += 64) op[q * os.h + i] = x;
+    }
   }
   if (bad) c = 0;
-  if (panel == 0 && h == 0 && tid == 0) seq.info[b] = make_int2(max(n, 0), c);
+  if (blockIdx.x == 0 && h == 0 && tid == 0) seq.info[b] = make_int2(max(n, 0), c);
   if (t0 >= c) return;
   const int R = min(c - t0, kPanel);
   const bf16* kb = k + b * ks.b + h * ks.h + (int64_t)t0 * ks.t;
@@ -109,12 +131,13 @@ __global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __r
     if (r < R) {
       x = ld8_cols(kb + r * ks.t, cc * 8, d, vec);
       const int j = n + t0 + r;
-      *reinterpret_cast<bf16x8*>(paged_at(kp, prefill_row(seq, kp, tbl[prefill_page(seq, j)], j, h)) + cc * 8) = x;
+      if (r / each == share)
+        *reinterpret_cast<bf16x8*>(paged_at(kp, prefill_row(seq, kp, tbl[prefill_page(seq, j)], j, h)) + cc * 8) = x;
     }
     *reinterpret_cast<bf16x8*>(tile_at<W>(rows, r, cc)) = x;
   }
   __syncthreads();
-  char* pm = pmat + (((int64_t)b * seq.Hkv + h) * gridDim.x + panel) * kPanelBytes;
+  char* pm = pmat + (((int64_t)b * seq.Hkv + h) * (gridDim.x >> 2) + panel) * kPanelBytes;
   {
     const int r = tid >> 1, half = tid & 1;
     float nn = 0.f;
@@ -128,13 +151,13 @@ __global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __r
       norm[r] = rsqrtf(nn / (float)d + eps);
       // 1 / P_tt; the exponent is the small difference of two terms of size sqrt(d): in fp64
       const double ms = (double)nn / d;
-      reinterpret_cast<float*>(pm + kPanelInv)[r] =
-          __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / f.s - f.s * d * ms / (ms + eps))));
+      inv[r] = __builtin_amdgcn_exp2f((float)(1.4426950408889634 * (1.0 / f.s - f.s * d * ms / (ms + eps))));
+      if (share == 0) reinterpret_cast<float*>(pm + kPanelInv)[r] = inv[r];
     }
   }
   __syncthreads();
   // tiles (i, j), j <= i, of 32 x 32: S^T = K_j . K_i, lane <-> row of i, element <-> row of j
-  for (int idx = w; idx < 36; idx += 8) {
+  for (int idx = 4 * w + share; idx < 36; idx += 32) {
     int i = (int)((sqrtf(8.f * idx + 1.f) - 1.f) * 0.5f);
     if ((i + 1) * (i + 2) / 2 <= idx) ++i;
     if (i * (i + 1) / 2 > idx) --i;
@@ -146,17 +169,15 @@ __global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __r
       sc = mfma32(ld8(tile_at<W>(rows, 32 * j + l32, 2 * st + g)), ld8(tile_at<W>(rows, 32 * i + l32, 2 * st + g)), sc);
     float nr[16];
     lds_rows16(&norm[32 * j], g, nr);
-    const float c1 = f.sl2 * norm[32 * i + l32];
+    const float c1 = f.sl2 * norm[32 * i + l32], over = -inv[32 * i + l32];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(c1 * nr[e], sc[e], -f.c0));
+    for (int e = 0; e < 16; ++e) sc[e] = over * __builtin_amdgcn_exp2f(fmaf(c1 * nr[e], sc[e], -f.c0));
     if (i == j) {
       float* dg = reinterpret_cast<float*>(pm + kPanelDiag) + i * 1024;
 #pragma unroll
       for (int e = 0; e < 16; ++e) dg[drow(e, g) * 32 + l32] = l32 > drow(e, g) ? sc[e] : 0.f;
     } else {
       bf16* op = reinterpret_cast<bf16*>(pm) + (i * (i - 1) / 2 + j) * kPanelTile;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = -sc[e];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const bf16x8 hi = pack_b(sc, q), lo = pack_lo(sc, q, hi);
@@ -262,7 +283,7 @@ struct SweepSmem {
       float o[2][64][W + 4], m[4][64], l[4][64];
     } fin;
   } u;
-  float nn[8][32];  // per wave: 1 / rms of a sub-tile's keys
+  float nr[kSweepKeys];  // couple: 1 / rms of the tile's keys
 };
 
 // Lane part of the offset of paged_tr_a's first read at row0 = 0 of a tile; the second read is 8 rows on
@@ -387,19 +408,31 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void l
       stage(jt + 1, idn, buf ^ 1);
       if (jt + 2 < ntile) idn = page_id(jt + 2);
     }
-    if (active && jb <= most) {
-      const bf16* tk = sm.u.st.k[buf];
-      const bf16* tv = sm.u.st.v[buf];
-      const bool mask = jb + kSweepKeys - 1 > free;
+    const bf16* tk = sm.u.st.k[buf];
+    const bf16* tv = sm.u.st.v[buf];
+    const bool work = active && jb <= most, mask = jb + kSweepKeys - 1 > free;
+    if constexpr (!ATTEND) {  // four lanes a key
+      const int r = tid >> 2;
+      float nn = 0.f;
+#pragma unroll
+      for (int cc = 0; cc < CPR; cc += 4)
+        if (CPR % 4 == 0 || cc + (tid & 3) < CPR) nn = dot8(ld8(tile_at<W>(tk, r, cc + (tid & 3))), nn);
+      nn = lanes_sum<4>(nn);
+      if ((tid & 3) == 0) sm.nr[r] = rsqrtf(nn / (float)d + eps);
+    }
+    f32x16 s[NMT];
+    if (work) {
+#pragma unroll
+      for (int i = 0; i < NMT; ++i) {
+        const int mt = kg + KSP * i;
+        s[i] = zero16();
+#pragma unroll
+        for (int st = 0; st < NKS; ++st) s[i] = mfma32(ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g)), xb[st], s[i]);
+      }
+    }
+    if constexpr (!ATTEND) __syncthreads();
+    if (work) {
       if constexpr (ATTEND) {
-        f32x16 s[NMT];
-#pragma unroll
-        for (int i = 0; i < NMT; ++i) {
-          const int mt = kg + KSP * i;
-          s[i] = zero16();
-#pragma unroll
-          for (int st = 0; st < NKS; ++st) s[i] = mfma32(ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g)), xb[st], s[i]);
-        }
         if (mask) {
 #pragma unroll
           for (int i = 0; i < NMT; ++i)
@@ -440,27 +473,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void l
 #pragma unroll
         for (int i = 0; i < NMT; ++i) {
           const int mt = kg + KSP * i;
-          f32x16 s = zero16();
-          float nn = 0.f;
-#pragma unroll
-          for (int st = 0; st < NKS; ++st) {
-            const bf16x8 kf = ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g));
-            s = mfma32(kf, xb[st], s);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) nn = fmaf((float)kf[e], (float)kf[e], nn);
-          }
-          nn = wave_sum32(nn);
-          if (g == 0) sm.nn[w][l32] = rsqrtf(nn / (float)d + eps);
           float nr[16];
-          lds_rows16(&sm.nn[w][0], g, nr);
+          lds_rows16(&sm.nr[32 * mt], g, nr);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(c1 * nr[e], s[e], -f.c0));
-            s[e] = mask && jb + mt * 32 + drow(e, g) > lim ? 0.f : p;
+          for (int e = 0; e < 16; ++e) s[i][e] = __builtin_amdgcn_exp2f(fmaf(c1 * nr[e], s[i][e], -f.c0));
+          if (mask) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (jb + mt * 32 + drow(e, g) > lim) s[i][e] = 0.f;
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const bf16x8 hi = pack_b(s, k), lo = pack_lo(s, k, hi);
+            const bf16x8 hi = pack_b(s[i], k), lo = pack_lo(s[i], k, hi);
 #pragma unroll
             for (int q = 0; q < NDT; ++q) {
               const bf16x8 a = tile_tr<W>(tv, tr[q], mt * 32 + 16 * k);
@@ -639,96 +663,126 @@ __global__ __launch_bounds__(256) void lucid_prefill_join_kernel(const bf16* __r
 }
 
 // --------------------------------------------------------------------------------------------
-// One panel's rows in order: x_t = y_t / P_tt, w_t = bf16(x_t), y_u -= P_ut w_t for u > t.  Grid (Hkv, B), a wave for
-// each 32 columns, which are independent: it holds all rows of the panel (lane <-> column, elements <-> rows), goes
-// through a block of 32 rows by itself, and takes it out of the blocks behind it with MFMAs, the block's rows as
-// they are in its registers as the second operand.
+// One panel's rows in order: with z_t = y_t / P_tt, w_t = bf16(z_t) and z_u -= P_ut / P_uu w_t for u > t.  Grid (32 columns,
+// Hkv, B), one wave: columns are independent, and a wave holds all rows of its own (lane <-> column, elements <->
+// rows of a block of 32).  It goes through a block by itself, row by row, each row's value from one lane half to the
+// other in the VALU, and takes it out of the blocks behind with MFMAs, the block's rows as they stand in registers as the
+// second operand.  The chain of 256 dependent rows bounds it, not the 145 KB of P it stages.
+// (The blocks are one loop over registers that move up by a block: with its eight blocks written out the kernel's 60 KB of
+// instructions, each run once, took 41 us to fetch.)
 // --------------------------------------------------------------------------------------------
 template <int W>
-__global__ __launch_bounds__(64 * ((W + 31) / 32)) __attribute__((amdgpu_waves_per_eu(1))) void lucid_prefill_solve_kernel(
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1))) void lucid_prefill_solve_kernel(
     const char* __restrict__ pmat, int panels, int panel, const float* __restrict__ y, int64_t yrows, PagedPool vp,
     PrefillBatch seq, int d) {
-  constexpr int NW = (W + 31) / 32;
   __shared__ __attribute__((aligned(16))) struct {
     char p[kPanelBytes];
     unsigned off[kPanel];
   } sm;
-  const int h = blockIdx.x, b = blockIdx.y;
+  const int h = blockIdx.y, b = blockIdx.z;
   const int2 info = seq.info[b];
   const int R = min(info.y - panel * kPanel, kPanel);
   if (R <= 0) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 5, l32 = lane & 31;
+  const int lane = threadIdx.x, g = lane >> 5, l32 = lane & 31;
   const int nb = (R + 31) / 32;  // blocks with rows
   const int64_t bh = (int64_t)b * seq.Hkv + h;
   const char* pm = pmat + (bh * panels + panel) * kPanelBytes;
   auto fetch = [&](size_t first, int pieces) {  // 1 KB each
-    for (int i = w; i < pieces; i += NW)
+    for (int i = 0; i < pieces; ++i)
       __builtin_amdgcn_global_load_lds(reinterpret_cast<const bf16*>(pm + first) + i * 512 + lane * 8,
                                        reinterpret_cast<bf16*>(sm.p + first) + i * 512, 16, 0, 0);
   };
   fetch(kPanelInv, 1);
   fetch(kPanelDiag, 4 * nb);
-  fetch(0, 4 * (nb * (nb - 1) / 2));
   const int n = info.x + panel * kPanel;
-  for (int r = tid; r < R; r += 64 * NW) {
+  for (int r = lane; r < R; r += 64) {  // (those behind stay as they are: read, not used)
     const int j = n + r;
     sm.off[r] = prefill_row(seq, vp, seq.table[b * seq.tstride + prefill_page(seq, j)], j, h);
   }
-  const int col = 32 * w + l32;
+  const int col = 32 * blockIdx.x + l32;
   const bool on = col < d;
-  f32x16 acc[kPanelBlocks];
-  const float* yb = y + (bh * yrows + panel * kPanel) * W + col;
+  f32x16 acc[kPanelBlocks];  // of the block at hand and those behind it
+  const float* yb = y + (bh * yrows + panel * kPanel) * W + min(col, W - 1);
 #pragma unroll
   for (int i = 0; i < kPanelBlocks; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int r = 32 * i + drow(e, g);
-      acc[i][e] = on && r < R ? yb[(int64_t)r * W] : 0.f;
-    }
+    for (int e = 0; e < 16; ++e) acc[i][e] = yb[min(32 * i + drow(e, g), R - 1) * W];
+  fetch(0, 4 * (nb * (nb - 1) / 2));
   dma_wait();
   __syncthreads();
-  const bf16* off = reinterpret_cast<const bf16*>(sm.p);
   const float* inv = reinterpret_cast<const float*>(sm.p + kPanelInv);
 #pragma unroll
   for (int i = 0; i < kPanelBlocks; ++i) {
-    if (i < nb) {
-      const float* dg = reinterpret_cast<const float*>(sm.p + kPanelDiag) + i * 1024;
-      f32x16 fin;
+    float iv[16];
+    lds_rows16(inv + 32 * i, g, iv);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) fin[e] = 0.f;
+    for (int e = 0; e < 16; ++e) acc[i][e] = 32 * i + drow(e, g) < R ? acc[i][e] * iv[e] : 0.f;
+    asm volatile("" ::: "memory");  // a block's comparisons at a time
+  }
+  const float* dg = reinterpret_cast<const float*>(sm.p + kPanelDiag) + 4 * g;
+#pragma unroll 1
+  for (int i = 0; i < nb; ++i, dg += 1024) {
+    f32x16 fin;
 #pragma unroll
-      for (int t = 0; t < 32; ++t) {
-        const int e_t = 4 * (t >> 3) + (t & 3), g_t = (t >> 2) & 1;
-        const float x = acc[i][e_t] * inv[32 * i + t];
-        const unsigned u = __builtin_bit_cast(unsigned, (float)(bf16)x);
-        const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // the first half's, the second's
-        const float wt = __builtin_bit_cast(float, g_t ? (unsigned)both[1] : (unsigned)both[0]);
-        fin[e_t] = g == g_t ? wt : fin[e_t];
+    for (int e = 0; e < 16; ++e) fin[e] = 0.f;
+    // P of row t arrives kAhead rows before its turn
+    constexpr int kAhead = 3;
+    f32x4 p[kAhead + 1][4];
+    auto ask = [&](int t) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (8 * q + 7 <= t) continue;  // no row of these is behind t
-          const f32x4 p = *reinterpret_cast<const f32x4*>(dg + 32 * t + 8 * q + 4 * g);
+      for (int q = 0; q < 4; ++q)
+        if (8 * q + 7 > t) p[t % (kAhead + 1)][q] = *reinterpret_cast<const f32x4*>(dg + 32 * t + 8 * q);
+    };
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (8 * q + 4 + k > t) acc[i][4 * q + k] = fmaf(-p[k], wt, acc[i][4 * q + k]);
-        }
+    for (int t = 0; t < kAhead; ++t) ask(t);
+#pragma unroll
+    for (int t = 0; t < 32; ++t) {
+      const int e_t = 4 * (t >> 3) + (t & 3), g_t = (t >> 2) & 1;
+      if (t + kAhead < 32) ask(t + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+      const unsigned u = __builtin_bit_cast(unsigned, (float)(bf16)acc[0][e_t]);
+      const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // the first half's, the second's
+      const float wt = __builtin_bit_cast(float, g_t ? (unsigned)both[1] : (unsigned)both[0]);
+      fin[e_t] = g == g_t ? wt : fin[e_t];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (8 * q + 4 + k > t) acc[0][4 * q + k] = fmaf(p[t % (kAhead + 1)][q][k], wt, acc[0][4 * q + k]);
+    }
+    const bf16x8 w0 = pack_b(fin, 0), w1 = pack_b(fin, 1);
+    // the blocks behind, each one place up; what lies behind the last one is not looked at again
+    auto take = [&](auto first, auto last) {
+      constexpr int K0 = decltype(first)::value, K1 = decltype(last)::value;
+      const bf16* tile[K1 - K0 + 1];
+#pragma unroll
+      for (int k = K0; k <= K1; ++k) {
+        const int at = min(i + k, nb - 1);
+        tile[k - K0] = reinterpret_cast<const bf16*>(sm.p) + (at * (at - 1) / 2 + min(i, at - 1)) * kPanelTile + lane * 8;
       }
-      const bf16x8 w0 = pack_b(fin, 0), w1 = pack_b(fin, 1);
 #pragma unroll
-      for (int k = i + 1; k < kPanelBlocks; ++k)
-        if (k < nb) {
-          const bf16* tile = off + (k * (k - 1) / 2 + i) * kPanelTile + lane * 8;
-          acc[k] = mfma32(ld8(tile), w0, acc[k]);
-          acc[k] = mfma32(ld8(tile + 512), w0, acc[k]);
-          acc[k] = mfma32(ld8(tile + 1024), w1, acc[k]);
-          acc[k] = mfma32(ld8(tile + 1536), w1, acc[k]);
-        }
-      if (col < W) {
+      for (int part = 0; part < 4; ++part)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int r = 32 * i + drow(e, g);
-          if (r < R) paged_at(vp, sm.off[r])[col] = (bf16)(on ? fin[e] : 0.f);
-        }
+        for (int k = K0; k <= K1; ++k)
+          acc[part < 3 ? k : k - 1] = mfma32(ld8(tile[k - K0] + 512 * part), part < 2 ? w0 : w1, acc[k]);
+    };
+    if (i + 1 < nb) take(std::integral_constant<int, 1>{}, std::integral_constant<int, 3>{});
+    if (i + 4 < nb) take(std::integral_constant<int, 4>{}, std::integral_constant<int, 7>{});
+    if (col < W) {
+      unsigned at[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const u32x4 r = *reinterpret_cast<const u32x4*>(&sm.off[32 * i + 8 * q + 4 * g]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) at[4 * q + k] = r[k];
+      }
+      if (32 * (i + 1) <= R) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) paged_at(vp, at[e])[col] = (bf16)(on ? fin[e] : 0.f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (32 * i + drow(e, g) < R) paged_at(vp, at[e])[col] = (bf16)(on ? fin[e] : 0.f);
       }
     }
   }

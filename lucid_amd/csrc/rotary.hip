@@ -29,18 +29,30 @@ struct RotaryCall {
   int B, T, d, part;
   int tokens;      // of a workgroup
   float scale, dir;  // dir -1: the gradient
-  int units;       // of a head: part / 2 / V of pairs, then (d - part) / V of columns that stay
+  int turning, units;        // units of a head: those of pairs, and with those of columns that stay
+  int stay;                  // columns of a unit that stay: V or 2 V
   float per_unit, per_head;  // 1 / units, 1 / (units (Hq + Hkv))
 };
+
+template <bool PAST, typename V>
+__device__ __forceinline__ void rotary_put(void* to, const V& x) {
+  if constexpr (PAST)
+    __builtin_nontemporal_store(x, static_cast<V*>(to));
+  else
+    *static_cast<V*>(to) = x;
+}
 
 // i / n by the reciprocal r of n: exact for i < 2^22
 __device__ __forceinline__ int div_by(int i, float r) { return (int)(((float)i + 0.5f) * r); }
 
-// V pairs a unit: V columns of either half, or 2 V adjacent ones.  256 threads.
-template <typename T, int V, bool INTER>
+// V pairs a unit: V columns of either half, or 2 V adjacent ones.  A run that is no whole number of units
+// ends in one that overlaps the one before (the same values twice), so that any head dim goes in 16-byte accesses, which
+// need no alignment.  256 threads.
+// PAST: results pass the caches by (the launcher's rule).
+template <typename T, int V, bool INTER, bool PAST>
 __global__ __launch_bounds__(256) void lucid_rotary_kernel(const RotaryCall c) {
-  typedef T TV __attribute__((ext_vector_type(V)));
-  typedef T T2 __attribute__((ext_vector_type(2 * V)));
+  typedef T TV __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  typedef T T2 __attribute__((ext_vector_type(2 * V), aligned(sizeof(T))));
   __shared__ __attribute__((aligned(16))) float2 turn[kRotaryTokens][kRotaryPairs];
   const int half = c.part / 2;
   const int64_t all = (int64_t)c.B * c.T, t0 = (int64_t)blockIdx.x * c.tokens;
@@ -63,7 +75,7 @@ __global__ __launch_bounds__(256) void lucid_rotary_kernel(const RotaryCall c) {
     turn[tk][p] = make_float2(cs * c.scale, sn * c.scale * c.dir);
   }
   __syncthreads();
-  const int heads = c.q.heads + c.k.heads, work = n * heads * c.units, turning = half / V;
+  const int heads = c.q.heads + c.k.heads, work = n * heads * c.units;
 #pragma unroll 2
   for (int i = threadIdx.x; i < work; i += 256) {
     const int tk = div_by(i, c.per_head), rest = i - tk * heads * c.units;
@@ -71,40 +83,40 @@ __global__ __launch_bounds__(256) void lucid_rotary_kernel(const RotaryCall c) {
     const int u = rest - h * c.units;
     const bool isk = h >= c.q.heads;
     if (isk) h -= c.q.heads;
-    const int64_t tok = t0 + tk, b = tok / c.T, t = tok - b * c.T;
+    const int64_t tok = t0 + tk, bt = tok / c.T, t = tok - bt * c.T;
     const Strides xs = isk ? c.k.xs : c.q.xs, ys = isk ? c.k.ys : c.q.ys;
-    const T* x = static_cast<const T*>(isk ? c.k.x : c.q.x) + b * xs.b + h * xs.h + t * xs.t;
-    T* y = static_cast<T*>(isk ? c.k.y : c.q.y) + b * ys.b + h * ys.h + t * ys.t;
-    if (u >= turning) {
-      const int col = c.part + (u - turning) * V;
-      *reinterpret_cast<TV*>(y + col) = *reinterpret_cast<const TV*>(x + col);
+    const T* x = static_cast<const T*>(isk ? c.k.x : c.q.x) + bt * xs.b + h * xs.h + t * xs.t;
+    T* y = static_cast<T*>(isk ? c.k.y : c.q.y) + bt * ys.b + h * ys.h + t * ys.t;
+    if (u >= c.turning) {
+      const int col = min(c.part + (u - c.turning) * c.stay, c.d - c.stay);
+      if (INTER && c.stay == 2 * V)
+        rotary_put<PAST>(y + col, *reinterpret_cast<const T2*>(x + col));
+      else
+        rotary_put<PAST>(y + col, *reinterpret_cast<const TV*>(x + col));
       continue;
     }
-    const float2* tn = &turn[tk][u * V];
-    if constexpr (INTER && V == 1) {  // pairs at any address
-      const float a = (float)x[2 * u], bb = (float)x[2 * u + 1];
-      y[2 * u] = (T)fmaf(a, tn->x, -(bb * tn->y));
-      y[2 * u + 1] = (T)fmaf(bb, tn->x, a * tn->y);
-    } else if constexpr (INTER) {
-      const T2 z = *reinterpret_cast<const T2*>(x + 2 * u * V);
+    const int p0 = min(u * V, half - V);  // first pair
+    const float2* tn = &turn[tk][p0];
+    if constexpr (INTER) {
+      const T2 z = *reinterpret_cast<const T2*>(x + 2 * p0);
       T2 o;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float a = (float)z[2 * e], bb = (float)z[2 * e + 1];
-        o[2 * e] = (T)fmaf(a, tn[e].x, -(bb * tn[e].y));
-        o[2 * e + 1] = (T)fmaf(bb, tn[e].x, a * tn[e].y);
+        const float a = (float)z[2 * e], b = (float)z[2 * e + 1];
+        o[2 * e] = (T)fmaf(a, tn[e].x, -(b * tn[e].y));
+        o[2 * e + 1] = (T)fmaf(b, tn[e].x, a * tn[e].y);
       }
-      *reinterpret_cast<T2*>(y + 2 * u * V) = o;
+      rotary_put<PAST>(y + 2 * p0, o);
     } else {
-      const TV a = *reinterpret_cast<const TV*>(x + u * V), bb = *reinterpret_cast<const TV*>(x + half + u * V);
+      const TV a = *reinterpret_cast<const TV*>(x + p0), b = *reinterpret_cast<const TV*>(x + half + p0);
       TV o, p;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        o[e] = (T)fmaf((float)a[e], tn[e].x, -((float)bb[e] * tn[e].y));
-        p[e] = (T)fmaf((float)bb[e], tn[e].x, (float)a[e] * tn[e].y);
+        o[e] = (T)fmaf((float)a[e], tn[e].x, -((float)b[e] * tn[e].y));
+        p[e] = (T)fmaf((float)b[e], tn[e].x, (float)a[e] * tn[e].y);
       }
-      *reinterpret_cast<TV*>(y + u * V) = o;
-      *reinterpret_cast<TV*>(y + half + u * V) = p;
+      rotary_put<PAST>(y + p0, o);
+      rotary_put<PAST>(y + half + p0, p);
     }
   }
 }

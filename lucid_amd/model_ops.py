@@ -32,6 +32,7 @@ dim 64; the loss: a vocabulary that is a multiple of 8) and raise otherwise; the
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import operator
 from typing import NamedTuple
@@ -269,31 +270,53 @@ class RotaryPositions(NamedTuple):
 _ROTARY_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
+@functools.lru_cache(maxsize=4096)
+def _strides(stride: tuple):
+    """The first three of a tensor's strides as the C entry points take them (they only read the array)."""
+    return (ctypes.c_int64 * 3)(*stride[:3])
+
+
+def _tracked(*tensors: torch.Tensor) -> bool:
+    """Whether a result of these needs an autograd function: a gradient, or a tangent of forward-mode differentiation
+    (which the functions refuse)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    # (the level first: 1 of the 2 us that asking two tensors for a tangent takes)
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _rotary(q, k, positions, inv_freq, interleaved, scale, inverse):
     """q and k (either may be None) turned, into new [B, T, H, d] buffers seen as [B, H, T, d]."""
-    some = q if q is not None else k
+    some = k if q is None else q
     B, _, T, d = some.shape
-    args, outs = [], []
-    for x in (q, k):
-        if x is None:
-            args += [None, None, None, None, 0]
-            outs.append(None)
-            continue
-        x = x if x.stride(3) == 1 or d == 1 else x.contiguous()
-        H = x.shape[1]
-        y = torch.empty((B, T, H, d), dtype=x.dtype, device=x.device)
-        args += [x, (ctypes.c_int64 * 3)(*x.stride()[:3]), y.data_ptr(), (ctypes.c_int64 * 3)(T * H * d, d, H * d), H]
-        outs.append(y.transpose(1, 2))
+    dtype, dev = some.dtype, some.device
+    qo = ko = None
+    qa = ka = (None, None, None, None, 0)
+    if q is not None:
+        if q.stride(3) != 1 and d > 1:
+            q = q.contiguous()
+        H = q.shape[1]
+        qo = torch.empty((B, T, H, d), dtype=dtype, device=dev)
+        qa = (q.data_ptr(), _strides(q.stride()), qo.data_ptr(), _strides((T * H * d, d, H * d)), H)
+        qo = qo.transpose(1, 2)
+    if k is not None:
+        if k.stride(3) != 1 and d > 1:
+            k = k.contiguous()
+        H = k.shape[1]
+        ko = torch.empty((B, T, H, d), dtype=dtype, device=dev)
+        ka = (k.data_ptr(), _strides(k.stride()), ko.data_ptr(), _strides((T * H * d, d, H * d)), H)
+        ko = ko.transpose(1, 2)
+    ps = positions.stride()
     lib = _lib.load()
-    pb, pt = (0, positions.stride(0)) if positions.dim() == 1 else (0 if positions.shape[0] == 1 else positions.stride(0),
-                                                                      positions.stride(1))
-    with _lib.on(some.device):
-        rc = lib.lucid_rotary(*(a.data_ptr() if torch.is_tensor(a) else a for a in args), positions.data_ptr(),
-                              int(positions.dtype == torch.int64), pb, pt, inv_freq.data_ptr(),
-                              int(inv_freq.dtype == torch.float64), B, T, d, 2 * inv_freq.numel(), scale, int(interleaved),
-                              int(inverse), _ROTARY_DTYPES[some.dtype], _lib.stream_handle(some.device))
+    with _lib.on(dev):
+        rc = lib.lucid_rotary(*qa, *ka, positions.data_ptr(), positions.dtype is torch.int64,
+                              0 if len(ps) == 1 or positions.shape[0] == 1 else ps[0], ps[-1], inv_freq.data_ptr(),
+                              inv_freq.dtype is torch.float64, B, T, d, 2 * inv_freq.shape[0], scale, interleaved, inverse,
+                              _ROTARY_DTYPES[dtype], _lib.stream_handle(dev))
     _lib.check(lib, rc, "lucid_rotary")
-    return tuple(outs)
+    return qo, ko
 
 
 class RotaryFunction(torch.autograd.Function):
@@ -333,7 +356,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     if q.dtype not in _ROTARY_DTYPES or (k is not None and (k.dtype != q.dtype or k.device != dev)):
         raise TypeError(f"{what}: bf16 or fp32 queries and keys of one dtype on one GPU, got {q.dtype}"
                         + (f" / {k.dtype} on {k.device}" if k is not None else ""))
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or (k.shape[0], *k.shape[2:]) != (q.shape[0], *q.shape[2:]))):
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
         raise ValueError(f"{what}: q [B, Hq, T, d] and k [B, Hkv, T, d], got {tuple(q.shape)}"
                          + (f" and {tuple(k.shape)}" if k is not None else ""))
     B, _, T, d = q.shape
@@ -347,9 +370,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
                          f"{tuple(inv_freq.shape)} on {inv_freq.device}")
     if inv_freq.requires_grad:
         raise NotImplementedError(f"{what}: no gradient of the frequencies")
-    tracked = [x for x in (q, k) if x is not None]
-    if torch.is_grad_enabled() and any(x.requires_grad for x in tracked) \
-            or any(forward_ad.unpack_dual(x).tangent is not None for x in tracked):
+    if _tracked(q) or (k is not None and _tracked(k)):
         return RotaryFunction.apply(q, k, positions, inv_freq, bool(interleaved), float(scale))
     return _rotary(q, k, positions, inv_freq, bool(interleaved), float(scale), False)
 
@@ -560,30 +581,28 @@ class _Constraints(NamedTuple):
     allowed: torch.Tensor | None
 
 
-def _row_stride(t: torch.Tensor | None) -> int:
-    return 0 if t is None or t.shape[0] == 1 else t.stride(0)
+def _rows_at(t: torch.Tensor | None) -> tuple:
+    """(address, row stride) of the rows of a constraint; 0 for one row that all share, and no address for none."""
+    if t is None or t.shape[1] == 0:
+        return None, 0
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0
 
 
 def _number(x) -> tuple:
-    return (x.data_ptr(), 0.0) if torch.is_tensor(x) else (None, x)
-
-
-def _at(t: torch.Tensor | None):
-    return None if t is None or t.numel() == 0 else t.data_ptr()
+    return (x.data_ptr(), 1.0) if isinstance(x, torch.Tensor) else (None, x)
 
 
 def _constrain(logits: torch.Tensor, c: _Constraints) -> torch.Tensor:
     rows, T, sb, st = _logit_rows(logits)
     V, dev = logits.shape[-1], logits.device
     out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    rep, one = _number(c.repetition), 1.0
     lib = _lib.load()
     with _lib.on(dev):
         rc = lib.lucid_constrain_logits(
-            rows.data_ptr(), sb, st, out.numel() // V, T, V, _LP_DTYPES[logits.dtype], _at(c.history), _row_stride(c.history),
-            0 if c.history is None else c.history.shape[1], _at(c.prompt_lens), rep[0], rep[1] if rep[0] is None else one,
-            *_number(c.presence), *_number(c.frequency), _at(c.bias), _row_stride(c.bias), _at(c.allowed),
-            _row_stride(c.allowed), out.data_ptr(), _lib.stream_handle(dev))
+            rows.data_ptr(), sb, st, out.numel() // V, T, V, _LP_DTYPES[logits.dtype], *_rows_at(c.history),
+            0 if c.history is None else c.history.shape[1], None if c.prompt_lens is None else c.prompt_lens.data_ptr(),
+            *_number(c.repetition), *_number(c.presence), *_number(c.frequency), *_rows_at(c.bias), *_rows_at(c.allowed),
+            out.data_ptr(), _lib.stream_handle(dev))
     _lib.check(lib, rc, "lucid_constrain_logits")
     return out
 
@@ -592,7 +611,7 @@ class ConstrainLogitsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits: torch.Tensor, *constraints):
         c = _Constraints(*constraints)
-        number = not torch.is_tensor(c.repetition)
+        number = not isinstance(c.repetition, torch.Tensor)
         ctx.repetition = c.repetition if number else None
         ctx.save_for_backward(logits, c.history, None if number else c.repetition, c.allowed)
         return _constrain(logits, c)
@@ -608,9 +627,9 @@ class ConstrainLogitsFunction(torch.autograd.Function):
         lib = _lib.load()
         with _lib.on(dev):
             rc = lib.lucid_constrain_logits_bwd(
-                rows.data_ptr(), sb, st, dlogits.numel() // V, T, V, _LP_DTYPES[logits.dtype], _at(history),
-                _row_stride(history), 0 if history is None else history.shape[1], _at(repetition),
-                1.0 if ctx.repetition is None else ctx.repetition, _at(allowed), _row_stride(allowed), g.data_ptr(),
+                rows.data_ptr(), sb, st, dlogits.numel() // V, T, V, _LP_DTYPES[logits.dtype], *_rows_at(history),
+                0 if history is None else history.shape[1],
+                *_number(ctx.repetition if repetition is None else repetition), *_rows_at(allowed), g.data_ptr(),
                 dlogits.data_ptr(), _lib.stream_handle(dev))
         _lib.check(lib, rc, "lucid_constrain_logits_bwd")
         return (dlogits,) + (None,) * len(_Constraints._fields)
@@ -647,17 +666,18 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
         """t [..., last] as [R, last] with contiguous rows ([1, last] for one row that all share)."""
         if t is None:
             return None
-        if not torch.is_tensor(t) or t.dtype != dtype or t.device != dev:
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != dev:
             raise TypeError(f"{what}: {name} must be a {dtype} tensor on {dev}")
         if t.requires_grad:
             raise NotImplementedError(f"{what}: no gradient of {name}")
         if t.dim() < 1 or (last is not None and t.shape[-1] != last) or not (t.shape[:-1] == lead or (shared and t.dim() == 1)):
             raise ValueError(f"{what}: {name} {tuple(t.shape)} does not fit logits {tuple(logits.shape)}")
-        t = t.reshape(1 if t.shape[:-1] != lead else lead.numel(), t.shape[-1])
+        if t.dim() != 2:
+            t = t.reshape(1 if t.shape[:-1] != lead else lead.numel(), t.shape[-1])
         return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
     def number(name, x):
-        if not torch.is_tensor(x):
+        if not isinstance(x, torch.Tensor):
             return float(x)
         if x.dtype != torch.float32 or x.device != dev or x.shape != lead:
             raise ValueError(f"{what}: {name} must be a number or fp32 {tuple(lead)} on {dev}")
@@ -668,13 +688,13 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
     if prompt_lens is not None:
         if history is None:
             raise ValueError(f"{what}: prompt_lens without a history")
-        if not torch.is_tensor(prompt_lens) or prompt_lens.dtype != torch.int32 or prompt_lens.shape != lead \
+        if not isinstance(prompt_lens, torch.Tensor) or prompt_lens.dtype != torch.int32 or prompt_lens.shape != lead \
                 or prompt_lens.device != dev:
             raise ValueError(f"{what}: prompt_lens must be int32 {tuple(lead)} on {dev}")
         prompt_lens = prompt_lens.contiguous()
     c = _Constraints(rows("history", history, torch.int64, None, False), prompt_lens, number("repetition", repetition),
                      number("presence", presence), number("frequency", frequency), rows("bias", bias, torch.float32, V, True),
                      rows("allowed", allowed, torch.int32, -(-V // 32), True))
-    if logits.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(logits).tangent is not None:
+    if _tracked(logits):
         return ConstrainLogitsFunction.apply(logits, *c)
-    return _constrain(logits.detach(), c)
+    return _constrain(logits, c)
