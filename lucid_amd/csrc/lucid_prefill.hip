@@ -65,11 +65,20 @@ __device__ __forceinline__ bf16x8 ld8_cols(const bf16* row, int c, int d, bool v
   return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// Chunk c (8 columns) of row r of a tile of rows in LDS
+// A tile of rows in LDS, chunk c (8 columns) of row r at c ^ tile_key(r).  Two kinds of reads have to find distinct banks
+// among 64: 16 consecutive rows at one chunk (the rows of a first operand, 16 lanes of 16 bytes at a time) and 4 rows from a
+// multiple of 4 at 4 adjacent chunks (a transposing read, 32 lanes of 8 bytes).  Rows of 256 bytes: the row's number in 16
+// with its low and high half exchanged; rows of 128 bytes, two to a round of the banks: that of the pair in 8, its bits
+// reversed.  Rows of 160 and 192 bytes stay as they are (some pairs of reads meet).
+template <int W>
+__device__ __forceinline__ int tile_key(int r) {
+  if constexpr (W == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  if constexpr (W == 64) return ((r & 2) << 1) | ((r & 4) >> 1) | ((r & 8) >> 3);
+  return 0;
+}
 template <int W, typename T>
 __device__ __forceinline__ T* tile_at(T* tile, int r, int c) {
-  if constexpr (paged_swizzled(W)) return tile + r * W + ((c ^ (r & 7)) << 3);
-  return tile + r * W + c * 8;
+  return tile + r * W + ((c ^ tile_key<W>(r)) << 3);
 }
 
 // --------------------------------------------------------------------------------------------
@@ -272,48 +281,58 @@ struct SweepParts {
   float* l;  // [slots][RT]  running sum, attend
 };
 
-template <int W>
+template <int W, int KT>
 struct SweepSmem {
   union {
     // staged tiles, filled by direct global -> LDS loads (the transposing reads of W = 80 end 32 bytes behind a tile)
     struct {
-      bf16 k[2][kSweepKeys * W], v[2][kSweepKeys * W + 64];
+      bf16 k[2][KT * W], v[2][KT * W + 64];
     } st;
     struct {
       float o[2][64][W + 4], m[4][64], l[4][64];
     } fin;
   } u;
-  float nr[kSweepKeys];  // couple: 1 / rms of the tile's keys
+  float nr[2][KT];  // couple: 1 / rms of a tile's keys
 };
 
-// Lane part of the offset of paged_tr_a's first read at row0 = 0 of a tile; the second read is 8 rows on
+// The transposing reads of MFMA A operands (paged_tr_a) from such a tile: the lane's offsets at row 0 for column block
+// col0 and its rows of the first and of the second read, 8 on (their keys differ); row0, a multiple of 16, adds row0 W
+struct TileTr {
+  int o1, o2;
+};
 template <int W>
-__device__ __forceinline__ int tile_tr_off(int col0) {
+__device__ __forceinline__ TileTr tile_tr_off(int col0) {
   const int lane = threadIdx.x & 63, s = lane & 15;
   const int col = col0 + 16 * ((lane >> 4) & 1) + 4 * (s & 3), r1 = 4 * (lane >> 5) + (s >> 2);
-  if constexpr (paged_swizzled(W)) return r1 * W + ((((col >> 3) ^ (r1 & 7)) << 3) | (col & 7));
-  return r1 * W + col;
+  return TileTr{r1 * W + (((col >> 3) ^ tile_key<W>(r1)) << 3) + (col & 7),
+                (r1 + 8) * W + (((col >> 3) ^ tile_key<W>(r1 + 8)) << 3) + (col & 7)};
 }
 template <int W>
-__device__ __forceinline__ bf16x8 tile_tr(const bf16* tile, int off, int row0) {
+__device__ __forceinline__ bf16x8 tile_tr(const bf16* tile, const TileTr& o, int row0) {
   typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
-  const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + off + row0 * W));
-  const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + off + (row0 + 8) * W));
+  const bf16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + o.o1 + row0 * W));
+  const bf16x4 v2 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + o.o2 + row0 * W));
   return bf16x8{v1[0], v1[1], v1[2], v1[3], v2[0], v2[1], v2[2], v2[3]};
 }
 
-// Eight waves over tiles of 128 keys, staged once for all of them; KSP waves share 32 rows and take every KSP-th
-// 32 keys (RT = 256 / KSP rows).  Lane <-> row: S^T[j][i] = K_j . x_i, then acc^T[col][i] += w^T[col][j] p^T[j][i].
+// Waves of a SIMD: as many as the registers of the instances leave place for
+constexpr int sweep_waves(int W, int NW) { return NW == 8 ? 2 : W == 64 ? 4 : W == 128 ? 2 : 3; }
+
+// NW waves over tiles of 16 NW keys, staged once for all of them; a wave holds NT tiles of 32 rows, KSP waves share them and
+// take every KSP-th 32 keys (RT = 32 NT NW / KSP rows).  Lane <-> row: S^T[j][i] = K_j . x_i, then acc^T[col][i] +=
+// w^T[col][j] p^T[j][i].
 //   attend: x = q, rows (token, query head of the group) token by token, online softmax
 //   couple: x = the new keys, p = P as a bf16 pair; y = v - acc.  panel >= 0: not the cached keys but those of that
 //           panel of new rows, out of the y of the rows behind it.  Grid (row tiles, Hkv, B) then, else by SweepPlan.
-template <int W, bool ATTEND, int KSP>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void lucid_prefill_sweep_kernel(
+template <int W, bool ATTEND, int KSP, int NW, int NT>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_waves(W, NW)))) void lucid_prefill_sweep_kernel(
     const bf16* __restrict__ x, Strides xs, int vec, const bf16* __restrict__ v, Strides vs, PagedPool kp, PagedPool vp,
     PrefillBatch seq, SweepGrid grid, int panel, PagedScale f, float eps, int d, float* __restrict__ y, int64_t yrows,
     bf16* __restrict__ o, Strides os, int ovec, SweepParts part) {
-  constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = CPR / 2, NMT = 4 / KSP, RT = 256 / KSP;
-  __shared__ __attribute__((aligned(16))) SweepSmem<W> sm;
+  constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = CPR / 2, KT = 16 * NW, NMT = KT / 32 / KSP;
+  constexpr int RT = 32 * NT * NW / KSP;
+  static_assert(KSP == 1 || (NT == 1 && RT == 64), "the join of key groups holds 64 rows");
+  __shared__ __attribute__((aligned(16))) SweepSmem<W, KT> sm;
   SweepItem it;
   int row_base = 0;
   if (!ATTEND && panel >= 0) {
@@ -339,34 +358,72 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void l
   const int b = it.b, h = it.h, n = it.n, GX = grid.GX;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
   const int rw = w / KSP, kg = w % KSP;
-  const int rows = it.c * GX, row0 = row_base + it.tile * RT + 32 * rw;  // of this wave
+  const int rows = it.c * GX, row0 = row_base + it.tile * RT + 32 * NT * rw;  // of this wave
   const bool active = row0 < rows;
-  const int row = row0 + l32, rr = min(row, rows - 1), t = rr / GX, hq = h * GX + (rr - t * GX);
+  int row[NT], t[NT], hq[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    row[u] = row0 + 32 * u + l32;
+    const int r = min(row[u], rows - 1);
+    t[u] = r / GX;
+    hq[u] = h * GX + (r - t[u] * GX);
+  }
   // attend: no row of this workgroup sees a key beyond its last token's
   const int last = min(row_base + (it.tile + 1) * RT, rows) - 1;
   const int j0 = it.j0, j1 = ATTEND ? min(it.j1, n + last / GX + 1) : it.j1;
-  const int lim = ATTEND ? min(j1 - 1, n + t) : j1 - 1;                         // the lane's last key,
-  const int free = ATTEND ? min(j1 - 1, n + min(row0, rows - 1) / GX) : j1 - 1;  // and one that all lanes of the wave see
-  const int most = ATTEND ? n + min(row0 + 31, rows - 1) / GX : j1 - 1;          // and beyond it none does
-  const int ntile = (j1 - j0 + kSweepKeys - 1) / kSweepKeys;
+  int lim[NT];  // the lane's last key,
+#pragma unroll
+  for (int u = 0; u < NT; ++u) lim[u] = ATTEND ? min(j1 - 1, n + t[u]) : j1 - 1;
+  const int free = ATTEND ? min(j1 - 1, n + min(row0, rows - 1) / GX) : j1 - 1;      // one that all lanes of the wave see,
+  const int most = ATTEND ? n + min(row0 + 32 * NT - 1, rows - 1) / GX : j1 - 1;  // and one beyond which none does
+  const int ntile = (j1 - j0 + KT - 1) / KT;
 
-  // staging: waves 0-3 the keys, 4-7 V', 32 rows each
+  // staging: half of the waves the keys, the others V', 32 rows each
   const int32_t* tbl = seq.table + b * seq.tstride;
-  const int quarter = w & 3;
-  const bool isv = w >= 4;
+  const int part_of = w % (NW / 2);
+  const bool isv = w >= NW / 2;
   const PagedPool pool = isv ? vp : kp;
-  auto key_of = [&](int tile) { return min(j0 + kSweepKeys * tile + 32 * quarter + l32, j1 - 1); };
-  auto page_id = [&](int tile) { return tbl[prefill_page(seq, key_of(tile))]; };
+  auto key_of = [&](int tile) { return min(j0 + KT * tile + 32 * part_of + l32, j1 - 1); };
+  // Pages of whole runs of 32 rows: a wave's rows of a tile lie in one page, whose place is scalar work, and the lanes' offsets
+  // in it are those of every tile.  The last tile, whose rows may end before it does, goes row by row in any case.
+  const bool runs = seq.page % 32 == 0 && j0 % 32 == 0 && pool.row < (1u << 22);
+  unsigned lane_off[NST];
+#pragma unroll
+  for (int i = 0; i < NST; ++i) {
+    const int q = i * 64 + lane, r = q / CPR;
+    lane_off[i] = 16 * (r * pool.row + ((q % CPR) ^ tile_key<W>(r)));
+  }
+  auto whole = [&](int tile) { return runs && j0 + KT * (tile + 1) <= j1; };
+  auto page_id = [&](int tile) {
+    const int j = whole(tile) ? j0 + KT * tile + 32 * part_of : key_of(tile);
+    return tbl[prefill_page(seq, j)];
+  };
   auto stage = [&](int tile, int id, int buf) {
+    bf16* dst = (isv ? sm.u.st.v[buf] : sm.u.st.k[buf]) + 32 * part_of * W;
+    if (whole(tile)) {
+      const char* base = reinterpret_cast<const char*>(
+          paged_at(pool, prefill_row(seq, pool, __builtin_amdgcn_readfirstlane(id), j0 + KT * tile + 32 * part_of, h)));
+#pragma unroll
+      for (int i = 0; i < NST; ++i)
+        __builtin_amdgcn_global_load_lds(reinterpret_cast<const bf16*>(base + lane_off[i]), dst + i * 512, 16, 0, 0);
+      return;
+    }
     const unsigned off = prefill_row(seq, pool, id, key_of(tile), h);
-    bf16* dst = (isv ? sm.u.st.v[buf] : sm.u.st.k[buf]) + 32 * quarter * W;
 #pragma unroll
     for (int i = 0; i < NST; ++i) {
-      const int q = i * 64 + lane, r = q / CPR;
-      int c = q % CPR;
-      if constexpr (paged_swizzled(W)) c ^= r & 7;
+      const int q = i * 64 + lane, r = q / CPR, c = (q % CPR) ^ tile_key<W>(r);
       __builtin_amdgcn_global_load_lds(paged_at(pool, __shfl((int)off, r, 64)) + c * 8, dst + i * 512, 16, 0, 0);
     }
+  };
+  // couple: once a wave's own keys have landed it works out their norms, two lanes a key
+  auto norms = [&](int buf) {
+    if (ATTEND || isv) return;
+    const int r = 32 * part_of + (lane >> 1);
+    float nn = 0.f;
+#pragma unroll
+    for (int cc = 0; cc < CPR; cc += 2) nn = dot8(ld8(tile_at<W>(sm.u.st.k[buf], r, cc + (lane & 1))), nn);
+    nn += dpp_f32<kDppXor1>(nn);
+    if ((lane & 1) == 0) sm.nr[buf][r] = rsqrtf(nn / (float)d + eps);
   };
   int idn = 0;
   if (ntile > 0) {
@@ -375,150 +432,185 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void l
     stage(0, id0, 0);
   }
   const float c = f.sl2;
-  bf16x8 xb[NKS];
-  {
-    const bf16* xr = x + b * xs.b + (ATTEND ? hq : h) * xs.h + t * xs.t;
+  bf16x8 xb[NT][NKS];
+  float c1[NT], m[NT], lsum[NT];
+  f32x16 acc[NT][NDT];
 #pragma unroll
-    for (int st = 0; st < NKS; ++st) xb[st] = ld8_cols(xr, 16 * st + 8 * g, d, vec);
+  for (int u = 0; u < NT; ++u) {
+    const bf16* xr = x + b * xs.b + (ATTEND ? hq[u] : h) * xs.h + t[u] * xs.t;
+#pragma unroll
+    for (int st = 0; st < NKS; ++st) xb[u][st] = ld8_cols(xr, 16 * st + 8 * g, d, vec);
+#pragma unroll
+    for (int q = 0; q < NDT; ++q) acc[u][q] = zero16();
+    m[u] = PREFILL_NEG;
+    lsum[u] = 0.f;
+    c1[u] = 0.f;
   }
-  float c1 = 0.f;
   if constexpr (!ATTEND) {
-    float nt = 0.f;
 #pragma unroll
-    for (int st = 0; st < NKS; ++st)
+    for (int u = 0; u < NT; ++u) {
+      float nt = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) nt = fmaf((float)xb[st][e], (float)xb[st][e], nt);
-    c1 = c * rsqrtf(wave_sum32(nt) / (float)d + eps);
+      for (int st = 0; st < NKS; ++st) nt = dot8(xb[u][st], nt);
+      c1[u] = c * rsqrtf(wave_sum32(nt) / (float)d + eps);
+    }
   }
-  f32x16 acc[NDT];
-#pragma unroll
-  for (int q = 0; q < NDT; ++q) acc[q] = zero16();
-  float m = PREFILL_NEG, lsum = 0.f;
-  int tr[NDT];
+  TileTr tr[NDT];
 #pragma unroll
   for (int q = 0; q < NDT; ++q) tr[q] = tile_tr_off<W>(32 * q);
   // the rows have landed before the loop (else every tile's first product waits for the next tile's loads)
 #pragma unroll
-  for (int st = 0; st < NKS; ++st) asm volatile("" ::"v"(xb[st]));
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int st = 0; st < NKS; ++st) asm volatile("" ::"v"(xb[u][st]));
   dma_wait();
+  if (ntile > 0) norms(0);
   __syncthreads();
   for (int jt = 0; jt < ntile; ++jt) {
-    const int buf = jt & 1, jb = j0 + kSweepKeys * jt;
+    const int buf = jt & 1, jb = j0 + KT * jt;
     if (jt + 1 < ntile) {
       stage(jt + 1, idn, buf ^ 1);
       if (jt + 2 < ntile) idn = page_id(jt + 2);
     }
-    const bf16* tk = sm.u.st.k[buf];
-    const bf16* tv = sm.u.st.v[buf];
-    const bool work = active && jb <= most, mask = jb + kSweepKeys - 1 > free;
-    if constexpr (!ATTEND) {  // four lanes a key
-      const int r = tid >> 2;
-      float nn = 0.f;
-#pragma unroll
-      for (int cc = 0; cc < CPR; cc += 4)
-        if (CPR % 4 == 0 || cc + (tid & 3) < CPR) nn = dot8(ld8(tile_at<W>(tk, r, cc + (tid & 3))), nn);
-      nn = lanes_sum<4>(nn);
-      if ((tid & 3) == 0) sm.nr[r] = rsqrtf(nn / (float)d + eps);
-    }
-    f32x16 s[NMT];
-    if (work) {
-#pragma unroll
-      for (int i = 0; i < NMT; ++i) {
-        const int mt = kg + KSP * i;
-        s[i] = zero16();
-#pragma unroll
-        for (int st = 0; st < NKS; ++st) s[i] = mfma32(ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g)), xb[st], s[i]);
-      }
-    }
-    if constexpr (!ATTEND) __syncthreads();
-    if (work) {
+    if (active && jb <= most) {
+      const bf16* tk = sm.u.st.k[buf];
+      const bf16* tv = sm.u.st.v[buf];
+      const bool mask = jb + KT - 1 > free;
       if constexpr (ATTEND) {
-        if (mask) {
-#pragma unroll
-          for (int i = 0; i < NMT; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (jb + (kg + KSP * i) * 32 + drow(e, g) > lim) s[i][e] = -INFINITY;
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NMT; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[i][e]);
-        mx = wave_max32(mx) * c;
-        if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {  // rescale only where a row grows by 2^8
-          const float mnew = fmaxf(m, mx);
-          const float alpha = __builtin_amdgcn_exp2f(m - mnew);
-          m = mnew;
-          lsum *= alpha;
-#pragma unroll
-          for (int q = 0; q < NDT; ++q)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[q][e] *= alpha;
-        }
+        f32x16 s[NMT][NT];
 #pragma unroll
         for (int i = 0; i < NMT; ++i) {
           const int mt = kg + KSP * i;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], c, -m));
-          const bf16x8 p0 = pack_b(s[i], 0), p1 = pack_b(s[i], 1);
-          lsum = add_sum8(p1, add_sum8(p0, lsum));  // sum of the bf16 P of the product
+          for (int u = 0; u < NT; ++u) s[i][u] = zero16();
+#pragma unroll
+          for (int st = 0; st < NKS; ++st) {
+            const bf16x8 kf = ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g));
+#pragma unroll
+            for (int u = 0; u < NT; ++u) s[i][u] = mfma32(kf, xb[u][st], s[i][u]);
+          }
+        }
+        if (mask) {
+#pragma unroll
+          for (int i = 0; i < NMT; ++i)
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (jb + (kg + KSP * i) * 32 + drow(e, g) > lim[u]) s[i][u][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < NMT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[i][u][e]);
+          mx = wave_max32(mx) * c;
+          if (__builtin_amdgcn_ballot_w64(mx > m[u] + 8.0f)) {  // rescale only where a row grows by 2^8
+            const float mnew = fmaxf(m[u], mx);
+            const float alpha = __builtin_amdgcn_exp2f(m[u] - mnew);
+            m[u] = mnew;
+            lsum[u] *= alpha;
+#pragma unroll
+            for (int q = 0; q < NDT; ++q)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[u][q][e] *= alpha;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NMT; ++i) {
+          const int mt = kg + KSP * i;
+          bf16x8 p0[NT], p1[NT];
+#pragma unroll
+          for (int u = 0; u < NT; ++u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[i][u][e] = __builtin_amdgcn_exp2f(fmaf(s[i][u][e], c, -m[u]));
+            p0[u] = pack_b(s[i][u], 0);
+            p1[u] = pack_b(s[i][u], 1);
+            lsum[u] = add_sum8(p1[u], add_sum8(p0[u], lsum[u]));  // sum of the bf16 P of the product
+          }
 #pragma unroll
           for (int q = 0; q < NDT; ++q) {
-            acc[q] = mfma32(tile_tr<W>(tv, tr[q], mt * 32), p0, acc[q]);
-            acc[q] = mfma32(tile_tr<W>(tv, tr[q], mt * 32 + 16), p1, acc[q]);
+            const bf16x8 a0 = tile_tr<W>(tv, tr[q], mt * 32), a1 = tile_tr<W>(tv, tr[q], mt * 32 + 16);
+#pragma unroll
+            for (int u = 0; u < NT; ++u) acc[u][q] = mfma32(a0, p0[u], acc[u][q]);
+#pragma unroll
+            for (int u = 0; u < NT; ++u) acc[u][q] = mfma32(a1, p1[u], acc[u][q]);
           }
         }
       } else {
 #pragma unroll
         for (int i = 0; i < NMT; ++i) {
           const int mt = kg + KSP * i;
+          f32x16 s[NT];
+#pragma unroll
+          for (int u = 0; u < NT; ++u) s[u] = zero16();
+#pragma unroll
+          for (int st = 0; st < NKS; ++st) {
+            const bf16x8 kf = ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g));
+#pragma unroll
+            for (int u = 0; u < NT; ++u) s[u] = mfma32(kf, xb[u][st], s[u]);
+          }
           float nr[16];
-          lds_rows16(&sm.nr[32 * mt], g, nr);
+          lds_rows16(&sm.nr[buf][32 * mt], g, nr);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[i][e] = __builtin_amdgcn_exp2f(fmaf(c1 * nr[e], s[i][e], -f.c0));
-          if (mask) {
+          for (int u = 0; u < NT; ++u) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (jb + mt * 32 + drow(e, g) > lim) s[i][e] = 0.f;
+            for (int e = 0; e < 16; ++e) s[u][e] = __builtin_amdgcn_exp2f(fmaf(c1[u] * nr[e], s[u][e], -f.c0));
+            if (mask) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (jb + mt * 32 + drow(e, g) > lim[u]) s[u][e] = 0.f;
+            }
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const bf16x8 hi = pack_b(s[i], k), lo = pack_lo(s[i], k, hi);
+            bf16x8 hi[NT], lo[NT];
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+              hi[u] = pack_b(s[u], k);
+              lo[u] = pack_lo(s[u], k, hi[u]);
+            }
 #pragma unroll
             for (int q = 0; q < NDT; ++q) {
               const bf16x8 a = tile_tr<W>(tv, tr[q], mt * 32 + 16 * k);
-              acc[q] = mfma32(a, hi, acc[q]);
-              acc[q] = mfma32(a, lo, acc[q]);
+#pragma unroll
+              for (int u = 0; u < NT; ++u) acc[u][q] = mfma32(a, hi[u], acc[u][q]);
+#pragma unroll
+              for (int u = 0; u < NT; ++u) acc[u][q] = mfma32(a, lo[u], acc[u][q]);
             }
           }
         }
       }
     }
     dma_wait();
+    if (jt + 1 < ntile) norms(buf ^ 1);
     __syncthreads();
   }
-  float l = ATTEND ? wave_sum32(lsum) : 0.f;
+  float l[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) l[u] = ATTEND ? wave_sum32(lsum[u]) : 0.f;
   if constexpr (KSP > 1) {  // the key groups' sums joined in the waves of group 0
     const int r = 32 * rw + l32;
     if constexpr (ATTEND) {
       if (g == 0) {
-        sm.u.fin.m[kg][r] = m;
-        sm.u.fin.l[kg][r] = l;
+        sm.u.fin.m[kg][r] = m[0];
+        sm.u.fin.l[kg][r] = l[0];
       }
       __syncthreads();
       float M = sm.u.fin.m[0][r];
 #pragma unroll
       for (int k = 1; k < KSP; ++k) M = fmaxf(M, sm.u.fin.m[k][r]);
-      l = 0.f;
+      l[0] = 0.f;
 #pragma unroll
-      for (int k = 0; k < KSP; ++k) l = fmaf(sm.u.fin.l[k][r], __builtin_amdgcn_exp2f(sm.u.fin.m[k][r] - M), l);
-      const float a = __builtin_amdgcn_exp2f(m - M);
-      m = M;
+      for (int k = 0; k < KSP; ++k) l[0] = fmaf(sm.u.fin.l[k][r], __builtin_amdgcn_exp2f(sm.u.fin.m[k][r] - M), l[0]);
+      const float a = __builtin_amdgcn_exp2f(m[0] - M);
+      m[0] = M;
 #pragma unroll
       for (int q = 0; q < NDT; ++q)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[q][e] *= a;
+        for (int e = 0; e < 16; ++e) acc[0][q][e] *= a;
     }
 #pragma unroll
     for (int half = KSP / 2; half >= 1; half /= 2) {
@@ -530,7 +622,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void l
           for (int e = 0; e < 16; e += 4)
             if (32 * q + drow(e, 0) < W)
               *reinterpret_cast<f32x4*>(&sm.u.fin.o[kg - half][r][32 * q + drow(e, g)]) =
-                  f32x4{acc[q][e], acc[q][e + 1], acc[q][e + 2], acc[q][e + 3]};
+                  f32x4{acc[0][q][e], acc[0][q][e + 1], acc[0][q][e + 2], acc[0][q][e + 3]};
       }
       __syncthreads();
       if (kg < half) {
@@ -541,67 +633,68 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void l
             if (32 * q + drow(e, 0) < W) {
               const f32x4 z = *reinterpret_cast<const f32x4*>(&sm.u.fin.o[kg][r][32 * q + drow(e, g)]);
 #pragma unroll
-              for (int u = 0; u < 4; ++u) acc[q][e + u] += z[u];
+              for (int u = 0; u < 4; ++u) acc[0][q][e + u] += z[u];
             }
       }
     }
     if (kg != 0) return;
   }
-  if (row >= rows) return;
-  if (it.slot >= 0) {
-    const int64_t at = (int64_t)it.slot * RT + 32 * rw + l32;
 #pragma unroll
-    for (int q = 0; q < NDT; ++q)
+  for (int r = 0; r < NT; ++r) {
+    if (row[r] >= rows) continue;
+    if (it.slot >= 0) {
+      const int64_t at = (int64_t)it.slot * RT + 32 * (NT * rw + r) + l32;
 #pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        if (32 * q + drow(e, 0) < W)
-          *reinterpret_cast<f32x4*>(part.o + at * W + 32 * q + drow(e, g)) =
-              f32x4{acc[q][e], acc[q][e + 1], acc[q][e + 2], acc[q][e + 3]};
-    if (ATTEND && g == 0) {
-      part.m[at] = m;
-      part.l[at] = l;
+      for (int q = 0; q < NDT; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          if (32 * q + drow(e, 0) < W)
+            *reinterpret_cast<f32x4*>(part.o + at * W + 32 * q + drow(e, g)) =
+                f32x4{acc[r][q][e], acc[r][q][e + 1], acc[r][q][e + 2], acc[r][q][e + 3]};
+      if (ATTEND && g == 0) {
+        part.m[at] = m[r];
+        part.l[at] = l[r];
+      }
+    } else if constexpr (ATTEND) {
+      const float inv = 1.f / l[r];
+      bf16* op = o + b * os.b + hq[r] * os.h + t[r] * os.t;
+#pragma unroll
+      for (int q = 0; q < NDT; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int col = 32 * q + drow(e, g);
+          bf16x4 z;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) z[u] = (bf16)(acc[r][q][e + u] * inv);
+          if (ovec && col + 4 <= d) {
+            *reinterpret_cast<bf16x4*>(op + col) = z;
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (col + u < d) op[col + u] = z[u];
+          }
+        }
+    } else {
+      float* yp = y + (((int64_t)b * seq.Hkv + h) * yrows + t[r]) * W;
+      const bf16* vr = v + b * vs.b + h * vs.h + t[r] * vs.t;
+#pragma unroll
+      for (int q = 0; q < NDT; ++q)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int col = 32 * q + drow(e, g);
+          if (32 * q + drow(e, 0) >= W) continue;
+          f32x4 z;
+          if (panel >= 0) {
+            z = *reinterpret_cast<const f32x4*>(yp + col);
+          } else {
+            const bf16x4 v4 = ld4_cols(vr, col, d, ovec);
+            z = f32x4{(float)v4[0], (float)v4[1], (float)v4[2], (float)v4[3]};
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) z[u] -= acc[r][q][e + u];
+          *reinterpret_cast<f32x4*>(yp + col) = z;
+        }
     }
-    return;
-  }
-  if constexpr (ATTEND) {
-    const float inv = 1.f / l;
-    bf16* op = o + b * os.b + hq * os.h + t * os.t;
-#pragma unroll
-    for (int q = 0; q < NDT; ++q)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int col = 32 * q + drow(e, g);
-        bf16x4 z;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) z[u] = (bf16)(acc[q][e + u] * inv);
-        if (ovec && col + 4 <= d) {
-          *reinterpret_cast<bf16x4*>(op + col) = z;
-        } else {
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (col + u < d) op[col + u] = z[u];
-        }
-      }
-  } else {
-    float* yp = y + (((int64_t)b * seq.Hkv + h) * yrows + t) * W;
-    const bf16* vr = v + b * vs.b + h * vs.h + t * vs.t;
-#pragma unroll
-    for (int q = 0; q < NDT; ++q)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int col = 32 * q + drow(e, g);
-        if (32 * q + drow(e, 0) >= W) continue;
-        f32x4 z;
-        if (panel >= 0) {
-          z = *reinterpret_cast<const f32x4*>(yp + col);
-        } else {
-          const bf16x4 r = ld4_cols(vr, col, d, false);
-          z = f32x4{(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) z[u] -= acc[q][e + u];
-        *reinterpret_cast<f32x4*>(yp + col) = z;
-      }
   }
 }
 

@@ -14,8 +14,8 @@ namespace {
 // Results of so many bytes pass the 256 MB cache by
 constexpr int64_t kPastBytes = 100000000;
 
-// Items that a sweep aims at: one or two rounds of the chip
-constexpr int kPrefillTarget = 512;
+// Slots of 128 rows for the parts of a sweep
+constexpr int kPrefillSlots = 1024;
 
 struct PrefillWs {
   int2* info;       // [B]
@@ -26,7 +26,10 @@ struct PrefillWs {
 };
 
 // Rows of a workgroup of a sweep: 64 with four waves to 32 rows where there are few
-int sweep_rows(int64_t rows) { return rows <= 128 ? 64 : 256; }
+int sweep_rows(int64_t rows, bool attend, int W) { return rows <= 128 ? 64 : attend && W <= 96 ? 128 : 256; }
+
+// Items that it aims at: one round of the chip
+int sweep_target(int RT, int W, bool attend) { return RT == 128 ? (W == 64 ? 1024 : 768) : 256; }
 
 PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
   const size_t panels = ((size_t)L + lucid::kPanel - 1) / lucid::kPanel;
@@ -41,7 +44,7 @@ PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
   w.info = reinterpret_cast<int2*>(take((size_t)B * 8));
   w.pmat = take((size_t)B * Hkv * panels * lucid::kPanelBytes);
   w.y = reinterpret_cast<float*>(take((size_t)B * Hkv * panels * lucid::kPanel * W * 4));
-  const size_t rows = (size_t)kPrefillTarget * 256;
+  const size_t rows = (size_t)kPrefillSlots * 128;
   w.part.o = reinterpret_cast<float*>(take(rows * W * 4));
   w.part.m = reinterpret_cast<float*>(take(rows * 4));
   w.part.l = reinterpret_cast<float*>(take(rows * 4));
@@ -73,8 +76,8 @@ int prefill_sweep(const PrefillCall& c, int panel) {
   const int G = c.Hq / c.seq.Hkv, GX = ATTEND ? G : 1;
   const int panels = (c.seq.L + lucid::kPanel - 1) / lucid::kPanel;
   const int64_t rows = (int64_t)c.seq.L * GX, yrows = (int64_t)panels * lucid::kPanel;
-  const int RT = panel >= 0 ? 64 : sweep_rows(rows);
-  const lucid::SweepGrid grid{GX, RT, ATTEND, kPrefillTarget};
+  const int RT = panel >= 0 ? 64 : sweep_rows(rows, ATTEND, W);
+  const lucid::SweepGrid grid{GX, RT, ATTEND, sweep_target(RT, W, ATTEND)};
   const bf16* x = ATTEND ? c.q : c.k;
   const int64_t* xs = ATTEND ? c.qs : c.ks;
   const int vec = rows_of_4(x, xs, 2), vvec = rows_of_4(c.v, c.vs, 2);
@@ -83,20 +86,22 @@ int prefill_sweep(const PrefillCall& c, int panel) {
   if (panel >= 0) {
     blocks = dim3((unsigned)((c.seq.L - lucid::kPanel * (panel + 1) + RT - 1) / RT), c.seq.Hkv, c.seq.B);
   } else {
-    const int64_t most = (int64_t)c.seq.B * c.seq.Hkv * ((rows + RT - 1) / RT) + kPrefillTarget;
+    const int64_t most = (int64_t)c.seq.B * c.seq.Hkv * ((rows + RT - 1) / RT) + grid.target;
     blocks = dim3((unsigned)((most + 7) / 8 * 8));
   }
-  auto go = [&](auto kernel) -> int {
-    LUCID_LAUNCH_B(ATTEND ? "lucid_prefill_attend_kernel" : "lucid_prefill_couple_kernel", kernel, blocks, dim3(512), c.st, x,
+  auto go = [&](auto kernel, int threads) -> int {
+    LUCID_LAUNCH_B(ATTEND ? "lucid_prefill_attend_kernel" : "lucid_prefill_couple_kernel", kernel, blocks, dim3(threads), c.st, x,
                    S(xs), vec, c.v, S(c.vs), c.kp, c.vp, c.seq, grid, panel, c.scale, c.eps, c.D, c.ws.y, yrows, c.o, S(c.os),
                    ovec, c.ws.part);
     return LUCID_OK;
   };
-  const int rc = RT == 64 ? go(lucid::lucid_prefill_sweep_kernel<W, ATTEND, 4>) : go(lucid::lucid_prefill_sweep_kernel<W, ATTEND, 1>);
+  constexpr int NW = ATTEND && W <= 96 ? 4 : 8;
+  const int rc = RT == 64 ? go(lucid::lucid_prefill_sweep_kernel<W, ATTEND, 4, 8, 1>, 512)
+                          : go(lucid::lucid_prefill_sweep_kernel<W, ATTEND, 1, NW, 1>, 64 * NW);
   if (rc || panel >= 0) return rc;
   // (rows of fewer tiles than two least parts are never cut)
   if ((int64_t)c.seq.M * c.seq.page <= (2 * lucid::kSweepLeast - 1) * lucid::kSweepKeys) return LUCID_OK;
-  LUCID_LAUNCH("lucid_prefill_join_kernel", (lucid::lucid_prefill_join_kernel<W, ATTEND>), dim3(kPrefillTarget / 2, RT / 16), c.st,
+  LUCID_LAUNCH("lucid_prefill_join_kernel", (lucid::lucid_prefill_join_kernel<W, ATTEND>), dim3(grid.target / 2, RT / 16), c.st,
                c.v, S(c.vs), vvec, c.seq, grid, c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
   return LUCID_OK;
 }
