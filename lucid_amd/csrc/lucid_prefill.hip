@@ -198,87 +198,115 @@ __global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __r
 }
 
 // --------------------------------------------------------------------------------------------
-// How a sweep is cut into workgroups, worked out by every wave from the sequences' lengths: tiles of RT of a
-// sequence's rows (GX for each token), for each kv head; and, where there are fewer than `target` of
-// them, cuts along the keys in proportion to their number, so that all items together are at most target + the
-// uncut ones.  A cut item leaves its part in a slot.
+// How a sweep is shared out, worked out by every wave from the sequences' lengths.  All row tiles (RT of a sequence's
+// rows, GX for each token) of all kv heads and sequences stand in one line, each as long as its keys' staged tiles, and
+// every workgroup takes an equal share of it: whole row tiles, and at either end part of one, along the keys.  A part
+// goes to slot 2 s of share s if it holds the share's beginning, else to 2 s + 1.  (Whole row tiles cut into equal parts
+// instead left a last round half empty: 4 sequences of 300 to 512 tokens of 32/4 heads of 64 columns behind 8192 rows, 181 us.)
+// Places without keys lead every row tile: what beginning and ending one costs.  A share's end at the beginning of a row
+// tile, or anywhere in a short one, goes back to where it starts.
 // --------------------------------------------------------------------------------------------
 struct SweepGrid {
-  int GX, RT, attend, target;
+  int GX, RT, attend, target;  // target: shares at most
+  int whole;                   // staged tiles of a row tile that is not cut at all
 };
-struct SweepItem {
+struct SweepPiece {
   int b, h, n, c, tile, j0, j1;
-  int slot, splits, tiles;  // slot -1: not cut
+  int slot;   // -1: a whole row tile
+  int place;  // the row tile's first (its keys follow kSweepLead behind)
+  int len;    // its staged tiles
 };
-constexpr int kSweepLeast = 4;  // staged tiles of an item that is cut off
+constexpr int kSweepLeast = 4;  // places of a share, at least
+constexpr int kSweepLead = 4;   // places before a row tile's keys
+constexpr int kSweepSnap = 2;   // staged tiles at a row tile's beginning that are not cut off
 
 struct SweepPlan {
-  const PrefillBatch& s;
-  const SweepGrid& a;
-  int64_t total;  // staged tiles of all row tiles
+  PrefillBatch s;
+  SweepGrid a;
+  int total, per;  // places of the line and of a share (their number fits: the host's check)
+  int2 x0;         // sequence `lane` of the first 64
   __device__ __forceinline__ int tiles(const int2& x) const { return (x.y * a.GX + a.RT - 1) / a.RT; }
   __device__ __forceinline__ int keys(const int2& x) const { return x.x + (a.attend ? x.y : 0); }
-  __device__ __forceinline__ int2 at(int b) const { return b < s.B ? s.info[b] : make_int2(0, 0); }
-  __device__ __forceinline__ int splits(const int2& x) const {
-    const int len = (keys(x) + kSweepKeys - 1) / kSweepKeys;
-    return max(1, min(len / kSweepLeast, (int)((int64_t)len * a.target / max(total, (int64_t)1))));
-  }
+  __device__ __forceinline__ int len(const int2& x) const { return max(1, (keys(x) + kSweepKeys - 1) / kSweepKeys); }
+  __device__ __forceinline__ int2 at(int b) const { return b < 64 ? x0 : b < s.B ? s.info[b] : make_int2(0, 0); }
+  __device__ __forceinline__ SweepPlan() {}
   __device__ __forceinline__ SweepPlan(const PrefillBatch& seq, const SweepGrid& grid) : s(seq), a(grid), total(0) {
-    for (int b0 = 0; b0 < s.B; b0 += 64) {
-      const int2 x = at(b0 + (threadIdx.x & 63));
-      total += (int64_t)s.Hkv * tiles(x) * ((keys(x) + kSweepKeys - 1) / kSweepKeys);
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o, 64);
-  }
-  // Item number `id`; cut: among the row tiles of the sequences that are cut, of which j0 and j1 say nothing
-  __device__ __forceinline__ bool find(int id, bool cut, SweepItem& it) const {
     const int lane = threadIdx.x & 63;
-    int base = 0, slots = 0;
+    x0 = lane < s.B ? s.info[lane] : make_int2(0, 0);
     for (int b0 = 0; b0 < s.B; b0 += 64) {
       const int2 x = at(b0 + lane);
-      const int tl = tiles(x), sp = splits(x);
-      const int own = sp > 1 ? s.Hkv * tl * sp : 0;  // slots
-      const int num = cut ? (sp > 1 ? s.Hkv * tl : 0) : s.Hkv * tl * sp;
-      const int end = base + wave_scan(num), send = slots + wave_scan(own);
-      const unsigned long long hit = __ballot(id < end);
+      total += __builtin_amdgcn_readlane(wave_scan(s.Hkv * tiles(x) * (len(x) + kSweepLead)), 63);
+    }
+    per = max(kSweepLeast, (total + a.target - 1) / a.target);
+  }
+  // The row tile at a place (below total)
+  __device__ __forceinline__ void find(int place, SweepPiece& it) const {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int b0 = 0; b0 < s.B; b0 += 64) {
+      const int2 x = at(b0 + lane);
+      const int tl = tiles(x), ln = len(x), end = base + wave_scan(s.Hkv * tl * (ln + kSweepLead));
+      const unsigned long long hit = __ballot(place < end);
       if (hit) {
         const int l = __builtin_amdgcn_readfirstlane(__ffsll(hit) - 1);
         it.b = b0 + l;
         it.n = __builtin_amdgcn_readlane(x.x, l);
         it.c = __builtin_amdgcn_readlane(x.y, l);
-        it.tiles = __builtin_amdgcn_readlane(tl, l);
-        it.splits = __builtin_amdgcn_readlane(sp, l);
-        int k = id - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(num, l));
-        const int first = __builtin_amdgcn_readlane(send, l) - __builtin_amdgcn_readlane(own, l);
-        if (cut) {
-          it.tile = k % it.tiles;
-          it.h = k / it.tiles;
-          it.slot = first + it.h * it.splits * it.tiles + it.tile;
-          return true;
-        }
-        it.slot = it.splits > 1 ? first + k : -1;
-        it.tile = k % it.tiles;
-        k /= it.tiles;
-        const int part = k % it.splits;
-        it.h = k / it.splits;
-        const int len = keys(make_int2(it.n, it.c)), all = (len + kSweepKeys - 1) / kSweepKeys;
-        it.j0 = (int)((int64_t)all * part / it.splits) * kSweepKeys;
-        it.j1 = min(len, (int)((int64_t)all * (part + 1) / it.splits) * kSweepKeys);
+        it.len = __builtin_amdgcn_readlane(ln, l);
+        const int t = __builtin_amdgcn_readlane(tl, l);
+        const int each = it.len + kSweepLead, first = __builtin_amdgcn_readlane(end, l) - s.Hkv * t * each;
+        const int k = (place - first) / each;
+        it.h = k / t;
+        it.tile = k - it.h * t;
+        it.place = first + k * each;
+        return;
+      }
+      base = __builtin_amdgcn_readlane(end, 63);
+    }
+  }
+  // Row tile number k of all; false: there are not so many
+  __device__ __forceinline__ bool number(int k, SweepPiece& it) const {
+    const int lane = threadIdx.x & 63;
+    int base = 0, place = 0;
+    for (int b0 = 0; b0 < s.B; b0 += 64) {
+      const int2 x = at(b0 + lane);
+      const int num = s.Hkv * tiles(x), end = base + wave_scan(num), places = num * (len(x) + kSweepLead),
+                pend = place + wave_scan(places);
+      const unsigned long long hit = __ballot(k < end);
+      if (hit) {
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll(hit) - 1);
+        it.b = b0 + l;
+        it.n = __builtin_amdgcn_readlane(x.x, l);
+        it.c = __builtin_amdgcn_readlane(x.y, l);
+        it.len = __builtin_amdgcn_readlane(len(x), l);
+        const int t = __builtin_amdgcn_readlane(tiles(x), l), i = k - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(num, l));
+        it.h = i / t;
+        it.tile = i - it.h * t;
+        it.place = __builtin_amdgcn_readlane(pend, l) - __builtin_amdgcn_readlane(places, l) + i * (it.len + kSweepLead);
         return true;
       }
       base = __builtin_amdgcn_readlane(end, 63);
-      slots = __builtin_amdgcn_readlane(send, 63);
+      place = __builtin_amdgcn_readlane(pend, 63);
     }
-    it.tile = base;  // the number of items
     return false;
+  }
+  // Places from a row tile's first on at which no share ends
+  __device__ __forceinline__ int uncut(const SweepPiece& it) const {
+    return it.len <= a.whole ? it.len + kSweepLead : kSweepLead + kSweepSnap;
+  }
+  // Where share number k begins (its row tile goes to it)
+  __device__ __forceinline__ int begin(int k, SweepPiece& it) const {
+    const int place = k * per;
+    if (place >= total) return total;
+    find(place, it);
+    return place - it.place < uncut(it) ? it.place : place;
   }
 };
 
 struct SweepParts {
-  float* o;  // [slots][RT][W]
-  float* m;  // [slots][RT]  running max (log2 domain), attend
-  float* l;  // [slots][RT]  running sum, attend
+  float* o;  // [2 shares][RT][W]
+  float* m;  // [2 shares][RT]  running max (log2 domain), attend
+  float* l;  // [2 shares][RT]  running sum, attend
 };
 
 template <int W, int KT>
@@ -316,26 +344,49 @@ __device__ __forceinline__ bf16x8 tile_tr(const bf16* tile, const TileTr& o, int
 }
 
 // Waves of a SIMD: as many as the registers of the instances leave place for
-constexpr int sweep_waves(int W, int NW) { return NW == 8 ? 2 : W == 64 ? 4 : W == 128 ? 2 : 3; }
+constexpr int sweep_waves(int NW) { return NW == 8 ? 2 : 3; }
 
 // NW waves over tiles of 16 NW keys, staged once for all of them; a wave holds NT tiles of 32 rows, KSP waves share them and
 // take every KSP-th 32 keys (RT = 32 NT NW / KSP rows).  Lane <-> row: S^T[j][i] = K_j . x_i, then acc^T[col][i] +=
 // w^T[col][j] p^T[j][i].
 //   attend: x = q, rows (token, query head of the group) token by token, online softmax
-//   couple: x = the new keys, p = P as a bf16 pair; y = v - acc.  panel >= 0: not the cached keys but those of that
-//           panel of new rows, out of the y of the rows behind it.  Grid (row tiles, Hkv, B) then, else by SweepPlan.
-template <int W, bool ATTEND, int KSP, int NW, int NT>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_waves(W, NW)))) void lucid_prefill_sweep_kernel(
+//   couple: x = the new keys, p = P as a bf16 pair; y = v - acc
+//   inner:  as couple, with the keys of one panel of new rows and out of the y of the rows behind it; grid (row
+//           tiles, Hkv, B), where the others go by SweepPlan
+enum class Sweep { Couple, Attend, Inner };
+template <int W, Sweep MODE, int KSP, int NW, int NT>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_waves(NW)))) void lucid_prefill_sweep_kernel(
     const bf16* __restrict__ x, Strides xs, int vec, const bf16* __restrict__ v, Strides vs, PagedPool kp, PagedPool vp,
     PrefillBatch seq, SweepGrid grid, int panel, PagedScale f, float eps, int d, float* __restrict__ y, int64_t yrows,
     bf16* __restrict__ o, Strides os, int ovec, SweepParts part) {
+  constexpr bool ATTEND = MODE == Sweep::Attend, LINE = MODE != Sweep::Inner;
   constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = CPR / 2, KT = 16 * NW, NMT = KT / 32 / KSP;
   constexpr int RT = 32 * NT * NW / KSP;
   static_assert(KSP == 1 || (NT == 1 && RT == 64), "the join of key groups holds 64 rows");
   __shared__ __attribute__((aligned(16))) SweepSmem<W, KT> sm;
-  SweepItem it;
-  int row_base = 0;
-  if (!ATTEND && panel >= 0) {
+  int share = 0, start = 0, place = 0, end = 1, row_base = 0;
+  SweepPiece it;
+  SweepPlan plan;
+  if constexpr (LINE) {
+    plan = SweepPlan(seq, grid);
+    // ids go round robin over the 8 XCDs: each takes a run of shares, the row tiles of one kv head next to each other
+    const int num = (plan.total + plan.per - 1) / plan.per, each = (num + 7) >> 3;
+    share = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= each || share >= num) return;
+    SweepPiece behind;
+    end = plan.begin(share + 1, behind);
+    start = place = plan.begin(share, it);
+  }
+  while (place < end) {
+  if constexpr (LINE) {
+    if (place != start) plan.find(place, it);
+    const int first = it.place + kSweepLead, next = min(end, first + it.len);
+    it.j0 = max(place - first, 0) * kSweepKeys;
+    it.j1 = min(plan.keys(make_int2(it.n, it.c)), (next - first) * kSweepKeys);
+    it.slot = place == it.place && next == first + it.len ? -1 : 2 * share + (place == start ? 0 : 1);
+    place = next;
+  } else {
+    place = end;
     it.b = blockIdx.z;
     it.h = blockIdx.y;
     it.tile = blockIdx.x;
@@ -347,16 +398,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_w
     it.j1 = it.j0 + kPanel;
     it.slot = -1;
     if (row_base + it.tile * RT >= it.c) return;
-  } else {
-    const SweepPlan plan(seq, grid);
-    // ids go round robin over the 8 XCDs: each takes a run of items, the row tiles of one part next to each other
-    SweepItem none;
-    plan.find(0x7fffffff, false, none);
-    const int per = (none.tile + 7) >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || !plan.find(id, false, it)) return;
   }
   const int b = it.b, h = it.h, n = it.n, GX = grid.GX;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // what follows from it is worked out here, not kept in registers across the pieces
+  const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
   const int rw = w / KSP, kg = w % KSP;
   const int rows = it.c * GX, row0 = row_base + it.tile * RT + 32 * NT * rw;  // of this wave
   const bool active = row0 < rows;
@@ -540,6 +586,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_w
           }
         }
       } else {
+        // (the masked and the whole tile as two bodies, so that no branch parts the sub-tiles, spill up to 283 registers:
+        // 2048 tokens of 32/8 heads of 128 columns behind 32768 rows 394 -> 850 us)
 #pragma unroll
         for (int i = 0; i < NMT; ++i) {
           const int mt = kg + KSP * i;
@@ -637,11 +685,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_w
             }
       }
     }
-    if (kg != 0) return;
   }
 #pragma unroll
   for (int r = 0; r < NT; ++r) {
-    if (row[r] >= rows) continue;
+    if (kg != 0 || row[r] >= rows) continue;
     if (it.slot >= 0) {
       const int64_t at = (int64_t)it.slot * RT + 32 * (NT * rw + r) + l32;
 #pragma unroll
@@ -684,7 +731,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_w
           const int col = 32 * q + drow(e, g);
           if (32 * q + drow(e, 0) >= W) continue;
           f32x4 z;
-          if (panel >= 0) {
+          if (!LINE) {
             z = *reinterpret_cast<const f32x4*>(yp + col);
           } else {
             const bf16x4 v4 = ld4_cols(vr, col, d, ovec);
@@ -696,12 +743,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_w
         }
     }
   }
+  if (LINE && KSP > 1 && place < end) __syncthreads();  // the join's rows are read before the next piece's tiles come
+  }
 }
 
 // --------------------------------------------------------------------------------------------
-// The parts of the row tiles that were cut along the keys, joined.  Grid (target / 2, RT / 16), 256 threads: 16 rows
-// of a row tile, W / 4 lanes a row.
+// The parts of the row tiles that a share's end cuts, joined.  Grid (row tiles at most, pieces of one), 256 threads: a piece of
+// join_rows(W) rows, W / 4 lanes a row.
 // --------------------------------------------------------------------------------------------
+constexpr int join_rows(int W) { return 256 / (W / 4); }
 template <int W, bool ATTEND>
 __global__ __launch_bounds__(256) void lucid_prefill_join_kernel(const bf16* __restrict__ v, Strides vs, int vec,
                                                                  PrefillBatch seq, SweepGrid grid, int d, float* __restrict__ y,
@@ -709,28 +759,46 @@ __global__ __launch_bounds__(256) void lucid_prefill_join_kernel(const bf16* __r
                                                                  SweepParts part) {
   constexpr int CG = W / 4;
   const SweepPlan plan(seq, grid);
-  SweepItem it;
-  if (!plan.find(blockIdx.x, true, it)) return;
+  SweepPiece it;
+  if (!plan.number(blockIdx.x, it)) return;
+  // the last share that begins at its first place, or the one that has it beside others
+  const int share = (it.place + plan.uncut(it) - 1) / plan.per;
+  const int parts = (it.place + kSweepLead + it.len - 1) / plan.per - share + 1;
+  if (parts == 1) return;
+  const int slot0 = 2 * share + (share * plan.per >= it.place ? 0 : 1);
   const int GX = grid.GX, rows = it.c * GX;
-  for (int i = threadIdx.x; i < 16 * CG; i += 256) {
-    const int r = 16 * blockIdx.y + i / CG, col = 4 * (i % CG), row = it.tile * grid.RT + r;
-    if (row >= rows) return;
+  {
+    const int i = threadIdx.x, r = join_rows(W) * blockIdx.y + i / CG, col = 4 * (i % CG), row = it.tile * grid.RT + r;
+    if (i >= join_rows(W) * CG || r >= grid.RT || row >= rows) return;
     const int t = row / GX, hq = it.h * GX + (row - t * GX);
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
     float M = PREFILL_NEG, l = 0.f;
-    for (int p = 0; p < it.splits; ++p) {
-      const int64_t at = ((int64_t)it.slot + (int64_t)p * it.tiles) * grid.RT + r;
-      const f32x4 x = *reinterpret_cast<const f32x4*>(part.o + at * W + col);
-      if constexpr (ATTEND) {
-        const float m = part.m[at], mn = fmaxf(M, m);
-        const float a = __builtin_amdgcn_exp2f(M - mn), e = __builtin_amdgcn_exp2f(m - mn);
-        l = fmaf(l, a, part.l[at] * e);
+    constexpr int UN = 8;  // parts asked for at a time (those beyond the last: the last, with the weight 0)
+    for (int p0 = 0; p0 < parts; p0 += UN) {
+      f32x4 x[UN];
+      float m[UN], lp[UN];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) z[u] = fmaf(z[u], a, x[u] * e);
-        M = mn;
-      } else {
+      for (int k = 0; k < UN; ++k) {
+        const int p = min(p0 + k, parts - 1);
+        const int64_t at = (int64_t)(p == 0 ? slot0 : 2 * (share + p)) * grid.RT + r;
+        x[k] = *reinterpret_cast<const f32x4*>(part.o + at * W + col);
+        m[k] = ATTEND ? part.m[at] : 0.f;
+        lp[k] = ATTEND ? part.l[at] : 0.f;
+      }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) z[u] += x[u];
+      for (int k = 0; k < UN; ++k) {
+        const bool on = p0 + k < parts;
+        if constexpr (ATTEND) {
+          const float mn = on ? fmaxf(M, m[k]) : M;
+          const float a = __builtin_amdgcn_exp2f(M - mn), e = on ? __builtin_amdgcn_exp2f(m[k] - mn) : 0.f;
+          l = fmaf(l, a, lp[k] * e);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) z[u] = fmaf(z[u], a, x[k][u] * e);
+          M = mn;
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) z[u] += on ? x[k][u] : 0.f;
+        }
       }
     }
     if constexpr (ATTEND) {

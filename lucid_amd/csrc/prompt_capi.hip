@@ -14,8 +14,6 @@ namespace {
 // Results of so many bytes pass the 256 MB cache by
 constexpr int64_t kPastBytes = 100000000;
 
-// Slots of 128 rows for the parts of a sweep
-constexpr int kPrefillSlots = 1024;
 
 struct PrefillWs {
   int2* info;       // [B]
@@ -27,9 +25,8 @@ struct PrefillWs {
 
 // Rows of a workgroup of a sweep: 64 with four waves to 32 rows where there are few
 int sweep_rows(int64_t rows, bool attend, int W) { return rows <= 128 ? 64 : attend && W <= 96 ? 128 : 256; }
-
-// Items that it aims at: one round of the chip
-int sweep_target(int RT, int W, bool attend) { return RT == 128 ? (W == 64 ? 1024 : 768) : 256; }
+// Shares of the line: one round of the chip, whose CUs hold three workgroups of 128 rows, and one of the others
+int sweep_target(int RT) { return RT == 128 ? 768 : 256; }
 
 PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
   const size_t panels = ((size_t)L + lucid::kPanel - 1) / lucid::kPanel;
@@ -44,7 +41,8 @@ PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
   w.info = reinterpret_cast<int2*>(take((size_t)B * 8));
   w.pmat = take((size_t)B * Hkv * panels * lucid::kPanelBytes);
   w.y = reinterpret_cast<float*>(take((size_t)B * Hkv * panels * lucid::kPanel * W * 4));
-  const size_t rows = (size_t)kPrefillSlots * 128;
+  size_t rows = 0;  // of the parts of any sweep
+  for (int RT : {64, 128, 256}) rows = std::max(rows, (size_t)2 * sweep_target(RT) * RT);
   w.part.o = reinterpret_cast<float*>(take(rows * W * 4));
   w.part.m = reinterpret_cast<float*>(take(rows * 4));
   w.part.l = reinterpret_cast<float*>(take(rows * 4));
@@ -52,10 +50,15 @@ PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
   return w;
 }
 
+// Places of a row tile in the line of a sweep, at most
+int64_t prefill_len(int page, int max_pages) {
+  return ((int64_t)page * max_pages + lucid::kSweepKeys - 1) / lucid::kSweepKeys + lucid::kSweepLead;
+}
+
 bool prefill_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int D) {
   return B > 0 && B <= 65535 && Hkv > 0 && Hkv <= 65535 && Hq > 0 && Hq % Hkv == 0 && L > 0 && page > 0 && max_pages > 0 &&
          page_width(D) && (int64_t)page * max_pages <= (1 << 30) && (int64_t)L * (Hq / Hkv) <= (1 << 24) &&
-         (int64_t)B * Hkv * (((int64_t)L * (Hq / Hkv) + 63) / 64) <= (1 << 24);
+         (int64_t)B * Hkv * (((int64_t)L * (Hq / Hkv) + 63) / 64) * prefill_len(page, max_pages) < (1 << 30);
 }
 
 struct PrefillCall {
@@ -71,39 +74,42 @@ struct PrefillCall {
   hipStream_t st;
 };
 
-template <int W, bool ATTEND>
-int prefill_sweep(const PrefillCall& c, int panel) {
-  const int G = c.Hq / c.seq.Hkv, GX = ATTEND ? G : 1;
+template <int W, lucid::Sweep MODE>
+int prefill_sweep(const PrefillCall& c, int panel = 0) {
+  using lucid::Sweep;
+  constexpr bool ATTEND = MODE == Sweep::Attend, LINE = MODE != Sweep::Inner;
+  const int GX = ATTEND ? c.Hq / c.seq.Hkv : 1;
   const int panels = (c.seq.L + lucid::kPanel - 1) / lucid::kPanel;
   const int64_t rows = (int64_t)c.seq.L * GX, yrows = (int64_t)panels * lucid::kPanel;
-  const int RT = panel >= 0 ? 64 : sweep_rows(rows, ATTEND, W);
-  const lucid::SweepGrid grid{GX, RT, ATTEND, sweep_target(RT, W, ATTEND)};
+  const int RT = LINE ? sweep_rows(rows, ATTEND, W) : 64;
+  const int64_t tiles = (int64_t)c.seq.B * c.seq.Hkv * ((rows + RT - 1) / RT);  // at most
+  // staged tiles of a sequence's keys, at most: where they are few, no row tile is cut and nothing is joined
+  const int64_t most = prefill_len(c.seq.page, c.seq.M) - lucid::kSweepLead;
+  const lucid::SweepGrid grid{GX, RT, ATTEND, sweep_target(RT), most <= 8 ? 8 : 4};
   const bf16* x = ATTEND ? c.q : c.k;
   const int64_t* xs = ATTEND ? c.qs : c.ks;
   const int vec = rows_of_4(x, xs, 2), vvec = rows_of_4(c.v, c.vs, 2);
   const int ovec = ATTEND ? c.D % 4 == 0 && rows_of_4(c.o, c.os, 2) : vvec;
-  dim3 blocks;
-  if (panel >= 0) {
-    blocks = dim3((unsigned)((c.seq.L - lucid::kPanel * (panel + 1) + RT - 1) / RT), c.seq.Hkv, c.seq.B);
-  } else {
-    const int64_t most = (int64_t)c.seq.B * c.seq.Hkv * ((rows + RT - 1) / RT) + grid.target;
-    blocks = dim3((unsigned)((most + 7) / 8 * 8));
-  }
+  const dim3 blocks = LINE ? dim3((grid.target + 7) / 8 * 8)
+                           : dim3((unsigned)((c.seq.L - lucid::kPanel * (panel + 1) + RT - 1) / RT), c.seq.Hkv, c.seq.B);
   auto go = [&](auto kernel, int threads) -> int {
-    LUCID_LAUNCH_B(ATTEND ? "lucid_prefill_attend_kernel" : "lucid_prefill_couple_kernel", kernel, blocks, dim3(threads), c.st, x,
-                   S(xs), vec, c.v, S(c.vs), c.kp, c.vp, c.seq, grid, panel, c.scale, c.eps, c.D, c.ws.y, yrows, c.o, S(c.os),
-                   ovec, c.ws.part);
+    LUCID_LAUNCH_B(ATTEND ? "lucid_prefill_attend_kernel" : LINE ? "lucid_prefill_couple_kernel" : "lucid_prefill_inner_kernel",
+                   kernel, blocks, dim3(threads), c.st, x, S(xs), vec, c.v, S(c.vs), c.kp, c.vp, c.seq, grid, panel, c.scale, c.eps,
+                   c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
     return LUCID_OK;
   };
-  constexpr int NW = ATTEND && W <= 96 ? 4 : 8;
-  const int rc = RT == 64 ? go(lucid::lucid_prefill_sweep_kernel<W, ATTEND, 4, 8, 1>, 512)
-                          : go(lucid::lucid_prefill_sweep_kernel<W, ATTEND, 1, NW, 1>, 64 * NW);
-  if (rc || panel >= 0) return rc;
-  // (rows of fewer tiles than two least parts are never cut)
-  if ((int64_t)c.seq.M * c.seq.page <= (2 * lucid::kSweepLeast - 1) * lucid::kSweepKeys) return LUCID_OK;
-  LUCID_LAUNCH("lucid_prefill_join_kernel", (lucid::lucid_prefill_join_kernel<W, ATTEND>), dim3(grid.target / 2, RT / 16), c.st,
-               c.v, S(c.vs), vvec, c.seq, grid, c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
-  return LUCID_OK;
+  if constexpr (!LINE) {
+    return go(lucid::lucid_prefill_sweep_kernel<W, MODE, 4, 8, 1>, 512);
+  } else {
+    constexpr int NW = ATTEND && W <= 96 ? 4 : 8;
+    const int rc = RT == 64 ? go(lucid::lucid_prefill_sweep_kernel<W, MODE, 4, 8, 1>, 512)
+                            : go(lucid::lucid_prefill_sweep_kernel<W, MODE, 1, NW, 1>, 64 * NW);
+    if (rc || most <= grid.whole) return rc;
+    LUCID_LAUNCH("lucid_prefill_join_kernel", (lucid::lucid_prefill_join_kernel<W, ATTEND>),
+                 dim3((unsigned)tiles, (RT + lucid::join_rows(W) - 1) / lucid::join_rows(W)), c.st, c.v, S(c.vs), vvec, c.seq,
+                 grid, c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
+    return LUCID_OK;
+  }
 }
 
 template <int W>
@@ -113,14 +119,14 @@ int prefill(const PrefillCall& c) {
   LUCID_LAUNCH_B("lucid_prefill_prep_kernel", lucid::lucid_prefill_prep_kernel<W>, dim3(4 * panels, c.seq.Hkv, c.seq.B), dim3(512),
                  c.st, c.k, S(c.ks), (int)rows_of_4(c.k, c.ks, 2), c.kp, c.seq, c.scale, c.eps, c.D, c.ws.pmat, c.o, S(c.os),
                  (int)(c.D % 4 == 0 && rows_of_4(c.o, c.os, 2)), c.Hq / c.seq.Hkv);
-  if (int rc = prefill_sweep<W, false>(c, -1)) return rc;
+  if (int rc = prefill_sweep<W, lucid::Sweep::Couple>(c)) return rc;
   for (int p = 0; p < panels; ++p) {
     LUCID_LAUNCH_B("lucid_prefill_solve_kernel", lucid::lucid_prefill_solve_kernel<W>, dim3((W + 31) / 32, c.seq.Hkv, c.seq.B),
                    dim3(64), c.st, c.ws.pmat, panels, p, c.ws.y, yrows, c.vp, c.seq, c.D);
     if (p + 1 < panels)
-      if (int rc = prefill_sweep<W, false>(c, p)) return rc;
+      if (int rc = prefill_sweep<W, lucid::Sweep::Inner>(c, p)) return rc;
   }
-  return prefill_sweep<W, true>(c, -1);
+  return prefill_sweep<W, lucid::Sweep::Attend>(c);
 }
 
 template <typename T, bool INTER>
@@ -210,7 +216,7 @@ int lucid_prefill_paged(const void* q, const int64_t* q_strides, const void* k, 
   if (!page_width(D)) return fail("head_dim must be in [1, 128], got " + std::to_string(D));
   if (!prefill_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D))
     return fail("lucid_prefill_paged: B, Hq, Hkv, L, page_size and max_pages positive, Hq a multiple of Hkv, B and Hkv at most "
-                "65535, at most 2^30 rows a sequence, 2^24 rows of query heads to a kv head and 2^24 tiles of 64 of them in all");
+                "65535, at most 2^30 rows a sequence, 2^24 rows of query heads to a kv head, and 2^30 tiles of 64 of them and 128 rows in all");
   if (num_pages < 1) return fail("lucid_prefill_paged: the pools have no pages");
   if (!q || !q_strides || !k || !k_strides || !v || !v_strides || !o || !o_strides || !page_table || !cache_lens || !ws)
     return fail("lucid_prefill_paged: null argument");
