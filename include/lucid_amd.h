@@ -53,7 +53,8 @@ extern "C" {
 #define LUCID_PRECISION_EXACT 2 /* hi/lo split products for every head */
 
 /* ABI version of this header (bumped whenever an entry point changes or goes): 6; and the number of
- * times that entry points have been added to that version: 1 (serving from a paged cache). */
+ * times that entry points have been added to that version: 2 (serving from a paged cache; prompts in chunks
+ * behind it, rotary positions, constraints on logits). */
 int lucid_abi_version(void);
 int lucid_abi_minor(void);
 
@@ -398,8 +399,9 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
  * and in slots without a sequence.  The new rows' V' go to the pages only (bf16).  Any cutting of a prompt into
  * calls of this and of lucid_decode_paged gives the same rows up to rounding.  A sequence whose table names a page
  * outside the pool among those it needs, or is too short for the new rows, gets NaN in o and nothing is
- * written for it.  Cached rows and the tokens' rows must be finite, scale positive.  At most 65535 sequences and kv heads, 2^24 rows of
- * query heads (L Hq / Hkv) to a kv head.
+ * written for it.  Cached rows and the tokens' rows must be finite, scale positive.  At most 65535 sequences and kv
+ * heads, 2^24 rows of query heads (L Hq / Hkv) to a kv head, 2^23 tiles of 64 of these in all, and 2^30 pairs of such
+ * tiles and tiles of 128 of the rows that a table holds.
  * ws: lucid_prefill_paged_workspace_bytes (0 on bad sizes), 256-byte aligned, one per call in flight. */
 size_t lucid_prefill_paged_workspace_bytes(int B, int Hq, int Hkv, int L, int page_size, int max_pages, int D);
 int lucid_prefill_paged(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,

@@ -58,6 +58,7 @@ int64_t prefill_len(int page, int max_pages) {
 bool prefill_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int D) {
   return B > 0 && B <= 65535 && Hkv > 0 && Hkv <= 65535 && Hq > 0 && Hq % Hkv == 0 && L > 0 && page > 0 && max_pages > 0 &&
          page_width(D) && (int64_t)page * max_pages <= (1 << 30) && (int64_t)L * (Hq / Hkv) <= (1 << 24) &&
+         (int64_t)B * Hkv * (((int64_t)L * (Hq / Hkv) + 63) / 64) <= (1 << 23) &&
          (int64_t)B * Hkv * (((int64_t)L * (Hq / Hkv) + 63) / 64) * prefill_len(page, max_pages) < (1 << 30);
 }
 
@@ -216,7 +217,8 @@ int lucid_prefill_paged(const void* q, const int64_t* q_strides, const void* k, 
   if (!page_width(D)) return fail("head_dim must be in [1, 128], got " + std::to_string(D));
   if (!prefill_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D))
     return fail("lucid_prefill_paged: B, Hq, Hkv, L, page_size and max_pages positive, Hq a multiple of Hkv, B and Hkv at most "
-                "65535, at most 2^30 rows a sequence, 2^24 rows of query heads to a kv head, and 2^30 tiles of 64 of them and 128 rows in all");
+                "65535, at most 2^30 rows a sequence, 2^24 rows of query heads to a kv head, 2^23 tiles of 64 of them in all, and "
+                "2^30 pairs of these and of tiles of 128 rows");
   if (num_pages < 1) return fail("lucid_prefill_paged: the pools have no pages");
   if (!q || !q_strides || !k || !k_strides || !v || !v_strides || !o || !o_strides || !page_table || !cache_lens || !ws)
     return fail("lucid_prefill_paged: null argument");

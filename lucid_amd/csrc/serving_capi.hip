@@ -409,6 +409,6 @@ int lucid_token_logprobs_bwd(const void* logits, int64_t batch_stride, int64_t r
   return go((bf16)0.f, past ? lucid_token_logprobs_bwd_kernel<bf16, true> : lucid_token_logprobs_bwd_kernel<bf16, false>);
 }
 
-int lucid_abi_minor(void) { return 1; }
+int lucid_abi_minor(void) { return 2; }
 
 }  // extern "C"

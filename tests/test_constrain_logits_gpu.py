@@ -230,3 +230,65 @@ def test_refusals():
             (dict(presence=torch.ones(2, device="cuda", requires_grad=True)), NotImplementedError, "gradient")):
         with pytest.raises(err, match=text):
             O.constrain_logits(x, **kw)
+
+
+def test_tangents_and_second_derivatives_are_refused():
+    from torch.autograd import forward_ad
+    x = torch.randn(2, 100, device="cuda")
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        O.constrain_logits(forward_ad.make_dual(x, torch.ones_like(x)), bias=torch.zeros(100, device="cuda"))
+    leaf = x.clone().requires_grad_()
+    g, = torch.autograd.grad(O.constrain_logits(leaf).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("N", [300, 5000])
+def test_large_rows_and_their_gradient(N):
+    """Results of 100 MB and more pass the caches by; both ways of finding what has occurred."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    R, V = 1700, 32000
+    x = torch.randn(R, V, generator=g, device="cuda").to(BF)
+    h = history_of(g, R, N, V)
+    ok = torch.rand(R, V, generator=g, device="cuda") < 0.8
+    grad = torch.randn(R, V, generator=g, device="cuda").to(BF)
+    leaf = x.clone().requires_grad_()
+    y = O.constrain_logits(leaf, history=h, repetition=1.25, presence=0.5, frequency=0.125, allowed=bits_of(ok))
+    d, = torch.autograd.grad(y, leaf, grad)
+    for rows in (slice(0, 40), slice(R - 40, R)):
+        want, tol, slope = ref(x[rows], history=h[rows], repetition=1.25, presence=0.5, frequency=0.125, allowed=ok[rows])
+        close(y[rows].detach(), want, tol, "logits")
+        close(d[rows], slope * grad[rows].double(), 2 * 2.0 ** -24 * (slope * grad[rows].double()).abs(), "dlogits")
+
+
+def test_gradient_of_log_probabilities_through_the_constraints():
+    """d logprob / d logits = slope ([v = token] - p), against float64 autograd of the definition."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(6, 500, generator=g, device="cuda")
+    h = history_of(g, 6, 40, 500)
+    ok = torch.rand(6, 500, generator=g, device="cuda") < 0.5
+    tok = torch.randint(0, 500, (6,), generator=g, device="cuda")
+    ok[torch.arange(6), tok] = True
+    leaf = x.clone().requires_grad_()
+    lp = O.token_logprobs(O.constrain_logits(leaf, history=h, repetition=1.3, presence=0.2, allowed=bits_of(ok)), tok).logprobs
+    d, = torch.autograd.grad(lp.sum(), leaf)
+    y, _, slope = ref(x, history=h, repetition=1.3, presence=0.2, allowed=ok)
+    p = torch.softmax(y, -1)
+    want = slope * (torch.nn.functional.one_hot(tok, 500) - p)
+    # p in 32 bits from exponents of at most 16 in size: 2^-19 of it, and the product's rounding
+    assert ((d.double() - want).abs() <= 2.0 ** -18 * slope * p + 2.0 ** -22 * want.abs()).all()
+
+
+def test_two_streams_and_expanded_rows():
+    g = torch.Generator(device="cuda").manual_seed(10)
+    x = torch.randn(1, 9000, generator=g, device="cuda").expand(4, 9000)
+    h = history_of(g, 1, 50, 9000, pad=False).expand(4, 50)
+    want, tol, _ = ref(x, history=h, repetition=1.4)
+    torch.cuda.synchronize()
+    outs = []
+    for s in (torch.cuda.Stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(s):
+            outs.append(O.constrain_logits(x, history=h, repetition=1.4))
+    torch.cuda.synchronize()
+    for y in outs:
+        close(y, want, tol, "logits")

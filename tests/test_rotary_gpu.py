@@ -188,3 +188,59 @@ def test_refusals():
         O.rotary(q, k, pos, freq, scale=math.inf)
     with pytest.raises(ValueError, match="256"):
         O.rotary(*make(1, 9, 1, 1, 257, BF), pos, freq)
+
+
+def test_tangents_and_second_derivatives_are_refused():
+    from torch.autograd import forward_ad
+    q, k = make(1, 4, 2, 1, 64, F32)
+    pos, freq = torch.arange(4, device="cuda"), O.rope_frequencies(64)[0].cuda()
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            O.rotary(forward_ad.make_dual(q, torch.ones_like(q)), k, pos, freq)
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            O.rotary(q, forward_ad.make_dual(k, torch.ones_like(k)), pos, freq)
+    x = q.clone().requires_grad_()
+    g, = torch.autograd.grad(O.rotary(x, k, pos, freq)[0].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_a_large_pass_and_its_gradient():
+    """Results of 100 MB and more pass the caches by; a gradient that comes in as one value for all."""
+    q, k = make(1, 14000, 24, 8, 128, BF)
+    pos = torch.arange(14000, device="cuda")
+    freq = O.rope_frequencies(128)[0].cuda()
+    a, b = O.rotary(q, k, pos, freq)
+    for t in (0, 1, 4095, 13999):
+        close(a[:, :, t:t + 1], ref(q[:, :, t:t + 1], pos[t:t + 1], freq, False, 1.0), f"q at {t}")
+        close(b[:, :, t:t + 1], ref(k[:, :, t:t + 1], pos[t:t + 1], freq, False, 1.0), f"k at {t}")
+    x = q.clone().requires_grad_()
+    O.rotary(x, k, pos, freq)[0].sum().backward()
+    close(x.grad[:, :, -1:], ref(torch.ones_like(q[:, :, -1:]), pos[-1:], freq, False, 1.0, True), "dq")
+
+
+def test_captured_backward():
+    """A captured turn and its gradient on static leaves follow new values, while no eager graph of theirs lives."""
+    q, k = make(2, 16, 4, 2, 68, BF)
+    q, k = (x.detach().contiguous().requires_grad_() for x in (q, k))
+    pos = torch.arange(16, device="cuda") * 100
+    freq = O.rope_frequencies(68)[0].cuda()
+    g = torch.randn(2, 4, 16, 68, device="cuda").to(BF)
+
+    def step():
+        a, b = O.rotary(q, k, pos, freq)
+        return torch.autograd.grad((a, b), (q, k), (g, g[:, :2]))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dq, dk = step()
+    for _ in range(3):
+        g.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        close(dq, ref(g, pos, freq, False, 1.0, True), "dq")
+        close(dk, ref(g[:, :2], pos, freq, False, 1.0, True), "dk")
