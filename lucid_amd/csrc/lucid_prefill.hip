@@ -825,125 +825,110 @@ __global__ __launch_bounds__(256) void lucid_prefill_join_kernel(const bf16* __r
 
 // --------------------------------------------------------------------------------------------
 // One panel's rows in order: with z_t = y_t / P_tt, w_t = bf16(z_t) and z_u -= P_ut / P_uu w_t for u > t.  Grid (32 columns,
-// Hkv, B), one wave: columns are independent, and a wave holds all rows of its own (lane <-> column, elements <->
-// rows of a block of 32).  It goes through a block by itself, row by row, each row's value from one lane half to the
-// other in the VALU, and takes it out of the blocks behind with MFMAs, the block's rows as they stand in registers as the
-// second operand.  The chain of 256 dependent rows bounds it, not the 145 KB of P it stages.
-// (The blocks are one loop over registers that move up by a block: with its eight blocks written out the kernel's 60 KB of
-// instructions, each run once, took 41 us to fetch.)
+// Hkv, B), a wave for each block of 32 rows: columns are independent (lane <-> column, elements <-> rows).  A wave goes
+// through its block by itself, row by row, each row's value from one lane half to the other in the VALU; the waves of the
+// blocks behind wait for its rows, operands of theirs as they stand in registers, and take them out with MFMAs, their tile of
+// P fetched a block ahead.  The chain of 256 dependent rows bounds it.  (One wave for all blocks, with the panel's 145 KB of P
+// staged in LDS, took 24.5 us a panel where this takes 16.5.)
 // --------------------------------------------------------------------------------------------
 template <int W>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1))) void lucid_prefill_solve_kernel(
+__global__ __launch_bounds__(64 * kPanelBlocks) void lucid_prefill_solve_kernel(
     const char* __restrict__ pmat, int panels, int panel, const float* __restrict__ y, int64_t yrows, PagedPool vp,
     PrefillBatch seq, int d) {
   __shared__ __attribute__((aligned(16))) struct {
-    char p[kPanelBytes];
+    float diag[kPanelBlocks][1024];
+    bf16 w[kPanelBlocks][1024];  // a block's rows as two operands
     unsigned off[kPanel];
   } sm;
   const int h = blockIdx.y, b = blockIdx.z;
   const int2 info = seq.info[b];
   const int R = min(info.y - panel * kPanel, kPanel);
   if (R <= 0) return;
-  const int lane = threadIdx.x, g = lane >> 5, l32 = lane & 31;
-  const int nb = (R + 31) / 32;  // blocks with rows
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // this wave's block
+  const int nb = (R + 31) / 32;                                      // blocks with rows
   const int64_t bh = (int64_t)b * seq.Hkv + h;
   const char* pm = pmat + (bh * panels + panel) * kPanelBytes;
-  auto fetch = [&](size_t first, int pieces) {  // 1 KB each
-    for (int i = 0; i < pieces; ++i)
-      __builtin_amdgcn_global_load_lds(reinterpret_cast<const bf16*>(pm + first) + i * 512 + lane * 8,
-                                       reinterpret_cast<bf16*>(sm.p + first) + i * 512, 16, 0, 0);
-  };
-  fetch(kPanelInv, 1);
-  fetch(kPanelDiag, 4 * nb);
-  const int n = info.x + panel * kPanel;
-  for (int r = lane; r < R; r += 64) {  // (those behind stay as they are: read, not used)
-    const int j = n + r;
-    sm.off[r] = prefill_row(seq, vp, seq.table[b * seq.tstride + prefill_page(seq, j)], j, h);
-  }
+  const bf16* tiles = reinterpret_cast<const bf16*>(pm) + (own * (own - 1) / 2) * kPanelTile + lane * 8;
   const int col = 32 * blockIdx.x + l32;
   const bool on = col < d;
-  f32x16 acc[kPanelBlocks];  // of the block at hand and those behind it
-  const float* yb = y + (bh * yrows + panel * kPanel) * W + min(col, W - 1);
+  bf16x8 p0, p1, p2, p3;
+  auto fetch = [&](int j) {
+    p0 = ld8(tiles + j * kPanelTile);
+    p1 = ld8(tiles + j * kPanelTile + 512);
+    p2 = ld8(tiles + j * kPanelTile + 1024);
+    p3 = ld8(tiles + j * kPanelTile + 1536);
+  };
+  f32x16 z = zero16();
+  if (own < nb) {
 #pragma unroll
-  for (int i = 0; i < kPanelBlocks; ++i)
+    for (int i = 0; i < 4; ++i)
+      dma_1k(reinterpret_cast<const bf16*>(pm + kPanelDiag) + own * 2048 + i * 512,
+             reinterpret_cast<bf16*>(sm.diag[own]) + i * 512);
+    const float* yb = y + (bh * yrows + panel * kPanel) * W + min(col, W - 1);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[i][e] = yb[min(32 * i + drow(e, g), R - 1) * W];
-  fetch(0, 4 * (nb * (nb - 1) / 2));
+    for (int e = 0; e < 16; ++e) z[e] = yb[min(32 * own + drow(e, g), R - 1) * W];
+    float iv[16];
+    lds_rows16(reinterpret_cast<const float*>(pm + kPanelInv) + 32 * own, g, iv);
+    if (own > 0) fetch(0);
+    const int r = 32 * own + l32;
+    if (lane < 32 && r < R) {  // (those behind stay as they are: read, not used)
+      const int j = info.x + panel * kPanel + r;
+      sm.off[r] = prefill_row(seq, vp, seq.table[b * seq.tstride + prefill_page(seq, j)], j, h);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = 32 * own + drow(e, g) < R ? z[e] * iv[e] : 0.f;
+  }
   dma_wait();
   __syncthreads();
-  const float* inv = reinterpret_cast<const float*>(sm.p + kPanelInv);
-#pragma unroll
-  for (int i = 0; i < kPanelBlocks; ++i) {
-    float iv[16];
-    lds_rows16(inv + 32 * i, g, iv);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[i][e] = 32 * i + drow(e, g) < R ? acc[i][e] * iv[e] : 0.f;
-    asm volatile("" ::: "memory");  // a block's comparisons at a time
-  }
-  const float* dg = reinterpret_cast<const float*>(sm.p + kPanelDiag) + 4 * g;
 #pragma unroll 1
-  for (int i = 0; i < nb; ++i, dg += 1024) {
+  for (int i = 0; i < nb; ++i) {
     f32x16 fin;
+    if (own == i) {
+      const float* dg = sm.diag[i] + 4 * g;
+      // P of row t arrives kAhead rows before its turn
+      constexpr int kAhead = 3;
+      f32x4 p[kAhead + 1][4];
+      auto ask = [&](int t) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) fin[e] = 0.f;
-    // P of row t arrives kAhead rows before its turn
-    constexpr int kAhead = 3;
-    f32x4 p[kAhead + 1][4];
-    auto ask = [&](int t) {
+        for (int q = 0; q < 4; ++q)
+          if (8 * q + 7 > t) p[t % (kAhead + 1)][q] = *reinterpret_cast<const f32x4*>(dg + 32 * t + 8 * q);
+      };
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (8 * q + 7 > t) p[t % (kAhead + 1)][q] = *reinterpret_cast<const f32x4*>(dg + 32 * t + 8 * q);
-    };
+      for (int e = 0; e < 16; ++e) fin[e] = 0.f;
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t) ask(t);
+      for (int t = 0; t < kAhead; ++t) ask(t);
 #pragma unroll
-    for (int t = 0; t < 32; ++t) {
-      const int e_t = 4 * (t >> 3) + (t & 3), g_t = (t >> 2) & 1;
-      if (t + kAhead < 32) ask(t + kAhead);
-      __builtin_amdgcn_sched_barrier(0);
-      const unsigned u = __builtin_bit_cast(unsigned, (float)(bf16)acc[0][e_t]);
-      const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // the first half's, the second's
-      const float wt = __builtin_bit_cast(float, g_t ? (unsigned)both[1] : (unsigned)both[0]);
-      fin[e_t] = g == g_t ? wt : fin[e_t];
+      for (int t = 0; t < 32; ++t) {
+        const int e_t = 4 * (t >> 3) + (t & 3), g_t = (t >> 2) & 1;
+        if (t + kAhead < 32) ask(t + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned u = __builtin_bit_cast(unsigned, (float)(bf16)z[e_t]);
+        const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // the first half's, the second's
+        const float wt = __builtin_bit_cast(float, g_t ? (unsigned)both[1] : (unsigned)both[0]);
+        fin[e_t] = g == g_t ? wt : fin[e_t];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (8 * q + 4 + k > t) acc[0][4 * q + k] = fmaf(p[t % (kAhead + 1)][q][k], wt, acc[0][4 * q + k]);
+          for (int k = 0; k < 4; ++k)
+            if (8 * q + 4 + k > t) z[4 * q + k] = fmaf(p[t % (kAhead + 1)][q][k], wt, z[4 * q + k]);
+      }
+      *reinterpret_cast<bf16x8*>(sm.w[i] + lane * 8) = pack_b(fin, 0);
+      *reinterpret_cast<bf16x8*>(sm.w[i] + 512 + lane * 8) = pack_b(fin, 1);
     }
-    const bf16x8 w0 = pack_b(fin, 0), w1 = pack_b(fin, 1);
-    // the blocks behind, each one place up; what lies behind the last one is not looked at again
-    auto take = [&](auto first, auto last) {
-      constexpr int K0 = decltype(first)::value, K1 = decltype(last)::value;
-      const bf16* tile[K1 - K0 + 1];
+    __syncthreads();
+    if (own > i && own < nb) {
+      const bf16x8 w0 = ld8(sm.w[i] + lane * 8), w1 = ld8(sm.w[i] + 512 + lane * 8);
+      z = mfma32(p0, w0, z);
+      z = mfma32(p1, w0, z);
+      z = mfma32(p2, w1, z);
+      z = mfma32(p3, w1, z);
+      if (own > i + 1) fetch(i + 1);
+    } else if (own == i && col < W) {
 #pragma unroll
-      for (int k = K0; k <= K1; ++k) {
-        const int at = min(i + k, nb - 1);
-        tile[k - K0] = reinterpret_cast<const bf16*>(sm.p) + (at * (at - 1) / 2 + min(i, at - 1)) * kPanelTile + lane * 8;
-      }
-#pragma unroll
-      for (int part = 0; part < 4; ++part)
-#pragma unroll
-        for (int k = K0; k <= K1; ++k)
-          acc[part < 3 ? k : k - 1] = mfma32(ld8(tile[k - K0] + 512 * part), part < 2 ? w0 : w1, acc[k]);
-    };
-    if (i + 1 < nb) take(std::integral_constant<int, 1>{}, std::integral_constant<int, 3>{});
-    if (i + 4 < nb) take(std::integral_constant<int, 4>{}, std::integral_constant<int, 7>{});
-    if (col < W) {
-      unsigned at[16];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const u32x4 r = *reinterpret_cast<const u32x4*>(&sm.off[32 * i + 8 * q + 4 * g]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) at[4 * q + k] = r[k];
-      }
-      if (32 * (i + 1) <= R) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) paged_at(vp, at[e])[col] = (bf16)(on ? fin[e] : 0.f);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (32 * i + drow(e, g) < R) paged_at(vp, at[e])[col] = (bf16)(on ? fin[e] : 0.f);
+      for (int e = 0; e < 16; ++e) {
+        const int r = 32 * i + drow(e, g);
+        if (r < R) paged_at(vp, sm.off[r])[col] = (bf16)(on ? fin[e] : 0.f);
       }
     }
   }

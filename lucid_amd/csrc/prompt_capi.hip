@@ -123,7 +123,7 @@ int prefill(const PrefillCall& c) {
   if (int rc = prefill_sweep<W, lucid::Sweep::Couple>(c)) return rc;
   for (int p = 0; p < panels; ++p) {
     LUCID_LAUNCH_B("lucid_prefill_solve_kernel", lucid::lucid_prefill_solve_kernel<W>, dim3((W + 31) / 32, c.seq.Hkv, c.seq.B),
-                   dim3(64), c.st, c.ws.pmat, panels, p, c.ws.y, yrows, c.vp, c.seq, c.D);
+                   dim3(64 * lucid::kPanelBlocks), c.st, c.ws.pmat, panels, p, c.ws.y, yrows, c.vp, c.seq, c.D);
     if (p + 1 < panels)
       if (int rc = prefill_sweep<W, lucid::Sweep::Inner>(c, p)) return rc;
   }
