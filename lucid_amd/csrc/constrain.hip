@@ -3,7 +3,10 @@
 // N_rv the times that v occurs in the row's history from its prompt's end on:
 //   x = logit;  if v occurs in the history: x = x > 0 ? x / rho : x rho;  x = x - pi [N_rv > 0] - phi N_rv;
 //   x = x + bias_v;  -inf where v is not allowed
-// Its gradient is 1, 1 / rho or rho (by the logit's sign), 0 where v is not allowed.
+// Its gradient is 1, 1 / rho or rho (by the logit's sign), 0 where v is not allowed.  One read and one write of the rows, a
+// segment of 8192 values to a workgroup; each reads the row's whole history, which the caches hold.  HBM bounds large calls: 8192 rows
+// of 32000 bf16 values behind 500 tokens, 1.05 GB, 217 us, 4.8 TB/s, and their gradient, 1.05 GB, 245 us; 64 of 131072 behind
+// 4000, 35 MB, 16 us; 4 of 32003 fp32 values behind 100000 tokens 25 us, the history once for each of 5 segments.
 #include "logit_rows.h"
 
 namespace lucid {
@@ -45,9 +48,11 @@ constexpr int kConstrainHeld = 8;  // tokens of a history that a lane holds
 // How a workgroup finds the tokens of its segment that have occurred
 enum class History {
   None,
-  Held,  // up to 512 kConstrainHeld tokens: in registers, so that only their own counters are cleared, and a bit each
-         // tells which eight values have none
-  Long,  // any number: all counters cleared, one pass
+  Counted,  // a counter of each value in LDS (clearing only those of tokens held in registers, with a bit a value for the rest,
+            // was slower: 64 rows of 131072 behind 4000 tokens 16.3 -> 18.0 us, 256 of 32000 fp32 behind 2000 20.8 -> 22.9)
+  Held,     // the gradient of up to 512 kConstrainHeld tokens: a bit of each value for an occurrence and for a logit above 0, both
+            // from the tokens themselves, held in registers (8192 rows of 32000 behind 500 tokens, with the forward: 472 us; with
+            // counters, and the logits looked up value by value, 582)
 };
 
 // Grid R x segments.  BWD: x is the incoming gradient and raw the logits' row, whose sign is asked for where a
@@ -59,10 +64,10 @@ __global__ __launch_bounds__(kConstrainThreads) void lucid_constrain_kernel(cons
                                                                             int Tn, int V, int segs, ConstrainRows a,
                                                                             T* __restrict__ out) {
   constexpr int NT = kConstrainThreads, N = LpRow<T>::N, C = kConstrainSeg / NT / N;
-  constexpr bool COUNT = H == History::Long || (H == History::Held && !BWD);
-  __shared__ __attribute__((aligned(16))) unsigned count[COUNT ? kConstrainSeg : 4];
+  static_assert(BWD || H != History::Held, "a forward counts");
+  __shared__ __attribute__((aligned(16))) unsigned count[H == History::Counted ? kConstrainSeg : 4];
   __shared__ unsigned bits[H == History::Held ? kConstrainSeg / 32 : 1];
-  __shared__ unsigned plus[H == History::Held && BWD ? kConstrainSeg / 32 : 1];  // of tokens whose logit is positive
+  __shared__ unsigned plus[H == History::Held ? kConstrainSeg / 32 : 1];  // of tokens whose logit is positive
   const int r = blockIdx.x / segs, seg = blockIdx.x - r * segs, tid = threadIdx.x;
   const LpRow<T> row(lp_row(x, sb, st, Tn, r), V);
   const int q0 = seg * NT * C + tid, lo = row.first(seg * NT * C);  // (lo may be negative: the first chunk)
@@ -110,29 +115,21 @@ __global__ __launch_bounds__(kConstrainThreads) void lucid_constrain_kernel(cons
     unsigned at;
     if (tid < kConstrainSeg / 32) {
       bits[tid] = 0;
-      if (BWD) plus[tid] = 0;
+      plus[tid] = 0;
     }
     bool up[kConstrainHeld];
-    if constexpr (BWD) {
 #pragma unroll
-      for (int k = 0; k < kConstrainHeld; ++k)
-        up[k] = k * NT < a.N && constrain_names(held[k], lo, V, at) && (float)rr[held[k]] > 0.f;
-    }
-    if constexpr (COUNT) {
-#pragma unroll
-      for (int k = 0; k < kConstrainHeld; ++k)
-        if (k * NT < a.N && constrain_names(held[k], lo, V, at)) count[at] = 0;
-    }
+    for (int k = 0; k < kConstrainHeld; ++k)
+      up[k] = k * NT < a.N && constrain_names(held[k], lo, V, at) && (float)rr[held[k]] > 0.f;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kConstrainHeld; ++k)
       if (k * NT < a.N && constrain_names(held[k], lo, V, at)) {
         atomicOr(&bits[at >> 5], 1u << (at & 31));
-        if (BWD && up[k]) atomicOr(&plus[at >> 5], 1u << (at & 31));
-        if (COUNT && k * NT + tid >= from) atomicAdd(&count[at], 1u);
+        if (up[k]) atomicOr(&plus[at >> 5], 1u << (at & 31));
       }
     __syncthreads();
-  } else if constexpr (H == History::Long) {
+  } else if constexpr (H == History::Counted) {
     for (int i = tid; i < kConstrainSeg / 4; i += NT) *reinterpret_cast<u32x4*>(&count[4 * i]) = u32x4{0, 0, 0, 0};
     __syncthreads();
     for (int i0 = tid; i0 < a.N; i0 += kConstrainHeld * NT) {
@@ -168,10 +165,10 @@ __global__ __launch_bounds__(kConstrainThreads) void lucid_constrain_kernel(cons
       if constexpr (H == History::Held) {
         const unsigned b = bits[at >> 5] >> (at & 31);
         any = (b & ((1u << N) - 1)) != 0;
-        if (BWD) positive = plus[at >> 5] >> (at & 31);
+        positive = plus[at >> 5] >> (at & 31);
         if (any) {
 #pragma unroll
-          for (int e = 0; e < N; ++e) n[e] = b >> e & 1 ? kConstrainSeen | (COUNT ? count[at + e] : 0u) : 0u;
+          for (int e = 0; e < N; ++e) n[e] = b >> e & 1 ? kConstrainSeen : 0u;
         }
       } else {
 #pragma unroll

@@ -14,7 +14,9 @@
 //                               the sweep takes the solved one out of the later rows' y
 //   lucid_prefill_sweep_kernel  (attend) the softmax over all rows, cached and new
 //   lucid_prefill_join_kernel   parts of a sweep that was cut along the keys
-// The sweeps are the work: 4 (Hq + Hkv) d flops for each pair of a token and a row.
+// The sweeps are the work: 4 (Hq + Hkv) d flops for each pair of a token and a row.  2048 tokens of 32/8 heads of 128 columns
+// behind 32768 rows (1.42 TFLOP, 185 MB) take 1.70 ms: 1.17 of attending, 0.43 of coupling, 0.23 in the eight solves and the
+// seven inner sweeps between them, which are one chain.
 #include <type_traits>
 
 #include "paged_common.h"
@@ -83,7 +85,8 @@ __device__ __forceinline__ T* tile_at(T* tile, int r, int c) {
 
 // --------------------------------------------------------------------------------------------
 // Grid (4 panels of L, Hkv, B), 512 threads: four workgroups share a panel's rows to write and its tiles.  Every workgroup of
-// a sequence looks its page ids over itself.
+// a sequence looks its page ids over itself.  13 us for 2048 tokens of 8 heads of 128 columns: latency, a chain of loads (lengths,
+// page ids, rows) before 36 tiles of products.  (P as hi + lo bf16, about 17 bits: the solve sums up to 255 of them.)
 // --------------------------------------------------------------------------------------------
 template <int W>
 __global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __restrict__ k, Strides ks, int vec,
@@ -198,16 +201,20 @@ __global__ __launch_bounds__(512) void lucid_prefill_prep_kernel(const bf16* __r
 }
 
 // --------------------------------------------------------------------------------------------
-// How a sweep is shared out, worked out by every wave from the sequences' lengths.  All row tiles (RT of a sequence's
-// rows, GX for each token) of all kv heads and sequences stand in one line, each as long as its keys' staged tiles, and
+// How a sweep is shared out, worked out by every wave from the sequences' lengths and tokens.  All row tiles (RT of a
+// sequence's rows, GX for each token) of all kv heads and sequences stand in one line, each as long as its keys' staged tiles, and
 // every workgroup takes an equal share of it: whole row tiles, and at either end part of one, along the keys.  A part
 // goes to slot 2 s of share s if it holds the share's beginning, else to 2 s + 1.  (Whole row tiles cut into equal parts
 // instead left a last round half empty: 4 sequences of 300 to 512 tokens of 32/4 heads of 64 columns behind 8192 rows, 181 us.)
+// Row tiles have 64 rows (four waves to 32 of them) or 256.  A place of 64 takes about 1 / 3.2 of one of 256, and a row tile
+// costs as much again as 4 of its places: whichever sums to less.  (us of a call with 64 / 256 / as chosen: 16 sequences of 1 to
+// 256 tokens of 16/16 heads of 64 columns behind 500 to 4000 rows 131 / 173 / 138; 16 of 256 each behind 4000 434 / 311 / 304,
+// of 96 columns 695 / 409 / 412; 14 of 1 to 256 tokens of 32/4 heads of 68 columns behind 50 to 3500 77 / 85 / 74.)
 // Places without keys lead every row tile: what beginning and ending one costs.  A share's end at the beginning of a row
 // tile, or anywhere in a short one, goes back to where it starts.
 // --------------------------------------------------------------------------------------------
 struct SweepGrid {
-  int GX, RT, attend, target;  // target: shares at most
+  int GX, attend, target;      // target: shares at most
   int whole;                   // staged tiles of a row tile that is not cut at all
 };
 struct SweepPiece {
@@ -223,19 +230,36 @@ constexpr int kSweepSnap = 2;   // staged tiles at a row tile's beginning that a
 struct SweepPlan {
   PrefillBatch s;
   SweepGrid a;
+  int RT;          // rows of a row tile
   int total, per;  // places of the line and of a share (their number fits: the host's check)
   int2 x0;         // sequence `lane` of the first 64
-  __device__ __forceinline__ int tiles(const int2& x) const { return (x.y * a.GX + a.RT - 1) / a.RT; }
+  __device__ __forceinline__ int tiles(const int2& x) const { return (x.y * a.GX + RT - 1) / RT; }
   __device__ __forceinline__ int keys(const int2& x) const { return x.x + (a.attend ? x.y : 0); }
   __device__ __forceinline__ int len(const int2& x) const { return max(1, (keys(x) + kSweepKeys - 1) / kSweepKeys); }
   __device__ __forceinline__ int2 at(int b) const { return b < 64 ? x0 : b < s.B ? s.info[b] : make_int2(0, 0); }
   __device__ __forceinline__ SweepPlan() {}
-  __device__ __forceinline__ SweepPlan(const PrefillBatch& seq, const SweepGrid& grid) : s(seq), a(grid), total(0) {
+  // FORM: rows of a row tile, or 0: chosen here
+  template <int FORM>
+  __device__ __forceinline__ void init(const PrefillBatch& seq, const SweepGrid& grid) {
+    s = seq;
+    a = grid;
     const int lane = threadIdx.x & 63;
     x0 = lane < s.B ? s.info[lane] : make_int2(0, 0);
-    for (int b0 = 0; b0 < s.B; b0 += 64) {
-      const int2 x = at(b0 + lane);
-      total += __builtin_amdgcn_readlane(wave_scan(s.Hkv * tiles(x) * (len(x) + kSweepLead)), 63);
+    auto sum = [&](auto of) {
+      int all = 0;
+      for (int b0 = 0; b0 < s.B; b0 += 64) all += __builtin_amdgcn_readlane(wave_scan(of(at(b0 + lane))), 63);
+      return all;
+    };
+    auto places = [&](int rows) {
+      return sum([&](const int2& x) { return s.Hkv * ((x.y * a.GX + rows - 1) / rows) * (len(x) + kSweepLead); });
+    };
+    RT = FORM;
+    if constexpr (FORM == 0) {
+      const int many = places(64), few = places(256), tiles64 = sum([&](const int2& x) { return s.Hkv * ((x.y * a.GX + 63) / 64); });
+      RT = (float)many + 4.f * (float)tiles64 < 3.2f * (float)few ? 64 : 256;
+      total = RT == 64 ? many : few;
+    } else {
+      total = places(FORM);
     }
     per = max(kSweepLeast, (total + a.target - 1) / a.target);
   }
@@ -343,32 +367,30 @@ __device__ __forceinline__ bf16x8 tile_tr(const bf16* tile, const TileTr& o, int
   return bf16x8{v1[0], v1[1], v1[2], v1[3], v2[0], v2[1], v2[2], v2[3]};
 }
 
-// Waves of a SIMD: as many as the registers of the instances leave place for
-constexpr int sweep_waves(int NW) { return NW == 8 ? 2 : 3; }
-
-// NW waves over tiles of 16 NW keys, staged once for all of them; a wave holds NT tiles of 32 rows, KSP waves share them and
-// take every KSP-th 32 keys (RT = 32 NT NW / KSP rows).  Lane <-> row: S^T[j][i] = K_j . x_i, then acc^T[col][i] +=
+// Bound by the matrix units and the VALU beside them, which take turns (128 columns: MFMAs 49 % of the cycles, VALU 38 %; 1.0
+// PFLOP/s of a large product's 1.36).  Both products are written so that lanes stay rows: the scores leave the first as the
+// second's operand, without LDS.  Only tiles of 32 keys that some row does not see are masked.
+// Eight waves over tiles of 128 keys, staged once for all of them; KSP waves share 32 rows and take every KSP-th 32 keys
+// (RT = 256 / KSP rows).  Lane <-> row: S^T[j][i] = K_j . x_i, then acc^T[col][i] +=
 // w^T[col][j] p^T[j][i].
 //   attend: x = q, rows (token, query head of the group) token by token, online softmax
 //   couple: x = the new keys, p = P as a bf16 pair; y = v - acc
 //   inner:  as couple, with the keys of one panel of new rows and out of the y of the rows behind it; grid (row
 //           tiles, Hkv, B), where the others go by SweepPlan
 enum class Sweep { Couple, Attend, Inner };
-template <int W, Sweep MODE, int KSP, int NW, int NT>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_waves(NW)))) void lucid_prefill_sweep_kernel(
-    const bf16* __restrict__ x, Strides xs, int vec, const bf16* __restrict__ v, Strides vs, PagedPool kp, PagedPool vp,
-    PrefillBatch seq, SweepGrid grid, int panel, PagedScale f, float eps, int d, float* __restrict__ y, int64_t yrows,
-    bf16* __restrict__ o, Strides os, int ovec, SweepParts part) {
+template <int W, Sweep MODE, int KSP>
+__device__ __forceinline__ void prefill_sweep(
+    SweepSmem<W, kSweepKeys>& sm, const SweepPlan& plan, const bf16* x, const Strides& xs, int vec,
+    const bf16* v, const Strides& vs, const PagedPool& kp, const PagedPool& vp, const PrefillBatch& seq,
+    const SweepGrid& grid, int panel, const PagedScale& f, float eps, int d, float* y, int64_t yrows,
+    bf16* o, const Strides& os, int ovec, const SweepParts& part) {
   constexpr bool ATTEND = MODE == Sweep::Attend, LINE = MODE != Sweep::Inner;
-  constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = CPR / 2, KT = 16 * NW, NMT = KT / 32 / KSP;
-  constexpr int RT = 32 * NT * NW / KSP;
-  static_assert(KSP == 1 || (NT == 1 && RT == 64), "the join of key groups holds 64 rows");
-  __shared__ __attribute__((aligned(16))) SweepSmem<W, KT> sm;
+  constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = CPR / 2, KT = kSweepKeys, NMT = KT / 32 / KSP;
+  constexpr int NW = 8, NT = 1, RT = 32 * NW / KSP;
+  static_assert(KSP == 1 || RT == 64, "the join of key groups holds 64 rows");
   int share = 0, start = 0, place = 0, end = 1, row_base = 0;
   SweepPiece it;
-  SweepPlan plan;
   if constexpr (LINE) {
-    plan = SweepPlan(seq, grid);
     // ids go round robin over the 8 XCDs: each takes a run of shares, the row tiles of one kv head next to each other
     const int num = (plan.total + plan.per - 1) / plan.per, each = (num + 7) >> 3;
     share = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
@@ -747,20 +769,46 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sweep_w
   }
 }
 
+template <int W, Sweep MODE, int FORM>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void lucid_prefill_sweep_kernel(
+    const bf16* __restrict__ x, Strides xs, int vec, const bf16* __restrict__ v, Strides vs, PagedPool kp, PagedPool vp,
+    PrefillBatch seq, SweepGrid grid, int panel, PagedScale f, float eps, int d, float* __restrict__ y, int64_t yrows,
+    bf16* __restrict__ o, Strides os, int ovec, SweepParts part) {
+  __shared__ __attribute__((aligned(16))) SweepSmem<W, kSweepKeys> sm;
+  SweepPlan plan;
+  if constexpr (MODE != Sweep::Inner) plan.init<FORM>(seq, grid);
+  if constexpr (FORM != 64)
+    if (FORM == 256 || plan.RT == 256) {
+      prefill_sweep<W, MODE, 1>(sm, plan, x, xs, vec, v, vs, kp, vp, seq, grid, panel, f, eps, d, y, yrows, o, os, ovec, part);
+      return;
+    }
+  if constexpr (FORM != 256)
+    prefill_sweep<W, MODE, 4>(sm, plan, x, xs, vec, v, vs, kp, vp, seq, grid, panel, f, eps, d, y, yrows, o, os, ovec, part);
+}
+
 // --------------------------------------------------------------------------------------------
-// The parts of the row tiles that a share's end cuts, joined.  Grid (row tiles at most, pieces of one), 256 threads: a piece of
+// The parts of the row tiles that a share's end cuts, joined in fp32: 10 us for the two of 8 heads, 32 row tiles each, of 128
+// columns.  Grid (row tiles at most, pieces of one), 256 threads: a piece of
 // join_rows(W) rows, W / 4 lanes a row.
 // --------------------------------------------------------------------------------------------
 constexpr int join_rows(int W) { return 256 / (W / 4); }
-template <int W, bool ATTEND>
+constexpr int join_pieces(int W, int RT) { return (RT + join_rows(W) - 1) / join_rows(W); }
+template <int W, bool ATTEND, int FORM>
 __global__ __launch_bounds__(256) void lucid_prefill_join_kernel(const bf16* __restrict__ v, Strides vs, int vec,
                                                                  PrefillBatch seq, SweepGrid grid, int d, float* __restrict__ y,
                                                                  int64_t yrows, bf16* __restrict__ o, Strides os, int ovec,
                                                                  SweepParts part) {
   constexpr int CG = W / 4;
-  const SweepPlan plan(seq, grid);
+  SweepPlan plan;
+  plan.init<FORM>(seq, grid);
   SweepPiece it;
-  if (!plan.number(blockIdx.x, it)) return;
+  int tile = blockIdx.x, piece = blockIdx.y;
+  if constexpr (FORM == 0) {  // a line of them: the first pieces of all row tiles, then the second ones, ..
+    const int tiles = seq.B * seq.Hkv * ((seq.L * grid.GX + plan.RT - 1) / plan.RT), index = blockIdx.y * gridDim.x + blockIdx.x;
+    piece = index / tiles;
+    tile = index - piece * tiles;
+  }
+  if (!plan.number(tile, it)) return;
   // the last share that begins at its first place, or the one that has it beside others
   const int share = (it.place + plan.uncut(it) - 1) / plan.per;
   const int parts = (it.place + kSweepLead + it.len - 1) / plan.per - share + 1;
@@ -768,8 +816,9 @@ __global__ __launch_bounds__(256) void lucid_prefill_join_kernel(const bf16* __r
   const int slot0 = 2 * share + (share * plan.per >= it.place ? 0 : 1);
   const int GX = grid.GX, rows = it.c * GX;
   {
-    const int i = threadIdx.x, r = join_rows(W) * blockIdx.y + i / CG, col = 4 * (i % CG), row = it.tile * grid.RT + r;
-    if (i >= join_rows(W) * CG || r >= grid.RT || row >= rows) return;
+    const int i = threadIdx.x, r = join_rows(W) * piece + i / CG, col = 4 * (i % CG),
+              row = it.tile * plan.RT + r;
+    if (i >= join_rows(W) * CG || r >= plan.RT || row >= rows) return;
     const int t = row / GX, hq = it.h * GX + (row - t * GX);
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
     float M = PREFILL_NEG, l = 0.f;
@@ -780,7 +829,7 @@ __global__ __launch_bounds__(256) void lucid_prefill_join_kernel(const bf16* __r
 #pragma unroll
       for (int k = 0; k < UN; ++k) {
         const int p = min(p0 + k, parts - 1);
-        const int64_t at = (int64_t)(p == 0 ? slot0 : 2 * (share + p)) * grid.RT + r;
+        const int64_t at = (int64_t)(p == 0 ? slot0 : 2 * (share + p)) * plan.RT + r;
         x[k] = *reinterpret_cast<const f32x4*>(part.o + at * W + col);
         m[k] = ATTEND ? part.m[at] : 0.f;
         lp[k] = ATTEND ? part.l[at] : 0.f;

@@ -11,9 +11,11 @@
 
 namespace {
 
-// Results of so many bytes pass the 256 MB cache by
+// Results of so many bytes pass the 256 MB cache by (past it / through it, us: 131072 tokens of 40 heads of 128 bf16 columns
+// turned, 1.3 GB, 489 / 612; constraints on 1700 rows of 32000 bf16 values, 109 MB, 47 / 49, on 8192 with gradient 472 / 479)
 constexpr int64_t kPastBytes = 100000000;
 
+constexpr int kSweepShares = 256;  // of the line of a sweep: a workgroup to a CU
 
 struct PrefillWs {
   int2* info;       // [B]
@@ -22,11 +24,6 @@ struct PrefillWs {
   lucid::SweepParts part;  // slots of either sweep
   size_t bytes;
 };
-
-// Rows of a workgroup of a sweep: 64 with four waves to 32 rows where there are few
-int sweep_rows(int64_t rows, bool attend, int W) { return rows <= 128 ? 64 : attend && W <= 96 ? 128 : 256; }
-// Shares of the line: one round of the chip, whose CUs hold three workgroups of 128 rows, and one of the others
-int sweep_target(int RT) { return RT == 128 ? 768 : 256; }
 
 PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
   const size_t panels = ((size_t)L + lucid::kPanel - 1) / lucid::kPanel;
@@ -41,8 +38,7 @@ PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
   w.info = reinterpret_cast<int2*>(take((size_t)B * 8));
   w.pmat = take((size_t)B * Hkv * panels * lucid::kPanelBytes);
   w.y = reinterpret_cast<float*>(take((size_t)B * Hkv * panels * lucid::kPanel * W * 4));
-  size_t rows = 0;  // of the parts of any sweep
-  for (int RT : {64, 128, 256}) rows = std::max(rows, (size_t)2 * sweep_target(RT) * RT);
+  const size_t rows = (size_t)2 * kSweepShares * 256;  // of the parts of any sweep
   w.part.o = reinterpret_cast<float*>(take(rows * W * 4));
   w.part.m = reinterpret_cast<float*>(take(rows * 4));
   w.part.l = reinterpret_cast<float*>(take(rows * 4));
@@ -82,35 +78,40 @@ int prefill_sweep(const PrefillCall& c, int panel = 0) {
   const int GX = ATTEND ? c.Hq / c.seq.Hkv : 1;
   const int panels = (c.seq.L + lucid::kPanel - 1) / lucid::kPanel;
   const int64_t rows = (int64_t)c.seq.L * GX, yrows = (int64_t)panels * lucid::kPanel;
-  const int RT = LINE ? sweep_rows(rows, ATTEND, W) : 64;
-  const int64_t tiles = (int64_t)c.seq.B * c.seq.Hkv * ((rows + RT - 1) / RT);  // at most
-  // staged tiles of a sequence's keys, at most: where they are few, no row tile is cut and nothing is joined
+  // staged tiles of a sequence's keys, at most: where they are few, no row tile is cut and nothing is joined (37 tokens of
+  // 16/16 heads of 64 columns behind 300 rows: 35 us, cut and joined 42)
   const int64_t most = prefill_len(c.seq.page, c.seq.M) - lucid::kSweepLead;
-  const lucid::SweepGrid grid{GX, RT, ATTEND, sweep_target(RT), most <= 8 ? 8 : 4};
+  const lucid::SweepGrid grid{GX, ATTEND, kSweepShares, most <= 8 ? 8 : 4};
   const bf16* x = ATTEND ? c.q : c.k;
   const int64_t* xs = ATTEND ? c.qs : c.ks;
   const int vec = rows_of_4(x, xs, 2), vvec = rows_of_4(c.v, c.vs, 2);
   const int ovec = ATTEND ? c.D % 4 == 0 && rows_of_4(c.o, c.os, 2) : vvec;
-  const dim3 blocks = LINE ? dim3((grid.target + 7) / 8 * 8)
-                           : dim3((unsigned)((c.seq.L - lucid::kPanel * (panel + 1) + RT - 1) / RT), c.seq.Hkv, c.seq.B);
-  auto go = [&](auto kernel, int threads) -> int {
+  const dim3 blocks = LINE ? dim3(kSweepShares) : dim3((c.seq.L - lucid::kPanel * (panel + 1) + 63) / 64, c.seq.Hkv, c.seq.B);
+  auto go = [&](auto form) -> int {
+    constexpr int FORM = decltype(form)::value;
     LUCID_LAUNCH_B(ATTEND ? "lucid_prefill_attend_kernel" : LINE ? "lucid_prefill_couple_kernel" : "lucid_prefill_inner_kernel",
-                   kernel, blocks, dim3(threads), c.st, x, S(xs), vec, c.v, S(c.vs), c.kp, c.vp, c.seq, grid, panel, c.scale, c.eps,
-                   c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
+                   (lucid::lucid_prefill_sweep_kernel<W, MODE, FORM>), blocks, dim3(512), c.st, x, S(xs), vec, c.v, S(c.vs), c.kp,
+                   c.vp, c.seq, grid, panel, c.scale, c.eps, c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
+    if constexpr (LINE) {
+      if (most <= grid.whole) return LUCID_OK;
+      const int64_t heads = (int64_t)c.seq.B * c.seq.Hkv;
+      const int64_t fine = heads * ((rows + 63) / 64), wide = heads * ((rows + 255) / 256);  // row tiles at most
+      const int64_t all = std::max(fine * lucid::join_pieces(W, 64), wide * lucid::join_pieces(W, 256));
+      const dim3 pieces = FORM == 64    ? dim3((unsigned)fine, lucid::join_pieces(W, 64))
+                          : FORM == 256 ? dim3((unsigned)wide, lucid::join_pieces(W, 256))
+                                        : dim3((unsigned)std::min<int64_t>(all, 1 << 20), (unsigned)((all + (1 << 20) - 1) >> 20));
+      LUCID_LAUNCH("lucid_prefill_join_kernel", (lucid::lucid_prefill_join_kernel<W, ATTEND, FORM>), pieces, c.st, c.v, S(c.vs),
+                   vvec, c.seq, grid, c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
+    }
     return LUCID_OK;
   };
-  if constexpr (!LINE) {
-    return go(lucid::lucid_prefill_sweep_kernel<W, MODE, 4, 8, 1>, 512);
-  } else {
-    constexpr int NW = ATTEND && W <= 96 ? 4 : 8;
-    const int rc = RT == 64 ? go(lucid::lucid_prefill_sweep_kernel<W, MODE, 4, 8, 1>, 512)
-                            : go(lucid::lucid_prefill_sweep_kernel<W, MODE, 1, NW, 1>, 64 * NW);
-    if (rc || most <= grid.whole) return rc;
-    LUCID_LAUNCH("lucid_prefill_join_kernel", (lucid::lucid_prefill_join_kernel<W, ATTEND>),
-                 dim3((unsigned)tiles, (RT + lucid::join_rows(W) - 1) / lucid::join_rows(W)), c.st, c.v, S(c.vs), vvec, c.seq,
-                 grid, c.D, c.ws.y, yrows, c.o, S(c.os), ovec, c.ws.part);
-    return LUCID_OK;
-  }
+  // Up to 128 rows 64 to a row tile (100 tokens of 8/8 heads of 128 columns behind 8000 rows: 68 us, with 256 to a tile 76;
+  // 8 x 20 tokens of 32/8 heads behind 4000: 81 and 100), from 513 on 256 (with 64: 2048 tokens of 32/8 heads of 128 columns behind
+  // 32768 1.67 -> 2.25 ms; left to the plan, both kinds in one kernel, 1 % slower); between, the plan looks at the tokens.
+  if (!LINE || rows <= 128) return go(std::integral_constant<int, 64>{});
+  if constexpr (LINE)
+    if (rows <= 512) return go(std::integral_constant<int, 0>{});
+  return go(std::integral_constant<int, LINE ? 256 : 64>{});
 }
 
 template <int W>
@@ -194,8 +195,10 @@ int constrain_launch(const T* x, int64_t sb, int64_t st, const T* raw, int64_t r
     constexpr History H = decltype(h)::value;
     return past ? go(lucid::lucid_constrain_kernel<T, H, BWD, true>) : go(lucid::lucid_constrain_kernel<T, H, BWD, false>);
   };
-  if (a.N > lucid::kConstrainThreads * lucid::kConstrainHeld) return pick(std::integral_constant<History, History::Long>{});
-  return a.N ? pick(std::integral_constant<History, History::Held>{}) : pick(std::integral_constant<History, History::None>{});
+  if (a.N == 0) return pick(std::integral_constant<History, History::None>{});
+  if constexpr (BWD)
+    if (a.N <= lucid::kConstrainThreads * lucid::kConstrainHeld) return pick(std::integral_constant<History, History::Held>{});
+  return pick(std::integral_constant<History, History::Counted>{});
 }
 
 }  // namespace
@@ -277,6 +280,9 @@ int lucid_rotary(const void* q, const int64_t* q_strides, void* q_out, const int
   c.scale = (float)scale;
   c.dir = inverse ? -1.f : 1.f;
   const int64_t tokens = (int64_t)B * T;
+  // Two tokens share a workgroup where there are many.  us with one / two / four: 8 x 2048 tokens of 36 heads of 68 fp32 columns
+  // and their gradient 137 / 139 / 152, 131072 of 40 of 128 bf16, half of it turned, 598 / 503 / 491, 65536 interleaved whole
+  // 239 / 226 / 242; of kernel with one / two: 32 tokens 3.9 / 4.5, 512 to 2048 the same
   c.tokens = tokens >= 4096 ? lucid::kRotaryTokens : 1;
   const int64_t blocks = (tokens + c.tokens - 1) / c.tokens;
   if (blocks > 0x7fffffff / 256) return fail("lucid_rotary: too many tokens");
