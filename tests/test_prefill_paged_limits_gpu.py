@@ -140,3 +140,34 @@ def test_python_refusals():
     bad(ValueError, "new_lens", counts=c["counts"][:1])
     bad(ValueError, "page_table", table=c["table"][:1])
     assert call(dict(c, q=c["q"][:, :, :0], k=c["k"][:, :, :0], v=c["v"][:, :, :0])).shape == (2, 0, 4, 64)
+
+
+@pytest.mark.parametrize("d", [64, 68, 96, 128])
+@pytest.mark.parametrize("lens,counts", [([1500, 900, 2100], [256, 256, 256]), ([1500, 900, 2100, 40], [1, 130, 20, 64]),
+                                         ([0, 3000], [500, 512]), ([0, 3000, 77, 1025, 2500], [3, 65, 512, 1, 129])], ids=str)
+def test_full_and_ragged_chunks(d, lens, counts):
+    """129 to 512 rows a kv head: full chunks take 256 rows to a row tile, ragged ones 64, and both are cut along the keys."""
+    print(f"case d={d} {lens} {counts}", flush=True)
+    run(make(lens, counts, 2, 2, d, 64))
+    run(make(lens, [min(c, 170) for c in counts], 9, 3, d, 16, L=170, seed=1))
+
+
+def test_captured_call_goes_from_full_to_ragged():
+    """The same graph with chunks that fill their row tiles, and with ones that do not."""
+    c = make([800, 800, 800], [256, 256, 256], 4, 4, 64, 64)
+    pools = c["kp"].clone(), c["vp"].clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call(c)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = call(c)
+    for counts in ([256, 256, 256], [3, 70, 1], [256, 0, 200], [10, 10, 10]):
+        c["counts"].copy_(torch.tensor(counts, dtype=torch.int32))
+        c["kp"].copy_(pools[0])
+        c["vp"].copy_(pools[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        check(c, o, (pools[0].clone(), pools[1].clone()))
