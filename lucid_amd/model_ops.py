@@ -235,8 +235,12 @@ def rope_frequencies(dim: int, theta: float = 10000.0, scaling: dict | None = No
         length = float(scaling["original_max_position_embeddings"]) if kind in ("llama3", "yarn") else 0.0
     except KeyError as e:
         raise ValueError(f"lucid_amd.rope_frequencies: {kind} needs {e.args[0]!r}") from None
-    if not factor > 0.0 or length < 0.0:
+    if not factor > 0.0:
         raise ValueError(f"lucid_amd.rope_frequencies: the factor must be positive, got {factor}")
+    if kind in ("llama3", "yarn") and not length > 0.0:
+        raise ValueError(f"lucid_amd.rope_frequencies: {kind} needs positive original_max_position_embeddings, got {length}")
+    if kind == "yarn" and not theta > 1.0:
+        raise ValueError(f"lucid_amd.rope_frequencies: yarn needs a theta above 1, got {theta}")
     if kind == "linear":
         return freq / factor, 1.0
     if kind == "ntk":
@@ -672,6 +676,8 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
             raise NotImplementedError(f"{what}: no gradient of {name}")
         if t.dim() < 1 or (last is not None and t.shape[-1] != last) or not (t.shape[:-1] == lead or (shared and t.dim() == 1)):
             raise ValueError(f"{what}: {name} {tuple(t.shape)} does not fit logits {tuple(logits.shape)}")
+        if t.shape[-1] >= 1 << 30:
+            raise ValueError(f"{what}: {name} of fewer than 2^30 a row, got {t.shape[-1]}")
         if t.dim() != 2:
             t = t.reshape(1 if t.shape[:-1] != lead else lead.numel(), t.shape[-1])
         return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()

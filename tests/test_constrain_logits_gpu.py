@@ -292,3 +292,9 @@ def test_two_streams_and_expanded_rows():
     torch.cuda.synchronize()
     for y in outs:
         close(y, want, tol, "logits")
+
+
+def test_histories_beyond_32_bits_are_refused():
+    logits = torch.zeros(1, 10, device="cuda")
+    with pytest.raises(ValueError, match="fewer than"):
+        O.constrain_logits(logits, history=torch.zeros(1, 1, dtype=torch.int64, device="cuda").expand(1, 1 << 30))

@@ -60,3 +60,16 @@ def test_refusals():
     for dim in (-2, 3):
         with pytest.raises(ValueError, match="even"):
             rope_frequencies(dim)
+
+
+@pytest.mark.parametrize("kind", ["llama3", "yarn"])
+@pytest.mark.parametrize("length", [0, -8192, float("nan")])
+def test_lengths_that_are_none_are_refused(kind, length):
+    with pytest.raises(ValueError, match="original_max_position_embeddings"):
+        rope_frequencies(64, 10000.0, {"rope_type": kind, "factor": 4.0, "original_max_position_embeddings": length})
+
+
+@pytest.mark.parametrize("theta", [1.0, 0.5])
+def test_yarn_without_a_spread_of_wavelengths_is_refused(theta):
+    with pytest.raises(ValueError, match="theta"):
+        rope_frequencies(64, theta, {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096})
