@@ -369,7 +369,7 @@ __device__ __forceinline__ bf16x8 tile_tr(const bf16* tile, const TileTr& o, int
 
 // Bound by the matrix units and the VALU beside them, which take turns (128 columns: MFMAs 49 % of the cycles, VALU 38 %; 1.0
 // PFLOP/s of a large product's 1.36).  Both products are written so that lanes stay rows: the scores leave the first as the
-// second's operand, without LDS.  Only tiles of 32 keys that some row does not see are masked.
+// second's operand, without LDS.  Only tiles with a key that some row of the wave does not see are masked.
 // Eight waves over tiles of 128 keys, staged once for all of them; KSP waves share 32 rows and take every KSP-th 32 keys
 // (RT = 256 / KSP rows).  Lane <-> row: S^T[j][i] = K_j . x_i, then acc^T[col][i] +=
 // w^T[col][j] p^T[j][i].
@@ -386,7 +386,7 @@ __device__ __forceinline__ void prefill_sweep(
     bf16* o, const Strides& os, int ovec, const SweepParts& part) {
   constexpr bool ATTEND = MODE == Sweep::Attend, LINE = MODE != Sweep::Inner;
   constexpr int NKS = W / 16, NDT = (W + 31) / 32, CPR = W / 8, NST = CPR / 2, KT = kSweepKeys, NMT = KT / 32 / KSP;
-  constexpr int NW = 8, NT = 1, RT = 32 * NW / KSP;
+  constexpr int NW = 8, RT = 32 * NW / KSP;
   static_assert(KSP == 1 || RT == 64, "the join of key groups holds 64 rows");
   int share = 0, start = 0, place = 0, end = 1, row_base = 0;
   SweepPiece it;
@@ -426,24 +426,15 @@ __device__ __forceinline__ void prefill_sweep(
   asm volatile("" : "+v"(tid));  // what follows from it is worked out here, not kept in registers across the pieces
   const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, l32 = lane & 31;
   const int rw = w / KSP, kg = w % KSP;
-  const int rows = it.c * GX, row0 = row_base + it.tile * RT + 32 * NT * rw;  // of this wave
+  const int rows = it.c * GX, row0 = row_base + it.tile * RT + 32 * rw;  // of this wave
   const bool active = row0 < rows;
-  int row[NT], t[NT], hq[NT];
-#pragma unroll
-  for (int u = 0; u < NT; ++u) {
-    row[u] = row0 + 32 * u + l32;
-    const int r = min(row[u], rows - 1);
-    t[u] = r / GX;
-    hq[u] = h * GX + (r - t[u] * GX);
-  }
+  const int row = row0 + l32, mine = min(row, rows - 1), t = mine / GX, hq = h * GX + (mine - t * GX);  // of the lane
   // attend: no row of this workgroup sees a key beyond its last token's
   const int last = min(row_base + (it.tile + 1) * RT, rows) - 1;
   const int j0 = it.j0, j1 = ATTEND ? min(it.j1, n + last / GX + 1) : it.j1;
-  int lim[NT];  // the lane's last key,
-#pragma unroll
-  for (int u = 0; u < NT; ++u) lim[u] = ATTEND ? min(j1 - 1, n + t[u]) : j1 - 1;
-  const int free = ATTEND ? min(j1 - 1, n + min(row0, rows - 1) / GX) : j1 - 1;      // one that all lanes of the wave see,
-  const int most = ATTEND ? n + min(row0 + 32 * NT - 1, rows - 1) / GX : j1 - 1;  // and one beyond which none does
+  const int lim = ATTEND ? min(j1 - 1, n + t) : j1 - 1;                           // the lane's last key,
+  const int free = ATTEND ? min(j1 - 1, n + min(row0, rows - 1) / GX) : j1 - 1;  // one that all lanes of the wave see,
+  const int most = ATTEND ? n + min(row0 + 31, rows - 1) / GX : j1 - 1;  // and one beyond which none does
   const int ntile = (j1 - j0 + KT - 1) / KT;
 
   // staging: half of the waves the keys, the others V', 32 rows each
@@ -500,37 +491,26 @@ __device__ __forceinline__ void prefill_sweep(
     stage(0, id0, 0);
   }
   const float c = f.sl2;
-  bf16x8 xb[NT][NKS];
-  float c1[NT], m[NT], lsum[NT];
-  f32x16 acc[NT][NDT];
+  bf16x8 xb[NKS];
+  float c1 = 0.f, m = PREFILL_NEG, lsum = 0.f;
+  f32x16 acc[NDT];
+  const bf16* xr = x + b * xs.b + (ATTEND ? hq : h) * xs.h + t * xs.t;
 #pragma unroll
-  for (int u = 0; u < NT; ++u) {
-    const bf16* xr = x + b * xs.b + (ATTEND ? hq[u] : h) * xs.h + t[u] * xs.t;
+  for (int st = 0; st < NKS; ++st) xb[st] = ld8_cols(xr, 16 * st + 8 * g, d, vec);
 #pragma unroll
-    for (int st = 0; st < NKS; ++st) xb[u][st] = ld8_cols(xr, 16 * st + 8 * g, d, vec);
-#pragma unroll
-    for (int q = 0; q < NDT; ++q) acc[u][q] = zero16();
-    m[u] = PREFILL_NEG;
-    lsum[u] = 0.f;
-    c1[u] = 0.f;
-  }
+  for (int q = 0; q < NDT; ++q) acc[q] = zero16();
   if constexpr (!ATTEND) {
+    float nt = 0.f;
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      float nt = 0.f;
-#pragma unroll
-      for (int st = 0; st < NKS; ++st) nt = dot8(xb[u][st], nt);
-      c1[u] = c * rsqrtf(wave_sum32(nt) / (float)d + eps);
-    }
+    for (int st = 0; st < NKS; ++st) nt = dot8(xb[st], nt);
+    c1 = c * rsqrtf(wave_sum32(nt) / (float)d + eps);
   }
   TileTr tr[NDT];
 #pragma unroll
   for (int q = 0; q < NDT; ++q) tr[q] = tile_tr_off<W>(32 * q);
   // the rows have landed before the loop (else every tile's first product waits for the next tile's loads)
 #pragma unroll
-  for (int u = 0; u < NT; ++u)
-#pragma unroll
-    for (int st = 0; st < NKS; ++st) asm volatile("" ::"v"(xb[u][st]));
+  for (int st = 0; st < NKS; ++st) asm volatile("" ::"v"(xb[st]));
   dma_wait();
   if (ntile > 0) norms(0);
   __syncthreads();
@@ -545,66 +525,52 @@ __device__ __forceinline__ void prefill_sweep(
       const bf16* tv = sm.u.st.v[buf];
       const bool mask = jb + KT - 1 > free;
       if constexpr (ATTEND) {
-        f32x16 s[NMT][NT];
+        f32x16 s[NMT];
 #pragma unroll
         for (int i = 0; i < NMT; ++i) {
           const int mt = kg + KSP * i;
-#pragma unroll
-          for (int u = 0; u < NT; ++u) s[i][u] = zero16();
+          s[i] = zero16();
 #pragma unroll
           for (int st = 0; st < NKS; ++st) {
             const bf16x8 kf = ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g));
-#pragma unroll
-            for (int u = 0; u < NT; ++u) s[i][u] = mfma32(kf, xb[u][st], s[i][u]);
+            s[i] = mfma32(kf, xb[st], s[i]);
           }
         }
         if (mask) {
 #pragma unroll
           for (int i = 0; i < NMT; ++i)
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (jb + (kg + KSP * i) * 32 + drow(e, g) > lim[u]) s[i][u][e] = -INFINITY;
+            for (int e = 0; e < 16; ++e)
+              if (jb + (kg + KSP * i) * 32 + drow(e, g) > lim) s[i][e] = -INFINITY;
         }
+        float mx = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          float mx = -INFINITY;
+        for (int i = 0; i < NMT; ++i)
 #pragma unroll
-          for (int i = 0; i < NMT; ++i)
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[i][e]);
+        mx = wave_max32(mx) * c;
+        if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f)) {  // rescale only where a row grows by 2^8
+          const float mnew = fmaxf(m, mx);
+          const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+          m = mnew;
+          lsum *= alpha;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[i][u][e]);
-          mx = wave_max32(mx) * c;
-          if (__builtin_amdgcn_ballot_w64(mx > m[u] + 8.0f)) {  // rescale only where a row grows by 2^8
-            const float mnew = fmaxf(m[u], mx);
-            const float alpha = __builtin_amdgcn_exp2f(m[u] - mnew);
-            m[u] = mnew;
-            lsum[u] *= alpha;
+          for (int q = 0; q < NDT; ++q)
 #pragma unroll
-            for (int q = 0; q < NDT; ++q)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) acc[u][q][e] *= alpha;
-          }
+            for (int e = 0; e < 16; ++e) acc[q][e] *= alpha;
         }
 #pragma unroll
         for (int i = 0; i < NMT; ++i) {
           const int mt = kg + KSP * i;
-          bf16x8 p0[NT], p1[NT];
 #pragma unroll
-          for (int u = 0; u < NT; ++u) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[i][u][e] = __builtin_amdgcn_exp2f(fmaf(s[i][u][e], c, -m[u]));
-            p0[u] = pack_b(s[i][u], 0);
-            p1[u] = pack_b(s[i][u], 1);
-            lsum[u] = add_sum8(p1[u], add_sum8(p0[u], lsum[u]));  // sum of the bf16 P of the product
-          }
+          for (int e = 0; e < 16; ++e) s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], c, -m));
+          const bf16x8 p0 = pack_b(s[i], 0), p1 = pack_b(s[i], 1);
+          lsum = add_sum8(p1, add_sum8(p0, lsum));  // sum of the bf16 P of the product
 #pragma unroll
           for (int q = 0; q < NDT; ++q) {
             const bf16x8 a0 = tile_tr<W>(tv, tr[q], mt * 32), a1 = tile_tr<W>(tv, tr[q], mt * 32 + 16);
-#pragma unroll
-            for (int u = 0; u < NT; ++u) acc[u][q] = mfma32(a0, p0[u], acc[u][q]);
-#pragma unroll
-            for (int u = 0; u < NT; ++u) acc[u][q] = mfma32(a1, p1[u], acc[u][q]);
+            acc[q] = mfma32(a0, p0, acc[q]);
+            acc[q] = mfma32(a1, p1, acc[q]);
           }
         }
       } else {
@@ -613,42 +579,29 @@ __device__ __forceinline__ void prefill_sweep(
 #pragma unroll
         for (int i = 0; i < NMT; ++i) {
           const int mt = kg + KSP * i;
-          f32x16 s[NT];
-#pragma unroll
-          for (int u = 0; u < NT; ++u) s[u] = zero16();
+          f32x16 s = zero16();
 #pragma unroll
           for (int st = 0; st < NKS; ++st) {
             const bf16x8 kf = ld8(tile_at<W>(tk, mt * 32 + l32, 2 * st + g));
-#pragma unroll
-            for (int u = 0; u < NT; ++u) s[u] = mfma32(kf, xb[u][st], s[u]);
+            s = mfma32(kf, xb[st], s);
           }
           float nr[16];
           lds_rows16(&sm.nr[buf][32 * mt], g, nr);
 #pragma unroll
-          for (int u = 0; u < NT; ++u) {
+          for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(c1 * nr[e], s[e], -f.c0));
+          if (mask) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[u][e] = __builtin_amdgcn_exp2f(fmaf(c1[u] * nr[e], s[u][e], -f.c0));
-            if (mask) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (jb + mt * 32 + drow(e, g) > lim[u]) s[u][e] = 0.f;
-            }
+            for (int e = 0; e < 16; ++e)
+              if (jb + mt * 32 + drow(e, g) > lim) s[e] = 0.f;
           }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            bf16x8 hi[NT], lo[NT];
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-              hi[u] = pack_b(s[u], k);
-              lo[u] = pack_lo(s[u], k, hi[u]);
-            }
+            const bf16x8 hi = pack_b(s, k), lo = pack_lo(s, k, hi);
 #pragma unroll
             for (int q = 0; q < NDT; ++q) {
               const bf16x8 a = tile_tr<W>(tv, tr[q], mt * 32 + 16 * k);
-#pragma unroll
-              for (int u = 0; u < NT; ++u) acc[u][q] = mfma32(a, hi[u], acc[u][q]);
-#pragma unroll
-              for (int u = 0; u < NT; ++u) acc[u][q] = mfma32(a, lo[u], acc[u][q]);
+              acc[q] = mfma32(a, hi, acc[q]);
+              acc[q] = mfma32(a, lo, acc[q]);
             }
           }
         }
@@ -658,29 +611,27 @@ __device__ __forceinline__ void prefill_sweep(
     if (jt + 1 < ntile) norms(buf ^ 1);
     __syncthreads();
   }
-  float l[NT];
-#pragma unroll
-  for (int u = 0; u < NT; ++u) l[u] = ATTEND ? wave_sum32(lsum[u]) : 0.f;
+  float l = ATTEND ? wave_sum32(lsum) : 0.f;
   if constexpr (KSP > 1) {  // the key groups' sums joined in the waves of group 0
     const int r = 32 * rw + l32;
     if constexpr (ATTEND) {
       if (g == 0) {
-        sm.u.fin.m[kg][r] = m[0];
-        sm.u.fin.l[kg][r] = l[0];
+        sm.u.fin.m[kg][r] = m;
+        sm.u.fin.l[kg][r] = l;
       }
       __syncthreads();
       float M = sm.u.fin.m[0][r];
 #pragma unroll
       for (int k = 1; k < KSP; ++k) M = fmaxf(M, sm.u.fin.m[k][r]);
-      l[0] = 0.f;
+      l = 0.f;
 #pragma unroll
-      for (int k = 0; k < KSP; ++k) l[0] = fmaf(sm.u.fin.l[k][r], __builtin_amdgcn_exp2f(sm.u.fin.m[k][r] - M), l[0]);
-      const float a = __builtin_amdgcn_exp2f(m[0] - M);
-      m[0] = M;
+      for (int k = 0; k < KSP; ++k) l = fmaf(sm.u.fin.l[k][r], __builtin_amdgcn_exp2f(sm.u.fin.m[k][r] - M), l);
+      const float a = __builtin_amdgcn_exp2f(m - M);
+      m = M;
 #pragma unroll
       for (int q = 0; q < NDT; ++q)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[0][q][e] *= a;
+        for (int e = 0; e < 16; ++e) acc[q][e] *= a;
     }
 #pragma unroll
     for (int half = KSP / 2; half >= 1; half /= 2) {
@@ -692,7 +643,7 @@ __device__ __forceinline__ void prefill_sweep(
           for (int e = 0; e < 16; e += 4)
             if (32 * q + drow(e, 0) < W)
               *reinterpret_cast<f32x4*>(&sm.u.fin.o[kg - half][r][32 * q + drow(e, g)]) =
-                  f32x4{acc[0][q][e], acc[0][q][e + 1], acc[0][q][e + 2], acc[0][q][e + 3]};
+                  f32x4{acc[q][e], acc[q][e + 1], acc[q][e + 2], acc[q][e + 3]};
       }
       __syncthreads();
       if (kg < half) {
@@ -703,30 +654,28 @@ __device__ __forceinline__ void prefill_sweep(
             if (32 * q + drow(e, 0) < W) {
               const f32x4 z = *reinterpret_cast<const f32x4*>(&sm.u.fin.o[kg][r][32 * q + drow(e, g)]);
 #pragma unroll
-              for (int u = 0; u < 4; ++u) acc[0][q][e + u] += z[u];
+              for (int u = 0; u < 4; ++u) acc[q][e + u] += z[u];
             }
       }
     }
   }
-#pragma unroll
-  for (int r = 0; r < NT; ++r) {
-    if (kg != 0 || row[r] >= rows) continue;
+  if (kg == 0 && row < rows) {
     if (it.slot >= 0) {
-      const int64_t at = (int64_t)it.slot * RT + 32 * (NT * rw + r) + l32;
+      const int64_t at = (int64_t)it.slot * RT + 32 * rw + l32;
 #pragma unroll
       for (int q = 0; q < NDT; ++q)
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
           if (32 * q + drow(e, 0) < W)
             *reinterpret_cast<f32x4*>(part.o + at * W + 32 * q + drow(e, g)) =
-                f32x4{acc[r][q][e], acc[r][q][e + 1], acc[r][q][e + 2], acc[r][q][e + 3]};
+                f32x4{acc[q][e], acc[q][e + 1], acc[q][e + 2], acc[q][e + 3]};
       if (ATTEND && g == 0) {
-        part.m[at] = m[r];
-        part.l[at] = l[r];
+        part.m[at] = m;
+        part.l[at] = l;
       }
     } else if constexpr (ATTEND) {
-      const float inv = 1.f / l[r];
-      bf16* op = o + b * os.b + hq[r] * os.h + t[r] * os.t;
+      const float inv = 1.f / l;
+      bf16* op = o + b * os.b + hq * os.h + t * os.t;
 #pragma unroll
       for (int q = 0; q < NDT; ++q)
 #pragma unroll
@@ -734,7 +683,7 @@ __device__ __forceinline__ void prefill_sweep(
           const int col = 32 * q + drow(e, g);
           bf16x4 z;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) z[u] = (bf16)(acc[r][q][e + u] * inv);
+          for (int u = 0; u < 4; ++u) z[u] = (bf16)(acc[q][e + u] * inv);
           if (ovec && col + 4 <= d) {
             *reinterpret_cast<bf16x4*>(op + col) = z;
           } else {
@@ -744,8 +693,8 @@ __device__ __forceinline__ void prefill_sweep(
           }
         }
     } else {
-      float* yp = y + (((int64_t)b * seq.Hkv + h) * yrows + t[r]) * W;
-      const bf16* vr = v + b * vs.b + h * vs.h + t[r] * vs.t;
+      float* yp = y + (((int64_t)b * seq.Hkv + h) * yrows + t) * W;
+      const bf16* vr = v + b * vs.b + h * vs.h + t * vs.t;
 #pragma unroll
       for (int q = 0; q < NDT; ++q)
 #pragma unroll
@@ -760,7 +709,7 @@ __device__ __forceinline__ void prefill_sweep(
             z = f32x4{(float)v4[0], (float)v4[1], (float)v4[2], (float)v4[3]};
           }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) z[u] -= acc[r][q][e + u];
+          for (int u = 0; u < 4; ++u) z[u] -= acc[q][e + u];
           *reinterpret_cast<f32x4*>(yp + col) = z;
         }
     }
