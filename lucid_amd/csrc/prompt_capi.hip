@@ -25,7 +25,16 @@ struct PrefillWs {
   size_t bytes;
 };
 
-PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
+// Places of a row tile in the line of a sweep, at most
+int64_t prefill_len(int page, int max_pages) {
+  return ((int64_t)page * max_pages + lucid::kSweepKeys - 1) / lucid::kSweepKeys + lucid::kSweepLead;
+}
+
+// Staged tiles of a row tile that is not cut. Where a sequence can have no more (`tiles` of them at most), nothing is cut and
+// nothing joined (37 tokens of 16/16 heads of 64 columns behind 300 rows: 35 us, cut and joined 42)
+int sweep_whole(int64_t tiles) { return tiles <= 8 ? 8 : 4; }
+
+PrefillWs carve_prefill(void* base, int B, int Hq, int Hkv, int L, int page, int max_pages, int W) {
   const size_t panels = ((size_t)L + lucid::kPanel - 1) / lucid::kPanel;
   size_t off = 0;
   char* p = static_cast<char*>(base);
@@ -38,17 +47,14 @@ PrefillWs carve_prefill(void* base, int B, int Hkv, int L, int W) {
   w.info = reinterpret_cast<int2*>(take((size_t)B * 8));
   w.pmat = take((size_t)B * Hkv * panels * lucid::kPanelBytes);
   w.y = reinterpret_cast<float*>(take((size_t)B * Hkv * panels * lucid::kPanel * W * 4));
-  const size_t rows = (size_t)2 * kSweepShares * 256;  // of the parts of any sweep
+  // rows of the parts of either sweep: of two row tiles a share, of 64 rows at up to 128 to a kv head
+  const int64_t tiles = prefill_len(page, max_pages) - lucid::kSweepLead;
+  const size_t rows = tiles <= sweep_whole(tiles) ? 0 : (size_t)2 * kSweepShares * ((int64_t)L * (Hq / Hkv) <= 128 ? 64 : 256);
   w.part.o = reinterpret_cast<float*>(take(rows * W * 4));
   w.part.m = reinterpret_cast<float*>(take(rows * 4));
   w.part.l = reinterpret_cast<float*>(take(rows * 4));
   w.bytes = off;
   return w;
-}
-
-// Places of a row tile in the line of a sweep, at most
-int64_t prefill_len(int page, int max_pages) {
-  return ((int64_t)page * max_pages + lucid::kSweepKeys - 1) / lucid::kSweepKeys + lucid::kSweepLead;
 }
 
 bool prefill_sizes_ok(int B, int Hq, int Hkv, int L, int page, int max_pages, int D) {
@@ -78,10 +84,8 @@ int prefill_sweep(const PrefillCall& c, int panel = 0) {
   const int GX = ATTEND ? c.Hq / c.seq.Hkv : 1;
   const int panels = (c.seq.L + lucid::kPanel - 1) / lucid::kPanel;
   const int64_t rows = (int64_t)c.seq.L * GX, yrows = (int64_t)panels * lucid::kPanel;
-  // staged tiles of a sequence's keys, at most: where they are few, no row tile is cut and nothing is joined (37 tokens of
-  // 16/16 heads of 64 columns behind 300 rows: 35 us, cut and joined 42)
-  const int64_t most = prefill_len(c.seq.page, c.seq.M) - lucid::kSweepLead;
-  const lucid::SweepGrid grid{GX, ATTEND, kSweepShares, most <= 8 ? 8 : 4};
+  const int64_t most = prefill_len(c.seq.page, c.seq.M) - lucid::kSweepLead;  // staged tiles of a sequence's keys
+  const lucid::SweepGrid grid{GX, ATTEND, kSweepShares, sweep_whole(most)};
   const bf16* x = ATTEND ? c.q : c.k;
   const int64_t* xs = ATTEND ? c.qs : c.ks;
   const int vec = rows_of_4(x, xs, 2), vvec = rows_of_4(c.v, c.vs, 2);
@@ -207,7 +211,7 @@ extern "C" {
 
 size_t lucid_prefill_paged_workspace_bytes(int B, int Hq, int Hkv, int L, int page_size, int max_pages, int D) {
   if (!prefill_sizes_ok(B, Hq, Hkv, L, page_size, max_pages, D)) return 0;
-  return carve_prefill(nullptr, B, Hkv, L, page_width(D)).bytes;
+  return carve_prefill(nullptr, B, Hq, Hkv, L, page_size, max_pages, page_width(D)).bytes;
 }
 
 int lucid_prefill_paged(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -232,7 +236,7 @@ int lucid_prefill_paged(const void* q, const int64_t* q_strides, const void* k, 
   constexpr double kLog2e = 1.4426950408889634;
   const int W = page_width(D);
   PrefillCall c{(const bf16*)q, (const bf16*)k, (const bf16*)v, q_strides, k_strides, v_strides, o_strides, {}, {}, {},
-                (bf16*)o, carve_prefill(ws, B, Hkv, L, W), Hq, D,
+                (bf16*)o, carve_prefill(ws, B, Hq, Hkv, L, page_size, max_pages, W), Hq, D,
                 {scale, (float)(scale * kLog2e), (float)(kLog2e / scale)}, eps, static_cast<hipStream_t>(stream)};
   if (int rc = check_pool("k_pages", k_pages, k_page_strides, num_pages, Hkv, page_size, W, &c.kp)) return rc;
   if (int rc = check_pool("vp_pages", vp_pages, vp_page_strides, num_pages, Hkv, page_size, W, &c.vp)) return rc;

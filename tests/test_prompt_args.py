@@ -166,3 +166,12 @@ def test_chunks_of_a_cache():
     with pytest.raises(OutOfPages):
         cache.begin(1, 40)
     assert cache.length(a) == 10 and cache.begin(1, 2).chunk  # a refused pass changes nothing
+
+
+def test_workspaces_of_short_tables_and_few_rows(lib):
+    """Parts of row tiles are kept only where one can be cut, and 64 rows of each where that is what a row tile has."""
+    ws = lib.lucid_prefill_paged_workspace_bytes
+    short, few, many = (ws(1, 16, 16, L, 64, pages, 64) for L, pages in ((37, 16), (37, 17), (200, 17)))
+    assert short < 4 << 20  # 16 heads' panels (148 KB) and rows (64 KB)
+    assert few - short == 2 * 256 * 64 * (64 + 2) * 4
+    assert many - short == 2 * 256 * 256 * (64 + 2) * 4
