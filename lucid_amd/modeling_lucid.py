@@ -95,13 +95,27 @@ class LlamaRotaryEmbedding(nn.Module):
             # (float64, so not a buffer: those follow the module's dtype)
             self._freq, self.scale = rope_frequencies(part, config.rope_theta, config.rope_scaling)
             self.interleaved = config.rope_interleaved
+            self._placed = self._freq
+            self._table(inv_freq.device)
+
+    def _table(self, device: torch.device) -> torch.Tensor:
+        """The frequencies on ``device``, for this pass and those behind it: copied outside inference mode, whose tensors no
+        later pass could save for its backward."""
+        if self._placed.device != device:
+            with torch.inference_mode(False):
+                self._placed = self._freq.to(device)
+        return self._placed
+
+    def _apply(self, fn, recurse: bool = True):
+        super()._apply(fn, recurse)
+        if not self.plain:  # (a pass that is captured could not copy them from the host)
+            self._table(self.inv_freq.device)
+        return self
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, position_ids: torch.Tensor):
         if not self.plain:
-            if self._freq.device != x.device:
-                self._freq = self._freq.to(x.device)
-            return RotaryPositions(position_ids, self._freq, self.interleaved, self.scale)
+            return RotaryPositions(position_ids, self._table(x.device), self.interleaved, self.scale)
         freqs = position_ids[:, :, None].float() * self.inv_freq[None, None, :].to(x.device)
         emb = torch.cat((freqs, freqs), dim=-1)
         return emb.cos().to(x.dtype), emb.sin().to(x.dtype)
