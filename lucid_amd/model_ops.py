@@ -221,7 +221,7 @@ def rope_frequencies(dim: int, theta: float = 10000.0, scaling: dict | None = No
     0.1 ln(factor) + 1 if it is not given)."""
     if dim < 0 or dim % 2:
         raise ValueError(f"lucid_amd.rope_frequencies: an even number of columns, got {dim}")
-    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    i = torch.arange(0, dim, 2, dtype=torch.float64, device="cpu")
     freq = theta ** (-i / max(dim, 1))
     scaling = {} if scaling is None else dict(scaling)
     kind = scaling.get("rope_type", scaling.get("type", "default"))
@@ -256,7 +256,7 @@ def rope_frequencies(dim: int, theta: float = 10000.0, scaling: dict | None = No
 
     first = max(math.floor(pair(float(scaling.get("beta_fast", 32.0)))), 0)
     last = min(math.ceil(pair(float(scaling.get("beta_slow", 1.0)))), dim - 1)
-    keep = 1 - ((torch.arange(dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
+    keep = 1 - ((torch.arange(dim // 2, dtype=torch.float64, device="cpu") - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
     scale = scaling.get("attention_factor")
     scale = (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0) if scale is None else float(scale)
     return freq * keep + freq / factor * (1 - keep), scale
