@@ -208,6 +208,12 @@ def qkv_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, nq: int, n
     return QKVRopeFunction.apply(qkv, cos, sin, nq, nk)
 
 
+# Entries of a scaling that its type knows, beside the type and the length trained on
+_ROPE_ENTRIES = {"default": (), "linear": ("factor",), "ntk": ("factor",),
+                 "llama3": ("factor", "low_freq_factor", "high_freq_factor"),
+                 "yarn": ("factor", "beta_fast", "beta_slow", "attention_factor")}
+
+
 def rope_frequencies(dim: int, theta: float = 10000.0, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
     """Inverse frequencies (float64 ``[dim / 2]``, on the CPU) of ``dim`` turning columns, and the factor of the turned
     values: ``theta^(-2 i / dim)`` and 1, or scaled for contexts longer than the model was trained on.
@@ -218,18 +224,23 @@ def rope_frequencies(dim: int, theta: float = 10000.0, scaling: dict | None = No
     divided by ``factor``, those between are interpolated over the inverse wavelength); ``"yarn"`` (pairs that turn ``beta_fast`` (32) times
     or more in ``original_max_position_embeddings`` positions stay, those that turn ``beta_slow`` (1) times or less
     are divided by ``factor``, with a ramp over the pair's number between, and values are multiplied by ``attention_factor``,
-    0.1 ln(factor) + 1 if it is not given)."""
+    0.1 ln(factor) + 1 if it is not given).  An entry that is None is as if it were not there; entries that the type does not know are
+    refused (``original_max_position_embeddings`` may go with any)."""
     if dim < 0 or dim % 2:
         raise ValueError(f"lucid_amd.rope_frequencies: an even number of columns, got {dim}")
     i = torch.arange(0, dim, 2, dtype=torch.float64, device="cpu")
     freq = theta ** (-i / max(dim, 1))
-    scaling = {} if scaling is None else dict(scaling)
+    scaling = {} if scaling is None else {name: x for name, x in scaling.items() if x is not None}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in _ROPE_ENTRIES:
+        raise ValueError(f"lucid_amd.rope_frequencies: rope_type one of {tuple(_ROPE_ENTRIES)}, got {kind!r}")
+    if scaling.get("type", kind) != kind:
+        raise ValueError(f"lucid_amd.rope_frequencies: rope_type {kind!r} beside type {scaling['type']!r}")
+    unknown = sorted(set(scaling) - {"rope_type", "type", "original_max_position_embeddings", *_ROPE_ENTRIES[kind]})
+    if unknown:
+        raise ValueError(f"lucid_amd.rope_frequencies: {kind} does not know {', '.join(map(repr, unknown))}")
     if kind == "default" or dim == 0:
         return freq, 1.0
-    known = ("linear", "ntk", "llama3", "yarn")
-    if kind not in known:
-        raise ValueError(f"lucid_amd.rope_frequencies: rope_type one of {('default',) + known}, got {kind!r}")
     try:
         factor = float(scaling["factor"])
         length = float(scaling["original_max_position_embeddings"]) if kind in ("llama3", "yarn") else 0.0
