@@ -468,7 +468,8 @@ int lucid_rotary(const void* q, const int64_t* q_strides, void* q_out, const int
  * from place prompt_lens[r] on (null: from 0) has presence + n frequency taken off.  The three are numbers, or fp32
  * arrays [R] that replace them.  Then bias (fp32 [R][V], rows bias_stride apart; 0: one row for all) is added, and what the
  * mask allowed (bit v % 32 of word v / 32, rows allowed_stride words apart) has no bit for becomes -inf, whatever it
- * was.  The backward gives dlogits [R][V] from dout [R][V], both contiguous in the logits' dtype. */
+ * was.  The backward gives dlogits [R][V] from dout [R][V], both contiguous in the logits' dtype; it reads the logits where
+ * there is a history (N 0: they may be null). */
 int lucid_constrain_logits(const void* logits, int64_t batch_stride, int64_t row_stride, int R, int T, int V, int dtype,
                            const int64_t* history, int64_t history_stride, int N, const int32_t* prompt_lens,
                            const float* repetitions, float repetition, const float* presences, float presence,

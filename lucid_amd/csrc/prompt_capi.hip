@@ -169,7 +169,7 @@ int rotary_launch(lucid::RotaryCall c, unsigned blocks, hipStream_t st) {
 int constrain_segs(int V) { return (V + 7 + lucid::kConstrainSeg - 1) / lucid::kConstrainSeg; }
 
 int check_constrain(const std::string& w, const void* logits, int64_t sb, int64_t st, int R, int Tn, int V, int dtype,
-                    const lucid::ConstrainRows& a) {
+                    const lucid::ConstrainRows& a, bool raw = true) {  // raw: logits are read
   if (dtype != LUCID_DTYPE_BF16 && dtype != LUCID_DTYPE_F32) return fail(w + ": dtype LUCID_DTYPE_BF16 or LUCID_DTYPE_F32");
   if (R < 0 || Tn < 1 || R % Tn) return fail(w + ": R a multiple of the rows of a batch, got R=" + std::to_string(R));
   if (V < 1 || V > 2000000) return fail(w + ": V from 1 to 2000000, got " + std::to_string(V));
@@ -177,7 +177,7 @@ int check_constrain(const std::string& w, const void* logits, int64_t sb, int64_
   if (a.N < 0 || (a.N > 0 && R > 0 && !a.history)) return fail(w + ": a history of N tokens a row, N >= 0");
   if (!a.rep && !(a.rep0 > 0.f && std::isfinite(a.rep0))) return fail(w + ": the repetition penalty must be positive and finite");
   if ((!a.pres && !std::isfinite(a.pres0)) || (!a.freq && !std::isfinite(a.freq0))) return fail(w + ": penalties must be finite");
-  if (R > 0 && !logits) return fail(w + ": logits are null");
+  if (R > 0 && raw && !logits) return fail(w + ": logits are null");
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == LUCID_DTYPE_F32 ? 4 : 2)) return fail(w + ": logits are misaligned");
   if ((int64_t)R * constrain_segs(V) * 512 >= ((int64_t)1 << 32)) return fail(w + ": too many rows");
   return LUCID_OK;
@@ -320,7 +320,8 @@ int lucid_constrain_logits_bwd(const void* logits, int64_t batch_stride, int64_t
   g_last_error.clear();
   const lucid::ConstrainRows a{history, history_stride, N, nullptr, repetitions, nullptr, nullptr, repetition, 0.f, 0.f, nullptr,
                                0, allowed, allowed_stride};
-  if (int rc = check_constrain("lucid_constrain_logits_bwd", logits, batch_stride, row_stride, R, T, V, dtype, a)) return rc;
+  if (int rc = check_constrain("lucid_constrain_logits_bwd", logits, batch_stride, row_stride, R, T, V, dtype, a, N > 0))
+    return rc;
   if (R == 0) return LUCID_OK;
   if (!dout || !dlogits) return fail("lucid_constrain_logits_bwd: null argument");
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -628,21 +628,24 @@ class ConstrainLogitsFunction(torch.autograd.Function):
         c = _Constraints(*constraints)
         number = not isinstance(c.repetition, torch.Tensor)
         ctx.repetition = c.repetition if number else None
-        ctx.save_for_backward(logits, c.history, None if number else c.repetition, c.allowed)
+        # (the gradient depends on the logits through their sign, where a repetition penalty applies, and on nothing else)
+        signs = c.history is not None and c.history.shape[1] > 0 and not (number and c.repetition == 1.0)
+        ctx.save_for_backward(logits if signs else None, c.history if signs else None, None if number else c.repetition,
+                              c.allowed)
         return _constrain(logits, c)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: torch.Tensor):
         logits, history, repetition, allowed = ctx.saved_tensors
-        rows, T, sb, st = _logit_rows(logits)
-        V, dev = logits.shape[-1], logits.device
+        rows, T, sb, st = (None, 1, 0, 0) if logits is None else _logit_rows(logits)
+        V, dev = dout.shape[-1], dout.device
         g = dout.contiguous()
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        dlogits = torch.empty(dout.shape, dtype=dout.dtype, device=dev)
         lib = _lib.load()
         with _lib.on(dev):
             rc = lib.lucid_constrain_logits_bwd(
-                rows.data_ptr(), sb, st, dlogits.numel() // V, T, V, _LP_DTYPES[logits.dtype], *_rows_at(history),
+                None if rows is None else rows.data_ptr(), sb, st, dlogits.numel() // V, T, V, _LP_DTYPES[dout.dtype], *_rows_at(history),
                 0 if history is None else history.shape[1],
                 *_number(ctx.repetition if repetition is None else repetition), *_rows_at(allowed), g.data_ptr(),
                 dlogits.data_ptr(), _lib.stream_handle(dev))
