@@ -303,7 +303,8 @@ def _tracked(*tensors: torch.Tensor) -> bool:
 
 
 def _rotary(q, k, positions, inv_freq, interleaved, scale, inverse):
-    """q and k (either may be None) turned, into new [B, T, H, d] buffers seen as [B, H, T, d]."""
+    """q and k (either may be None) turned, into new tensors [B, H, T, d] laid out as [B, T, H, d] (no views, which could not be
+    changed in place behind an autograd function)."""
     some = k if q is None else q
     B, _, T, d = some.shape
     dtype, dev = some.dtype, some.device
@@ -313,16 +314,16 @@ def _rotary(q, k, positions, inv_freq, interleaved, scale, inverse):
         if q.stride(3) != 1 and d > 1:
             q = q.contiguous()
         H = q.shape[1]
-        qo = torch.empty((B, T, H, d), dtype=dtype, device=dev)
-        qa = (q.data_ptr(), _strides(q.stride()), qo.data_ptr(), _strides((T * H * d, d, H * d)), H)
-        qo = qo.transpose(1, 2)
+        by = (T * H * d, d, H * d, 1)
+        qo = torch.empty_strided((B, H, T, d), by, dtype=dtype, device=dev)
+        qa = (q.data_ptr(), _strides(q.stride()), qo.data_ptr(), _strides(by), H)
     if k is not None:
         if k.stride(3) != 1 and d > 1:
             k = k.contiguous()
         H = k.shape[1]
-        ko = torch.empty((B, T, H, d), dtype=dtype, device=dev)
-        ka = (k.data_ptr(), _strides(k.stride()), ko.data_ptr(), _strides((T * H * d, d, H * d)), H)
-        ko = ko.transpose(1, 2)
+        by = (T * H * d, d, H * d, 1)
+        ko = torch.empty_strided((B, H, T, d), by, dtype=dtype, device=dev)
+        ka = (k.data_ptr(), _strides(k.stride()), ko.data_ptr(), _strides(by), H)
     ps = positions.stride()
     lib = _lib.load()
     with _lib.on(dev):
@@ -362,8 +363,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     ``[1, T]`` or ``[B, T]``; ``inv_freq`` fp32 or fp64 ``[part / 2]`` (:func:`rope_frequencies`), part at most d.  With x =
     position inv_freq[i], the pair (a, b) number i of a row becomes scale (a cos x - b sin x, b cos x + a sin x): columns i and
     i + part / 2, or 2 i and 2 i + 1 where ``interleaved``; columns from part on stay as they are.  Angles are worked out in
-    64 bits (good for positions up to 2^31 and beyond), values in 32, rounded once.  Results are ``[B, H, T, d]`` views of
-    ``[B, T, H, d]`` buffers, as the projections leave them."""
+    64 bits (good for positions up to 2^31 and beyond), values in 32, rounded once.  Results are ``[B, H, T, d]``, laid out
+    as ``[B, T, H, d]`` as the projections leave them."""
     what = "lucid_amd.rotary"
     if not q.is_cuda:
         raise RuntimeError("lucid_amd: query must be a GPU tensor (no CPU path)")
