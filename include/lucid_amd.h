@@ -397,9 +397,10 @@ int lucid_decode_paged(const void* q, const int64_t* q_strides, const void* k, c
  * new_lens[b] tokens of sequence b (clamped to 0 .. L; null: L tokens each), for any number of them and at the rate of
  * a prefill.  The rows of q, k and v behind a sequence's tokens are padding and are not used; o is zero there
  * and in slots without a sequence.  The new rows' V' go to the pages only (bf16).  Any cutting of a prompt into
- * calls of this and of lucid_decode_paged gives the same rows up to rounding.  A sequence whose table names a page
- * outside the pool among those it needs, or is too short for the new rows, gets NaN in o and nothing is
- * written for it.  Cached rows and the tokens' rows must be finite, scale positive.  At most 65535 sequences and kv
+ * calls of this and of lucid_decode_paged gives the same rows up to rounding.  o's attention weights are single
+ * bf16 values here, pairs there: o is off by 0.0024 of its norm where lucid_decode_paged's is by 0.0017, the rounding
+ * of o itself.  A sequence whose table names a page outside the pool among those it needs, or is too short for the
+ * new rows, gets NaN in o and nothing is written for it.  Cached rows and the tokens' rows must be finite, scale positive.  At most 65535 sequences and kv
  * heads, 2^24 rows of query heads (L Hq / Hkv) to a kv head, 2^23 tiles of 64 of these in all, and 2^30 pairs of such
  * tiles and tiles of 128 of the rows that a table holds.
  * ws: lucid_prefill_paged_workspace_bytes (0 on bad sizes), 256-byte aligned, one per call in flight. */

@@ -27,6 +27,7 @@ inline int hip_status(const char* where) {
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
+// Workspaces hold operands whose blocks of rows must fill whole cache lines.
 inline int check_ws(const char* name, const void* p) {
   if (reinterpret_cast<uintptr_t>(p) % 256) return fail(std::string(name) + " must be 256-byte aligned");
   return LUCID_OK;

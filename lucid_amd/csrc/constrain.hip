@@ -5,8 +5,8 @@
 //   x = x + bias_v;  -inf where v is not allowed
 // Its gradient is 1, 1 / rho or rho (by the logit's sign), 0 where v is not allowed.  One read and one write of the rows, a
 // segment of 8192 values to a workgroup; each reads the row's whole history, which the caches hold.  HBM bounds large calls: 8192 rows
-// of 32000 bf16 values behind 500 tokens, 1.05 GB, 217 us, 4.8 TB/s, and their gradient, 1.05 GB, 245 us; 64 of 131072 behind
-// 4000, 35 MB, 16 us; 4 of 32003 fp32 values behind 100000 tokens 25 us, the history once for each of 5 segments.
+// of 32000 bf16 values behind 500 tokens, 1.05 GB, 236 us, 4.4 TB/s, and their gradient, 1.05 GB, 250 us; 64 of 131072 behind
+// 4000, 35 MB, 15 us; 4 of 32003 fp32 values behind 100000 tokens 24 us: 16 workgroups, each over its row's whole history.
 #include "logit_rows.h"
 
 namespace lucid {
@@ -49,7 +49,7 @@ constexpr int kConstrainHeld = 8;  // tokens of a history that a lane holds
 enum class History {
   None,
   Counted,  // a counter of each value in LDS (clearing only those of tokens held in registers, with a bit a value for the rest,
-            // was slower: 64 rows of 131072 behind 4000 tokens 16.3 -> 18.0 us, 256 of 32000 fp32 behind 2000 20.8 -> 22.9)
+            // was a tenth slower: 64 rows of 131072 behind 4000 tokens, 256 of 32000 fp32 behind 2000)
   Held,     // the gradient of up to 512 kConstrainHeld tokens: a bit of each value for an occurrence and for a logit above 0, both
             // from the tokens themselves, held in registers (8192 rows of 32000 behind 500 tokens, with the forward: 472 us; with
             // counters, and the logits looked up value by value, 582)

@@ -222,7 +222,6 @@ int check_dims(int B, int Hq, int Hkv, int T, int D) {
   return LUCID_OK;
 }
 
-// Workspaces hold the chain operands; their 64-row blocks must fill whole cache lines.
 int check_tensor(const char* name, const void* p, const int64_t* s, int mult = 8) {
   if (!p) return fail(std::string(name) + " is null");
   if (!s) return fail(std::string(name) + " strides are null");

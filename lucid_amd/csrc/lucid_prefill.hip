@@ -15,8 +15,9 @@
 //   lucid_prefill_sweep_kernel  (attend) the softmax over all rows, cached and new
 //   lucid_prefill_join_kernel   parts of a sweep that was cut along the keys
 // The sweeps are the work: 4 (Hq + Hkv) d flops for each pair of a token and a row.  2048 tokens of 32/8 heads of 128 columns
-// behind 32768 rows (1.42 TFLOP, 185 MB) take 1.70 ms: 1.17 of attending, 0.43 of coupling, 0.23 in the eight solves and the
-// seven inner sweeps between them, which are one chain.
+// behind 32768 rows (1.42 TFLOP, 185 MB) take 1.71 ms a call.  Its kernels traced one by one sum to 1.85 on the same card: 1.17 of
+// attending, 0.42 of coupling, 0.23 in the eight solves and the seven inner sweeps between them, which are one chain, and
+// 0.03 of prep and joins.
 #include <type_traits>
 
 #include "paged_common.h"
@@ -367,13 +368,19 @@ __device__ __forceinline__ bf16x8 tile_tr(const bf16* tile, const TileTr& o, int
   return bf16x8{v1[0], v1[1], v1[2], v1[3], v2[0], v2[1], v2[2], v2[3]};
 }
 
-// Bound by the matrix units and the VALU beside them, which take turns (128 columns: MFMAs 49 % of the cycles, VALU 38 %; 1.0
-// PFLOP/s of a large product's 1.36).  Both products are written so that lanes stay rows: the scores leave the first as the
+// Matrix units and VALU take turns: of a SIMD's cycles, attending at 128 columns has MFMAs in 52 % and the VALU in 41 % (0.97
+// PFLOP/s of a large product's 1.36), at 64 columns in 35 and 51 % (0.65), with the LDS read in 26 and 18 % of a CU's.  These are no
+// bounds of the chip: the kernels on contiguous rows reach 1.18 and 0.95 PFLOP/s; at 64 columns theirs hold 64 rows a wave, two products
+// for each operand read from LDS, where these waves hold 32.  Both products are written so that lanes stay rows: the scores leave the first as the
 // second's operand, without LDS.  Only tiles with a key that some row of the wave does not see are masked.
 // Eight waves over tiles of 128 keys, staged once for all of them; KSP waves share 32 rows and take every KSP-th 32 keys
 // (RT = 256 / KSP rows).  Lane <-> row: S^T[j][i] = K_j . x_i, then acc^T[col][i] +=
 // w^T[col][j] p^T[j][i].
-//   attend: x = q, rows (token, query head of the group) token by token, online softmax
+//   attend: x = q, rows (token, query head of the group) token by token, online softmax.  Its weights enter the second product
+//           as one bf16 and are summed as such, as in the kernels on contiguous rows: O is off by 0.0024 of its norm, 0.0017 of it
+//           the rounding of O itself.  As a pair (0.0017 in all) they would cost half the products of this sweep again: 2048 tokens
+//           of 32/8 heads of 128 columns behind 32768 rows 1.71 -> 2.20 ms, 4 x 512 of 32/4 of 64 behind 8192 262 -> 335 us.
+//           Nothing carries this rounding on, unlike the coupling's, whose errors the solve and the cache keep
 //   couple: x = the new keys, p = P as a bf16 pair; y = v - acc
 //   inner:  as couple, with the keys of one panel of new rows and out of the y of the rows behind it; grid (row
 //           tiles, Hkv, B), where the others go by SweepPlan
