@@ -628,11 +628,13 @@ class ConstrainLogitsFunction(torch.autograd.Function):
     def forward(ctx, logits: torch.Tensor, *constraints):
         c = _Constraints(*constraints)
         number = not isinstance(c.repetition, torch.Tensor)
-        ctx.repetition = c.repetition if number else None
         # (the gradient depends on the logits through their sign, where a repetition penalty applies, and on nothing else)
-        signs = c.history is not None and c.history.shape[1] > 0 and not (number and c.repetition == 1.0)
-        ctx.save_for_backward(logits if signs else None, c.history if signs else None, None if number else c.repetition,
-                              c.allowed)
+        if c.history is None or c.history.shape[1] == 0 or (number and c.repetition == 1.0):
+            ctx.repetition = 1.0
+            ctx.save_for_backward(None, None, None, c.allowed)
+        else:
+            ctx.repetition = c.repetition if number else None
+            ctx.save_for_backward(logits, c.history, None if number else c.repetition, c.allowed)
         return _constrain(logits, c)
 
     @staticmethod

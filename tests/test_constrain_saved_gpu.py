@@ -74,3 +74,18 @@ def test_shapes_of_a_gradient_without_logits():
         grad = torch.randn(*x.shape[:-1], 1001, generator=g, device="cuda").to(BF)[..., 1:]
         d, = torch.autograd.grad(O.constrain_logits(leaf, allowed=bits_of(ok)), leaf, grad)
         assert d.shape == x.shape and torch.equal(d, torch.where(ok, grad, 0.0).to(BF))
+
+
+def test_penalties_and_histories_may_change_where_the_gradient_does_not_ask_for_them():
+    """Without a history no penalty is kept, and without a repetition penalty no history."""
+    g, x, ok, h = make(F32)
+    rho = 0.5 + torch.rand(x.shape[0], generator=g, device="cuda")
+    phi = rho.clone()
+    leaf = x.clone().requires_grad_()
+    y = O.constrain_logits(leaf, repetition=rho, allowed=bits_of(ok))
+    z = O.constrain_logits(leaf, history=h, frequency=phi)
+    rho.fill_(2.0)
+    phi.fill_(2.0)
+    h.fill_(0)
+    (y[ok].sum() + z.sum()).backward()
+    assert torch.equal(leaf.grad, 1.0 + ok.float())
